@@ -35,11 +35,15 @@ EXPORTED = (
     "gf_batch_set_grads", "gf_batch_read", "gf_backward_noalloc", "gf_forward", "gf_backward_direct",
     "gf_forward_grads_offset", "gf_backward_direct_launches", "gf_fwd_bwd_fused", "gf_fwd_bwd_fused_supported",
     "gf_forward_kcap", "gf_backward_direct_kcap", "gf_forward_bin_info", "gf_read_bin_info", "gf_backward_train",
+    "gf_dropout_add", "gf_ff_saved_bytes", "gf_ff_workspace_bytes", "gf_ff_forward", "gf_ff_backward",
 )
 
 GF_PHASE_BIN, GF_PHASE_EMIT, GF_PHASE_RENDER = 0x1, 0x2, 0x4
 GF_PHASE_REDUCE, GF_PHASE_FINISH = 0x1, 0x2
 GF_PHASE_ALL = 0xFF
+
+GF_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+GF_ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}
 
 
 class GfFieldConfig(ctypes.Structure):
@@ -85,6 +89,24 @@ class GfBatchInfo(ctypes.Structure):
         ("emit_blocks", c_int64), ("finish_blocks", c_int64), ("plan_bytes", c_size_t),
         ("backward_buffers", c_int32), ("mask_clamp", c_int32), ("render_blocks", c_int64),
         ("tile_render", c_int32), ("wide_blocks", c_int32),
+    ]
+
+
+class GfDropout(ctypes.Structure):
+    """``gf_dropout``."""
+
+    _fields_ = [("p", c_double), ("seed", c_uint64), ("seed_device", c_void_p), ("offset", c_uint64)]
+
+
+class GfFfArgs(ctypes.Structure):
+    """``gf_ff_args``: a linear or gated product of the feed-forward block (device pointers)."""
+
+    _fields_ = [
+        ("dtype", c_int32), ("activation", c_int32), ("rows", c_int64), ("in_features", c_int64),
+        ("out_features", c_int64), ("x", c_void_p), ("ldx", c_int64), ("weight", c_void_p), ("ldw", c_int64),
+        ("bias", c_void_p), ("residual", c_void_p), ("ldr", c_int64), ("y", c_void_p), ("saved", c_void_p),
+        ("dy", c_void_p), ("lddy", c_int64), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p),
+        ("dropout", GfDropout),
     ]
 
 
@@ -159,12 +181,20 @@ def lib() -> ctypes.CDLL:
     L.gf_batch_read.argtypes = [_P, POINTER(GfBatchInfo), c_int32, POINTER(c_uint32), POINTER(c_int64),
                                 POINTER(c_double), _P]
     L.gf_selftest_softplus.argtypes = [POINTER(c_uint64), _P]
+    L.gf_dropout_add.argtypes = [c_int32, POINTER(GfDropout), c_int64, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P]
+    L.gf_ff_saved_bytes.argtypes = [POINTER(GfFfArgs)]
+    L.gf_ff_saved_bytes.restype = c_size_t
+    L.gf_ff_workspace_bytes.argtypes = [POINTER(GfFfArgs), c_int32]
+    L.gf_ff_workspace_bytes.restype = c_size_t
+    L.gf_ff_forward.argtypes = [POINTER(GfFfArgs), _P, c_size_t, _P]
+    L.gf_ff_backward.argtypes = [POINTER(GfFfArgs), _P, c_size_t, _P]
     for name in ("gf_tile_grid", "gf_forward_bin", "gf_forward_emit", "gf_forward_render",
                  "gf_backward", "gf_backward_reduce", "gf_backward_finish", "gf_read_status",
                  "gf_selftest_softplus", "gf_batch_plan", "gf_batch_forward", "gf_batch_backward",
                  "gf_batch_set_grads", "gf_batch_read", "gf_backward_noalloc", "gf_forward",
                  "gf_backward_direct", "gf_fwd_bwd_fused", "gf_forward_kcap", "gf_backward_direct_kcap",
-                 "gf_forward_bin_info", "gf_read_bin_info", "gf_backward_train"):
+                 "gf_forward_bin_info", "gf_read_bin_info", "gf_backward_train",
+                 "gf_dropout_add", "gf_ff_forward", "gf_ff_backward"):
         getattr(L, name).restype = c_int
     _LIB = L
     return L

@@ -1,6 +1,7 @@
 """Builds the native libraries in-tree.
 
-* ``guass_amd/libgaussfield.so``       gfx950 kernels + C ABI (hipcc, --offload-arch=gfx950)
+* ``guass_amd/libgaussfield.so``       gfx950 kernels + C ABI (hipcc, --offload-arch=gfx950): the fields'
+                                       (gaussfield.hip) and the feed-forward block's (feedforward.hip)
 * ``guass_amd/libgaussfield_host.so``  host build of the per-Gaussian geometry (g++), used by
                                        CPU tests to pin the exact arithmetic the GPU runs
 * ``oracle/_build/libm_sweep``         exhaustive libm check (test infrastructure)
@@ -17,11 +18,14 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
+GPU_SOURCES = [CSRC / "gaussfield.hip", CSRC / "feedforward.hip"]
 LIB = PKG / "libgaussfield.so"
 HOST_LIB = PKG / "libgaussfield_host.so"
 
@@ -55,10 +59,19 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError(f"build failed ({proc.returncode}): {' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
 
 
+def _compile_and_link(flags: list[str], lib: Path) -> None:
+    """The GPU sources, compiled at the same time, linked into ``lib``."""
+    flags = [f for f in flags if f != "-shared"]
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor() as pool:
+        objects = [Path(tmp) / f"{src.stem}.o" for src in GPU_SOURCES]
+        list(pool.map(lambda so: _run([hipcc(), *flags, "-c", str(so[0]), "-o", str(so[1])]), zip(GPU_SOURCES, objects)))
+        new = lib.with_suffix(".so.tmp")
+        _run([hipcc(), *flags, "-shared", *map(str, objects), "-o", str(new)])
+        os.replace(new, lib)
+
+
 def build_gpu_lib() -> Path:
-    tmp = LIB.with_suffix(".so.tmp")
-    _run([hipcc(), *HIP_FLAGS, str(CSRC / "gaussfield.hip"), "-o", str(tmp)])
-    os.replace(tmp, LIB)
+    _compile_and_link(HIP_FLAGS, LIB)
     return LIB
 
 
@@ -113,7 +126,7 @@ def build_sanitized(out_dir: Path = SANITIZE_DIR) -> dict[str, Path]:
     lib, host = out_dir / "libgaussfield.so", out_dir / "libgaussfield_host.so"
     hip = [f for f in HIP_FLAGS if f != "-O3"] + ["-O1", "-g"]
     host_only = [a for f in SANITIZE_FLAGS for a in ("-Xarch_host", f)]
-    _run([hipcc(), *hip, *host_only, str(CSRC / "gaussfield.hip"), "-o", str(lib)])
+    _compile_and_link([*hip, *host_only], lib)
     _run([clangxx(), "-O1", "-g", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off", *SANITIZE_FLAGS,
           str(CSRC / "host_geometry.cpp"), "-o", str(host)])
     return {"lib": lib, "host_lib": host}

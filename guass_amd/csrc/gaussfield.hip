@@ -57,6 +57,7 @@
 #include <vector>
 
 #include "../../include/gaussfield.h"
+#include "error.h"
 #include "geometry.h"
 
 #define GF_VERSION "gaussfield-mi355x 0.2.0"
@@ -5137,6 +5138,9 @@ int scratch_for_current_device(void** out) {
 }
 
 }  // namespace
+
+// feedforward.hip's errors, for the same gf_last_error().
+int gf_set_error(int code, const char* message) { return set_err(code, "%s", message); }
 
 // ------------------------------------------------------------------------------------------
 // C ABI.

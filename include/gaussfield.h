@@ -486,6 +486,69 @@ int gf_read_status(void* workspace, int32_t clear, uint32_t* status_host, void* 
  */
 int gf_selftest_softplus(uint64_t* checksum_host, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Feed-forward block (csrc/feedforward.hip): what surrounds the adapted linears of a transformer
+ * block's feed-forward half.  No counterpart in the reference.
+ *
+ *   dropout  y = residual + drop(x)
+ *   linear   y = residual + drop(x W^T + b)                    W [out, in], b [out]
+ *   gated    y = drop(value * act(gate)), (value, gate) = the first and the last `out` columns of
+ *            x W^T + b                                         W [2 out, in], b [2 out]
+ *
+ * drop: element (row, col) of the output takes 16 bits of Philox4x32-10 (Salmon et al., 2011): half-word
+ * col % 8 (low halves first) of the block with counter (col / 8, row, offset low, offset high) and key
+ * `seed`.  It is dropped (exactly 0, whatever it was) where they are below t = round(p * 65536), else
+ * multiplied by 65536 / (65536 - t).  No mask is stored: the backward makes it again.
+ *
+ * Matrices are row-major with unit column stride and a row stride (ld*, in elements) of at least their
+ * width; all are of one type, `dtype`; products and sums are accumulated in 32 bits.  bias, residual and
+ * the outputs that are not wanted are NULL.  dx [rows, in], dweight and dbias (shaped as weight and bias)
+ * are written whole, contiguous; the residual's gradient is dy itself. */
+#define GF_DTYPE_F32 0
+#define GF_DTYPE_BF16 1
+#define GF_DTYPE_F16 2
+
+#define GF_ACT_NONE 0      /* linear                                              */
+#define GF_ACT_GELU 1      /* gated: g Phi(g)                                     */
+#define GF_ACT_GELU_TANH 2 /* gated: g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2 */
+#define GF_ACT_SILU 3      /* gated: g / (1 + exp(-g))                            */
+
+typedef struct gf_dropout {
+  double p;                    /* share of the elements that are dropped, in [0, 1]             */
+  uint64_t seed;               /* Philox key                                                    */
+  const uint64_t* seed_device; /* not NULL: the key is read from here when the kernels run, so
+                                  that a captured graph can be replayed with another            */
+  uint64_t offset;             /* counter words 2 and 3: one value per call of a step           */
+} gf_dropout;
+
+typedef struct gf_ff_args {
+  int32_t dtype, activation;
+  int64_t rows, in_features, out_features;
+  const void* x;        int64_t ldx;
+  const void* weight;   int64_t ldw;
+  const void* bias;
+  const void* residual; int64_t ldr;  /* linear only                                            */
+  void* y;                            /* [rows, out], contiguous                                */
+  void* saved;                        /* gated: gf_ff_saved_bytes, written by a forward that a
+                                         backward follows (NULL: none) and read by it           */
+  const void* dy;       int64_t lddy; /* backward                                               */
+  void* dx;
+  void* dweight;
+  void* dbias;
+  gf_dropout dropout;
+} gf_ff_args;
+
+int gf_dropout_add(int32_t dtype, const gf_dropout* dropout, int64_t rows, int64_t cols, const void* x, int64_t ldx,
+                   const void* residual, int64_t ldr, void* y, int64_t ldy, void* stream);
+
+/* Bytes of `saved` (0 for linear) and of the workspace of a forward or backward with these arguments (their
+ * pointers' alignment counts, their contents do not); 0 on invalid arguments too (gf_last_error tells). */
+size_t gf_ff_saved_bytes(const gf_ff_args* args);
+size_t gf_ff_workspace_bytes(const gf_ff_args* args, int32_t backward);
+
+int gf_ff_forward(const gf_ff_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int gf_ff_backward(const gf_ff_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,473 @@
+"""The feed-forward operators (guass_amd/feedforward.py) against their definitions in 64 bits.
+
+The bounds are the oracle's (oracle/feedforward_oracle.py): what 32-bit sums and the roundings to the
+tensors' type may do, element by element.  No counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from guass_amd import _native as N
+from guass_amd import feedforward as ff
+from oracle import feedforward_oracle as fo
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+ids = lambda v: str(v).replace("torch.", "") if isinstance(v, torch.dtype) else None  # noqa: E731
+
+
+# ------------------------------------------------------------------------------------ the CPU
+
+
+@pytest.mark.parametrize("counter,key,want", [
+    # Random123's published known answers of philox4x32-10
+    ((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+    ((2**32 - 1,) * 4, (2**32 - 1,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+    ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0), (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1)),
+])
+def test_oracle_generator_known_answers(counter, key, want):
+    assert tuple(int(v) for v in fo.philox(np.array(counter, dtype=np.uint64), key)) == want
+
+
+@pytest.mark.parametrize("act", ff.ACTIVATIONS)
+def test_oracle_gradients_against_differences(act):
+    """dx, dweight and dbias of the oracle's formulas against central differences of its own forward."""
+    g = torch.Generator().manual_seed(0)
+    x, w, b, dy = (torch.randn(*s, generator=g, dtype=torch.float64) for s in ((3, 5), (8, 5), (8,), (3, 4)))
+    kw = dict(act=act, p=0.3, seed=7, offset=9)
+    loss = lambda: float((fo.gated(x, w, b, None, **kw)[0][0] * dy).sum())  # noqa: E731
+    grads = fo.gated(x, w, b, dy, **kw)[1:]
+    for t, (grad, _) in zip((x, w, b), grads):
+        flat = t.view(-1)
+        for i in range(flat.numel()):
+            old = float(flat[i])
+            flat[i] = old + 1e-5
+            up = loss()
+            flat[i] = old - 1e-5
+            down = loss()
+            flat[i] = old
+            assert abs((up - down) / 2e-5 - float(grad.reshape(-1)[i])) < 1e-8
+
+
+def test_oracle_sees_a_planted_mistake():
+    """The bounds tell a neighbour's mask, a swapped half and a missing scale from the right result."""
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.randn(4, 16, generator=g, dtype=torch.float64), torch.randn(16, 16, generator=g, dtype=torch.float64)
+    kw = dict(p=0.25, seed=3, dtype=torch.bfloat16)
+    value, bound = fo.gated(x, w, None, None, offset=0, **kw)[0]
+    wrong = [fo.gated(x, w, None, None, offset=1, **kw)[0][0], fo.gated(x, w.roll(8, 0), None, None, offset=0, **kw)[0][0],
+             value * 0.75]
+    for other in wrong:
+        assert ((other - value).abs() > bound).any()
+
+
+def test_refusals_without_a_gpu():
+    x, w = torch.zeros(2, 8), torch.zeros(4, 8)
+    for call in (lambda: ff.gated_linear(x, w), lambda: ff.linear_dropout_add(x, w), lambda: ff.dropout_add(x, p=0.1, seed=0)):
+        with pytest.raises(RuntimeError, match="x must be a CUDA tensor"):
+            call()
+    with pytest.raises(ValueError, match="activation must be one of"):
+        ff.gated_linear(x, w, activation="relu")
+    with pytest.raises(TypeError, match="x must be a tensor"):
+        ff.dropout_add([1.0], p=0.1, seed=0)
+
+
+def _args(**kw):
+    a = N.GfFfArgs()
+    base = dict(dtype=1, activation=1, rows=4, in_features=16, out_features=8, x=4096, ldx=16, weight=4096, ldw=16, y=4096,
+                dy=4096, lddy=8, saved=4096)
+    for k, v in {**base, **kw}.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(dtype=3), "unknown dtype"), (dict(activation=4), "unknown activation"), (dict(rows=-1), "rows must not be negative"),
+    (dict(in_features=0), "must be positive"), (dict(out_features=0), "must be positive"), (dict(rows=2**31), "too large"),
+    (dict(x=None), "x must not be NULL"), (dict(weight=None), "weight must not be NULL"),
+    (dict(ldx=15), "row stride 15 is below its width 16"), (dict(ldw=15), "row stride 15"),
+    (dict(x=4097), "not aligned to its type"), (dict(dropout=N.GfDropout(1.5, 0, None, 0)), "p must lie in"),
+    (dict(dropout=N.GfDropout(math.nan, 0, None, 0)), "p must lie in"),
+])
+@pytest.mark.parametrize("phase", ["forward", "backward"])
+def test_abi_refuses_before_device_work(kw, msg, phase):
+    lib = N.lib()
+    a = _args(**kw)
+    rc = getattr(lib, f"gf_ff_{phase}")(ctypes.byref(a), None, 0, None)
+    assert rc == 1 and msg in lib.gf_last_error().decode()
+
+
+def test_abi_refuses_a_small_workspace_and_a_gated_residual():
+    lib = N.lib()
+    a = _args()
+    need = lib.gf_ff_workspace_bytes(ctypes.byref(a), 1)
+    assert need >= 4 * 16 * 2
+    assert lib.gf_ff_backward(ctypes.byref(a), 4096, need - 1, None) == 2
+    assert "workspace" in lib.gf_last_error().decode()
+    a = _args(residual=4096, ldr=8)
+    assert lib.gf_ff_forward(ctypes.byref(a), None, 0, None) == 1 and "residual" in lib.gf_last_error().decode()
+    assert lib.gf_ff_forward(None, None, 0, None) == 1 and lib.gf_ff_saved_bytes(None) == 0
+    d = N.GfDropout(0.5, 1, None, 0)
+    assert lib.gf_dropout_add(0, ctypes.byref(d), 2, 8, 4096, 7, None, 0, 4096, 8, None) == 1
+    assert lib.gf_dropout_add(0, None, 2, 8, 4096, 8, None, 0, 4096, 8, None) == 1
+    assert lib.gf_dropout_add(0, ctypes.byref(d), 0, 8, None, 0, None, 0, None, 0, None) == 0
+
+
+# ------------------------------------------------------------------------------------ the GPU
+
+
+def _say(*what):
+    print("[gpu-test] feedforward", *what, flush=True)
+
+
+def _rand(device, *shape, dtype, seed, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(dtype).to(device)
+
+
+def _close(got, want, what):
+    value, bound = want
+    got = got.detach().cpu().double()
+    assert got.shape == value.shape, what
+    off = (got - value).abs()
+    worst = (off - bound).max() if off.numel() else torch.zeros(())
+    assert bool((off <= bound).all()), f"{what}: {float(worst):.3e} past its bound, off {float(off.max()):.3e}"
+
+
+def _case(device, kind, rows, d, n, dtype, bias=True, residual=True, seed=0):
+    w_rows = 2 * n if kind == "gated" else n
+    t = {"x": _rand(device, rows, d, dtype=dtype, seed=seed), "w": _rand(device, w_rows, d, dtype=dtype, seed=seed + 1, std=d**-0.5),
+         "b": _rand(device, w_rows, dtype=dtype, seed=seed + 2, std=0.3) if bias else None,
+         "r": _rand(device, rows, n, dtype=dtype, seed=seed + 3) if residual and kind == "linear" else None,
+         "dy": _rand(device, rows, n, dtype=dtype, seed=seed + 4, std=0.5)}
+    return t
+
+
+def _check(kind, t, dtype, act="gelu", p=0.0, seed=11, offset=5, what=""):
+    """Forward without and with gradients, and the gradients, against the oracle."""
+    rng = dict(p=p, seed=seed, offset=offset)
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items() if v is not None and k != "dy"}
+    x, w, b, r = (leaves.get(k) for k in "xwbr")
+
+    def run():
+        if kind == "gated":
+            return ff.gated_linear(x, w, b, activation=act, **rng)
+        return ff.linear_dropout_add(x, w, b, r, **rng)
+
+    x2, dy2 = t["x"].reshape(-1, t["x"].shape[-1]), t["dy"].reshape(-1, t["dy"].shape[-1])
+    if kind == "gated":
+        want = fo.gated(x2, t["w"], t["b"], dy2, act=act, dtype=dtype, **rng)
+    else:
+        r2 = None if t["r"] is None else t["r"].reshape(dy2.shape)
+        want = fo.linear(x2, t["w"], t["b"], r2, dy2, dtype=dtype, **rng)
+    with torch.no_grad():
+        quiet = run()
+    y = run()
+    assert torch.equal(quiet, y), f"{what}: the forward differs where gradients are wanted"
+    _close(y.reshape(dy2.shape), want[0], f"{what} y")
+    names = [k for k in "xwbr" if k in leaves]
+    grads = dict(zip(names, torch.autograd.grad(y, [leaves[k] for k in names], t["dy"])))
+    _close(grads["x"].reshape(x2.shape), want[1], f"{what} dx")
+    _close(grads["w"], want[2], f"{what} dweight")
+    if "b" in grads:
+        _close(grads["b"], want[3], f"{what} dbias")
+    if "r" in grads:
+        assert torch.equal(grads["r"], t["dy"])
+    return y, grads
+
+
+# one token; tiny and odd; tile edges by one each way; widths past one tile; a long contraction
+SHAPES = [(1, 64, 64), (1, 1, 1), (2, 3, 5), (5, 9, 7), (16, 32, 24), (17, 40, 33), (33, 320, 96), (63, 65, 127), (64, 64, 128),
+          (65, 63, 129), (127, 256, 257), (128, 320, 640), (129, 328, 264), (300, 77, 100), (1000, 64, 72), (3, 2056, 16), (40, 8, 1288)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", ["gated", "linear"])
+def test_products(device, kind, shape, dtype):
+    _say("products", kind, shape, dtype)
+    t = _case(device, kind, *shape, dtype)
+    _check(kind, t, dtype, p=0.2, what=f"{kind} {shape}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows", [1, 8, 16, 31, 48, 64, 96, 200, 1025, 2500])
+@pytest.mark.parametrize("kind", ["gated", "linear"])
+def test_rows(device, kind, rows, dtype):
+    """Row counts on both sides of every way of splitting the work, at a wide block's sizes."""
+    d, n = (320, 1280) if kind == "gated" else (1280, 320)
+    _say("rows", kind, rows, dtype)
+    t = _case(device, kind, rows, d, n, dtype, seed=20)
+    _check(kind, t, dtype, p=0.1, what=f"{kind} rows {rows}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("act", ff.ACTIVATIONS)
+def test_activations_over_their_range(device, act, dtype):
+    """Gates from far below zero to far above it, tiny ones among them; no dropout, no bias."""
+    n = 256
+    gate = torch.cat((torch.linspace(-30, 30, n - 64), torch.logspace(-8, 0, 32), -torch.logspace(-8, 0, 32)))
+    w = torch.zeros(2 * n, 8)
+    w[:n, 0], w[n:, 1] = 1.0, gate
+    x = torch.zeros(3, 8)
+    x[:, 0], x[:, 1] = torch.tensor([1.0, -2.0, 0.5]), torch.tensor([1.0, 1.0, 0.25])
+    _say("activations", act, dtype)
+    t = {"x": x.to(dtype).to(device), "w": w.to(dtype).to(device), "b": None, "r": None,
+         "dy": _rand(device, 3, n, dtype=dtype, seed=3)}
+    y, _ = _check("gated", t, dtype, act=act, what=act)
+    assert bool(torch.isfinite(y).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("kind", ["gated", "linear"])
+def test_strides_and_alignment(device, kind, dtype):
+    """Rows of larger matrices, bases that are not 16-byte aligned, three dimensions, a transposed x, a dy that
+    is one broadcast number."""
+    rows, d, n = 48, 72, 40
+    t = _case(device, kind, rows, d, n, dtype, seed=30)
+    _say("strides", kind, dtype)
+    want, grads = _check(kind, t, dtype, p=0.1, what="plain")
+
+    def wide(m, left, right):
+        big = torch.full((m.shape[0] + 1, left + m.shape[1] + right), float("nan"), dtype=dtype, device=device)
+        big[:-1, left:left + m.shape[1]] = m
+        return big[:-1, left:left + m.shape[1]]
+
+    for left, right in ((8, 8), (1, 2), (16, 3)):
+        u = {k: wide(v, left, right) if v is not None and v.dim() == 2 else v for k, v in t.items()}
+        y, g = _check(kind, u, dtype, p=0.1, what=f"strided {left},{right}")
+        assert torch.equal(y, want) or dtype == torch.float32
+    flat = torch.empty(rows * d + 1, dtype=dtype, device=device)
+    u = dict(t, x=flat[1:].view(rows, d).copy_(t["x"]))
+    _check(kind, u, dtype, p=0.1, what="odd base")
+    u = dict(t, x=t["x"].t().contiguous().t())
+    _check(kind, u, dtype, p=0.1, what="transposed x")
+    u = {k: v.reshape(4, 12, -1) if k in ("x", "r", "dy") and v is not None else v for k, v in t.items()}
+    _check(kind, u, dtype, p=0.1, what="three dimensions")
+    u = dict(t, dy=torch.full((1, 1), 0.5, dtype=dtype, device=device).expand(rows, n))
+    _check(kind, u, dtype, p=0.1, what="broadcast dy")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 7), (1, 8), (3, 9), (64, 1280), (33, 321), (257, 8), (2, 5000), (1000, 3)])
+def test_dropout(device, rows, cols, dtype):
+    _say("dropout", rows, cols, dtype)
+    x, r, dy = (_rand(device, rows, cols, dtype=dtype, seed=40 + i) for i in range(3))
+    for p in (0.0, 0.1, 0.5, 0.99999, 1.0):
+        for seed, offset in ((0, 0), (2**63 + 12345, 2**40 + 3)):
+            rng = dict(p=p, seed=seed, offset=offset)
+            for res in (None, r):
+                xx = x.detach().requires_grad_(True)
+                rr = None if res is None else res.detach().requires_grad_(True)
+                y = ff.dropout_add(xx, rr, **rng)
+                _close(y, fo.dropout_add(x, res, dtype=dtype, **rng), f"dropout {p}")
+                y.backward(dy)
+                _close(xx.grad, fo.dropout_add(dy, None, dtype=dtype, **rng), f"dropout dx {p}")
+                if rr is not None:
+                    assert torch.equal(rr.grad, dy)
+
+
+@pytest.mark.gpu
+def test_dropout_layouts_and_the_share_kept(device):
+    """Strided and transposed matrices drop the same places; a scalar and an empty tensor go through; the share
+    of kept elements is p's to within five standard deviations; the fused forms drop the same places."""
+    _say("dropout layouts")
+    x = _rand(device, 512, 1000, dtype=torch.float32, seed=50)
+    rng = dict(p=0.3, seed=77, offset=1)
+    want = ff.dropout_add(x, **rng)
+    big = torch.full((512, 1013), float("nan"), device=device)
+    big[:, 5:1005] = x
+    assert torch.equal(ff.dropout_add(big[:, 5:1005], big[:, 5:1005], **rng), want + x)
+    assert torch.equal(ff.dropout_add(x.t().contiguous().t(), **rng), want)
+    assert torch.equal(ff.dropout_add(x.view(8, 64, 1000), **rng).view(512, 1000), want)
+    n = x.numel()
+    kept = float((want != 0).sum())
+    assert abs(kept - 0.7 * n) < 5 * math.sqrt(0.21 * n)
+    other = ff.dropout_add(x, **{**rng, "offset": 2})
+    both = float(((want != 0) & (other != 0)).sum())
+    assert abs(both - 0.49 * n) < 5 * math.sqrt(0.49 * 0.51 * n)
+    assert ff.dropout_add(torch.ones((), device=device), p=0.0, seed=0).item() == 1.0
+    assert ff.dropout_add(torch.ones(0, 4, device=device), p=0.5, seed=0).shape == (0, 4)
+    w, b = torch.eye(1000, device=device), None
+    assert torch.equal(ff.linear_dropout_add(x, w, b, **rng) != 0, want != 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_dropped_elements_are_zero_whatever_they_were(device, dtype):
+    _say("dropped nan", dtype)
+    rows, cols = 40, 64
+    keep = fo.keep_scale(rows, cols, 0.5, 9, 0) != 0
+    for bad in (math.nan, math.inf, -math.inf):
+        x = torch.where(keep, torch.ones(rows, cols, dtype=torch.float64), torch.tensor(bad, dtype=torch.float64)).to(dtype).to(device)
+        y = ff.dropout_add(x, p=0.5, seed=9)
+        assert torch.equal(y.cpu().double(), keep.double() * 2)
+        assert torch.equal(ff.dropout_add(x, x, p=0.5, seed=9).cpu().isfinite(), keep)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("kind", ["gated", "linear"])
+@pytest.mark.parametrize("rows", [5, 200])
+def test_nonfinite_rows_stay_their_own(device, kind, dtype, rows):
+    """A NaN or infinity in a row of x makes that row of the output not finite, and no other."""
+    _say("nonfinite", kind, rows, dtype)
+    t = _case(device, kind, rows, 96, 64, dtype, seed=60)
+    for bad in (math.nan, math.inf):
+        x = t["x"].clone()
+        x[3, 17] = bad
+        y = ff.gated_linear(x, t["w"], t["b"]) if kind == "gated" else ff.linear_dropout_add(x, t["w"], t["b"], t["r"])
+        fine = torch.isfinite(y).all(dim=1).cpu()
+        assert not bool(fine[3]) and int(fine.sum()) == rows - 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["gated", "linear"])
+def test_gradients_against_differences(device, kind):
+    """The kernels' own forward, differenced: a step of 2^-6 along random directions, whose third-order term and
+    rounding stay below the tolerance (the loss is a sum of at most 24 x 16 terms of order one, each good to
+    2^-20 or so: 2^-14 over a step of 2^-5 is 2^-9; the third-order term is about 2^-12)."""
+    _say("differences", kind)
+    rows, d, n = 24, 40, 16
+    t = _case(device, kind, rows, d, n, torch.float32, seed=70)
+    rng = dict(p=0.25, seed=5, offset=1)
+
+    def run(v):
+        if kind == "gated":
+            return ff.gated_linear(v["x"], v["w"], v["b"], **rng)
+        return ff.linear_dropout_add(v["x"], v["w"], v["b"], v["r"], **rng)
+
+    names = [k for k in "xwbr" if t[k] is not None]
+    leaves = {k: t[k].clone().requires_grad_(True) for k in names}
+    grads = torch.autograd.grad(run(leaves), list(leaves.values()), t["dy"])
+    for name, grad in zip(names, grads):
+        for s in range(3):
+            v = _rand(device, *t[name].shape, dtype=torch.float32, seed=80 + s)
+            v = v / v.norm()
+            up, down = (float((run({**t, name: t[name] + sign * 2.0**-6 * v}).double() * t["dy"].double()).sum()) for sign in (1, -1))
+            slope = float((grad.double() * v.double()).sum())
+            assert abs((up - down) / 2.0**-5 - slope) < 2.0**-8, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("kind", ["gated", "linear"])
+def test_only_what_is_wanted(device, kind, dtype):
+    """A frozen weight, a frozen bias or an x without gradient gives the others' gradients unchanged."""
+    _say("wanted", kind, dtype)
+    t = _case(device, kind, 70, 48, 32, dtype, seed=90)
+    _, full = _check(kind, t, dtype, p=0.1, what="all")
+    for name in ("x", "w", "b"):
+        v = {k: None if u is None else u.detach() for k, u in t.items()}
+        v[name].requires_grad_(True)
+        rng = dict(p=0.1, seed=11, offset=5)
+        y = (ff.gated_linear(v["x"], v["w"], v["b"], **rng) if kind == "gated"
+             else ff.linear_dropout_add(v["x"], v["w"], v["b"], v["r"], **rng))
+        got, = torch.autograd.grad(y, [v[name]], t["dy"])
+        assert torch.equal(got, full[name]), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["gated", "linear"])
+def test_no_rows(device, kind):
+    _say("no rows", kind)
+    t = _case(device, kind, 0, 16, 8, torch.bfloat16)
+    v = {k: u.detach().requires_grad_(True) for k, u in t.items() if u is not None and k != "dy"}
+    y = ff.gated_linear(v["x"], v["w"], v["b"]) if kind == "gated" else ff.linear_dropout_add(v["x"], v["w"], v["b"], v["r"])
+    assert y.shape == (0, 8)
+    y.sum().backward()
+    assert float(v["w"].grad.abs().sum()) == 0 and float(v["b"].grad.abs().sum()) == 0 and v["x"].grad.shape == (0, 16)
+
+
+@pytest.mark.gpu
+def test_gpu_refusals(device):
+    _say("refusals")
+    x, w = torch.zeros(4, 16, device=device), torch.zeros(8, 16, device=device)
+    bad = [
+        (lambda: ff.gated_linear(x, w[:7]), "even number of rows"),
+        (lambda: ff.gated_linear(x, w[:, :8]), "x has 16 features"),
+        (lambda: ff.gated_linear(x, w.half()), "weight must be torch.float32"),
+        (lambda: ff.gated_linear(x, w, torch.zeros(4, device=device)), "bias must have shape"),
+        (lambda: ff.gated_linear(x, w, torch.zeros(8)), "bias must be a CUDA tensor"),
+        (lambda: ff.gated_linear(x.double(), w.double()), "float32, bfloat16 or float16"),
+        (lambda: ff.linear_dropout_add(x, w[0]), "two dimensions"),
+        (lambda: ff.linear_dropout_add(x, w[:0]), "must not be empty"),
+        (lambda: ff.linear_dropout_add(x, w, None, torch.zeros(4, 16, device=device)), "residual must have shape"),
+        (lambda: ff.dropout_add(x, x[:2], p=0.1, seed=0), "residual must have x's shape"),
+        (lambda: ff.dropout_add(x, p=0.1, seed=torch.zeros(1, device=device)), "seed tensor"),
+        (lambda: ff.dropout_add(x, p=0.1, seed=torch.zeros(1, dtype=torch.int64)), "seed tensor"),
+    ]
+    for call, msg in bad:
+        with pytest.raises(RuntimeError, match=msg):
+            call()
+    for kw in (dict(p=-0.1, seed=0), dict(p=1.1, seed=0), dict(p=math.nan, seed=0), dict(p=0.1, seed=-1), dict(p=0.1, seed=2**64),
+               dict(p=0.1, seed=0, offset=-1)):
+        with pytest.raises(ValueError):
+            ff.dropout_add(x, **kw)
+    y = ff.dropout_add(x.requires_grad_(True), p=0.1, seed=0)
+    g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):  # differentiated once only
+        g.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_repeatable_and_on_another_stream(device, dtype):
+    """The same call gives the same bits, on a side stream too (whose inputs are made on it)."""
+    _say("streams", dtype)
+    t = _case(device, "gated", 600, 320, 192, dtype, seed=100)
+    first = _check("gated", t, dtype, p=0.1, what="default stream")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        u = {k: None if v is None else v * 1 for k, v in t.items()}
+        second = _check("gated", u, dtype, p=0.1, what="side stream")
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(first[0], second[0])
+    for k in first[1]:
+        assert torch.equal(first[1][k], second[1][k]), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows", [4, 300])
+def test_graph_replays_draw_by_the_seed_tensor(device, dtype, rows):
+    """Forward and backward kernels captured once; every replay, with other seeds and eager work between them,
+    equals the eager result of that seed."""
+    _say("graph", rows, dtype)
+    d, n = 64, 96
+    x, w, b, dy = (_rand(device, *s, dtype=dtype, seed=110 + i) for i, s in enumerate(((rows, d), (2 * n, d), (2 * n,), (rows, n))))
+    seed = torch.zeros(1, dtype=torch.int64, device=device)
+
+    def step(s):
+        h, saved = ff._linear_forward(x, w, b, None, "gelu", 0.3, s, 4, True)
+        grads = ff._linear_backward(x, w, saved, dy, "gelu", 0.3, s, 4, (True, True, True))
+        return [h, *grads, ff.dropout_add(h, h, p=0.5, seed=s, offset=6)]
+
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        step(seed)
+    torch.cuda.current_stream().wait_stream(warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(seed)
+    for value in (0, 1, 2**62 + 5, 1):
+        want = step(value)
+        torch.cuda.synchronize()
+        seed.fill_(value)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(out, want):
+            assert torch.equal(got, ref)
