@@ -80,7 +80,7 @@ def test_refusals_without_a_gpu():
 def _args(**kw):
     a = N.GfFfArgs()
     base = dict(dtype=1, activation=1, rows=4, in_features=16, out_features=8, x=4096, ldx=16, weight=4096, ldw=16, y=4096,
-                dy=4096, lddy=8, saved=4096)
+                dy=4096, lddy=8, saved=4096, dx=4096)
     for k, v in {**base, **kw}.items():
         setattr(a, k, v)
     return a
