@@ -30,6 +30,45 @@ int fail(int code, const char* msg) { return gf_set_error(code, msg); }
     if (e_ != hipSuccess) return fail(GF_E_HIP, "launch of %s failed: %s", name, hipGetErrorString(e_)); \
   } while (0)
 
+// 8 consecutive elements in 32 bits: 16 bytes (two times 16) a lane at whatever alignment, which global memory takes,
+// or where they are not `all` there the first n, one by one.
+template <typename T, int N>
+using Vec = T __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+
+template <typename T>
+__device__ inline void load8(float v[8], const T* p, bool all, int n) {
+  constexpr int W = 16 / sizeof(T);
+  if (all) {
+#pragma unroll
+    for (int i = 0; i < 8; i += W) {
+      const Vec<T, W> t = *(const Vec<T, W>*)(p + i);
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[i + j] = (float)t[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ inline void store8(T* p, const float v[8], bool all, int n) {
+  constexpr int W = 16 / sizeof(T);
+  if (all) {
+#pragma unroll
+    for (int i = 0; i < 8; i += W) {
+      Vec<T, W> t;
+#pragma unroll
+      for (int j = 0; j < W; ++j) t[j] = (T)v[i + j];
+      *(Vec<T, W>*)(p + i) = t;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = (T)v[j];
+  }
+}
+
 // ------------------------------------------------------------------------------------------
 // Dropout.
 
@@ -71,43 +110,77 @@ __device__ inline float dropped(const Drop& d, const uint32_t bits[4], int j, fl
   return h >= d.threshold ? v * d.scale : 0.0f;
 }
 
-// residual + drop(x), 8 elements of a row a thread.
-template <typename T>
-__global__ __launch_bounds__(256) void k_dropout(Drop d, int64_t rows, int64_t cols, const T* x, int64_t ldx, const T* res,
-                                                 int64_t ldr, T* y, int64_t ldy) {
+// residual + drop(x), 8 elements of a row a thread and turn.  A thread's next group is a fixed number of groups on, whole
+// rows and a rest of columns, so that nothing is divided in the loop.
+template <typename T, bool RESIDUAL>
+__global__ __launch_bounds__(256) void k_dropout(Drop d, int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx,
+                                                 const T* __restrict__ res, int64_t ldr, T* __restrict__ y, int64_t ldy) {
   load_key(d);
-  const int64_t groups = (cols + 7) / 8, total = rows * groups;
-  for (int64_t g = blockIdx.x * 256ll + threadIdx.x; g < total; g += gridDim.x * 256ll) {
-    const int64_t row = g / groups, group = g % groups;
-    uint32_t bits[4];
-    random_block(d, (uint32_t)row, (uint32_t)group, bits);
-    const int n = cols - 8 * group < 8 ? (int)(cols - 8 * group) : 8;
-    for (int j = 0; j < n; ++j) {
-      const int64_t c = 8 * group + j;
-      float v = dropped(d, bits, j, (float)x[row * ldx + c]);
-      if (res != nullptr) v += (float)res[row * ldr + c];
-      y[row * ldy + c] = (T)v;
+  const uint32_t groups = (uint32_t)((cols + 7) / 8);
+  const int64_t first = blockIdx.x * 256ll + threadIdx.x, all = gridDim.x * 256ll;
+  int64_t row = first / groups;
+  uint32_t group = (uint32_t)(first % groups);
+  const int64_t row_step = all / groups;
+  const uint32_t group_step = (uint32_t)(all % groups);
+  while (row < rows) {
+    const int64_t c = 8ll * group;
+    const int n = cols - c < 8 ? (int)(cols - c) : 8;
+    float v[8], r[8];
+    load8(v, x + row * ldx + c, n == 8, n);
+    if constexpr (RESIDUAL) load8(r, res + row * ldr + c, n == 8, n);
+    if (d.threshold != 0) {
+      uint32_t bits[4];
+      random_block(d, (uint32_t)row, group, bits);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = dropped(d, bits, j, v[j]);
     }
+    if constexpr (RESIDUAL)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += r[j];
+    store8(y + row * ldy + c, v, n == 8, n);
+    row += row_step, group += group_step;
+    if (group >= groups) group -= groups, ++row;
   }
 }
 
 // ------------------------------------------------------------------------------------------
-// Activations: act(g), and with it act'(g).
+// Activations: act(g), and with it act'(g).  Exponentials and reciprocals are the hardware's (1 unit in the last place).
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// Phi(-a) e^(a^2/2) for a >= 0 as t Q(t), t = 1 / (1 + p a): p and Q fitted (least squares reweighted to the largest
+// relative error) over a in [0, 14], where it is good to 9e-8; past that Phi(-a) is below the smallest float.
+__device__ inline float normal_tail(float a) {
+  const float t = rcp_fast(__builtin_fmaf(0.3045656383f, a, 1.0f));
+  float q = 0.0367617272f;
+  q = __builtin_fmaf(q, t, -0.153960079f);
+  q = __builtin_fmaf(q, t, 0.188459948f);
+  q = __builtin_fmaf(q, t, -0.0401414931f);
+  q = __builtin_fmaf(q, t, 0.122078776f);
+  q = __builtin_fmaf(q, t, 0.103001416f);
+  q = __builtin_fmaf(q, t, 0.122335792f);
+  q = __builtin_fmaf(q, t, 0.121463954f);
+  return q * t;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
 
 template <int ACT>
 __device__ inline float activation(float g, float* slope) {
-  if constexpr (ACT == GF_ACT_SILU) {  // g s, s = 1 / (1 + e^-g); s' = s (1 - s)
-    const float s = 1.0f / (1.0f + expf(-g));
-    if (slope != nullptr) *slope = s + g * s * (1.0f - s);
-    return g * s;
-  } else if constexpr (ACT == GF_ACT_GELU) {  // g Phi(g); Phi' = e^(-g^2/2) / sqrt(2 pi)
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
-    if (slope != nullptr) *slope = cdf + g * (0.39894228040143268f * expf(-0.5f * g * g));
+  if constexpr (ACT == GF_ACT_GELU) {  // g Phi(g); Phi' = e^(-g^2/2) / sqrt(2 pi)
+    const float e = exp2_fast(-0.5f * kLog2e * g * g), tail = normal_tail(fabsf(g)) * e;
+    const float cdf = g < 0.0f ? tail : 1.0f - tail;
+    if (slope != nullptr) *slope = __builtin_fmaf(0.39894228040143268f * g, e, cdf);
     return g * cdf;
+  } else if constexpr (ACT == GF_ACT_SILU) {  // g s, s = 1 / (1 + e^-g); s' = s (1 - s)
+    const float s = rcp_fast(1.0f + exp2_fast(-kLog2e * g));
+    if (slope != nullptr) *slope = __builtin_fmaf(g * s, 1.0f - s, s);
+    return g * s;
   } else {  // (1 + tanh u) / 2 = 1 / (1 + e^-2u), u = sqrt(2/pi) (g + 0.044715 g^3)
-    const float u2 = 1.5957691216057308f * g * (1.0f + 0.044715f * g * g);
-    const float s = 1.0f / (1.0f + expf(-u2));
-    if (slope != nullptr) *slope = s + g * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 3.0f * 0.044715f * g * g));
+    constexpr float c = 1.5957691216057308f;
+    const float s = rcp_fast(1.0f + exp2_fast(-c * kLog2e * g * __builtin_fmaf(0.044715f * g, g, 1.0f)));
+    if (slope != nullptr) *slope = __builtin_fmaf(g * s * (1.0f - s), c * __builtin_fmaf(3.0f * 0.044715f * g, g, 1.0f), s);
     return g * s;
   }
 }
@@ -165,7 +238,6 @@ struct Epilogue {
   void* saved;  // gated: the value's plane, then the gate's, [M, saved_ld]
   int64_t saved_ld;
   float* partial;  // not NULL: sums for k_join instead of all of the above, [split][M][N (gated: 2 N), whole groups of 8]
-  int32_t vec;     // out, bias and residual can be read and written 16 bytes at a time
   Drop drop;
 };
 
@@ -181,59 +253,20 @@ constexpr int kStep = 64;
 // n within 32 of the matrix instruction's row r = 8 a + 4 h + e
 __device__ inline int row_of(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
 
-template <typename T>
-__device__ inline void load8(float v[8], const T* p, bool vec, int n) {
-  if (vec) {
-    if constexpr (sizeof(T) == 2) {
-      using V = T __attribute__((ext_vector_type(8)));
-      const V t = *(const V*)p;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (float)t[j];
-    } else {
-      const f32x4 a = ((const f32x4*)p)[0], b = ((const f32x4*)p)[1];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.0f;
-  }
-}
-
-template <typename T>
-__device__ inline void store8(T* p, const float v[8], bool vec, int n) {
-  if (vec) {
-    if constexpr (sizeof(T) == 2) {
-      using V = T __attribute__((ext_vector_type(8)));
-      V t;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = (T)v[j];
-      *(V*)p = t;
-    } else {
-      ((f32x4*)p)[0] = f32x4{v[0], v[1], v[2], v[3]};
-      ((f32x4*)p)[1] = f32x4{v[4], v[5], v[6], v[7]};
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = (T)v[j];
-  }
-}
-
 // What follows the sums: 8 consecutive columns n.. of row m (gated: the value's in v, the gate's in g).
-// WHOLE: all 8 are inside and everything can be read and written 16 bytes at a time.
+// WHOLE: all 8 are inside.
 template <typename T, int ACT, bool WHOLE>
 __device__ inline void finish(const Epilogue& e, const Drop& drop, int64_t M, int64_t N, int64_t m, int64_t n, float v[8],
                               float g[8]) {
   const int left = N - n < 8 ? (int)(N - n) : 8;
-  const bool vec = WHOLE || (e.vec && left == 8);
+  const bool all = WHOLE || left == 8;
   if (e.bias != nullptr) {
     float b[8];
-    load8(b, (const T*)e.bias + n, vec, left);
+    load8(b, (const T*)e.bias + n, all, left);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += b[j];
     if constexpr (ACT != GF_ACT_NONE) {
-      load8(b, (const T*)e.bias + N + n, vec, left);
+      load8(b, (const T*)e.bias + N + n, all, left);
 #pragma unroll
       for (int j = 0; j < 8; ++j) g[j] += b[j];
     }
@@ -254,11 +287,11 @@ __device__ inline void finish(const Epilogue& e, const Drop& drop, int64_t M, in
   }
   if (e.residual != nullptr) {
     float r[8];
-    load8(r, (const T*)e.residual + m * e.ldr + n, vec, left);
+    load8(r, (const T*)e.residual + m * e.ldr + n, all, left);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += r[j];
   }
-  store8((T*)e.out + m * N + n, v, vec, left);
+  store8((T*)e.out + m * N + n, v, all, left);
 }
 
 // One operand's way from memory into LDS.  ROWS: its rows of the tile.  HALF: the tile takes HALF rows of the value,
@@ -266,8 +299,9 @@ __device__ inline void finish(const Epilogue& e, const Drop& drop, int64_t M, in
 template <bool KC, int ROWS, int THREADS, int HALF>
 struct Stage {
   static constexpr int kBytes = ROWS * kStep * 2;
-  static constexpr int kLoads = kBytes / (THREADS * 16);  // a lane's loads a step
-  static_assert(kBytes % (THREADS * 16) == 0 && ROWS % 64 == 0 && HALF % 8 == 0);
+  static constexpr int kPieces = kBytes / 1024;  // one load of a wave each
+  static constexpr int kWaves = THREADS / 64, kLoads = (kPieces + kWaves - 1) / kWaves;
+  static_assert(ROWS % 32 == 0 && HALF % 8 == 0);
 
   uint32_t off[kLoads];
   int32_t k_of[kLoads];  // the first k (of the step's 64) of each load
@@ -281,7 +315,7 @@ struct Stage {
     advance = (KC ? kStep : kStep * a.ld) * 2;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int piece = (wave * kLoads + i) * 64 + lane;  // the 16 bytes of LDS that the lane fills
+      const int piece = (i * kWaves + wave) * 64 + lane;  // the 16 bytes of LDS that the lane fills
       if constexpr (KC) {
         const int r = piece / 8, chunk = (piece % 8) ^ swizzle(r);
         int64_t row = HALF ? r / (2 * HALF + !HALF) * HALF + r % (HALF + !HALF) : r;
@@ -297,10 +331,13 @@ struct Stage {
     }
   }
 
-  // Which 16 bytes of an LDS row hold which: their number is xored with this.  K-contiguous: rows that row_of gives
-  // 8 consecutive lanes differ in it.  Row-contiguous: the 4 k that 16 lanes read differ in their 32 bytes.
+  // Which 16 bytes of an LDS row hold which: their number is xored with this.  LDS has 64 banks of 4 bytes.
+  // K-contiguous, rows of 128 bytes: of the 16 lanes that read together, those of rows of one parity differ in it.
+  // Row-contiguous: 32 lanes read 64 bytes of 4 consecutive k together, which go to different quarters of the banks;
+  // rows of an odd number of 64 bytes do so by themselves.
   __device__ static int swizzle(int r) {
-    return KC ? (r & 3) | ((r >> 3) & 1) << 2 : (r & (ROWS / 16 - 1) & 7) << 1;
+    if constexpr (KC) return (r >> 1) & 7;
+    return ROWS % 128 == 0 ? (r & 3) << 2 : ROWS % 64 == 0 ? (r & 2) << 1 : 0;
   }
 
   __device__ void seek(int64_t steps) { base += steps * advance; }
@@ -310,7 +347,8 @@ struct Stage {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int piece = wave * kLoads + i;  // a wave's 1024 bytes
+      const int piece = i * kWaves + wave;
+      if ((i + 1) * kWaves > kPieces && piece >= kPieces) break;
       const uint8_t* b = base;
       if constexpr (HALF != 0) b += (piece * 8 / HALF) % 2 ? gate : 0;
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, 0x80000000, 0x00020000);
@@ -327,15 +365,12 @@ struct Stage {
       return *(const half8*)(lds + row * 128 + r * 128 + (((2 * s + (lane >> 5)) ^ swizzle(r)) << 4));
     } else {
       // 16 lanes read 4 k of 16 rows, a lane 4 rows of one k, and get 4 k of one row each
-      const int i = lane & 15, q = 4 * ((lane >> 4) & 1) + (i & 3);  // q: which 4 matrix-instruction rows
-      const int r = row + row_of(4 * q);
+      const int i = lane & 15, r = row + row_of(16 * ((lane >> 4) & 1) + 4 * (i & 3)), k = 8 * (lane >> 5) + (i >> 2);
+      const uint8_t* at = lds + k * ROWS * 2 + (((r >> 3) ^ swizzle(k)) << 4) + (r & 7) * 2;  // swizzle(k): of k % 4 alone
       half4 part[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int k = 16 * s + 8 * (lane >> 5) + 4 * u + (i >> 2);
-        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) half4*)(lds + k * ROWS * 2 + (((r >> 3) ^ swizzle(k)) << 4) + (r & 7) * 2));
-      }
+      for (int u = 0; u < 2; ++u)
+        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) half4*)(at + (16 * s + 4 * u) * ROWS * 2));
       return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
@@ -345,44 +380,56 @@ struct Stage {
 // 2^-16 of a0 b0 leave out 3 2^-24 of a b.  Smallest first.
 __device__ constexpr int kPlaneP[6] = {2, 0, 1, 1, 0, 0}, kPlaneQ[6] = {0, 2, 1, 0, 1, 0};
 
-// One step of a workgroup: the loads of a later step into `to`, the products of this one out of `from`.  The two are
-// different LDS arrays and said to be (__restrict__): otherwise the compiler waits for the loads before it reads.
-template <typename T, typename SP, typename SQ, int TM, int TN, typename Load>
-__device__ __forceinline__ void step(uint8_t* __restrict__ to, const uint8_t* __restrict__ from, bool more, Load& load, int wm, int wn,
-                                     f32x16 (&acc)[TN / 32][TM / 32]) {
-  if (more) load(to);
+template <typename SP, typename SQ, int TM, int TN>
+__device__ __forceinline__ void read(const uint8_t* from, int s, int wm, int wn, half8 (&fp)[TM / 32], half8 (&fq)[TN / 32]) {
 #pragma unroll
-  for (int s = 0; s < kStep / 16; ++s) {
-    half8 fp[TM / 32], fq[TN / 32];
+  for (int i = 0; i < TM / 32; ++i) fp[i] = SP::fragment(from, wm + 32 * i, s);
 #pragma unroll
-    for (int i = 0; i < TM / 32; ++i) fp[i] = SP::fragment(from, wm + 32 * i, s);
-#pragma unroll
-    for (int j = 0; j < TN / 32; ++j) fq[j] = SQ::fragment(from + SP::kBytes, wn + 32 * j, s);
-#pragma unroll
-    for (int j = 0; j < TN / 32; ++j)
-#pragma unroll
-      for (int i = 0; i < TM / 32; ++i) acc[j][i] = mfma<T>(fq[j], fp[i], acc[j][i]);
-  }
+  for (int j = 0; j < TN / 32; ++j) fq[j] = SQ::fragment(from + SP::kBytes, wn + 32 * j, s);
 }
 
-// All of this wave's LDS reads are done and all but its last `loads` loads are in LDS; then all waves'.
-template <int LOADS>
+// This wave's LDS reads are done and its loads are in LDS; then all waves'.
 __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070 | (LOADS & 15) | (LOADS >> 4) << 14);  // vmcnt(LOADS) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
-template <typename T, bool PKC, bool QKC, int ACT, int WM, int WN, int TM, int TN, int STAGES>
-__global__ __launch_bounds__(WM * WN * 64, 2) void k_product(Shape sh, Matrix p, Matrix q, int64_t second, Epilogue e) {
+// One step of a workgroup.  Its first fragments are in slot 0 already; those of 16 k more are read while the matrix
+// cores work on the ones before, the next step's first ones too, so that nobody waits behind the barrier.  Where the
+// barrier is passed, `cur` has been read by all and takes the loads of the step after next.
+// cur and nxt are different LDS arrays and said to be (__restrict__): otherwise the compiler waits for the loads
+// before any read.
+template <typename T, typename SP, typename SQ, int TM, int TN, typename Load>
+__device__ __forceinline__ void step(uint8_t* __restrict__ cur, const uint8_t* __restrict__ nxt, int after, Load& load, int wm, int wn,
+                                     half8 (&fp)[2][TM / 32], half8 (&fq)[2][TN / 32], f32x16 (&acc)[TN / 32][TM / 32]) {
+  constexpr int kPhases = kStep / 16;
+#pragma unroll
+  for (int s = 0; s < kPhases; ++s) {
+    const int now = s & 1;
+    if (s + 1 < kPhases) {
+      read<SP, SQ, TM, TN>(cur, s + 1, wm, wn, fp[now ^ 1], fq[now ^ 1]);
+    } else if (after > 0) {
+      meet();
+      if (after > 1) load(cur);
+      read<SP, SQ, TM, TN>(nxt, 0, wm, wn, fp[now ^ 1], fq[now ^ 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < TN / 32; ++j)
+#pragma unroll
+      for (int i = 0; i < TM / 32; ++i) acc[j][i] = mfma<T>(fq[now][j], fp[now][i], acc[j][i]);
+  }
+}
+
+template <typename T, bool PKC, bool QKC, int ACT, int WM, int WN, int TM, int TN>
+__global__ __launch_bounds__(WM * WN * 64, (WM * TM + WN * TN) * kStep * 4 > 80 * 1024 ? WM * WN / 4 : WM * WN / 2) void k_product(Shape sh, Matrix p, Matrix q, int64_t second, Epilogue e) {
   constexpr bool kGated = ACT != GF_ACT_NONE;
   constexpr int kThreads = WM * WN * 64, BM = WM * TM, BN = WN * TN, BO = kGated ? BN / 2 : BN;
   constexpr int kPlanes = std::is_same_v<T, float> ? 6 : 1;
   using SP = Stage<PKC, BM, kThreads, 0>;
   using SQ = Stage<QKC, BN, kThreads, kGated ? TN / 2 : 0>;
-  constexpr int kBytes = SP::kBytes + SQ::kBytes, kLoads = SP::kLoads + SQ::kLoads;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds0[kBytes], lds1[kBytes], lds2[STAGES > 2 ? kBytes : 1024];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds0[SP::kBytes + SQ::kBytes], lds1[SP::kBytes + SQ::kBytes];
 
   // Workgroups go round the 8 dies by their number; a die gets consecutive tiles, in groups of 8 tile rows, so that
   // its cache sees the same rows of P and of Q again.
@@ -430,48 +477,25 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product(Shape sh, Matrix p,
   };
 
   const int total = steps * kPlanes;
-  if constexpr (STAGES == 2) {
-    load(lds0);
-    int t = 0;
-    for (; t + 1 < total; t += 2) {
-      meet<0>();
-      step<T, SP, SQ, TM, TN>(lds1, lds0, true, load, wm, wn, acc);
-      meet<0>();
-      step<T, SP, SQ, TM, TN>(lds0, lds1, t + 2 < total, load, wm, wn, acc);
-    }
-    if (t < total) {
-      meet<0>();
-      step<T, SP, SQ, TM, TN>(lds1, lds0, false, load, wm, wn, acc);
-    }
-  } else {
-    load(lds0);
-    if (total > 1) load(lds1);
-    int t = 0;
-    for (; t + 4 < total; t += 3) {
-      meet<kLoads>();
-      step<T, SP, SQ, TM, TN>(lds2, lds0, true, load, wm, wn, acc);
-      meet<kLoads>();
-      step<T, SP, SQ, TM, TN>(lds0, lds1, true, load, wm, wn, acc);
-      meet<kLoads>();
-      step<T, SP, SQ, TM, TN>(lds1, lds2, true, load, wm, wn, acc);
-    }
-    // 1 to 4 steps are left, two of them loaded
-    for (bool first = true; t < total; t += 3, first = false) {
-      meet<0>();
-      step<T, SP, SQ, TM, TN>(lds2, lds0, t + 2 < total, load, wm, wn, acc);
-      if (t + 1 >= total) break;
-      meet<0>();
-      step<T, SP, SQ, TM, TN>(lds0, lds1, t + 3 < total, load, wm, wn, acc);
-      if (t + 2 >= total) break;
-      meet<0>();
-      step<T, SP, SQ, TM, TN>(lds1, lds2, false, load, wm, wn, acc);
-    }
+  half8 fp[2][TM / 32], fq[2][TN / 32];
+  load(lds0);
+  meet();
+  if (total > 1) load(lds1);
+  read<SP, SQ, TM, TN>(lds0, 0, wm, wn, fp[0], fq[0]);
+  int after = total - 1;
+  for (; after > 0; after -= 2) {
+    step<T, SP, SQ, TM, TN>(lds0, lds1, after, load, wm, wn, fp, fq, acc);
+    step<T, SP, SQ, TM, TN>(lds1, lds0, after - 1, load, wm, wn, fp, fq, acc);
   }
+  if (after == 0) step<T, SP, SQ, TM, TN>(lds0, lds1, 0, load, wm, wn, fp, fq, acc);
 
   // Lane l has, of each 32 x 32, row m = row_of(l % 32) and columns 16 h + 8 (l / 32) .. + 8 for h = 0, 1.
   Drop drop = e.drop;
   load_key(drop);
   constexpr int kOut = kGated ? TN / 64 : TN / 32;
+  float* const rest = (float*)lds0;  // [BM][16]: the last columns that are no whole group, finished at the end
+  const bool ragged = e.partial == nullptr && sh.N % 8 != 0 && n0 + BO > sh.N;
+  if (ragged) __syncthreads();  // everyone has read lds0
 #pragma unroll
   for (int i = 0; i < TM / 32; ++i) {
     const int64_t m = m0 + wm + 32 * i + row_of(lane & 31);
@@ -493,11 +517,125 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product(Shape sh, Matrix p,
           float* out = e.partial + ((int64_t)blockIdx.y * sh.M + m) * width * (kGated ? 2 : 1) + n;
           store8(out, v, true, 8);
           if constexpr (kGated) store8(out + width, g, true, 8);
+        } else if (n + 8 > sh.N) {
+          store8(rest + (m - m0) * 16, v, true, 8);
+          if constexpr (kGated) store8(rest + (m - m0) * 16 + 8, g, true, 8);
         } else {
           finish<T, ACT, true>(e, drop, sh.M, sh.N, m, n, v, g);
         }
       }
   }
+  if (!ragged) return;
+  __syncthreads();
+  for (int64_t m = m0 + threadIdx.x; m < m0 + BM && m < sh.M; m += kThreads) {
+    float v[8], g[8];
+    load8(v, rest + (m - m0) * 16, true, 8);
+    if constexpr (kGated) load8(g, rest + (m - m0) * 16 + 8, true, 8);
+    finish<T, ACT, false>(e, drop, sh.M, sh.N, m, sh.N / 8 * 8, v, g);
+  }
+}
+
+// The forward product of at most 16 G rows: bound by reading W once, so nothing of it goes through LDS.  A workgroup takes 16
+// output columns (gated: 16 of the value's and of the gate's), its waves interleaved chunks of 64 bytes along k; a lane
+// loads 16 bytes of W's row (lane % 16) and of x's straight into the matrix instruction's operands, at whatever
+// alignment.  32-bit operands are multiplied as such (16 x 16 x 4).  The waves' sums meet in LDS.
+template <typename T, int ACT, int G>
+__global__ __launch_bounds__(1024) void k_few(int64_t M, int64_t N, int64_t K, const T* __restrict__ x, int64_t ldx,
+                                              const T* __restrict__ w, int64_t ldw, Epilogue e) {
+  constexpr int H = ACT == GF_ACT_NONE ? 1 : 2, E = 16 / sizeof(T), kChunk = 4 * E, kAhead = G > 2 ? 2 : 4;
+  using V = Vec<T, E>;
+  __shared__ float sums[16][H][G][16][16 + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int64_t n0 = blockIdx.x * 16ll, at = (lane >> 4) * E;
+  const int64_t n = n0 + (lane & 15) < N ? n0 + (lane & 15) : N - 1;
+  const T *pw[H], *px[G];
+#pragma unroll
+  for (int h = 0; h < H; ++h) pw[h] = w + (n + h * N) * ldw + at;
+#pragma unroll
+  for (int g = 0; g < G; ++g) px[g] = x + (16 * g + (lane & 15) < M ? 16 * g + (lane & 15) : M - 1) * ldx + at;
+
+  f32x4 acc[H][G] = {};
+  auto multiply = [&](const V* a, const V* b) {
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[h][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[h][i], b[g][i], acc[h][g], 0, 0, 0);
+        } else if constexpr (std::is_same_v<T, f16>) {
+          acc[h][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a[h]), __builtin_bit_cast(f16x8, b[g]), acc[h][g], 0, 0, 0);
+        } else {
+          acc[h][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a[h]), __builtin_bit_cast(bf16x8, b[g]), acc[h][g], 0, 0, 0);
+        }
+      }
+  };
+  const int chunks = (int)(K / kChunk);  // whole ones
+  int c = wave;
+  for (; c + (kAhead - 1) * waves < chunks; c += kAhead * waves) {
+    V a[kAhead][H], b[kAhead][G];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+      for (int h = 0; h < H; ++h) a[u][h] = *(const V*)(pw[h] + (int64_t)(c + u * waves) * kChunk);
+#pragma unroll
+      for (int g = 0; g < G; ++g) b[u][g] = *(const V*)(px[g] + (int64_t)(c + u * waves) * kChunk);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) multiply(a[u], b[u]);
+  }
+  for (; c <= chunks; c += waves) {  // the rest, and the part of a chunk
+    const int64_t k = (int64_t)c * kChunk;
+    const int64_t left = K - k - at;
+    if (K - k <= 0) break;
+    V a[H], b[G];
+    if (c < chunks) {
+#pragma unroll
+      for (int h = 0; h < H; ++h) a[h] = *(const V*)(pw[h] + k);
+#pragma unroll
+      for (int g = 0; g < G; ++g) b[g] = *(const V*)(px[g] + k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) a[h][i] = i < left ? pw[h][k + i] : (T)0.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) b[g][i] = i < left ? px[g][k + i] : (T)0.0f;
+      }
+    }
+    multiply(a, b);
+  }
+
+  // Lane l has row l % 16 of each 16 and columns 4 (l / 16) .. + 4.
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sums[wave][h][g][lane & 15][4 * (lane >> 4) + r] = acc[h][g][r];
+  __syncthreads();
+  for (int t = threadIdx.x; t < H * G * 256; t += blockDim.x) {
+    float* const s = &sums[0][t / 256 / G][t / 256 % G][t / 16 % 16][t % 16];
+    float v = s[0];
+    for (int i = 1; i < waves; ++i) v += s[i * (H * G * 16 * 17)];
+    s[0] = v;
+  }
+  __syncthreads();
+  const int t = threadIdx.x;
+  const int64_t m = t / 2, col = n0 + t % 2 * 8;
+  if (m >= M || t >= 32 * G || col >= N) return;
+  Drop drop = e.drop;
+  load_key(drop);
+  float v[8], g[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    v[j] = sums[0][0][m / 16][m % 16][t % 2 * 8 + j];
+    if constexpr (H == 2) g[j] = sums[0][1][m / 16][m % 16][t % 2 * 8 + j];
+  }
+  if (col + 8 <= N)
+    finish<T, ACT, true>(e, drop, M, N, m, col, v, g);
+  else
+    finish<T, ACT, false>(e, drop, M, N, m, col, v, g);
 }
 
 // The products' parts, added in their order.
@@ -541,14 +679,14 @@ __device__ inline void split(float x, bf16 out[3]) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_pack(int64_t rows, int64_t cols, const T* x, int64_t ldx, int32_t vec, void* out,
-                                              int64_t ld, int64_t plane) {
+__global__ __launch_bounds__(256) void k_pack(int64_t rows, int64_t cols, const T* x, int64_t ldx, void* out, int64_t ld,
+                                              int64_t plane) {
   const int64_t groups = ld / 8;
   for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < rows * groups; t += gridDim.x * 256ll) {
     const int64_t row = t / groups, c = t % groups * 8;
     const int n = cols - c < 8 ? (int)(cols - c) : 8;
     float v[8];
-    load8(v, x + row * ldx + c, vec && n == 8, n);
+    load8(v, x + row * ldx + c, n == 8, n);
     if constexpr (std::is_same_v<T, float>) {
       bf16x8 o[3];
 #pragma unroll
@@ -569,8 +707,8 @@ __global__ __launch_bounds__(256) void k_pack(int64_t rows, int64_t cols, const 
 // ([rows, ld], in planes for 32 bits, zero past its columns), and its columns' sums: a workgroup takes 256 columns of dy
 // and `chunk` rows, 8 columns a thread in 8 interleaved rows, and leaves its sums in `sums` [row chunk][columns of dz].
 template <typename T, int ACT>
-__global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, int64_t chunk, const T* dy, int64_t lddy, int32_t vec,
-                                            const T* saved, int64_t saved_ld, void* dz, int64_t ld, int64_t plane, float* sums) {
+__global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, int64_t chunk, const T* dy, int64_t lddy, const T* saved,
+                                            int64_t saved_ld, void* dz, int64_t ld, int64_t plane, float* sums) {
   constexpr bool kGated = ACT != GF_ACT_NONE;
   constexpr int H = kGated ? 2 : 1;
   __shared__ float part[H][8][256 + 8];
@@ -583,7 +721,7 @@ __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, i
     const int64_t end = (blockIdx.y + 1) * chunk < rows ? (blockIdx.y + 1) * chunk : rows;
     for (int64_t row = blockIdx.y * chunk + line; row < end; row += 8) {
       float g[H][8];
-      load8(g[0], dy + row * lddy + c, vec && n == 8, n);
+      load8(g[0], dy + row * lddy + c, n == 8, n);
       if (d.threshold != 0) {
         uint32_t bits[4];
         random_block(d, (uint32_t)row, (uint32_t)(c >> 3), bits);
@@ -614,28 +752,22 @@ __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, i
         const int64_t at = row * ld + h * out + c;
         const bool last = h == H - 1 && c + 8 >= out;
         const int put = last ? (int)(ld - h * out - c) : n;
-        const bool whole = out % 8 == 0;
         if constexpr (std::is_same_v<T, float>) {
-          bf16 s[8][3];
+          float part[3][8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) split(g[h][j], s[j]);
+          for (int j = 0; j < 8; ++j) {
+            bf16 o[3];
+            split(g[h][j], o);
+            part[0][j] = (float)o[0], part[1][j] = (float)o[1], part[2][j] = (float)o[2];
+          }
 #pragma unroll
           for (int i = 0; i < 3; ++i) {
             bf16* to = (bf16*)dz + i * plane + at;
-            if (whole) {
-              bf16x8 o;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) o[j] = s[j][i];
-              *(bf16x8*)to = o;
-            } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (j < put) to[j] = s[j][i];
-              for (int j = 8; j < put; ++j) to[j] = (bf16)0.0f;
-            }
+            store8(to, part[i], put == 8, put);
+            for (int j = 8; j < put; ++j) to[j] = (bf16)0.0f;
           }
         } else {
-          store8((T*)dz + at, g[h], whole, put);
+          store8((T*)dz + at, g[h], put == 8, put);
           for (int j = 8; j < put; ++j) ((T*)dz)[at + j] = (T)0.0f;
         }
       }
@@ -658,12 +790,20 @@ __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, i
   }
 }
 
+// The chunks' sums of 32 columns a workgroup, added in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(256) void k_join_sums(int64_t chunks, int64_t cols, const float* sums, T* out) {
-  const int64_t c = blockIdx.x * 256ll + threadIdx.x;
-  if (c >= cols) return;
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
+  const int64_t c = blockIdx.x * 32ll + lane;
   float s = 0.0f;
-  for (int64_t i = 0; i < chunks; ++i) s += sums[i * cols + c];
+  if (c < cols)
+    for (int64_t i = line; i < chunks; i += 8) s += sums[i * cols + c];
+  part[line][lane] = s;
+  __syncthreads();
+  if (line != 0 || c >= cols) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) s += part[i][lane];
   out[c] = (T)s;
 }
 
@@ -778,8 +918,7 @@ int operand(Arena& ws, bool run, const void* x, int64_t rows, int64_t cols, int6
   const int64_t width = round_up(cols, 8), plane = rows * width;
   *out = {ws.take(plane * 2 * (kSplit ? 3 : 1)), width, plane, (int32_t)width};
   FF_RUN {
-    k_pack<T><<<blocks_for(rows * width / 8), 256, 0, s>>>(rows, cols, (const T*)x, ld, aligned(x, ld, sizeof(T)),
-                                                           (void*)out->p, width, plane);
+    k_pack<T><<<blocks_for(rows * width / 8), 256, 0, s>>>(rows, cols, (const T*)x, ld, (void*)out->p, width, plane);
     FF_LAUNCH_CHECK("k_pack");
   }
   return GF_OK;
@@ -787,26 +926,47 @@ int operand(Arena& ws, bool run, const void* x, int64_t rows, int64_t cols, int6
 
 constexpr int kUnits = 256;  // compute units
 
-template <typename T, bool PKC, bool QKC, int ACT, int WM, int WN, int TM, int TN, int STAGES>
+// How a product is cut: tiles of 256 x 256 or 128 x 128, and `splits` parts along k that k_join adds.
+struct Cut {
+  bool large;
+  int32_t splits;
+};
+
+// The cut whose estimated time is least, from what was measured over 4096 x 4096 x 8192 in bfloat16: a step of 64 takes
+// 1.64 us for one 256 x 256 tile on each compute unit (1.3 PFLOP/s) and 1.02 us for two of 128 x 128 (1.05 PFLOP/s: twice
+// the bytes from L2 for each operation), a round of workgroups about 7 and 3 us besides; the parts are written and read
+// back at about 4 TB/s.  So large tiles win where they fill the chip, small ones and splits where there are few.
+Cut choose_cut(int64_t M, int64_t columns, int64_t steps, int planes, int size) {
+  Cut best{};
+  double least = 1e300;
+  for (const bool large : {true, false}) {
+    const int64_t edge = large ? 256 : 128, tiles = ((M + edge - 1) / edge) * ((columns + edge - 1) / edge);
+    for (int64_t splits = 1; splits <= 32 && splits * 2 <= std::max<int64_t>(steps, 2); ++splits) {
+      const int64_t slots = large ? kUnits : 2 * kUnits, rounds = (tiles * splits + slots - 1) / slots;
+      const int64_t each = (steps + splits - 1) / splits;
+      double us = rounds * (each * planes * (large ? 1.64 : 1.02) + (large ? 7.0 : 3.0));
+      if (splits > 1) us += M * columns * (8.0 * splits + size) / 4e6 + 4.0;
+      if (us < least) least = us, best = {large, (int32_t)splits};
+    }
+  }
+  return best;
+}
+
+template <typename T, bool PKC, bool QKC, int ACT, int WM, int WN, int TM, int TN>
 int product_tiled(Arena& ws, bool run, int64_t M, int64_t N, int64_t K, const Matrix& p, const Matrix& q, int64_t second, Epilogue e,
-                  hipStream_t s) {
+                  int64_t splits, hipStream_t s) {
   constexpr int BM = WM * TM, BO = WN * TN / (ACT == GF_ACT_NONE ? 1 : 2);
   Shape sh{M, N, K, 0, 0, 1, 0};
   const int64_t tm = (M + BM - 1) / BM, tn = (N + BO - 1) / BO, steps = (K + kStep - 1) / kStep;
   if (tm * tn > (int64_t(1) << 30)) return fail(GF_E_INVALID_ARGUMENT, "rows, in_features or out_features too large");
   sh.tiles_m = (int32_t)tm, sh.tiles_n = (int32_t)tn;
-  // Fewer tiles than compute units: the steps are split among workgroups, at least 4 each, until there are two
-  // workgroups a unit.
-  int64_t splits = 1;
-  if (tm * tn < kUnits) splits = std::max<int64_t>(std::min<int64_t>(2 * kUnits / (tm * tn), steps / 4), 1);
   sh.steps = (int32_t)((steps + splits - 1) / splits);
   sh.splits = (int32_t)((steps + sh.steps - 1) / sh.steps);
+  const bool join = sh.splits > 1;
   e.partial = nullptr;
-  // Columns that are not whole, aligned groups of 8 are left to k_join too.
-  const bool join = sh.splits > 1 || N % 8 != 0 || !e.vec;
   if (join) e.partial = (float*)ws.take(sh.splits * M * round_up(N, 8) * (ACT == GF_ACT_NONE ? 1 : 2) * 4);
   FF_RUN {
-    k_product<T, PKC, QKC, ACT, WM, WN, TM, TN, STAGES><<<dim3((unsigned)(tm * tn), (unsigned)sh.splits), WM * WN * 64, 0, s>>>(sh, p, q, second, e);
+    k_product<T, PKC, QKC, ACT, WM, WN, TM, TN><<<dim3((unsigned)(tm * tn), (unsigned)sh.splits), WM * WN * 64, 0, s>>>(sh, p, q, second, e);
     FF_LAUNCH_CHECK("k_product");
     if (join) {
       k_join<T, ACT><<<blocks_for(M * ((N + 7) / 8)), 256, 0, s>>>(sh, e);
@@ -821,13 +981,21 @@ int product(Arena& ws, bool run, int64_t M, int64_t N, int64_t K, const Matrix& 
             hipStream_t s) {
   // a load's 32-bit offset spans a tile's rows (K-contiguous) or a step's (row-contiguous)
   if (std::max(p.ld, q.ld) * 2 * 256 >= (int64_t(1) << 31)) return fail(GF_E_INVALID_ARGUMENT, "row stride too large");
-  return product_tiled<T, PKC, QKC, ACT, 2, 2, 64, 64, 2>(ws, run, M, N, K, p, q, second, e, s);
+  const Cut cut = choose_cut(M, ACT == GF_ACT_NONE ? N : 2 * N, (K + kStep - 1) / kStep, std::is_same_v<T, float> ? 6 : 1,
+                             sizeof(T));
+  if (cut.large) return product_tiled<T, PKC, QKC, ACT, 2, 4, 128, 64>(ws, run, M, N, K, p, q, second, e, cut.splits, s);
+  return product_tiled<T, PKC, QKC, ACT, 2, 2, 64, 64>(ws, run, M, N, K, p, q, second, e, cut.splits, s);
 }
 
-int32_t vec_ok(const gf_ff_args& a, const void* out) {
-  const int size = size_of(a.dtype);
-  return aligned(out, a.out_features, size) && (a.bias == nullptr || aligned(a.bias, a.out_features, size)) &&
-         (a.residual == nullptr || aligned(a.residual, a.ldr, size));
+template <typename T, int ACT>
+int few(const gf_ff_args& a, const Epilogue& e, hipStream_t s) {
+  const dim3 grid((unsigned)((a.out_features + 15) / 16));
+  // 16 waves where each still has 4 chunks of 64 bytes or more, 8 else
+  const unsigned threads = a.in_features * (int64_t)sizeof(T) >= 16 * 4 * 64 ? 1024 : 512;
+  auto* kernel = a.rows <= 16 ? k_few<T, ACT, 1> : a.rows <= 32 ? k_few<T, ACT, 2> : k_few<T, ACT, 4>;
+  kernel<<<grid, threads, 0, s>>>(a.rows, a.out_features, a.in_features, (const T*)a.x, a.ldx, (const T*)a.weight, a.ldw, e);
+  FF_LAUNCH_CHECK("k_few");
+  return GF_OK;
 }
 
 // The forward's launches, or (run false) its workspace.
@@ -835,10 +1003,14 @@ int forward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
     return with_activation(a.activation, [&](auto act) {
+      const Epilogue e{a.y, a.bias, a.residual, a.ldr, a.saved, saved_ld(&a), nullptr, make_drop(a.dropout)};
+      if (a.rows <= 64) {
+        FF_RUN return few<T, act.value>(a, e, s);
+        return (int)GF_OK;
+      }
       Matrix x, w;
       FF_CHECK(operand<T>(ws, run, a.x, a.rows, a.in_features, a.ldx, s, &x));
       FF_CHECK(operand<T>(ws, run, a.weight, weight_rows(&a), a.in_features, a.ldw, s, &w));
-      const Epilogue e{a.y, a.bias, a.residual, a.ldr, a.saved, saved_ld(&a), nullptr, vec_ok(a, a.y), make_drop(a.dropout)};
       return product<T, true, true, act.value>(ws, run, a.rows, a.out_features, a.in_features, x, w, a.out_features, e, s);
     });
   });
@@ -871,11 +1043,11 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
         float* sums = a.dbias != nullptr ? (float*)ws.take(chunks * wr * 4) : nullptr;
         FF_RUN {
           k_dz<T, ACT><<<dim3((unsigned)across, (unsigned)chunks), 256, 0, s>>>(
-              drop, a.rows, out, chunk, (const T*)a.dy, a.lddy, aligned(a.dy, a.lddy, sizeof(T)), (const T*)a.saved, saved_ld(&a),
+              drop, a.rows, out, chunk, (const T*)a.dy, a.lddy, (const T*)a.saved, saved_ld(&a),
               make ? (void*)dz.p : nullptr, dz.ld, dz.plane, sums);
           FF_LAUNCH_CHECK("k_dz");
           if (sums != nullptr) {
-            k_join_sums<T><<<(unsigned)((wr + 255) / 256), 256, 0, s>>>(chunks, wr, sums, (T*)a.dbias);
+            k_join_sums<T><<<(unsigned)((wr + 31) / 32), 256, 0, s>>>(chunks, wr, sums, (T*)a.dbias);
             FF_LAUNCH_CHECK("k_join_sums");
           }
         }
@@ -884,13 +1056,13 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
       if (a.dx != nullptr) {
         Matrix w;
         FF_CHECK(operand<T>(ws, run, a.weight, wr, a.in_features, a.ldw, s, &w));
-        e.out = a.dx, e.vec = aligned(a.dx, a.in_features, sizeof(T));
+        e.out = a.dx;
         FF_CHECK((product<T, true, false, GF_ACT_NONE>(ws, run, a.rows, a.in_features, wr, dz, w, 0, e, s)));
       }
       if (a.dweight != nullptr) {
         Matrix x;
         FF_CHECK(operand<T>(ws, run, a.x, a.rows, a.in_features, a.ldx, s, &x));
-        e.out = a.dweight, e.vec = aligned(a.dweight, a.in_features, sizeof(T));
+        e.out = a.dweight;
         FF_CHECK((product<T, false, false, GF_ACT_NONE>(ws, run, wr, a.in_features, a.rows, dz, x, 0, e, s)));
       }
       return (int)GF_OK;
@@ -914,8 +1086,9 @@ int gf_dropout_add(int32_t dtype, const gf_dropout* dropout, int64_t rows, int64
   const Drop d = make_drop(*dropout);
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    k_dropout<T><<<blocks_for(rows * ((cols + 7) / 8)), 256, 0, (hipStream_t)stream>>>(d, rows, cols, (const T*)x, ldx, (const T*)residual, ldr,
-                                                                      (T*)y, ldy);
+    auto* kernel = residual != nullptr ? k_dropout<T, true> : k_dropout<T, false>;
+    kernel<<<blocks_for(rows * ((cols + 7) / 8)), 256, 0, (hipStream_t)stream>>>(d, rows, cols, (const T*)x, ldx, (const T*)residual, ldr, (T*)y,
+                                                                                 ldy);
     FF_LAUNCH_CHECK("k_dropout");
     return (int)GF_OK;
   });
