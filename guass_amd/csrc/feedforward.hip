@@ -300,6 +300,7 @@ template <bool KC, int ROWS, int THREADS, int HALF>
 struct Stage {
   static constexpr int kBytes = ROWS * kStep * 2;
   static constexpr int kPieces = kBytes / 1024;  // one load of a wave each
+  static constexpr int kReads = KC ? 1 : 2;       // LDS reads a fragment
   static constexpr int kWaves = THREADS / 64, kLoads = (kPieces + kWaves - 1) / kWaves;
   static_assert(ROWS % 32 == 0 && HALF % 8 == 0);
 
@@ -342,8 +343,8 @@ struct Stage {
 
   __device__ void seek(int64_t steps) { base += steps * advance; }
 
-  template <bool CUT>
-  __device__ void load(uint8_t* lds, int64_t left) const {
+  // left: how many of the k from here on are the matrix's
+  __device__ void load(uint8_t* lds, int left) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -352,7 +353,7 @@ struct Stage {
       const uint8_t* b = base;
       if constexpr (HALF != 0) b += (piece * 8 / HALF) % 2 ? gate : 0;
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, 0x80000000, 0x00020000);
-      const uint32_t o = CUT && k_of[i] >= left ? 0x80000000u : off[i];
+      const uint32_t o = k_of[i] < left ? off[i] : 0x80000000u;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + piece * 1024), 16, o, 0, 0, 0);
     }
   }
@@ -396,29 +397,42 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
 }
 
+// For the scheduler: a product, then its share of the LDS reads and of the loads, and so on.
+template <int PRODUCTS, int READS, int LOADS, int I = 0>
+__device__ __forceinline__ void interleave() {
+  if constexpr (I < PRODUCTS) {
+    constexpr int r = READS * (I + 1) / PRODUCTS - READS * I / PRODUCTS, l = LOADS * (I + 1) / PRODUCTS - LOADS * I / PRODUCTS;
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
+    if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x020, l, 0);
+    interleave<PRODUCTS, READS, LOADS, I + 1>();
+  }
+}
+
 // One step of a workgroup.  Its first fragments are in slot 0 already; those of 16 k more are read while the matrix
-// cores work on the ones before, the next step's first ones too, so that nobody waits behind the barrier.  Where the
-// barrier is passed, `cur` has been read by all and takes the loads of the step after next.
+// cores work on the ones before, the next step's first ones too (NEXT), so that nobody waits behind the barrier.  Where
+// the barrier is passed, `cur` has been read by all and takes the loads of the step after next (LOAD).
 // cur and nxt are different LDS arrays and said to be (__restrict__): otherwise the compiler waits for the loads
 // before any read.
-template <typename T, typename SP, typename SQ, int TM, int TN, typename Load>
-__device__ __forceinline__ void step(uint8_t* __restrict__ cur, const uint8_t* __restrict__ nxt, int after, Load& load, int wm, int wn,
+template <typename T, typename SP, typename SQ, int TM, int TN, bool NEXT, bool LOAD, int S = 0, typename Load>
+__device__ __forceinline__ void step(uint8_t* __restrict__ cur, const uint8_t* __restrict__ nxt, Load& load, int wm, int wn,
                                      half8 (&fp)[2][TM / 32], half8 (&fq)[2][TN / 32], f32x16 (&acc)[TN / 32][TM / 32]) {
-  constexpr int kPhases = kStep / 16;
-#pragma unroll
-  for (int s = 0; s < kPhases; ++s) {
-    const int now = s & 1;
-    if (s + 1 < kPhases) {
-      read<SP, SQ, TM, TN>(cur, s + 1, wm, wn, fp[now ^ 1], fq[now ^ 1]);
-    } else if (after > 0) {
+  if constexpr (S < kStep / 16) {
+    constexpr bool kLast = S + 1 == kStep / 16;
+    constexpr int kReads = kLast && !NEXT ? 0 : SP::kReads * (TM / 32) + SQ::kReads * (TN / 32);
+    if constexpr (!kLast) {
+      read<SP, SQ, TM, TN>(cur, S + 1, wm, wn, fp[~S & 1], fq[~S & 1]);
+    } else if constexpr (NEXT) {
       meet();
-      if (after > 1) load(cur);
-      read<SP, SQ, TM, TN>(nxt, 0, wm, wn, fp[now ^ 1], fq[now ^ 1]);
+      if constexpr (LOAD) load(cur);
+      read<SP, SQ, TM, TN>(nxt, 0, wm, wn, fp[~S & 1], fq[~S & 1]);
     }
 #pragma unroll
     for (int j = 0; j < TN / 32; ++j)
 #pragma unroll
-      for (int i = 0; i < TM / 32; ++i) acc[j][i] = mfma<T>(fq[now][j], fp[now][i], acc[j][i]);
+      for (int i = 0; i < TM / 32; ++i) acc[j][i] = mfma<T>(fq[S & 1][j], fp[S & 1][i], acc[j][i]);
+    interleave<TM / 32 * (TN / 32), kReads, kLast && LOAD ? SP::kLoads + SQ::kLoads : 0>();
+    step<T, SP, SQ, TM, TN, NEXT, LOAD, S + 1>(cur, nxt, load, wm, wn, fp, fq, acc);
   }
 }
 
@@ -453,41 +467,39 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * TM + WN * TN) * kStep * 4 > 80 
   const int wm = wave % WM * TM, wn = wave / WM * TN;
   f32x16 acc[TN / 32][TM / 32] = {};
 
-  int64_t left = sh.K - (int64_t)step0 * kStep;  // k from the next load's first on
-  int loaded = 0, plane = 0;                     // steps of this plane product loaded; which it is
+  const int first_left = (int)(sh.K - (int64_t)step0 * kStep);
+  int left = first_left;      // k from the next load's first on; none: loads read nothing and fill with zeros
+  int loaded = 0, plane = 0;  // steps of this plane product loaded; which it is
   auto load = [&](uint8_t* to) {
     if constexpr (kPlanes > 1) {
       if (loaded == 0) {
-        sp.base = p_base + kPlaneP[plane] * p.plane * 2;
-        sq.base = q_base + kPlaneQ[plane] * q.plane * 2;
-        left = sh.K - (int64_t)step0 * kStep;
+        const int i = plane < kPlanes ? plane : kPlanes - 1;
+        sp.base = p_base + kPlaneP[i] * p.plane * 2;
+        sq.base = q_base + kPlaneQ[i] * q.plane * 2;
+        left = plane < kPlanes ? first_left : 0;
       }
+      if (++loaded == steps) loaded = 0, ++plane;
     }
-    if (left >= kStep) {
-      sp.template load<false>(to, left);
-      sq.template load<false>(to + SP::kBytes, left);
-    } else {
-      sp.template load<true>(to, left);
-      sq.template load<true>(to + SP::kBytes, left);
-    }
+    sp.load(to, left);
+    sq.load(to + SP::kBytes, left);
     sp.seek(1);
     sq.seek(1);
     left -= kStep;
-    if (++loaded == steps) loaded = 0, ++plane;
   };
 
-  const int total = steps * kPlanes;
   half8 fp[2][TM / 32], fq[2][TN / 32];
   load(lds0);
   meet();
-  if (total > 1) load(lds1);
+  load(lds1);
   read<SP, SQ, TM, TN>(lds0, 0, wm, wn, fp[0], fq[0]);
-  int after = total - 1;
-  for (; after > 0; after -= 2) {
-    step<T, SP, SQ, TM, TN>(lds0, lds1, after, load, wm, wn, fp, fq, acc);
-    step<T, SP, SQ, TM, TN>(lds1, lds0, after - 1, load, wm, wn, fp, fq, acc);
+  int after = steps * kPlanes - 1;  // steps after the one to be done
+  for (; after >= 2; after -= 2) {
+    step<T, SP, SQ, TM, TN, true, true>(lds0, lds1, load, wm, wn, fp, fq, acc);
+    step<T, SP, SQ, TM, TN, true, true>(lds1, lds0, load, wm, wn, fp, fq, acc);
   }
-  if (after == 0) step<T, SP, SQ, TM, TN>(lds0, lds1, 0, load, wm, wn, fp, fq, acc);
+  if (after == 1) step<T, SP, SQ, TM, TN, true, false>(lds0, lds1, load, wm, wn, fp, fq, acc);
+  step<T, SP, SQ, TM, TN, false, false>(after == 1 ? lds1 : lds0, lds0, load, wm, wn, fp, fq, acc);
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the loads past the end have filled theirs while the LDS is still ours
 
   // Lane l has, of each 32 x 32, row m = row_of(l % 32) and columns 16 h + 8 (l / 32) .. + 8 for h = 0, 1.
   Drop drop = e.drop;
@@ -495,7 +507,7 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * TM + WN * TN) * kStep * 4 > 80 
   constexpr int kOut = kGated ? TN / 64 : TN / 32;
   float* const rest = (float*)lds0;  // [BM][16]: the last columns that are no whole group, finished at the end
   const bool ragged = e.partial == nullptr && sh.N % 8 != 0 && n0 + BO > sh.N;
-  if (ragged) __syncthreads();  // everyone has read lds0
+  if (ragged) meet();  // everyone has read lds0
 #pragma unroll
   for (int i = 0; i < TM / 32; ++i) {
     const int64_t m = m0 + wm + 32 * i + row_of(lane & 31);
@@ -926,27 +938,37 @@ int operand(Arena& ws, bool run, const void* x, int64_t rows, int64_t cols, int6
 
 constexpr int kUnits = 256;  // compute units
 
-// How a product is cut: tiles of 256 x 256 or 128 x 128, and `splits` parts along k that k_join adds.
+// How a product is cut into workgroups: tiles, and `splits` parts along k that k_join adds.
+enum class Tile { k256x256, k256x160, k128x128 };
 struct Cut {
-  bool large;
+  Tile tile;
   int32_t splits;
 };
 
-// The cut whose estimated time is least, from what was measured over 4096 x 4096 x 8192 in bfloat16: a step of 64 takes
-// 1.64 us for one 256 x 256 tile on each compute unit (1.3 PFLOP/s) and 1.02 us for two of 128 x 128 (1.05 PFLOP/s: twice
-// the bytes from L2 for each operation), a round of workgroups about 7 and 3 us besides; the parts are written and read
-// back at about 4 TB/s.  So large tiles win where they fill the chip, small ones and splits where there are few.
-Cut choose_cut(int64_t M, int64_t columns, int64_t steps, int planes, int size) {
+// The cut whose estimated time is least, from what was measured in bfloat16.  A step of 64 takes 1.59 us with a
+// 256 x 256 tile on each compute unit (4096 x 4096 x 8192: 203 us, 1.35 PFLOP/s), 1.18 us with 256 x 160
+// (8192 x 1280 x 10240, one round: 191 us, against 208 us in 160 tiles of 256 x 256) and 0.98 us with two of 128 x 128
+// (250 us for the first: twice the bytes from L2 for each operation).  Where not all units work, those that do run faster
+// (160 tiles: 1.30 us a step): the chip is held by its power.  A round costs about 7, 7 and 3 us besides, and split
+// parts are written and read back at about 4 TB/s.
+Cut choose_cut(int64_t M, int64_t columns, int64_t steps, bool gated, int planes, int size) {
+  constexpr struct {
+    Tile tile;
+    int64_t m, n, slots;
+    double step, round;
+  } kinds[] = {{Tile::k256x256, 256, 256, kUnits, 1.59, 7.0}, {Tile::k256x160, 256, 160, kUnits, 1.18, 7.0}, {Tile::k128x128, 128, 128, 2 * kUnits, 0.98, 3.0}};
   Cut best{};
   double least = 1e300;
-  for (const bool large : {true, false}) {
-    const int64_t edge = large ? 256 : 128, tiles = ((M + edge - 1) / edge) * ((columns + edge - 1) / edge);
+  for (const auto& k : kinds) {
+    if (gated && k.tile == Tile::k256x160) continue;  // its halves would not be whole matrix instructions
+    const int64_t tiles = ((M + k.m - 1) / k.m) * ((columns + k.n - 1) / k.n);
     for (int64_t splits = 1; splits <= 32 && splits * 2 <= std::max<int64_t>(steps, 2); ++splits) {
-      const int64_t slots = large ? kUnits : 2 * kUnits, rounds = (tiles * splits + slots - 1) / slots;
-      const int64_t each = (steps + splits - 1) / splits;
-      double us = rounds * (each * planes * (large ? 1.64 : 1.02) + (large ? 7.0 : 3.0));
+      const double each = (double)((steps + splits - 1) / splits) * planes * k.step;
+      const int64_t full = tiles * splits / k.slots, rest = tiles * splits % k.slots;
+      double us = full * (each + k.round);
+      if (rest != 0) us += each * std::max(0.72, 0.5 + 0.5 * rest / k.slots) + k.round;
       if (splits > 1) us += M * columns * (8.0 * splits + size) / 4e6 + 4.0;
-      if (us < least) least = us, best = {large, (int32_t)splits};
+      if (us < least) least = us, best = {k.tile, (int32_t)splits};
     }
   }
   return best;
@@ -981,9 +1003,11 @@ int product(Arena& ws, bool run, int64_t M, int64_t N, int64_t K, const Matrix& 
             hipStream_t s) {
   // a load's 32-bit offset spans a tile's rows (K-contiguous) or a step's (row-contiguous)
   if (std::max(p.ld, q.ld) * 2 * 256 >= (int64_t(1) << 31)) return fail(GF_E_INVALID_ARGUMENT, "row stride too large");
-  const Cut cut = choose_cut(M, ACT == GF_ACT_NONE ? N : 2 * N, (K + kStep - 1) / kStep, std::is_same_v<T, float> ? 6 : 1,
-                             sizeof(T));
-  if (cut.large) return product_tiled<T, PKC, QKC, ACT, 2, 4, 128, 64>(ws, run, M, N, K, p, q, second, e, cut.splits, s);
+  const Cut cut = choose_cut(M, ACT == GF_ACT_NONE ? N : 2 * N, (K + kStep - 1) / kStep, ACT != GF_ACT_NONE,
+                             std::is_same_v<T, float> ? 6 : 1, sizeof(T));
+  if constexpr (ACT == GF_ACT_NONE)
+    if (cut.tile == Tile::k256x160) return product_tiled<T, PKC, QKC, ACT, 8, 1, 32, 160>(ws, run, M, N, K, p, q, second, e, cut.splits, s);
+  if (cut.tile == Tile::k256x256) return product_tiled<T, PKC, QKC, ACT, 2, 4, 128, 64>(ws, run, M, N, K, p, q, second, e, cut.splits, s);
   return product_tiled<T, PKC, QKC, ACT, 2, 2, 64, 64>(ws, run, M, N, K, p, q, second, e, cut.splits, s);
 }
 
