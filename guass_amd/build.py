@@ -2,13 +2,14 @@
 
 * ``guass_amd/libgaussfield.so``       gfx950 kernels + C ABI (hipcc, --offload-arch=gfx950): the fields'
                                        (gaussfield.hip) and the feed-forward block's (feedforward.hip)
+* ``guass_amd/libguass_torch.so``       the feed-forward operators as torch operators over it (g++)
 * ``guass_amd/libgaussfield_host.so``  host build of the per-Gaussian geometry (g++), used by
                                        CPU tests to pin the exact arithmetic the GPU runs
 * ``oracle/_build/libm_sweep``         exhaustive libm check (test infrastructure)
 * ``_build/sanitize/``                 (``build_sanitized``, for the CPU tests) both libraries with
                                        their host code under ASan + UBSan
 
-``python -m guass_amd.build`` builds all three; ``build_all()`` is what ``__graft_entry__.build``
+``python -m guass_amd.build`` builds them all; ``build_all()`` is what ``__graft_entry__.build``
 calls.  Every call compiles (no up-to-date check), so a stale library is never picked up.
 """
 
@@ -28,6 +29,7 @@ CSRC = PKG / "csrc"
 GPU_SOURCES = [CSRC / "gaussfield.hip", CSRC / "feedforward.hip"]
 LIB = PKG / "libgaussfield.so"
 HOST_LIB = PKG / "libgaussfield_host.so"
+TORCH_LIB = PKG / "libguass_torch.so"
 
 # Packed FP32 instructions are disabled (-packed-fp32-ops: some of their forms have given wrong
 # results); fp32 denormals are kept (the bit-exact softplus path passes through subnormal expf results).
@@ -66,13 +68,29 @@ def _compile_and_link(flags: list[str], lib: Path) -> None:
         objects = [Path(tmp) / f"{src.stem}.o" for src in GPU_SOURCES]
         list(pool.map(lambda so: _run([hipcc(), *flags, "-c", str(so[0]), "-o", str(so[1])]), zip(GPU_SOURCES, objects)))
         new = lib.with_suffix(".so.tmp")
-        _run([hipcc(), *flags, "-shared", *map(str, objects), "-o", str(new)])
+        _run([hipcc(), *flags, "-shared", "-Wl,-soname,libgaussfield.so", *map(str, objects), "-o", str(new)])
         os.replace(new, lib)
 
 
 def build_gpu_lib() -> Path:
     _compile_and_link(HIP_FLAGS, LIB)
     return LIB
+
+
+def build_torch_lib() -> Path:
+    """The torch operators over libgaussfield.so (which it finds beside itself)."""
+    import torch
+
+    home = Path(torch.__file__).parent
+    rocm = Path(hipcc()).resolve().parent.parent
+    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{home / 'include'}",
+          f"-I{home / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{rocm / 'include'}", str(CSRC / "torch_ops.cpp"),
+          "-o", str(tmp), f"-L{home / 'lib'}", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
+          str(LIB), "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
 
 
 def build_host_lib() -> Path:
@@ -133,7 +151,7 @@ def build_sanitized(out_dir: Path = SANITIZE_DIR) -> dict[str, Path]:
 
 
 def build_all(verbose: bool = True) -> None:
-    for fn in (build_gpu_lib, build_host_lib, build_oracle_tools):
+    for fn in (build_gpu_lib, build_torch_lib, build_host_lib, build_oracle_tools):
         path = fn()
         if verbose:
             print(f"[guass_amd.build] built {path.relative_to(ROOT)}", flush=True)
