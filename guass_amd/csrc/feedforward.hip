@@ -191,7 +191,7 @@ using ActTag = std::integral_constant<int, ACT>;
 // ------------------------------------------------------------------------------------------
 // Products.  C[m, n] = sum over k of P(m, k) Q(n, k) on the matrix cores, accumulated in 32 bits.
 //
-// A workgroup computes a BM x BN tile, WM x WN waves a TM x TN part each, in steps of 64 along k.  An operand is
+// A workgroup computes a BM x BN tile, WM x WN waves a TM x TN part each, in steps of 64 (32) along k.  An operand is
 // either K-contiguous (its row in memory is a row of the tile: x and W forward, dz in dx) or row-contiguous
 // (memory's rows are the steps of k: W in dx, dz and x in dW); nothing is transposed in memory:
 //   K-contiguous   LDS [row][64 k], fragments by 16-byte reads;
@@ -248,7 +248,11 @@ struct Shape {
   int32_t steps;
 };
 
-constexpr int kStep = 64;
+// k that a step takes, and planes that an operand has: 32-bit operands come in three planes and a step of half the length.
+template <typename T>
+constexpr int kStep = std::is_same_v<T, float> ? 32 : 64;
+template <typename T>
+constexpr int kPlanes = std::is_same_v<T, float> ? 3 : 1;
 
 // n within 32 of the matrix instruction's row r = 8 a + 4 h + e
 __device__ inline int row_of(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
@@ -295,49 +299,50 @@ __device__ inline void finish(const Epilogue& e, const Drop& drop, int64_t M, in
 }
 
 // One operand's way from memory into LDS.  ROWS: its rows of the tile.  HALF: the tile takes HALF rows of the value,
-// HALF of the gate and so on (0: consecutive rows).
-template <bool KC, int ROWS, int THREADS, int HALF>
+// HALF of the gate and so on (0: consecutive rows).  STEP k in each of PLANES planes.
+template <bool KC, int ROWS, int WAVES, int HALF, int STEP, int PLANES>
 struct Stage {
-  static constexpr int kBytes = ROWS * kStep * 2;
-  static constexpr int kPieces = kBytes / 1024;  // one load of a wave each
-  static constexpr int kReads = KC ? 1 : 2;       // LDS reads a fragment
-  static constexpr int kWaves = THREADS / 64, kLoads = (kPieces + kWaves - 1) / kWaves;
-  static_assert(ROWS % 32 == 0 && HALF % 8 == 0);
+  static constexpr int kPlaneBytes = ROWS * STEP * 2, kBytes = PLANES * kPlaneBytes;
+  static constexpr int kPieces = kBytes / 1024, kPlanePieces = kPlaneBytes / 1024;  // one load of a wave each
+  static constexpr int kLoads = (kPieces + WAVES - 1) / WAVES;
+  static constexpr int kReads = (KC ? 1 : 2) * PLANES;  // LDS reads for 32 rows and 16 k
+  static constexpr int kRowBytes = KC ? STEP * 2 : ROWS * 2, kChunks = kRowBytes / 16;
+  static_assert(kPlaneBytes % 1024 == 0 && (HALF * STEP * 2) % 1024 == 0);
 
   uint32_t off[kLoads];
-  int32_t k_of[kLoads];  // the first k (of the step's 64) of each load
+  int32_t k_of[kLoads];  // the first k (of the step's) of each load
   const uint8_t* base;
-  int64_t gate, advance;  // bytes to the gate's rows; bytes a step
+  int64_t gate, plane, advance;  // bytes to the gate's rows, to the next plane, to the next step
 
   __device__ void init(const Matrix& a, int64_t row0, int64_t rows, int64_t second) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     base = (const uint8_t*)a.p + (KC ? row0 * a.ld : row0) * 2;
     gate = second * a.ld * 2;
-    advance = (KC ? kStep : kStep * a.ld) * 2;
+    plane = a.plane * 2;
+    advance = (KC ? STEP : STEP * a.ld) * 2;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int piece = (i * kWaves + wave) * 64 + lane;  // the 16 bytes of LDS that the lane fills
+      const int at = ((i * WAVES + wave) % kPlanePieces) * 64 + lane;  // the 16 bytes of the LDS plane that the lane fills
+      const int r = at / kChunks, chunk = (at % kChunks) ^ swizzle(r);
       if constexpr (KC) {
-        const int r = piece / 8, chunk = (piece % 8) ^ swizzle(r);
         int64_t row = HALF ? r / (2 * HALF + !HALF) * HALF + r % (HALF + !HALF) : r;
         row = row < rows - row0 ? row : rows - row0 - 1;
         off[i] = (uint32_t)((row * a.ld + chunk * 8) * 2);
         k_of[i] = chunk * 8;
       } else {
-        const int k = piece / (ROWS / 8), chunk = (piece % (ROWS / 8)) ^ swizzle(k);
         const int64_t last = a.width - row0 - 8, col = chunk * 8 < last ? chunk * 8 : last;
-        off[i] = (uint32_t)((k * a.ld + col) * 2);
-        k_of[i] = k;
+        off[i] = (uint32_t)((r * a.ld + col) * 2);
+        k_of[i] = r;
       }
     }
   }
 
   // Which 16 bytes of an LDS row hold which: their number is xored with this.  LDS has 64 banks of 4 bytes.
-  // K-contiguous, rows of 128 bytes: of the 16 lanes that read together, those of rows of one parity differ in it.
+  // K-contiguous: 16 lanes read the same k of 16 rows together; rows that begin at the same bank differ in it.
   // Row-contiguous: 32 lanes read 64 bytes of 4 consecutive k together, which go to different quarters of the banks;
   // rows of an odd number of 64 bytes do so by themselves.
   __device__ static int swizzle(int r) {
-    if constexpr (KC) return (r >> 1) & 7;
+    if constexpr (KC) return STEP == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
     return ROWS % 128 == 0 ? (r & 3) << 2 : ROWS % 64 == 0 ? (r & 2) << 1 : 0;
   }
 
@@ -348,10 +353,11 @@ struct Stage {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int piece = i * kWaves + wave;
-      if ((i + 1) * kWaves > kPieces && piece >= kPieces) break;
+      const int piece = i * WAVES + wave;
+      if ((i + 1) * WAVES > kPieces && piece >= kPieces) break;
       const uint8_t* b = base;
-      if constexpr (HALF != 0) b += (piece * 8 / HALF) % 2 ? gate : 0;
+      if constexpr (PLANES > 1) b += piece / kPlanePieces * plane;
+      if constexpr (HALF != 0) b += piece % kPlanePieces * 1024 / (HALF * STEP * 2) % 2 ? gate : 0;
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, 0x80000000, 0x00020000);
       const uint32_t o = k_of[i] < left ? off[i] : 0x80000000u;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + piece * 1024), 16, o, 0, 0, 0);
@@ -363,31 +369,31 @@ struct Stage {
     const int lane = threadIdx.x & 63;
     if constexpr (KC) {
       const int r = row_of(lane & 31);
-      return *(const half8*)(lds + row * 128 + r * 128 + (((2 * s + (lane >> 5)) ^ swizzle(r)) << 4));
+      return *(const half8*)(lds + row * kRowBytes + r * kRowBytes + (((2 * s + (lane >> 5)) ^ swizzle(r)) << 4));
     } else {
       // 16 lanes read 4 k of 16 rows, a lane 4 rows of one k, and get 4 k of one row each
       const int i = lane & 15, r = row + row_of(16 * ((lane >> 4) & 1) + 4 * (i & 3)), k = 8 * (lane >> 5) + (i >> 2);
-      const uint8_t* at = lds + k * ROWS * 2 + (((r >> 3) ^ swizzle(k)) << 4) + (r & 7) * 2;  // swizzle(k): of k % 4 alone
+      const uint8_t* at = lds + k * kRowBytes + (((r >> 3) ^ swizzle(k)) << 4) + (r & 7) * 2;  // swizzle(k): of k % 4 alone
       half4 part[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) half4*)(at + (16 * s + 4 * u) * ROWS * 2));
+        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) half4*)(at + (16 * s + 4 * u) * kRowBytes));
       return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
+  }
+
+  template <int COUNT>
+  __device__ static void fragments(const uint8_t* lds, int row, int s, half8 (&out)[PLANES][COUNT]) {
+#pragma unroll
+    for (int c = 0; c < PLANES; ++c)
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) out[c][i] = fragment(lds + c * kPlaneBytes, row + 32 * i, s);
   }
 };
 
 // Planes of a 32-bit matrix times planes of another: a = a0 + a1 + a2 exactly, 8 bits each, so the six products down to
 // 2^-16 of a0 b0 leave out 3 2^-24 of a b.  Smallest first.
-__device__ constexpr int kPlaneP[6] = {2, 0, 1, 1, 0, 0}, kPlaneQ[6] = {0, 2, 1, 0, 1, 0};
-
-template <typename SP, typename SQ, int TM, int TN>
-__device__ __forceinline__ void read(const uint8_t* from, int s, int wm, int wn, half8 (&fp)[TM / 32], half8 (&fq)[TN / 32]) {
-#pragma unroll
-  for (int i = 0; i < TM / 32; ++i) fp[i] = SP::fragment(from, wm + 32 * i, s);
-#pragma unroll
-  for (int j = 0; j < TN / 32; ++j) fq[j] = SQ::fragment(from + SP::kBytes, wn + 32 * j, s);
-}
+constexpr int kPlaneP[6] = {2, 0, 1, 1, 0, 0}, kPlaneQ[6] = {0, 2, 1, 0, 1, 0};
 
 // This wave's LDS reads are done and its loads are in LDS; then all waves'.
 __device__ __forceinline__ void meet() {
@@ -416,33 +422,43 @@ __device__ __forceinline__ void interleave() {
 // before any read.
 template <typename T, typename SP, typename SQ, int TM, int TN, bool NEXT, bool LOAD, int S = 0, typename Load>
 __device__ __forceinline__ void step(uint8_t* __restrict__ cur, const uint8_t* __restrict__ nxt, Load& load, int wm, int wn,
-                                     half8 (&fp)[2][TM / 32], half8 (&fq)[2][TN / 32], f32x16 (&acc)[TN / 32][TM / 32]) {
-  if constexpr (S < kStep / 16) {
-    constexpr bool kLast = S + 1 == kStep / 16;
-    constexpr int kReads = kLast && !NEXT ? 0 : SP::kReads * (TM / 32) + SQ::kReads * (TN / 32);
+                                     half8 (&fp)[2][kPlanes<T>][TM / 32], half8 (&fq)[2][kPlanes<T>][TN / 32],
+                                     f32x16 (&acc)[TN / 32][TM / 32]) {
+  if constexpr (S < kStep<T> / 16) {
+    constexpr bool kLast = S + 1 == kStep<T> / 16;
+    constexpr int kReads = kLast && !NEXT ? 0 : SP::kReads * (TM / 32) + SQ::kReads * (TN / 32), kTimes = kPlanes<T> == 1 ? 1 : 6;
     if constexpr (!kLast) {
-      read<SP, SQ, TM, TN>(cur, S + 1, wm, wn, fp[~S & 1], fq[~S & 1]);
+      SP::template fragments<TM / 32>(cur, wm, S + 1, fp[~S & 1]);
+      SQ::template fragments<TN / 32>(cur + SP::kBytes, wn, S + 1, fq[~S & 1]);
     } else if constexpr (NEXT) {
       meet();
       if constexpr (LOAD) load(cur);
-      read<SP, SQ, TM, TN>(nxt, 0, wm, wn, fp[~S & 1], fq[~S & 1]);
+      SP::template fragments<TM / 32>(nxt, wm, 0, fp[~S & 1]);
+      SQ::template fragments<TN / 32>(nxt + SP::kBytes, wn, 0, fq[~S & 1]);
     }
 #pragma unroll
-    for (int j = 0; j < TN / 32; ++j)
+    for (int c = 0; c < kTimes; ++c)
 #pragma unroll
-      for (int i = 0; i < TM / 32; ++i) acc[j][i] = mfma<T>(fq[S & 1][j], fp[S & 1][i], acc[j][i]);
-    interleave<TM / 32 * (TN / 32), kReads, kLast && LOAD ? SP::kLoads + SQ::kLoads : 0>();
+      for (int j = 0; j < TN / 32; ++j)
+#pragma unroll
+        for (int i = 0; i < TM / 32; ++i)
+          acc[j][i] = mfma<T>(fq[S & 1][kTimes == 1 ? 0 : kPlaneQ[c]][j], fp[S & 1][kTimes == 1 ? 0 : kPlaneP[c]][i], acc[j][i]);
+    interleave<TM / 32 * (TN / 32) * kTimes, kReads, kLast && LOAD ? SP::kLoads + SQ::kLoads : 0>();
     step<T, SP, SQ, TM, TN, NEXT, LOAD, S + 1>(cur, nxt, load, wm, wn, fp, fq, acc);
   }
 }
 
 template <typename T, bool PKC, bool QKC, int ACT, int WM, int WN, int TM, int TN>
-__global__ __launch_bounds__(WM * WN * 64, (WM * TM + WN * TN) * kStep * 4 > 80 * 1024 ? WM * WN / 4 : WM * WN / 2) void k_product(Shape sh, Matrix p, Matrix q, int64_t second, Epilogue e) {
+constexpr int kStageBytes = (WM * TM + WN * TN) * kStep<T> * 2 * kPlanes<T>;
+
+// Waves a SIMD: by how many workgroups' double buffers the 160 KB of LDS hold, one or two.
+template <typename T, bool PKC, bool QKC, int ACT, int WM, int WN, int TM, int TN>
+__global__ __launch_bounds__(WM * WN * 64, WM * WN / (kStageBytes<T, PKC, QKC, ACT, WM, WN, TM, TN> * 2 > 80 * 1024 ? 4 : 2)) void k_product(
+    Shape sh, Matrix p, Matrix q, int64_t second, Epilogue e) {
   constexpr bool kGated = ACT != GF_ACT_NONE;
-  constexpr int kThreads = WM * WN * 64, BM = WM * TM, BN = WN * TN, BO = kGated ? BN / 2 : BN;
-  constexpr int kPlanes = std::is_same_v<T, float> ? 6 : 1;
-  using SP = Stage<PKC, BM, kThreads, 0>;
-  using SQ = Stage<QKC, BN, kThreads, kGated ? TN / 2 : 0>;
+  constexpr int kThreads = WM * WN * 64, BM = WM * TM, BN = WN * TN, BO = kGated ? BN / 2 : BN, kK = kStep<T>;
+  using SP = Stage<PKC, BM, WM * WN, 0, kK, kPlanes<T>>;
+  using SQ = Stage<QKC, BN, WM * WN, kGated ? TN / 2 : 0, kK, kPlanes<T>>;
   __shared__ __attribute__((aligned(1024))) uint8_t lds0[SP::kBytes + SQ::kBytes], lds1[SP::kBytes + SQ::kBytes];
 
   // Workgroups go round the 8 dies by their number; a die gets consecutive tiles, in groups of 8 tile rows, so that
@@ -452,7 +468,7 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * TM + WN * TN) * kStep * 4 > 80 
   const int group = tile / (8 * sh.tiles_n), in_group = tile % (8 * sh.tiles_n);
   const int height = sh.tiles_m - 8 * group < 8 ? sh.tiles_m - 8 * group : 8;
   const int64_t m0 = (int64_t)(8 * group + in_group % height) * BM, n0 = (int64_t)(in_group / height) * BO;
-  const int step0 = blockIdx.y * sh.steps, all = (int)((sh.K + kStep - 1) / kStep);
+  const int step0 = blockIdx.y * sh.steps, all = (int)((sh.K + kK - 1) / kK);
   const int steps = all - step0 < sh.steps ? all - step0 : sh.steps;
 
   SP sp;
@@ -461,38 +477,27 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * TM + WN * TN) * kStep * 4 > 80 
   sq.init(q, n0, sh.N, second);
   sp.seek(step0);
   sq.seek(step0);
-  const uint8_t *p_base = sp.base, *q_base = sq.base;
 
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wm = wave % WM * TM, wn = wave / WM * TN;
   f32x16 acc[TN / 32][TM / 32] = {};
 
-  const int first_left = (int)(sh.K - (int64_t)step0 * kStep);
-  int left = first_left;      // k from the next load's first on; none: loads read nothing and fill with zeros
-  int loaded = 0, plane = 0;  // steps of this plane product loaded; which it is
+  int left = (int)(sh.K - (int64_t)step0 * kK);  // k from the next load's first on; none: loads read nothing and fill with zeros
   auto load = [&](uint8_t* to) {
-    if constexpr (kPlanes > 1) {
-      if (loaded == 0) {
-        const int i = plane < kPlanes ? plane : kPlanes - 1;
-        sp.base = p_base + kPlaneP[i] * p.plane * 2;
-        sq.base = q_base + kPlaneQ[i] * q.plane * 2;
-        left = plane < kPlanes ? first_left : 0;
-      }
-      if (++loaded == steps) loaded = 0, ++plane;
-    }
     sp.load(to, left);
     sq.load(to + SP::kBytes, left);
     sp.seek(1);
     sq.seek(1);
-    left -= kStep;
+    left -= kK;
   };
 
-  half8 fp[2][TM / 32], fq[2][TN / 32];
+  half8 fp[2][kPlanes<T>][TM / 32], fq[2][kPlanes<T>][TN / 32];
   load(lds0);
   meet();
   load(lds1);
-  read<SP, SQ, TM, TN>(lds0, 0, wm, wn, fp[0], fq[0]);
-  int after = steps * kPlanes - 1;  // steps after the one to be done
+  SP::template fragments<TM / 32>(lds0, wm, 0, fp[0]);
+  SQ::template fragments<TN / 32>(lds0 + SP::kBytes, wn, 0, fq[0]);
+  int after = steps - 1;  // steps after the one to be done
   for (; after >= 2; after -= 2) {
     step<T, SP, SQ, TM, TN, true, true>(lds0, lds1, load, wm, wn, fp, fq, acc);
     step<T, SP, SQ, TM, TN, true, true>(lds1, lds0, load, wm, wn, fp, fq, acc);
@@ -939,35 +944,43 @@ int operand(Arena& ws, bool run, const void* x, int64_t rows, int64_t cols, int6
 constexpr int kUnits = 256;  // compute units
 
 // How a product is cut into workgroups: tiles, and `splits` parts along k that k_join adds.
-enum class Tile { k256x256, k256x160, k128x128 };
+enum class Tile { k256x256, k256x160, k256x128, k128x128 };
 struct Cut {
   Tile tile;
   int32_t splits;
 };
 
-// The cut whose estimated time is least, from what was measured in bfloat16.  A step of 64 takes 1.59 us with a
+struct TileKind {
+  Tile tile;
+  int64_t m, n, slots;  // slots: workgroups at a time
+  double step, round;   // us
+};
+
+// The cut whose estimated time is least, from what was measured.  In 16 bits a step of 64 takes 1.59 us with a
 // 256 x 256 tile on each compute unit (4096 x 4096 x 8192: 203 us, 1.35 PFLOP/s), 1.18 us with 256 x 160
 // (8192 x 1280 x 10240, one round: 191 us, against 208 us in 160 tiles of 256 x 256) and 0.98 us with two of 128 x 128
 // (250 us for the first: twice the bytes from L2 for each operation).  Where not all units work, those that do run faster
 // (160 tiles: 1.30 us a step): the chip is held by its power.  A round costs about 7, 7 and 3 us besides, and split
-// parts are written and read back at about 4 TB/s.
-Cut choose_cut(int64_t M, int64_t columns, int64_t steps, bool gated, int planes, int size) {
-  constexpr struct {
-    Tile tile;
-    int64_t m, n, slots;
-    double step, round;
-  } kinds[] = {{Tile::k256x256, 256, 256, kUnits, 1.59, 7.0}, {Tile::k256x160, 256, 160, kUnits, 1.18, 7.0}, {Tile::k128x128, 128, 128, 2 * kUnits, 0.98, 3.0}};
+// parts are written and read back at about 4 TB/s.  In 32 bits a step of 32 takes 2.35 us with 256 x 128 and 1.25 us with
+// 128 x 128 on each unit (4096 x 4096 x 2048: 284 to 329 us and 302 to 344 us, by the operands' layouts).
+constexpr TileKind kTiles16[] = {{Tile::k256x256, 256, 256, kUnits, 1.59, 7.0}, {Tile::k256x160, 256, 160, kUnits, 1.18, 7.0}, {Tile::k128x128, 128, 128, 2 * kUnits, 0.98, 3.0}};
+constexpr TileKind kTiles32[] = {{Tile::k256x128, 256, 128, kUnits, 2.35, 7.0}, {Tile::k128x128, 128, 128, kUnits, 1.25, 4.0}};
+
+template <bool F32>
+Cut choose_cut(int64_t M, int64_t columns, int64_t steps, bool gated) {
+  constexpr const TileKind* kinds = F32 ? kTiles32 : kTiles16;
   Cut best{};
   double least = 1e300;
-  for (const auto& k : kinds) {
+  for (int i = 0; i < (F32 ? 2 : 3); ++i) {
+    const TileKind& k = kinds[i];
     if (gated && k.tile == Tile::k256x160) continue;  // its halves would not be whole matrix instructions
     const int64_t tiles = ((M + k.m - 1) / k.m) * ((columns + k.n - 1) / k.n);
     for (int64_t splits = 1; splits <= 32 && splits * 2 <= std::max<int64_t>(steps, 2); ++splits) {
-      const double each = (double)((steps + splits - 1) / splits) * planes * k.step;
+      const double each = (double)((steps + splits - 1) / splits) * k.step;
       const int64_t full = tiles * splits / k.slots, rest = tiles * splits % k.slots;
       double us = full * (each + k.round);
       if (rest != 0) us += each * std::max(0.72, 0.5 + 0.5 * rest / k.slots) + k.round;
-      if (splits > 1) us += M * columns * (8.0 * splits + size) / 4e6 + 4.0;
+      if (splits > 1) us += M * columns * (8.0 * splits + (F32 ? 4 : 2)) / 4e6 + 4.0;
       if (us < least) least = us, best = {k.tile, (int32_t)splits};
     }
   }
@@ -979,7 +992,7 @@ int product_tiled(Arena& ws, bool run, int64_t M, int64_t N, int64_t K, const Ma
                   int64_t splits, hipStream_t s) {
   constexpr int BM = WM * TM, BO = WN * TN / (ACT == GF_ACT_NONE ? 1 : 2);
   Shape sh{M, N, K, 0, 0, 1, 0};
-  const int64_t tm = (M + BM - 1) / BM, tn = (N + BO - 1) / BO, steps = (K + kStep - 1) / kStep;
+  const int64_t tm = (M + BM - 1) / BM, tn = (N + BO - 1) / BO, steps = (K + kStep<T> - 1) / kStep<T>;
   if (tm * tn > (int64_t(1) << 30)) return fail(GF_E_INVALID_ARGUMENT, "rows, in_features or out_features too large");
   sh.tiles_m = (int32_t)tm, sh.tiles_n = (int32_t)tn;
   sh.steps = (int32_t)((steps + splits - 1) / splits);
@@ -1003,12 +1016,18 @@ int product(Arena& ws, bool run, int64_t M, int64_t N, int64_t K, const Matrix& 
             hipStream_t s) {
   // a load's 32-bit offset spans a tile's rows (K-contiguous) or a step's (row-contiguous)
   if (std::max(p.ld, q.ld) * 2 * 256 >= (int64_t(1) << 31)) return fail(GF_E_INVALID_ARGUMENT, "row stride too large");
-  const Cut cut = choose_cut(M, ACT == GF_ACT_NONE ? N : 2 * N, (K + kStep - 1) / kStep, ACT != GF_ACT_NONE,
-                             std::is_same_v<T, float> ? 6 : 1, sizeof(T));
-  if constexpr (ACT == GF_ACT_NONE)
-    if (cut.tile == Tile::k256x160) return product_tiled<T, PKC, QKC, ACT, 8, 1, 32, 160>(ws, run, M, N, K, p, q, second, e, cut.splits, s);
-  if (cut.tile == Tile::k256x256) return product_tiled<T, PKC, QKC, ACT, 2, 4, 128, 64>(ws, run, M, N, K, p, q, second, e, cut.splits, s);
-  return product_tiled<T, PKC, QKC, ACT, 2, 2, 64, 64>(ws, run, M, N, K, p, q, second, e, cut.splits, s);
+  const Cut cut = choose_cut<std::is_same_v<T, float>>(M, ACT == GF_ACT_NONE ? N : 2 * N, (K + kStep<T> - 1) / kStep<T>, ACT != GF_ACT_NONE);
+#define FF_TILED(...) return product_tiled<T, PKC, QKC, ACT, __VA_ARGS__>(ws, run, M, N, K, p, q, second, e, cut.splits, s)
+  if constexpr (std::is_same_v<T, float>) {
+    if (cut.tile == Tile::k256x128) FF_TILED(4, 2, 64, 64);
+    FF_TILED(4, 2, 32, 64);
+  } else {
+    if constexpr (ACT == GF_ACT_NONE)
+      if (cut.tile == Tile::k256x160) FF_TILED(8, 1, 32, 160);
+    if (cut.tile == Tile::k256x256) FF_TILED(2, 4, 128, 64);
+    FF_TILED(2, 2, 64, 64);
+  }
+#undef FF_TILED
 }
 
 template <typename T, int ACT>
@@ -1059,9 +1078,9 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
         dz.p = ws.take(dz.plane * 2 * (kSplit ? 3 : 1));
       }
       if (make || a.dbias != nullptr) {
-        // rows in chunks of at least 32 until there are about 4 workgroups a compute unit
+        // rows in chunks of at least 8 until there are about 4 workgroups a compute unit
         const int64_t across = (out + 255) / 256;
-        int64_t chunks = std::max<int64_t>(std::min<int64_t>(4 * kUnits / across, a.rows / 32), 1);
+        int64_t chunks = std::max<int64_t>(std::min<int64_t>(4 * kUnits / across, a.rows / 8), 1);
         const int64_t chunk = (a.rows + chunks - 1) / chunks;
         chunks = (a.rows + chunk - 1) / chunk;
         float* sums = a.dbias != nullptr ? (float*)ws.take(chunks * wr * 4) : nullptr;
