@@ -235,7 +235,7 @@ struct Epilogue {
   const void* bias;
   const void* residual;
   int64_t ldr;
-  void* saved;  // gated: the value's plane, then the gate's, [M, saved_ld]
+  void* saved;  // gated: see Saved
   int64_t saved_ld;
   float* partial;  // not NULL: sums for k_join instead of all of the above, [split][M][N (gated: 2 N), whole groups of 8]
   Drop drop;
@@ -257,6 +257,65 @@ constexpr int kPlanes = std::is_same_v<T, float> ? 3 : 1;
 // n within 32 of the matrix instruction's row r = 8 a + 4 h + e
 __device__ inline int row_of(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
 
+// What a gated forward leaves for its backward: value and gate of [rows, ld], ld whole groups of 8.  In 32 bits two
+// planes of floats.  For 16-bit tensors floats of fewer bits, 12 significant ones (bfloat16) or 16 (float16): the upper
+// 16 bits of the float in two planes, the bits below them of value and gate together in a third.  A rounding to the
+// tensors' own type here would count in dx and dW as much as the two that are needed, of dz and of the result itself
+// (1.7 instead of 1.4 roundings); the third plane costs a quarter (half) more bytes than that.
+template <typename T>
+struct Saved {
+  static constexpr bool kFloat = std::is_same_v<T, float>;
+  static constexpr int kExtra = std::is_same_v<T, bf16> ? 4 : 8;  // bits below the upper 16
+  using Low = std::conditional_t<kExtra == 4, uint8_t, uint16_t>;
+  static constexpr int64_t kBytes = kFloat ? 8 : 4 + sizeof(Low);  // an element
+
+  void* p;
+  int64_t rows, ld;
+
+  __device__ Vec<uint16_t, 8>* high(int64_t row, int64_t col) const { return (Vec<uint16_t, 8>*)((uint16_t*)p + row * ld + col); }
+  __device__ Vec<Low, 8>* low(int64_t row, int64_t col) const { return (Vec<Low, 8>*)((Low*)((uint16_t*)p + 2 * rows * ld) + row * ld + col); }
+
+  // to the nearest, halves up; a NaN as it is, or its bits could carry into the sign
+  __device__ static uint32_t rounded(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    return x == x ? b + (0x8000u >> kExtra) : b;
+  }
+
+  __device__ void put(int64_t row, int64_t col, const float v[8], const float g[8]) const {
+    if constexpr (kFloat) {
+      store8((float*)p + row * ld + col, v, true, 8);
+      store8((float*)p + (rows + row) * ld + col, g, true, 8);
+    } else {
+      Vec<uint16_t, 8> a, b;
+      Vec<Low, 8> l;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t x = rounded(v[j]), y = rounded(g[j]);
+        a[j] = (uint16_t)(x >> 16), b[j] = (uint16_t)(y >> 16);
+        l[j] = (Low)((x & 0xffffu) >> (16 - kExtra) | ((y & 0xffffu) >> (16 - kExtra)) << kExtra);
+      }
+      *high(row, col) = a;
+      *high(rows + row, col) = b;
+      *low(row, col) = l;
+    }
+  }
+
+  __device__ void get(int64_t row, int64_t col, float v[8], float g[8]) const {
+    if constexpr (kFloat) {
+      load8(v, (const float*)p + row * ld + col, true, 8);
+      load8(g, (const float*)p + (rows + row) * ld + col, true, 8);
+    } else {
+      const Vec<uint16_t, 8> a = *high(row, col), b = *high(rows + row, col);
+      const Vec<Low, 8> l = *low(row, col);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = __builtin_bit_cast(float, (uint32_t)a[j] << 16 | (l[j] & ((1u << kExtra) - 1)) << (16 - kExtra));
+        g[j] = __builtin_bit_cast(float, (uint32_t)b[j] << 16 | (uint32_t)(l[j] >> kExtra) << (16 - kExtra));
+      }
+    }
+  }
+};
+
 // What follows the sums: 8 consecutive columns n.. of row m (gated: the value's in v, the gate's in g).
 // WHOLE: all 8 are inside.
 template <typename T, int ACT, bool WHOLE>
@@ -276,10 +335,7 @@ __device__ inline void finish(const Epilogue& e, const Drop& drop, int64_t M, in
     }
   }
   if constexpr (ACT != GF_ACT_NONE) {
-    if (e.saved != nullptr) {  // its rows are padded to whole groups of 8
-      store8((T*)e.saved + m * e.saved_ld + n, v, true, 8);
-      store8((T*)e.saved + (M + m) * e.saved_ld + n, g, true, 8);
-    }
+    if (e.saved != nullptr) Saved<T>{e.saved, M, e.saved_ld}.put(m, n, v, g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= activation<ACT>(g[j], nullptr);
   }
@@ -724,7 +780,7 @@ __global__ __launch_bounds__(256) void k_pack(int64_t rows, int64_t cols, const 
 // ([rows, ld], in planes for 32 bits, zero past its columns), and its columns' sums: a workgroup takes 256 columns of dy
 // and `chunk` rows, 8 columns a thread in 8 interleaved rows, and leaves its sums in `sums` [row chunk][columns of dz].
 template <typename T, int ACT>
-__global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, int64_t chunk, const T* dy, int64_t lddy, const T* saved,
+__global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, int64_t chunk, const T* dy, int64_t lddy, void* saved,
                                             int64_t saved_ld, void* dz, int64_t ld, int64_t plane, float* sums) {
   constexpr bool kGated = ACT != GF_ACT_NONE;
   constexpr int H = kGated ? 2 : 1;
@@ -747,8 +803,7 @@ __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, i
       }
       if constexpr (kGated) {
         float value[8], gate[8];
-        load8(value, saved + row * saved_ld + c, true, 8);
-        load8(gate, saved + (rows + row) * saved_ld + c, true, 8);
+        Saved<T>{saved, rows, saved_ld}.get(row, c, value, gate);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float slope;
@@ -1086,7 +1141,7 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
         float* sums = a.dbias != nullptr ? (float*)ws.take(chunks * wr * 4) : nullptr;
         FF_RUN {
           k_dz<T, ACT><<<dim3((unsigned)across, (unsigned)chunks), 256, 0, s>>>(
-              drop, a.rows, out, chunk, (const T*)a.dy, a.lddy, (const T*)a.saved, saved_ld(&a),
+              drop, a.rows, out, chunk, (const T*)a.dy, a.lddy, a.saved, saved_ld(&a),
               make ? (void*)dz.p : nullptr, dz.ld, dz.plane, sums);
           FF_LAUNCH_CHECK("k_dz");
           if (sums != nullptr) {
@@ -1139,7 +1194,8 @@ int gf_dropout_add(int32_t dtype, const gf_dropout* dropout, int64_t rows, int64
 
 size_t gf_ff_saved_bytes(const gf_ff_args* args) {
   if (check_shape(args) != GF_OK || args->activation == GF_ACT_NONE) return 0;
-  return (size_t)(2 * args->rows * saved_ld(args) * size_of(args->dtype));
+  const int64_t element = args->dtype == GF_DTYPE_F32 ? Saved<float>::kBytes : args->dtype == GF_DTYPE_BF16 ? Saved<bf16>::kBytes : Saved<f16>::kBytes;
+  return (size_t)(args->rows * saved_ld(args) * element);
 }
 
 size_t gf_ff_workspace_bytes(const gf_ff_args* args, int32_t is_backward) {
