@@ -232,7 +232,9 @@ class GaussianLinear(nn.Linear):
     def _delta_apply_row_chunk(self) -> int:
         return min(self.out_features, max(max(1, int(self.adapter_config.tile_out)), 64))
 
-    def forward(self, input: Tensor) -> Tensor:
+    def merged_weight(self) -> Tensor:
+        """weight + adapter_scale * delta-W, differentiable in the Gaussians: what ``delta_apply="merged"`` multiplies
+        by, and what operators that take a weight (guass_amd.feedforward) get of this layer."""
         pending = self._batched_delta
         if pending is not None and pending[2] == "merged_weight":
             # weight + adapter_scale * delta-W, written by GaussianFieldBatch's render (the same
@@ -243,13 +245,18 @@ class GaussianLinear(nn.Linear):
             self.__dict__["last_forward_metadata"] = {
                 "execution_mode": self.adapter_config.execution_mode, "accumulate_backend": "batched_fields",
                 "delta_w_norm": norm, "linear_composition": "merged_weight"}
-            return F.linear(input, merged, self._parameters["bias"])
+            return merged
         delta_weight = self.compute_delta_weight().to(dtype=self.weight.dtype)
-        if self.adapter_config.delta_apply == "merged":
-            metadata = dict(self.last_forward_metadata)
-            metadata["linear_composition"] = "merged_weight"
-            self.last_forward_metadata = metadata
-            return F.linear(input, self.weight + delta_weight, self.bias)
+        metadata = dict(self.last_forward_metadata)
+        metadata["linear_composition"] = "merged_weight"
+        self.last_forward_metadata = metadata
+        return self.weight + delta_weight
+
+    def forward(self, input: Tensor) -> Tensor:
+        pending = self._batched_delta
+        if self.adapter_config.delta_apply == "merged" or (pending is not None and pending[2] == "merged_weight"):
+            return F.linear(input, self.merged_weight(), self._parameters["bias"])
+        delta_weight = self.compute_delta_weight().to(dtype=self.weight.dtype)
         base = F.linear(input, self.weight, self.bias)
         chunk = self._delta_apply_row_chunk()
         metadata = dict(self.last_forward_metadata)
@@ -261,6 +268,54 @@ class GaussianLinear(nn.Linear):
             r1 = min(r0 + chunk, self.out_features)
             out[..., r0:r1].add_(F.linear(input, delta_weight[r0:r1, :], None))
         return out
+
+
+class GaussianFeedForward(nn.Module):
+    """The feed-forward half of a transformer block on adapted linears (``ff.net.0.proj`` and ``ff.net.2`` of the
+    reference's target model): residual + out_dropout(out(dropout(value * act(gate)))), (value, gate) the two halves
+    of proj(x).  Both layers' weights are taken merged (from GaussianFieldBatch's render where that ran, else rendered
+    here) by the kernels of guass_amd.feedforward; nothing of the inner width is kept but what the backward reads.
+
+    In training mode ``forward`` needs a ``seed`` where something is dropped: an int, or an int64 tensor on the device that
+    a captured graph can be given anew.  The two dropouts draw at counters 2 ``offset`` and 2 ``offset`` + 1, so give
+    every block of a model, and every step of one seed, an offset of its own.
+    """
+
+    def __init__(self, proj: GaussianLinear, out: GaussianLinear, *, activation: str = "gelu", dropout: float = 0.0,
+                 out_dropout: float = 0.0) -> None:
+        super().__init__()
+        from guass_amd.feedforward import ACTIVATIONS
+
+        for name, ly in (("proj", proj), ("out", out)):
+            if not isinstance(ly, GaussianLinear):
+                raise TypeError(f"{name} is not a GaussianLinear")
+        if proj.out_features != 2 * out.in_features:
+            raise ValueError(f"proj must make value and gate of out's {out.in_features} features (got {proj.out_features})")
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation must be one of {ACTIVATIONS} (got {activation!r})")
+        for name, p in (("dropout", dropout), ("out_dropout", out_dropout)):
+            if not 0.0 <= p <= 1.0:
+                raise ValueError(f"{name} must lie in [0, 1] (got {p})")
+        self.proj, self.out = proj, out
+        self.activation, self.dropout, self.out_dropout = activation, float(dropout), float(out_dropout)
+
+    @classmethod
+    def from_linears(cls, proj: nn.Linear, out: nn.Linear, adapter_config: GaussianAdapterConfig, **kwargs) -> "GaussianFeedForward":
+        return cls(GaussianLinear.from_linear(proj, adapter_config), GaussianLinear.from_linear(out, adapter_config), **kwargs)
+
+    def forward(self, input: Tensor, residual: Tensor | None = None, *, seed: int | Tensor | None = None,
+                offset: int = 0) -> Tensor:
+        from guass_amd.feedforward import gated_linear, linear_dropout_add
+
+        p, out_p = (self.dropout, self.out_dropout) if self.training else (0.0, 0.0)
+        if seed is None:
+            if p or out_p:
+                raise ValueError("a training forward with dropout needs a seed")
+            seed = 0
+        h = gated_linear(input, self.proj.merged_weight(), self.proj.bias, activation=self.activation, p=p, seed=seed,
+                         offset=2 * offset)
+        return linear_dropout_add(h, self.out.merged_weight(), self.out.bias, residual, p=out_p, seed=seed,
+                                  offset=2 * offset + 1)
 
 
 class _null:

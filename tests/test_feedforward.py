@@ -118,6 +118,24 @@ def test_abi_refuses_a_small_workspace_and_a_gated_residual():
     assert lib.gf_dropout_add(0, ctypes.byref(d), 0, 8, None, 0, None, 0, None, 0, None) == 0
 
 
+def test_block_checks_its_layers():
+    from guass_amd.layers import GaussianAdapterConfig, GaussianFeedForward, GaussianLinear
+
+    cfg = GaussianAdapterConfig(init_num_gaussians=4)
+    proj, out = GaussianLinear(8, 24, adapter_config=cfg), GaussianLinear(12, 8, adapter_config=cfg)
+    block = GaussianFeedForward(proj, out, dropout=0.1)
+    with pytest.raises(ValueError, match="needs a seed"):
+        block(torch.zeros(2, 8))
+    with pytest.raises(TypeError, match="out is not a GaussianLinear"):
+        GaussianFeedForward(proj, torch.nn.Linear(12, 8))
+    with pytest.raises(ValueError, match="value and gate"):
+        GaussianFeedForward(out, proj)
+    with pytest.raises(ValueError, match="activation"):
+        GaussianFeedForward(proj, out, activation="relu")
+    with pytest.raises(ValueError, match="out_dropout"):
+        GaussianFeedForward(proj, out, out_dropout=-1.0)
+
+
 # ------------------------------------------------------------------------------------ the GPU
 
 
@@ -471,3 +489,57 @@ def test_graph_replays_draw_by_the_seed_tensor(device, dtype, rows):
         torch.cuda.synchronize()
         for got, ref in zip(out, want):
             assert torch.equal(got, ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batched", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+def test_adapted_block_trains_as_its_parts_do(device, dtype, batched):
+    """A whole step of the block (weights rendered with their deltas, both products, both dropouts, the residual) against
+    the same layers composed of torch's operations with the same masks: output and the Gaussians' gradients.  In
+    float32 both sides round like 32-bit sums (the gradients' bar is the field's, 1e-4 of their norm); in bfloat16 the
+    composition rounds the inner activation, its parts and every gradient of them, about eight roundings of 2^-9
+    each way, independent: 2% of the norm is beyond four times their sum."""
+    from guass_amd.layers import GaussianAdapterConfig, GaussianFeedForward, GaussianFieldBatch, GaussianLinear
+
+    if batched and dtype != torch.float32:
+        pytest.skip("the batch writes merged weights in float32 only; the layer then merges by itself")
+    _say("block", dtype, batched)
+    torch.manual_seed(0)
+    cfg = GaussianAdapterConfig(init_num_gaussians=48, init_amp_scale=0.05, tile_out=16, tile_in=16, delta_apply="merged")
+    dim, inner, rows, seed, offset = 64, 96, 130, 99, 3
+    block = GaussianFeedForward(GaussianLinear(dim, 2 * inner, adapter_config=cfg, device=device, dtype=dtype),
+                                GaussianLinear(inner, dim, adapter_config=cfg, device=device, dtype=dtype),
+                                dropout=0.2, out_dropout=0.1)
+    x, r, dy = (_rand(device, rows, dim, dtype=dtype, seed=130 + i) for i in range(3))
+    x.requires_grad_(True)
+    batch = GaussianFieldBatch([block.proj, block.out]) if batched else None
+    params = [p for ly in (block.proj, block.out) for p in ly.get_gaussian_parameters().values()]
+
+    def fused():
+        return block(x, r, seed=seed, offset=offset)
+
+    def parts():
+        z = torch.nn.functional.linear(x, block.proj.merged_weight(), block.proj.bias)
+        value, gate = z.chunk(2, dim=-1)
+        k1 = fo.keep_scale(rows, inner, 0.2, seed, 2 * offset).to(device, dtype)
+        k2 = fo.keep_scale(rows, dim, 0.1, seed, 2 * offset + 1).to(device, dtype)
+        h = value * torch.nn.functional.gelu(gate) * k1
+        return torch.nn.functional.linear(h, block.out.merged_weight(), block.out.bias) * k2 + r
+
+    results = []
+    for run in (fused, parts):
+        if batched:
+            batch.render()
+        y = run()
+        results.append([y.detach(), *torch.autograd.grad(y, [x, *params], dy)])
+    limit = 1e-4 if dtype == torch.float32 else 2e-2
+    for a, b in zip(*results):
+        assert float((a.double() - b.double()).norm() / b.double().norm()) < limit
+    block.eval()
+    with torch.no_grad():
+        plain = torch.nn.functional.linear(x, block.proj.merged_weight(), block.proj.bias)
+        value, gate = plain.double().chunk(2, dim=-1)
+        want = (value * torch.nn.functional.gelu(gate)) @ block.out.merged_weight().double().t() + block.out.bias.double()
+        got = block(x)
+    assert float((got.double() - want).norm() / want.norm()) < limit
