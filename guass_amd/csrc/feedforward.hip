@@ -405,7 +405,7 @@ struct Stage {
   __device__ void seek(int64_t steps) { base += steps * advance; }
 
   // left: how many of the k from here on are the matrix's
-  __device__ void load(uint8_t* lds, int left) const {
+  __device__ void load(uint8_t* lds, int offset, int left) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -416,34 +416,34 @@ struct Stage {
       if constexpr (HALF != 0) b += piece % kPlanePieces * 1024 / (HALF * STEP * 2) % 2 ? gate : 0;
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, 0x80000000, 0x00020000);
       const uint32_t o = k_of[i] < left ? off[i] : 0x80000000u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + piece * 1024), 16, o, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(lds + (uint32_t)(offset + piece * 1024)), 16, o, 0, 0, 0);
     }
   }
 
   // The fragment of 32 rows from `row` on and 16 k from 16 s on: lane l has row row_of(l % 32) and 8 k from 8 (l / 32) on.
-  __device__ static half8 fragment(const uint8_t* lds, int row, int s) {
+  __device__ static half8 fragment(const uint8_t* lds, int offset, int row, int s) {
     const int lane = threadIdx.x & 63;
     if constexpr (KC) {
       const int r = row_of(lane & 31);
-      return *(const half8*)(lds + row * kRowBytes + r * kRowBytes + (((2 * s + (lane >> 5)) ^ swizzle(r)) << 4));
+      return *(const half8*)(lds + (uint32_t)(offset + (row + r) * kRowBytes + (((2 * s + (lane >> 5)) ^ swizzle(r)) << 4)));
     } else {
       // 16 lanes read 4 k of 16 rows, a lane 4 rows of one k, and get 4 k of one row each
       const int i = lane & 15, r = row + row_of(16 * ((lane >> 4) & 1) + 4 * (i & 3)), k = 8 * (lane >> 5) + (i >> 2);
-      const uint8_t* at = lds + k * kRowBytes + (((r >> 3) ^ swizzle(k)) << 4) + (r & 7) * 2;  // swizzle(k): of k % 4 alone
+      const int at = offset + k * kRowBytes + (((r >> 3) ^ swizzle(k)) << 4) + (r & 7) * 2;  // swizzle(k): of k % 4 alone
       half4 part[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) half4*)(at + (16 * s + 4 * u) * kRowBytes));
+        part[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) half4*)(lds + (uint32_t)(at + (16 * s + 4 * u) * kRowBytes)));
       return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
 
   template <int COUNT>
-  __device__ static void fragments(const uint8_t* lds, int row, int s, half8 (&out)[PLANES][COUNT]) {
+  __device__ static void fragments(const uint8_t* lds, int offset, int row, int s, half8 (&out)[PLANES][COUNT]) {
 #pragma unroll
     for (int c = 0; c < PLANES; ++c)
 #pragma unroll
-      for (int i = 0; i < COUNT; ++i) out[c][i] = fragment(lds + c * kPlaneBytes, row + 32 * i, s);
+      for (int i = 0; i < COUNT; ++i) out[c][i] = fragment(lds, offset + c * kPlaneBytes, row + 32 * i, s);
   }
 };
 
@@ -474,23 +474,23 @@ __device__ __forceinline__ void interleave() {
 // One step of a workgroup.  Its first fragments are in slot 0 already; those of 16 k more are read while the matrix
 // cores work on the ones before, the next step's first ones too (NEXT), so that nobody waits behind the barrier.  Where
 // the barrier is passed, `cur` has been read by all and takes the loads of the step after next (LOAD).
-// cur and nxt are different LDS arrays and said to be (__restrict__): otherwise the compiler waits for the loads
-// before any read.
+// cur and nxt are different LDS arrays, and every access is one offset from one of them: what the compiler cannot tell
+// apart by that, it waits for all loads before reading.
 template <typename T, typename SP, typename SQ, int TM, int TN, bool NEXT, bool LOAD, int S = 0, typename Load>
-__device__ __forceinline__ void step(uint8_t* __restrict__ cur, const uint8_t* __restrict__ nxt, Load& load, int wm, int wn,
+__device__ __forceinline__ void step(uint8_t* cur, const uint8_t* nxt, Load& load, int wm, int wn,
                                      half8 (&fp)[2][kPlanes<T>][TM / 32], half8 (&fq)[2][kPlanes<T>][TN / 32],
                                      f32x16 (&acc)[TN / 32][TM / 32]) {
   if constexpr (S < kStep<T> / 16) {
     constexpr bool kLast = S + 1 == kStep<T> / 16;
     constexpr int kReads = kLast && !NEXT ? 0 : SP::kReads * (TM / 32) + SQ::kReads * (TN / 32), kTimes = kPlanes<T> == 1 ? 1 : 6;
     if constexpr (!kLast) {
-      SP::template fragments<TM / 32>(cur, wm, S + 1, fp[~S & 1]);
-      SQ::template fragments<TN / 32>(cur + SP::kBytes, wn, S + 1, fq[~S & 1]);
+      SP::template fragments<TM / 32>(cur, 0, wm, S + 1, fp[~S & 1]);
+      SQ::template fragments<TN / 32>(cur, SP::kBytes, wn, S + 1, fq[~S & 1]);
     } else if constexpr (NEXT) {
       meet();
       if constexpr (LOAD) load(cur);
-      SP::template fragments<TM / 32>(nxt, wm, 0, fp[~S & 1]);
-      SQ::template fragments<TN / 32>(nxt + SP::kBytes, wn, 0, fq[~S & 1]);
+      SP::template fragments<TM / 32>(nxt, 0, wm, 0, fp[~S & 1]);
+      SQ::template fragments<TN / 32>(nxt, SP::kBytes, wn, 0, fq[~S & 1]);
     }
 #pragma unroll
     for (int c = 0; c < kTimes; ++c)
@@ -540,8 +540,8 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / (kStageBytes<T, PKC, QKC, A
 
   int left = (int)(sh.K - (int64_t)step0 * kK);  // k from the next load's first on; none: loads read nothing and fill with zeros
   auto load = [&](uint8_t* to) {
-    sp.load(to, left);
-    sq.load(to + SP::kBytes, left);
+    sp.load(to, 0, left);
+    sq.load(to, SP::kBytes, left);
     sp.seek(1);
     sq.seek(1);
     left -= kK;
@@ -551,8 +551,8 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / (kStageBytes<T, PKC, QKC, A
   load(lds0);
   meet();
   load(lds1);
-  SP::template fragments<TM / 32>(lds0, wm, 0, fp[0]);
-  SQ::template fragments<TN / 32>(lds0 + SP::kBytes, wn, 0, fq[0]);
+  SP::template fragments<TM / 32>(lds0, 0, wm, 0, fp[0]);
+  SQ::template fragments<TN / 32>(lds0, SP::kBytes, wn, 0, fq[0]);
   int after = steps - 1;  // steps after the one to be done
   for (; after >= 2; after -= 2) {
     step<T, SP, SQ, TM, TN, true, true>(lds0, lds1, load, wm, wn, fp, fq, acc);
