@@ -261,7 +261,8 @@ __device__ inline int row_of(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) 
 // planes of floats.  For 16-bit tensors floats of fewer bits, 12 significant ones (bfloat16) or 16 (float16): the upper
 // 16 bits of the float in two planes, the bits below them of value and gate together in a third.  A rounding to the
 // tensors' own type here would count in dx and dW as much as the two that are needed, of dz and of the result itself
-// (1.7 instead of 1.4 roundings); the third plane costs a quarter (half) more bytes than that.
+// (1.7 instead of 1.4 roundings); the third plane costs a quarter (half) more bytes than that.  Written past the caches:
+// nobody reads it before the backward (16384 x 320 -> 1280: 74 -> 60 us, 8192 x 1280 -> 5120: 252 -> 244 us).
 template <typename T>
 struct Saved {
   static constexpr bool kFloat = std::is_same_v<T, float>;
@@ -283,8 +284,11 @@ struct Saved {
 
   __device__ void put(int64_t row, int64_t col, const float v[8], const float g[8]) const {
     if constexpr (kFloat) {
-      store8((float*)p + row * ld + col, v, true, 8);
-      store8((float*)p + (rows + row) * ld + col, g, true, 8);
+#pragma unroll
+      for (int u = 0; u < 8; u += 4) {
+        __builtin_nontemporal_store(f32x4{v[u], v[u + 1], v[u + 2], v[u + 3]}, (f32x4*)((float*)p + row * ld + col + u));
+        __builtin_nontemporal_store(f32x4{g[u], g[u + 1], g[u + 2], g[u + 3]}, (f32x4*)((float*)p + (rows + row) * ld + col + u));
+      }
     } else {
       Vec<uint16_t, 8> a, b;
       Vec<Low, 8> l;
@@ -294,9 +298,9 @@ struct Saved {
         a[j] = (uint16_t)(x >> 16), b[j] = (uint16_t)(y >> 16);
         l[j] = (Low)((x & 0xffffu) >> (16 - kExtra) | ((y & 0xffffu) >> (16 - kExtra)) << kExtra);
       }
-      *high(row, col) = a;
-      *high(rows + row, col) = b;
-      *low(row, col) = l;
+      __builtin_nontemporal_store(a, high(row, col));
+      __builtin_nontemporal_store(b, high(rows + row, col));
+      __builtin_nontemporal_store(l, low(row, col));
     }
   }
 
@@ -459,6 +463,13 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
 }
 
+// A wave's LDS writes before are seen by its reads after (and the other way round).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // For the scheduler: a product, then its share of the LDS reads and of the loads, and so on.
 template <int PRODUCTS, int READS, int LOADS, int I = 0>
 __device__ __forceinline__ void interleave() {
@@ -562,49 +573,65 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / (kStageBytes<T, PKC, QKC, A
   step<T, SP, SQ, TM, TN, false, false>(after == 1 ? lds1 : lds0, lds0, load, wm, wn, fp, fq, acc);
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the loads past the end have filled theirs while the LDS is still ours
 
-  // Lane l has, of each 32 x 32, row m = row_of(l % 32) and columns 16 h + 8 (l / 32) .. + 8 for h = 0, 1.
+  // Lane l has, of each 32 x 32, row m = row_of(l % 32) and columns 16 h + 8 (l / 32) .. + 8 for h = 0, 1.  Stored like
+  // that a line of memory would be written in as many parts as it has 32 bytes, so a wave's 32 rows and at most 64
+  // columns (gated: 64 of each half) go through its part of LDS and come out row by row, 8 columns a lane.
+  // LDS rows of 16-byte pieces, whose number is xored with the row's against bank conflicts.
+  constexpr int kOut = kGated ? TN / 64 : TN / 32, kBlock = kOut < 2 ? kOut : 2, kWidth = kBlock * 32 * (kGated ? 2 : 1);
+  static_assert(WM * WN * 32 * kWidth * 4 <= 2 * (SP::kBytes + SQ::kBytes));
+  constexpr int kHalf = (SP::kBytes + SQ::kBytes) / (32 * kWidth * 4);  // waves whose part is in lds0
+  float* const part = (float*)(wave < kHalf ? lds0 : lds1) + (wave < kHalf ? wave : wave - kHalf) * 32 * kWidth;
+  auto piece = [&](int row, int col) { return (f32x4*)(part + row * kWidth + (((col >> 2) ^ (row & (kWidth / 4 - 1) & 15)) << 2)); };
   Drop drop = e.drop;
   load_key(drop);
-  constexpr int kOut = kGated ? TN / 64 : TN / 32;
-  float* const rest = (float*)lds0;  // [BM][16]: the last columns that are no whole group, finished at the end
-  const bool ragged = e.partial == nullptr && sh.N % 8 != 0 && n0 + BO > sh.N;
-  if (ragged) meet();  // everyone has read lds0
+  meet();  // everyone has read lds0 and lds1
 #pragma unroll
   for (int i = 0; i < TM / 32; ++i) {
-    const int64_t m = m0 + wm + 32 * i + row_of(lane & 31);
-    if (m >= sh.M) continue;
 #pragma unroll
-    for (int j = 0; j < kOut; ++j)
+    for (int j0 = 0; j0 < kOut; j0 += kBlock) {
+      const int blocks = kOut - j0 < kBlock ? kOut - j0 : kBlock;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t n = n0 + (kGated ? wn / 2 : wn) + 32 * j + 16 * h + 8 * (lane >> 5);
-        if (n >= sh.N) continue;
+      for (int b = 0; b < blocks; ++b)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {  // 4 columns each
+          const int row = row_of(lane & 31), col = 32 * b + 16 * (u >> 1) + 8 * (lane >> 5) + 4 * (u & 1);
+          *piece(row, col) = f32x4{acc[j0 + b][i][4 * u], acc[j0 + b][i][4 * u + 1], acc[j0 + b][i][4 * u + 2], acc[j0 + b][i][4 * u + 3]};
+          if constexpr (kGated) {
+            const f32x16& g = acc[kOut + j0 + b][i];
+            *piece(row, kWidth / 2 + col) = f32x4{g[4 * u], g[4 * u + 1], g[4 * u + 2], g[4 * u + 3]};
+          }
+        }
+      wave_sync();
+#pragma unroll 1
+      for (int t = lane; t < 32 * 4 * blocks; t += 64) {
+        const int row = t / (4 * blocks), col = t % (4 * blocks) * 8;
+        const int64_t m = m0 + wm + 32 * i + row, n = n0 + (kGated ? wn / 2 : wn) + 32 * j0 + col;
+        if (m >= sh.M || n >= sh.N) continue;
         float v[8], g[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          v[r] = acc[j][i][8 * h + r];
-          if constexpr (kGated) g[r] = acc[kOut + j][i][8 * h + r];
+        for (int u = 0; u < 2; ++u) {
+          const f32x4 x = *piece(row, col + 4 * u);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[4 * u + r] = x[r];
+          if constexpr (kGated) {
+            const f32x4 y = *piece(row, kWidth / 2 + col + 4 * u);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) g[4 * u + r] = y[r];
+          }
         }
         if (e.partial != nullptr) {
           const int64_t width = (sh.N + 7) / 8 * 8;
           float* out = e.partial + ((int64_t)blockIdx.y * sh.M + m) * width * (kGated ? 2 : 1) + n;
           store8(out, v, true, 8);
           if constexpr (kGated) store8(out + width, g, true, 8);
-        } else if (n + 8 > sh.N) {
-          store8(rest + (m - m0) * 16, v, true, 8);
-          if constexpr (kGated) store8(rest + (m - m0) * 16 + 8, g, true, 8);
-        } else {
+        } else if (n + 8 <= sh.N) {
           finish<T, ACT, true>(e, drop, sh.M, sh.N, m, n, v, g);
+        } else {
+          finish<T, ACT, false>(e, drop, sh.M, sh.N, m, n, v, g);
         }
       }
-  }
-  if (!ragged) return;
-  __syncthreads();
-  for (int64_t m = m0 + threadIdx.x; m < m0 + BM && m < sh.M; m += kThreads) {
-    float v[8], g[8];
-    load8(v, rest + (m - m0) * 16, true, 8);
-    if constexpr (kGated) load8(g, rest + (m - m0) * 16 + 8, true, 8);
-    finish<T, ACT, false>(e, drop, sh.M, sh.N, m, sh.N / 8 * 8, v, g);
+      wave_sync();
+    }
   }
 }
 
@@ -869,8 +896,10 @@ __global__ __launch_bounds__(256) void k_join_sums(int64_t chunks, int64_t cols,
   const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
   const int64_t c = blockIdx.x * 32ll + lane;
   float s = 0.0f;
-  if (c < cols)
+  if (c < cols) {
+#pragma unroll 4
     for (int64_t i = line; i < chunks; i += 8) s += sums[i * cols + c];
+  }
   part[line][lane] = s;
   __syncthreads();
   if (line != 0 || c >= cols) return;
@@ -1077,10 +1106,14 @@ int product(Arena& ws, bool run, int64_t M, int64_t N, int64_t K, const Matrix& 
     if (cut.tile == Tile::k256x128) FF_TILED(4, 2, 64, 64);
     FF_TILED(4, 2, 32, 64);
   } else {
-    if constexpr (ACT == GF_ACT_NONE)
+    if constexpr (ACT == GF_ACT_NONE) {
       if (cut.tile == Tile::k256x160) FF_TILED(8, 1, 32, 160);
-    if (cut.tile == Tile::k256x256) FF_TILED(2, 4, 128, 64);
-    FF_TILED(2, 2, 64, 64);
+      if (cut.tile == Tile::k256x256) FF_TILED(2, 4, 128, 64);
+      FF_TILED(2, 2, 64, 64);
+    } else {  // waves of 128 columns: 64 of each half, whole lines of the output
+      if (cut.tile == Tile::k256x256) FF_TILED(4, 2, 64, 128);
+      FF_TILED(4, 1, 32, 128);
+    }
   }
 #undef FF_TILED
 }
