@@ -306,11 +306,16 @@ struct Saved {
 
   __device__ void get(int64_t row, int64_t col, float v[8], float g[8]) const {
     if constexpr (kFloat) {
-      load8(v, (const float*)p + row * ld + col, true, 8);
-      load8(g, (const float*)p + (rows + row) * ld + col, true, 8);
+#pragma unroll
+      for (int u = 0; u < 8; u += 4) {
+        const f32x4 a = __builtin_nontemporal_load((const f32x4*)((const float*)p + row * ld + col + u));
+        const f32x4 b = __builtin_nontemporal_load((const f32x4*)((const float*)p + (rows + row) * ld + col + u));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[u + j] = a[j], g[u + j] = b[j];
+      }
     } else {
-      const Vec<uint16_t, 8> a = *high(row, col), b = *high(rows + row, col);
-      const Vec<Low, 8> l = *low(row, col);
+      const Vec<uint16_t, 8> a = __builtin_nontemporal_load(high(row, col)), b = __builtin_nontemporal_load(high(rows + row, col));
+      const Vec<Low, 8> l = __builtin_nontemporal_load(low(row, col));
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[j] = __builtin_bit_cast(float, (uint32_t)a[j] << 16 | (l[j] & ((1u << kExtra) - 1)) << (16 - kExtra));
