@@ -783,15 +783,25 @@ __device__ inline void split(float x, bf16 out[3]) {
   }
 }
 
+struct PackJob {
+  int64_t rows, cols;
+  const void* x;
+  int64_t ldx;
+  void* out;
+  int64_t ld, plane;
+};
+
+// Up to two matrices in one launch: the first `blocks0` workgroups the first, the others the second.
 template <typename T>
-__global__ __launch_bounds__(256) void k_pack(int64_t rows, int64_t cols, const T* x, int64_t ldx, void* out, int64_t ld,
-                                              int64_t plane) {
-  const int64_t groups = ld / 8;
-  for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < rows * groups; t += gridDim.x * 256ll) {
+__global__ __launch_bounds__(256) void k_pack(PackJob job0, PackJob job1, unsigned blocks0) {
+  const bool second = blockIdx.x >= blocks0;
+  const PackJob a = second ? job1 : job0;
+  const int64_t groups = a.ld / 8, block = second ? blockIdx.x - blocks0 : blockIdx.x, all = (second ? gridDim.x - blocks0 : blocks0) * 256ll;
+  for (int64_t t = block * 256 + threadIdx.x; t < a.rows * groups; t += all) {
     const int64_t row = t / groups, c = t % groups * 8;
-    const int n = cols - c < 8 ? (int)(cols - c) : 8;
+    const int n = a.cols - c < 8 ? (int)(a.cols - c) : 8;
     float v[8];
-    load8(v, x + row * ldx + c, n == 8, n);
+    load8(v, (const T*)a.x + row * a.ldx + c, n == 8, n);
     if constexpr (std::is_same_v<T, float>) {
       bf16x8 o[3];
 #pragma unroll
@@ -801,19 +811,20 @@ __global__ __launch_bounds__(256) void k_pack(int64_t rows, int64_t cols, const 
         o[0][j] = s[0], o[1][j] = s[1], o[2][j] = s[2];
       }
 #pragma unroll
-      for (int i = 0; i < 3; ++i) *(bf16x8*)((bf16*)out + i * plane + row * ld + c) = o[i];
+      for (int i = 0; i < 3; ++i) *(bf16x8*)((bf16*)a.out + i * a.plane + row * a.ld + c) = o[i];
     } else {
-      store8((T*)out + row * ld + c, v, true, 8);
+      store8((T*)a.out + row * a.ld + c, v, true, 8);
     }
   }
 }
 
 // dz: the gradient of x W^T + b from dy (gated: the value's columns, then the gate's), as the products read it
 // ([rows, ld], in planes for 32 bits, zero past its columns), and its columns' sums: a workgroup takes 256 columns of dy
-// and `chunk` rows, 8 columns a thread in 8 interleaved rows, and leaves its sums in `sums` [row chunk][columns of dz].
+// and `chunk` rows, 8 columns a thread in 8 interleaved rows, and leaves its sums in `sums` [row chunk][columns of dz],
+// or, of one chunk, in dbias.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, int64_t chunk, const T* dy, int64_t lddy, void* saved,
-                                            int64_t saved_ld, void* dz, int64_t ld, int64_t plane, float* sums) {
+                                            int64_t saved_ld, void* dz, int64_t ld, int64_t plane, float* sums, T* dbias) {
   constexpr bool kGated = ACT != GF_ACT_NONE;
   constexpr int H = kGated ? 2 : 1;
   __shared__ float part[H][8][256 + 8];
@@ -877,7 +888,7 @@ __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, i
       }
     }
   }
-  if (sums == nullptr) return;
+  if (sums == nullptr && dbias == nullptr) return;
 #pragma unroll
   for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -890,7 +901,10 @@ __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, i
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += part[h][i][threadIdx.x];
-    sums[blockIdx.y * width + h * out + col] = s;
+    if (dbias != nullptr)
+      dbias[h * out + col] = (T)s;  // one chunk
+    else
+      sums[blockIdx.y * width + h * out + col] = s;
   }
 }
 
@@ -1011,20 +1025,36 @@ struct Arena {
   }
 };
 
+template <typename T>
+bool reads_in_place(const void* x, int64_t cols, int64_t ld) {
+  return !std::is_same_v<T, float> && aligned(x, ld, 2) && cols % 8 == 0;
+}
+
 #define FF_RUN if (run)  // nothing is launched while the workspace is counted
 
-// x as a product reads it: itself where it can be, else packed.
+// The matrices that have to be packed, and their launch.
+struct Packs {
+  PackJob job[2];
+  int n = 0;
+};
+
+// x as a product reads it: itself where it can be, else what `packs` is given to make.
 template <typename T>
-int operand(Arena& ws, bool run, const void* x, int64_t rows, int64_t cols, int64_t ld, hipStream_t s, Matrix* out) {
-  constexpr bool kSplit = std::is_same_v<T, float>;
-  if (!kSplit && aligned(x, ld, 2) && cols % 8 == 0) {
-    *out = {x, ld, 0, (int32_t)cols};
-    return GF_OK;
-  }
+Matrix operand(Arena& ws, Packs& packs, const void* x, int64_t rows, int64_t cols, int64_t ld) {
+  if (reads_in_place<T>(x, cols, ld)) return {x, ld, 0, (int32_t)cols};
+  constexpr int kBytes = 2 * kPlanes<T>;
   const int64_t width = round_up(cols, 8), plane = rows * width;
-  *out = {ws.take(plane * 2 * (kSplit ? 3 : 1)), width, plane, (int32_t)width};
-  FF_RUN {
-    k_pack<T><<<blocks_for(rows * width / 8), 256, 0, s>>>(rows, cols, (const T*)x, ld, (void*)out->p, width, plane);
+  void* const out = ws.take(plane * kBytes);
+  packs.job[packs.n++] = {rows, cols, x, ld, out, width, plane};
+  return {out, width, plane, (int32_t)width};
+}
+
+template <typename T>
+int pack(bool run, const Packs& packs, hipStream_t s) {
+  FF_RUN if (packs.n != 0) {
+    unsigned blocks[2] = {};
+    for (int i = 0; i < packs.n; ++i) blocks[i] = blocks_for(packs.job[i].rows * packs.job[i].ld / 8);
+    k_pack<T><<<blocks[0] + blocks[1], 256, 0, s>>>(packs.job[0], packs.job[packs.n - 1], blocks[0]);
     FF_LAUNCH_CHECK("k_pack");
   }
   return GF_OK;
@@ -1050,7 +1080,7 @@ struct TileKind {
 // (8192 x 1280 x 10240, one round: 191 us, against 208 us in 160 tiles of 256 x 256) and 0.98 us with two of 128 x 128
 // (250 us for the first: twice the bytes from L2 for each operation).  Where not all units work, those that do run faster
 // (160 tiles: 1.30 us a step): the chip is held by its power.  A round costs about 7, 7 and 3 us besides, and split
-// parts are written and read back at about 4 TB/s.  In 32 bits a step of 32 takes 2.35 us with 256 x 128 and 1.25 us with
+// parts are written and read back at about 4 TB/s, by one more launch.  In 32 bits a step of 32 takes 2.35 us with 256 x 128 and 1.25 us with
 // 128 x 128 on each unit (4096 x 4096 x 2048: 284 to 329 us and 302 to 344 us, by the operands' layouts).
 constexpr TileKind kTiles16[] = {{Tile::k256x256, 256, 256, kUnits, 1.59, 7.0}, {Tile::k256x160, 256, 160, kUnits, 1.18, 7.0}, {Tile::k128x128, 128, 128, 2 * kUnits, 0.98, 3.0}};
 constexpr TileKind kTiles32[] = {{Tile::k256x128, 256, 128, kUnits, 2.35, 7.0}, {Tile::k128x128, 128, 128, kUnits, 1.25, 4.0}};
@@ -1069,7 +1099,7 @@ Cut choose_cut(int64_t M, int64_t columns, int64_t steps, bool gated) {
       const int64_t full = tiles * splits / k.slots, rest = tiles * splits % k.slots;
       double us = full * (each + k.round);
       if (rest != 0) us += each * std::max(0.72, 0.5 + 0.5 * rest / k.slots) + k.round;
-      if (splits > 1) us += M * columns * (8.0 * splits + (F32 ? 4 : 2)) / 4e6 + 4.0;
+      if (splits > 1) us += M * columns * (8.0 * splits + (F32 ? 4 : 2)) / 4e6 + 8.0;
       if (us < least) least = us, best = {k.tile, (int32_t)splits};
     }
   }
@@ -1144,9 +1174,10 @@ int forward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
         FF_RUN return few<T, act.value>(a, e, s);
         return (int)GF_OK;
       }
-      Matrix x, w;
-      FF_CHECK(operand<T>(ws, run, a.x, a.rows, a.in_features, a.ldx, s, &x));
-      FF_CHECK(operand<T>(ws, run, a.weight, weight_rows(&a), a.in_features, a.ldw, s, &w));
+      Packs packs;
+      const Matrix x = operand<T>(ws, packs, a.x, a.rows, a.in_features, a.ldx);
+      const Matrix w = operand<T>(ws, packs, a.weight, weight_rows(&a), a.in_features, a.ldw);
+      FF_CHECK(pack<T>(run, packs, s));
       return product<T, true, true, act.value>(ws, run, a.rows, a.out_features, a.in_features, x, w, a.out_features, e, s);
     });
   });
@@ -1162,25 +1193,27 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
       const Drop drop = make_drop(a.dropout);
       const bool products = a.dx != nullptr || a.dweight != nullptr;
       Matrix dz{};
-      // linear, nothing dropped: dz is dy
-      const bool same = ACT == GF_ACT_NONE && drop.threshold == 0;
-      if (same && products) FF_CHECK(operand<T>(ws, run, a.dy, a.rows, out, a.lddy, s, &dz));
+      Packs packs;
+      // linear, nothing dropped: dz is dy, where the products can read it so
+      const bool same = ACT == GF_ACT_NONE && drop.threshold == 0 && reads_in_place<T>(a.dy, out, a.lddy);
+      if (same && products) dz = operand<T>(ws, packs, a.dy, a.rows, out, a.lddy);
       const bool make = products && !same;
       if (make) {
         dz.ld = round_up(wr, 8), dz.plane = a.rows * dz.ld, dz.width = (int32_t)dz.ld;
-        dz.p = ws.take(dz.plane * 2 * (kSplit ? 3 : 1));
+        dz.p = ws.take(dz.plane * 2 * kPlanes<T>);
       }
       if (make || a.dbias != nullptr) {
-        // rows in chunks of at least 8 until there are about 4 workgroups a compute unit
+        // rows in chunks of at least 8 until there are about 4 workgroups a compute unit; up to 64 rows in one chunk, whose
+        // sums are the bias's gradient (a launch less)
         const int64_t across = (out + 255) / 256;
-        int64_t chunks = std::max<int64_t>(std::min<int64_t>(4 * kUnits / across, a.rows / 8), 1);
+        int64_t chunks = a.rows <= 64 ? 1 : std::max<int64_t>(std::min<int64_t>(4 * kUnits / across, a.rows / 8), 1);
         const int64_t chunk = (a.rows + chunks - 1) / chunks;
         chunks = (a.rows + chunk - 1) / chunk;
-        float* sums = a.dbias != nullptr ? (float*)ws.take(chunks * wr * 4) : nullptr;
+        float* sums = a.dbias != nullptr && chunks > 1 ? (float*)ws.take(chunks * wr * 4) : nullptr;
         FF_RUN {
           k_dz<T, ACT><<<dim3((unsigned)across, (unsigned)chunks), 256, 0, s>>>(
-              drop, a.rows, out, chunk, (const T*)a.dy, a.lddy, a.saved, saved_ld(&a),
-              make ? (void*)dz.p : nullptr, dz.ld, dz.plane, sums);
+              drop, a.rows, out, chunk, (const T*)a.dy, a.lddy, a.saved, saved_ld(&a), make ? (void*)dz.p : nullptr, dz.ld, dz.plane, sums,
+              sums == nullptr ? (T*)a.dbias : nullptr);
           FF_LAUNCH_CHECK("k_dz");
           if (sums != nullptr) {
             k_join_sums<T><<<(unsigned)((wr + 31) / 32), 256, 0, s>>>(chunks, wr, sums, (T*)a.dbias);
@@ -1188,16 +1221,16 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
           }
         }
       }
+      Matrix w{}, x{};
+      if (a.dx != nullptr) w = operand<T>(ws, packs, a.weight, wr, a.in_features, a.ldw);
+      if (a.dweight != nullptr) x = operand<T>(ws, packs, a.x, a.rows, a.in_features, a.ldx);
+      FF_CHECK(pack<T>(run, packs, s));
       Epilogue e{};
       if (a.dx != nullptr) {
-        Matrix w;
-        FF_CHECK(operand<T>(ws, run, a.weight, wr, a.in_features, a.ldw, s, &w));
         e.out = a.dx;
         FF_CHECK((product<T, true, false, GF_ACT_NONE>(ws, run, a.rows, a.in_features, wr, dz, w, 0, e, s)));
       }
       if (a.dweight != nullptr) {
-        Matrix x;
-        FF_CHECK(operand<T>(ws, run, a.x, a.rows, a.in_features, a.ldx, s, &x));
         e.out = a.dweight;
         FF_CHECK((product<T, false, false, GF_ACT_NONE>(ws, run, wr, a.in_features, a.rows, dz, x, 0, e, s)));
       }
