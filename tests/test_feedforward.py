@@ -543,3 +543,32 @@ def test_adapted_block_trains_as_its_parts_do(device, dtype, batched):
         want = (value * torch.nn.functional.gelu(gate)) @ block.out.merged_weight().double().t() + block.out.bias.double()
         got = block(x)
     assert float((got.double() - want).norm() / want.norm()) < limit
+
+
+# (kind, rows, in, out): odd sizes at which the products take each of the large tiles, in each operand layout
+LARGE = [("gated", 4089, 331, 2037), ("linear", 4089, 331, 4075), ("linear", 8100, 328, 1279), ("linear", 4089, 4075, 331),
+         ("linear", 331, 4075, 4089), ("gated", 1030, 1031, 2090), ("gated", 4000, 2201, 600), ("linear", 331, 1279, 8100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("kind,rows,d,n", LARGE)
+def test_large_tiles(device, kind, rows, d, n, dtype):
+    _say("large tiles", kind, rows, d, n, dtype)
+    t = _case(device, kind, rows, d, n, dtype, seed=140)
+    _check(kind, t, dtype, p=0.1, what=f"large {kind} {rows}x{d}->{n}")
+
+
+@pytest.mark.gpu
+def test_phases_refuse_what_does_not_fit(device):
+    """The backward phase by itself: a gradient of another shape, and a gated product without what its forward keeps."""
+    _say("phases")
+    x, w = torch.zeros(4, 16, device=device), torch.zeros(8, 16, device=device)
+    want = (True, True, True)
+    with pytest.raises(RuntimeError, match="dy must have shape"):
+        ff._linear_backward(x, w, None, torch.zeros(4, 16, device=device), None, 0.0, 0, 0, want)
+    for saved in (None, torch.zeros(8, dtype=torch.uint8, device=device)):
+        with pytest.raises(RuntimeError, match="saved must be"):
+            ff._linear_backward(x, w, saved, torch.zeros(4, 4, device=device), "gelu", 0.0, 0, 0, want)
+    dx, dw, db = ff._linear_backward(x, w, None, torch.ones(4, 8, device=device), None, 0.0, 0, 0, (False, True, False))
+    assert dx is None and db is None and dw.shape == w.shape
