@@ -18,6 +18,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <type_traits>
+#include <utility>
 
 #include "../../include/gaussfield.h"
 #include "error.h"
@@ -258,6 +259,7 @@ struct Epilogue {
   int64_t saved_ld;
   float* partial;  // not NULL: sums for k_join instead of all of the above, [split][M][N (gated: 2 N), whole groups of 8]
   Drop drop;
+  float scale = 1.0f;  // of the sums of a product without activation, before everything else
 };
 
 struct Shape {
@@ -351,6 +353,9 @@ __device__ inline void finish(const Epilogue& e, const Drop& drop, int64_t M, in
                               float g[8]) {
   const int left = N - n < 8 ? (int)(N - n) : 8;
   const bool all = WHOLE || left == 8;
+  if constexpr (ACT == GF_ACT_NONE)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= e.scale;
   if (e.bias != nullptr) {
     float b[8];
     load8(b, (const T*)e.bias + n, all, left);
@@ -841,16 +846,18 @@ __global__ __launch_bounds__(256) void k_pack(PackJob job0, PackJob job1, unsign
   }
 }
 
-// dz: the gradient of x W^T + b from dy (gated: the value's columns, then the gate's; dv = d act(g), dg = d v act'(g), d
-// the masked and scaled dy).  16-bit dz is rounded to the tensors' type, because the matrix cores take it so: of the same
-// size as dx's and dW's own rounding, which makes 1.4 of one; the bias's sums take it before.  Bound by memory:
+// dz: the gradient of x W^T + b from dy.  Linear: the masked dy as it is; the scale of what is kept is left to the sums
+// (`scale` for the bias's, Epilogue::scale for the products), so that nothing is rounded here and nothing can overflow.
+// Gated: the value's columns, then the gate's; dv = d act(g), dg = d v act'(g), d the masked and scaled dy.  In 16 bits
+// they are rounded to the tensors' type, because the matrix cores take it so: of the same size as dx's and dW's own
+// rounding, which makes 1.4 of one; the bias's sums take them before.  Bound by memory:
 // 8192 x 5120 gated in bfloat16 84 us (462 MB, 5.5 TB/s).  It is written as the products read it
 // ([rows, ld], in planes for 32 bits, zero past its columns), and its columns' sums: a workgroup takes 256 columns of dy
 // and `chunk` rows, 8 columns a thread in 8 interleaved rows, and leaves its sums in `sums` [row chunk][columns of dz],
 // or, of one chunk, in dbias.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, int64_t chunk, const T* dy, int64_t lddy, void* saved,
-                                            int64_t saved_ld, void* dz, int64_t ld, int64_t plane, float* sums, T* dbias) {
+                                            int64_t saved_ld, void* dz, int64_t ld, int64_t plane, float* sums, T* dbias, float scale) {
   constexpr bool kGated = ACT != GF_ACT_NONE;
   constexpr int H = kGated ? 2 : 1;
   __shared__ float part[H][8][256 + 8];
@@ -927,6 +934,7 @@ __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, i
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += part[h][i][threadIdx.x];
+    s *= scale;
     if (dbias != nullptr)
       dbias[h * out + col] = (T)s;  // one chunk
     else
@@ -1216,7 +1224,9 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
     return with_activation(a.activation, [&](auto act) {
       constexpr int ACT = act.value;
       constexpr bool kSplit = std::is_same_v<T, float>;
-      const Drop drop = make_drop(a.dropout);
+      Drop drop = make_drop(a.dropout);
+      Epilogue e{};
+      if (ACT == GF_ACT_NONE) std::swap(drop.scale, e.scale);
       const bool products = a.dx != nullptr || a.dweight != nullptr;
       Matrix dz{};
       Packs packs;
@@ -1239,7 +1249,7 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
         FF_RUN {
           k_dz<T, ACT><<<dim3((unsigned)across, (unsigned)chunks), 256, 0, s>>>(
               drop, a.rows, out, chunk, (const T*)a.dy, a.lddy, a.saved, saved_ld(&a), make ? (void*)dz.p : nullptr, dz.ld, dz.plane, sums,
-              sums == nullptr ? (T*)a.dbias : nullptr);
+              sums == nullptr ? (T*)a.dbias : nullptr, e.scale);
           FF_LAUNCH_CHECK("k_dz");
           if (sums != nullptr) {
             k_join_sums<T><<<(unsigned)((wr + 31) / 32), 256, 0, s>>>(chunks, wr, sums, (T*)a.dbias);
@@ -1251,7 +1261,6 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
       if (a.dx != nullptr) w = operand<T>(ws, packs, a.weight, wr, a.in_features, a.ldw);
       if (a.dweight != nullptr) x = operand<T>(ws, packs, a.x, a.rows, a.in_features, a.ldx);
       FF_CHECK(pack<T>(run, packs, s));
-      Epilogue e{};
       if (a.dx != nullptr) {
         e.out = a.dx;
         FF_CHECK((product<T, true, false, GF_ACT_NONE>(ws, run, a.rows, a.in_features, wr, dz, w, 0, e, s)));

@@ -1,0 +1,118 @@
+"""How near the feed-forward operators come to their definitions as a whole, and over their types' whole range.
+
+Beside the element-by-element bounds of tests/test_feedforward.py, whose worst cases are wide: the root of the
+mean square of an output's error, against that of the output, with limits that follow from how independent
+roundings add up.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from guass_amd import feedforward as ff
+from oracle import feedforward_oracle as fo
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+ids = lambda v: str(v).replace("torch.", "") if isinstance(v, torch.dtype) else None  # noqa: E731
+RNG = dict(seed=11, offset=5)
+
+
+def _say(*what):
+    print("[gpu-test] feedforward precision", *what, flush=True)
+
+
+def _rand(device, *shape, dtype, seed, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(dtype).to(device)
+
+
+def _case(device, kind, rows, d, n, dtype, seed):
+    w_rows = 2 * n if kind == "gated" else n
+    return {"x": _rand(device, rows, d, dtype=dtype, seed=seed), "w": _rand(device, w_rows, d, dtype=dtype, seed=seed + 1, std=d**-0.5),
+            "b": _rand(device, w_rows, dtype=dtype, seed=seed + 2, std=0.3), "dy": _rand(device, rows, n, dtype=dtype, seed=seed + 3, std=0.5)}
+
+
+def _exact(kind, t, act, p):
+    """y, dx, dweight and dbias in 64 bits, where the tensors are."""
+    x, w, b, dy = (None if t[k] is None else t[k].double() for k in ("x", "w", "b", "dy"))
+    n = dy.shape[1]
+    keep = fo.keep_scale(*dy.shape, p, **RNG).to(x.device)
+    z = x @ w.t()
+    if b is not None:
+        z = z + b
+    if kind == "linear":
+        y, dz = z * keep, dy * keep
+    else:
+        a, slope = fo.activation(z[:, n:], act)
+        y = z[:, :n] * a * keep
+        dz = torch.cat((dy * keep * a, dy * keep * z[:, :n] * slope), dim=1)
+    return [y, dz @ w, dz.t() @ x] + ([] if b is None else [dz.sum(0)])
+
+
+def _run(kind, t, act, p):
+    leaves = [t[k].detach().requires_grad_(True) for k in ("x", "w", "b") if t[k] is not None]
+    if kind == "gated":
+        y = ff.gated_linear(*leaves, activation=act, p=p, **RNG)
+    else:
+        y = ff.linear_dropout_add(*leaves, p=p, **RNG)
+    return [y.detach(), *torch.autograd.grad(y, leaves, t["dy"])]
+
+
+def _rms(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+def _limits(kind, dtype, want, inner):
+    """For y, dx, dweight and dbias, each a sum of inner[i] terms.
+
+    32 bits: six products for each term leave out at most 8 2^-24 of it, and 6 n additions each round by 1/sqrt(12) of a unit of
+    the sum so far, which is at most 2^-23 of it and whose mean square is half the final one's: sqrt(6 n / 24) 2^-23.
+    16 bits: what rounding the right result once does to it (measured on the result itself), with a tenth on top, which is
+    more than what 32-bit sums add; for a gated product's dx and dweight twice that rounding, independently, because dz is
+    rounded to the tensors' type too.
+    """
+    out = []
+    for i, (v, n) in enumerate(zip(want, inner)):
+        if dtype == torch.float32:
+            out.append((8 + math.sqrt(n)) * 2.0**-24)
+        else:
+            out.append(1.1 * _rms(v.to(dtype), v) * (math.sqrt(2) if kind == "gated" and i in (1, 2) else 1))
+    return out
+
+
+def _check(device, kind, rows, d, n, dtype, act="gelu", p=0.0, seed=200, change=None):
+    t = _case(device, kind, rows, d, n, dtype, seed)
+    if change is not None:
+        t = change(t)
+    want = _exact(kind, t, act, p)
+    inner = (d, t["w"].shape[0], rows, rows)
+    for name, got, v, limit in zip(("y", "dx", "dweight", "dbias"), _run(kind, t, act, p), want, _limits(kind, dtype, want, inner)):
+        off = _rms(got, v)
+        _say(kind, (rows, d, n), ids(dtype), act, p, name, f"{off:.3e} of {limit:.3e}")
+        assert off <= limit, f"{name}: {off:.3e}, limit {limit:.3e}"
+
+
+# every tile shape of every operand layout, few rows, splits along k, odd sizes
+SIZES = [(48, 320, 264), (300, 640, 1000), (1025, 2560, 640), (4089, 331, 2037), (8100, 328, 1279), (4089, 2037, 331)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.0, 0.1])
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_linear_loses_its_outputs_rounding_only(device, size, dtype, p):
+    _check(device, "linear", *size, dtype, p=p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [40, 300])
+def test_linear_gradients_beyond_float16(device, rows):
+    """What is kept times 1 / (1 - p) passes float16's largest number, or falls among its smallest; the gradients do
+    neither."""
+    large = lambda t: dict(t, b=None, dy=(t["dy"] * 16000).clamp(-60000, 60000), w=t["w"] * 2.0**-8, x=t["x"] * 2.0**-8)  # noqa: E731
+    _check(device, "linear", rows, 72, 104, torch.float16, p=0.9, change=large)
+    small = lambda t: dict(t, b=None, dy=t["dy"] * 2.0**-18, w=t["w"] * 2.0**5, x=t["x"] * 2.0**5)  # noqa: E731
+    _check(device, "linear", rows, 72, 104, torch.float16, p=0.1, change=small)
