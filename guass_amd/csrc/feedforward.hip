@@ -6,10 +6,11 @@
 //   k_product   every other product, on the matrix cores, its epilogue fused (bias, activation, dropout, residual)
 //   k_join      adds the parts of a product that was split along k, with the same epilogue
 //   k_dz        the products' gradient from dy (dropout and activation undone) and its column sums
+//   k_peak      that gradient's largest element, for its scale (gated, float16)
 //   k_pack      32-bit operands into three bfloat16 planes, unaligned 16-bit ones into aligned rows
 //   k_join_sums the column sums' chunks
 //
-// Forward: k_few, or (k_pack,) k_product (, k_join).  Backward: k_dz (, k_join_sums) (, k_pack), k_product for dx and for
+// Forward: k_few, or (k_pack,) k_product (, k_join).  Backward: (k_peak,) k_dz (, k_join_sums) (, k_pack), k_product for dx and for
 // dW (, k_join each).  No atomics: every sum has one order, so a call's results depend on its inputs alone.
 #include <hip/hip_runtime.h>
 
@@ -260,7 +261,10 @@ struct Epilogue {
   float* partial;  // not NULL: sums for k_join instead of all of the above, [split][M][N (gated: 2 N), whole groups of 8]
   Drop drop;
   float scale = 1.0f;  // of the sums of a product without activation, before everything else
+  const float* scale_at = nullptr;  // where it is read from instead, or NULL
 };
+
+__device__ inline float scale_of(const Epilogue& e) { return e.scale_at != nullptr ? *e.scale_at : e.scale; }
 
 struct Shape {
   int64_t M, N, K;      // N: output columns (gated: the value's)
@@ -349,13 +353,13 @@ struct Saved {
 // What follows the sums: 8 consecutive columns n.. of row m (gated: the value's in v, the gate's in g).
 // WHOLE: all 8 are inside.
 template <typename T, int ACT, bool WHOLE>
-__device__ inline void finish(const Epilogue& e, const Drop& drop, int64_t M, int64_t N, int64_t m, int64_t n, float v[8],
+__device__ inline void finish(const Epilogue& e, const Drop& drop, float scale, int64_t M, int64_t N, int64_t m, int64_t n, float v[8],
                               float g[8]) {
   const int left = N - n < 8 ? (int)(N - n) : 8;
   const bool all = WHOLE || left == 8;
   if constexpr (ACT == GF_ACT_NONE)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= e.scale;
+    for (int j = 0; j < 8; ++j) v[j] *= scale;
   if (e.bias != nullptr) {
     float b[8];
     load8(b, (const T*)e.bias + n, all, left);
@@ -613,6 +617,7 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / (kStageBytes<T, PKC, QKC, A
   auto piece = [&](int row, int col) { return (f32x4*)(part + row * kWidth + (((col >> 2) ^ (row & (kWidth / 4 - 1) & 15)) << 2)); };
   Drop drop = e.drop;
   load_key(drop);
+  const float scale = scale_of(e);
   meet();  // everyone has read lds0 and lds1
 #pragma unroll
   for (int i = 0; i < TM / 32; ++i) {
@@ -654,9 +659,9 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / (kStageBytes<T, PKC, QKC, A
           store8(out, v, true, 8);
           if constexpr (kGated) store8(out + width, g, true, 8);
         } else if (n + 8 <= sh.N) {
-          finish<T, ACT, true>(e, drop, sh.M, sh.N, m, n, v, g);
+          finish<T, ACT, true>(e, drop, scale, sh.M, sh.N, m, n, v, g);
         } else {
-          finish<T, ACT, false>(e, drop, sh.M, sh.N, m, n, v, g);
+          finish<T, ACT, false>(e, drop, scale, sh.M, sh.N, m, n, v, g);
         }
       }
       wave_sync();
@@ -763,9 +768,9 @@ __global__ __launch_bounds__(1024) void k_few(int64_t M, int64_t N, int64_t K, c
     if constexpr (H == 2) g[j] = sums[0][1][m / 16][m % 16][t % 2 * 8 + j];
   }
   if (col + 8 <= N)
-    finish<T, ACT, true>(e, drop, M, N, m, col, v, g);
+    finish<T, ACT, true>(e, drop, 1.0f, M, N, m, col, v, g);
   else
-    finish<T, ACT, false>(e, drop, M, N, m, col, v, g);
+    finish<T, ACT, false>(e, drop, 1.0f, M, N, m, col, v, g);
 }
 
 // The products' parts, added in their order.
@@ -774,6 +779,7 @@ __global__ __launch_bounds__(256) void k_join(Shape sh, Epilogue e) {
   constexpr bool kGated = ACT != GF_ACT_NONE;
   Drop drop = e.drop;
   load_key(drop);
+  const float scale = scale_of(e);
   const int64_t groups = (sh.N + 7) / 8, width = groups * 8 * (kGated ? 2 : 1);
   for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < sh.M * groups; t += gridDim.x * 256ll) {
     const int64_t m = t / groups, n = t % groups * 8;
@@ -789,7 +795,7 @@ __global__ __launch_bounds__(256) void k_join(Shape sh, Epilogue e) {
         for (int j = 0; j < 8; ++j) g[j] += part[j];
       }
     }
-    finish<T, ACT, false>(e, drop, sh.M, sh.N, m, n, v, g);
+    finish<T, ACT, false>(e, drop, scale, sh.M, sh.N, m, n, v, g);
   }
 }
 
@@ -850,14 +856,90 @@ __global__ __launch_bounds__(256) void k_pack(PackJob job0, PackJob job1, unsign
 // (`scale` for the bias's, Epilogue::scale for the products), so that nothing is rounded here and nothing can overflow.
 // Gated: the value's columns, then the gate's; dv = d act(g), dg = d v act'(g), d the masked and scaled dy.  In 16 bits
 // they are rounded to the tensors' type, because the matrix cores take it so: of the same size as dx's and dW's own
-// rounding, which makes 1.4 of one; the bias's sums take them before.  Bound by memory:
-// 8192 x 5120 gated in bfloat16 84 us (462 MB, 5.5 TB/s).  It is written as the products read it
+// rounding, which makes 1.4 of one; the bias's sums take them before.
+// 8 columns from c on, of which n are the matrix's; zero past those.
+template <typename T, int ACT, int H>
+__device__ inline void make_dz(const Drop& d, int64_t rows, const T* dy, int64_t lddy, void* saved, int64_t saved_ld, int64_t row, int64_t c,
+                               int n, float (&g)[H][8]) {
+  load8(g[0], dy + row * lddy + c, n == 8, n);
+  if (d.threshold != 0) {
+    uint32_t bits[4];
+    random_block(d, (uint32_t)row, (uint32_t)(c >> 3), bits);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[0][j] = dropped(d, bits, j, g[0][j]);
+  }
+  if constexpr (H == 2) {
+    float value[8], gate[8];
+    Saved<T>{saved, rows, saved_ld}.get(row, c, value, gate);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float slope;
+      const float a = activation<ACT>(gate[j], &slope), v = g[0][j];
+      g[0][j] = j < n ? v * a : 0.0f;
+      g[1][j] = j < n ? v * value[j] * slope : 0.0f;
+    }
+  }
+}
+
+// A product of a gradient, a value and a slope leaves float16's range at either end where dx and dW do not, so a gated dz
+// in float16 is stored times a power of two that brings its largest finite element (k_peak) to [2^14, 2^15), which
+// dx's and dW's sums take back (Epilogue::scale_at).  An element keeps its 11 bits down to 2^-29 of the largest, and lies within
+// 2^-40 of that below.  That costs one pass over dy, value and gate more.
+template <typename T, int ACT>
+constexpr bool kScaledDz = std::is_same_v<T, f16> && ACT != GF_ACT_NONE;
+constexpr int kPeaks = 1024;  // workgroups, and their maxima
+
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void k_peak(Drop d, int64_t rows, int64_t out, const T* dy, int64_t lddy, void* saved, int64_t saved_ld,
+                                              float* peaks) {
+  __shared__ float part[256];
+  load_key(d);
+  const int64_t groups = (out + 7) / 8;
+  float peak = 0.0f;
+  for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < rows * groups; t += gridDim.x * 256ll) {
+    const int64_t row = t / groups, c = t % groups * 8;
+    float g[2][8];
+    make_dz<T, ACT>(d, rows, dy, lddy, saved, saved_ld, row, c, out - c < 8 ? (int)(out - c) : 8, g);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = fabsf(g[h][j]);
+        if (a < INFINITY) peak = fmaxf(peak, a);  // a NaN is not
+      }
+  }
+  part[threadIdx.x] = peak;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  peak = fmaxf(fmaxf(part[threadIdx.x], part[threadIdx.x + 64]), fmaxf(part[threadIdx.x + 128], part[threadIdx.x + 192]));
+#pragma unroll
+  for (int i = 32; i > 0; i >>= 1) peak = fmaxf(peak, __shfl_xor(peak, i));
+  if (threadIdx.x == 0) peaks[blockIdx.x] = peak;
+}
+
+// The power of two of k_peak's maxima, for the whole workgroup.
+__device__ inline float dz_factor(const float* peaks, int count) {
+  __shared__ float part[4];
+  float peak = 0.0f;
+  for (int i = threadIdx.x; i < count; i += 256) peak = fmaxf(peak, peaks[i]);
+#pragma unroll
+  for (int i = 32; i > 0; i >>= 1) peak = fmaxf(peak, __shfl_xor(peak, i));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = peak;
+  __syncthreads();
+  peak = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  if (peak == 0.0f) return 1.0f;
+  const int e = (int)(__builtin_bit_cast(uint32_t, peak) >> 23);  // peak in [2^(e - 127), 2^(e - 126))
+  return __builtin_bit_cast(float, (uint32_t)(127 + min(127 + 14 - e, 120)) << 23);
+}
+
+// dz, bound by memory: 8192 x 5120 gated in bfloat16 84 us (462 MB, 5.5 TB/s).  It is written as the products read it
 // ([rows, ld], in planes for 32 bits, zero past its columns), and its columns' sums: a workgroup takes 256 columns of dy
 // and `chunk` rows, 8 columns a thread in 8 interleaved rows, and leaves its sums in `sums` [row chunk][columns of dz],
-// or, of one chunk, in dbias.
+// or, of one chunk, in dbias.  `peaks`: k_peak's, followed by the place for the power of two's inverse (NULL: no such).
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, int64_t chunk, const T* dy, int64_t lddy, void* saved,
-                                            int64_t saved_ld, void* dz, int64_t ld, int64_t plane, float* sums, T* dbias, float scale) {
+                                            int64_t saved_ld, void* dz, int64_t ld, int64_t plane, float* sums, T* dbias, float scale,
+                                            float* peaks, int peak_count) {
   constexpr bool kGated = ACT != GF_ACT_NONE;
   constexpr int H = kGated ? 2 : 1;
   __shared__ float part[H][8][256 + 8];
@@ -865,37 +947,26 @@ __global__ __launch_bounds__(256) void k_dz(Drop d, int64_t rows, int64_t out, i
   const int lane = threadIdx.x & 31, line = threadIdx.x >> 5;
   const int64_t c = (blockIdx.x * 32ll + lane) * 8, width = H * out;
   const int n = c >= out ? 0 : out - c < 8 ? (int)(out - c) : 8;
-  float sum[H][8] = {};
+  float sum[H][8] = {}, factor = 1.0f;
+  if constexpr (kScaledDz<T, ACT>) {
+    if (peaks != nullptr) {
+      factor = dz_factor(peaks, peak_count);
+      if (blockIdx.x + blockIdx.y == 0 && threadIdx.x == 0) peaks[kPeaks] = 1.0f / factor;  // exact
+    }
+  }
   if (n > 0) {
     const int64_t end = (blockIdx.y + 1) * chunk < rows ? (blockIdx.y + 1) * chunk : rows;
     for (int64_t row = blockIdx.y * chunk + line; row < end; row += 8) {
       float g[H][8];
-      load8(g[0], dy + row * lddy + c, n == 8, n);
-      if (d.threshold != 0) {
-        uint32_t bits[4];
-        random_block(d, (uint32_t)row, (uint32_t)(c >> 3), bits);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[0][j] = dropped(d, bits, j, g[0][j]);
-      }
-      if constexpr (kGated) {
-        float value[8], gate[8];
-        Saved<T>{saved, rows, saved_ld}.get(row, c, value, gate);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float slope;
-          const float a = activation<ACT>(gate[j], &slope), v = g[0][j];
-          g[0][j] = v * a;
-          g[1][j] = v * value[j] * slope;
-        }
-      }
+      make_dz<T, ACT>(d, rows, dy, lddy, saved, saved_ld, row, c, n, g);
 #pragma unroll
       for (int h = 0; h < H; ++h) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j >= n) g[h][j] = 0.0f;
-          sum[h][j] += g[h][j];
-        }
+        for (int j = 0; j < 8; ++j) sum[h][j] += g[h][j];
         if (dz == nullptr) continue;
+        if constexpr (kScaledDz<T, ACT>)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[h][j] *= factor;
         // the last columns' store also clears what follows them, up to ld
         const int64_t at = row * ld + h * out + c;
         const bool last = h == H - 1 && c + 8 >= out;
@@ -1245,11 +1316,23 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
         int64_t chunks = a.rows <= 64 ? 1 : std::max<int64_t>(std::min<int64_t>(4 * kUnits / across, a.rows / 8), 1);
         const int64_t chunk = (a.rows + chunks - 1) / chunks;
         chunks = (a.rows + chunk - 1) / chunk;
+        float* peaks = nullptr;
+        const int peak_blocks = (int)std::min<int64_t>((a.rows * ((out + 7) / 8) + 255) / 256, kPeaks);
+        if (kScaledDz<T, ACT> && make) {
+          peaks = (float*)ws.take((kPeaks + 1) * 4);
+          FF_RUN e.scale_at = peaks + kPeaks;
+        }
         float* sums = a.dbias != nullptr && chunks > 1 ? (float*)ws.take(chunks * wr * 4) : nullptr;
         FF_RUN {
+          if constexpr (kScaledDz<T, ACT>) {
+            if (make) {
+              k_peak<T, ACT><<<peak_blocks, 256, 0, s>>>(drop, a.rows, out, (const T*)a.dy, a.lddy, a.saved, saved_ld(&a), peaks);
+              FF_LAUNCH_CHECK("k_peak");
+            }
+          }
           k_dz<T, ACT><<<dim3((unsigned)across, (unsigned)chunks), 256, 0, s>>>(
               drop, a.rows, out, chunk, (const T*)a.dy, a.lddy, a.saved, saved_ld(&a), make ? (void*)dz.p : nullptr, dz.ld, dz.plane, sums,
-              sums == nullptr ? (T*)a.dbias : nullptr, e.scale);
+              sums == nullptr ? (T*)a.dbias : nullptr, e.scale, peaks, peak_blocks);
           FF_LAUNCH_CHECK("k_dz");
           if (sums != nullptr) {
             k_join_sums<T><<<(unsigned)((wr + 31) / 32), 256, 0, s>>>(chunks, wr, sums, (T*)a.dbias);

@@ -116,3 +116,46 @@ def test_linear_gradients_beyond_float16(device, rows):
     _check(device, "linear", rows, 72, 104, torch.float16, p=0.9, change=large)
     small = lambda t: dict(t, b=None, dy=t["dy"] * 2.0**-18, w=t["w"] * 2.0**5, x=t["x"] * 2.0**5)  # noqa: E731
     _check(device, "linear", rows, 72, 104, torch.float16, p=0.1, change=small)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("act", ff.ACTIVATIONS)
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_gated_loses_its_outputs_rounding_and_the_gradients(device, size, act, dtype):
+    _check(device, "gated", *size, dtype, act=act, p=0.1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [40, 300])
+def test_gated_gradients_beyond_float16(device, rows):
+    """dy times the value passes float16's largest number (values near 1000), or falls among its smallest; dx and dweight do
+    neither.  A NaN and an infinity in one row of dy leave the others' dx as it was."""
+    def large(t):
+        n = t["dy"].shape[1]
+        b = t["b"].clone()
+        b[:n] = 1000.0
+        return dict(t, b=b, dy=t["dy"] * 300, w=t["w"] * 2.0**-8, x=t["x"] * 2.0**-8)
+
+    t = large(_case(device, "gated", rows, 72, 104, torch.float16, 200))
+    n = t["dy"].shape[1]
+    want = _exact("gated", t, "gelu", 0.1)
+    assert float((t["dy"].double() * 1000).abs().max()) > 65504
+    got = _run("gated", t, "gelu", 0.1)
+    limits = _limits("gated", torch.float16, want, (72, 2 * n, rows, rows))
+    for i in range(3):  # dbias passes the range by itself
+        assert _rms(got[i], want[i]) <= limits[i]
+
+    small = lambda t: dict(t, b=t["b"] * 0, dy=t["dy"] * 2.0**-16, w=t["w"] * 2.0**2, x=t["x"] * 2.0**-5)  # noqa: E731
+    t = small(_case(device, "gated", rows, 72, 104, torch.float16, 200))
+    want = _exact("gated", t, "gelu", 0.1)
+    got = _run("gated", t, "gelu", 0.1)
+    limits = _limits("gated", torch.float16, want, (72, 2 * n, rows, rows))
+    for i in range(4):
+        assert _rms(got[i], want[i]) <= limits[i]
+
+    t = large(_case(device, "gated", rows, 72, 104, torch.float16, 200))
+    t["dy"][3, 5], t["dy"][7, 6] = math.nan, math.inf
+    dx = _run("gated", t, "gelu", 0.0)[1]
+    fine = torch.isfinite(dx).all(dim=1).cpu()
+    assert not fine[3] and not fine[7] and int(fine.sum()) == rows - 2
