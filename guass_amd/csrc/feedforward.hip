@@ -120,10 +120,11 @@ __device__ inline void random_block(const Drop& d, uint32_t row, uint32_t group,
   out[0] = c0, out[1] = c1, out[2] = c2, out[3] = c3;
 }
 
-__device__ inline float dropped(const Drop& d, const uint32_t bits[4], int j, float v) {
-  const uint32_t h = (bits[j >> 1] >> (16 * (j & 1))) & 0xffffu;
-  return h >= d.threshold ? v * d.scale : 0.0f;
+__device__ inline bool kept(const Drop& d, const uint32_t bits[4], int j) {
+  return ((bits[j >> 1] >> (16 * (j & 1))) & 0xffffu) >= d.threshold;
 }
+
+__device__ inline float dropped(const Drop& d, const uint32_t bits[4], int j, float v) { return kept(d, bits, j) ? v * d.scale : 0.0f; }
 
 // residual + drop(x), 8 elements of a row a thread and turn.  A thread's next group is a fixed number of groups on, whole
 // rows and a rest of columns, so that nothing is divided in the loop.  Bound by memory: 32768 x 2560 bfloat16 60 us a pass
@@ -856,17 +857,21 @@ __global__ __launch_bounds__(256) void k_pack(PackJob job0, PackJob job1, unsign
 // (`scale` for the bias's, Epilogue::scale for the products), so that nothing is rounded here and nothing can overflow.
 // Gated: the value's columns, then the gate's; dv = d act(g), dg = d v act'(g), d the masked and scaled dy.  In 16 bits
 // they are rounded to the tensors' type, because the matrix cores take it so: of the same size as dx's and dW's own
-// rounding, which makes 1.4 of one; the bias's sums take them before.
+// rounding, which makes 1.4 of one; the bias's sums take them before.  A dropped place's are zero whatever its value and
+// gate are: the output there is 0, not 0 times them.
 // 8 columns from c on, of which n are the matrix's; zero past those.
 template <typename T, int ACT, int H>
 __device__ inline void make_dz(const Drop& d, int64_t rows, const T* dy, int64_t lddy, void* saved, int64_t saved_ld, int64_t row, int64_t c,
                                int n, float (&g)[H][8]) {
   load8(g[0], dy + row * lddy + c, n == 8, n);
+  bool there[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) there[j] = j < n;
   if (d.threshold != 0) {
     uint32_t bits[4];
     random_block(d, (uint32_t)row, (uint32_t)(c >> 3), bits);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) g[0][j] = dropped(d, bits, j, g[0][j]);
+    for (int j = 0; j < 8; ++j) there[j] = there[j] && kept(d, bits, j), g[0][j] = there[j] ? g[0][j] * d.scale : 0.0f;
   }
   if constexpr (H == 2) {
     float value[8], gate[8];
@@ -875,8 +880,8 @@ __device__ inline void make_dz(const Drop& d, int64_t rows, const T* dy, int64_t
     for (int j = 0; j < 8; ++j) {
       float slope;
       const float a = activation<ACT>(gate[j], &slope), v = g[0][j];
-      g[0][j] = j < n ? v * a : 0.0f;
-      g[1][j] = j < n ? v * value[j] * slope : 0.0f;
+      g[0][j] = there[j] ? v * a : 0.0f;
+      g[1][j] = there[j] ? v * value[j] * slope : 0.0f;
     }
   }
 }

@@ -159,3 +159,26 @@ def test_gated_gradients_beyond_float16(device, rows):
     dx = _run("gated", t, "gelu", 0.0)[1]
     fine = torch.isfinite(dx).all(dim=1).cpu()
     assert not fine[3] and not fine[7] and int(fine.sum()) == rows - 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [4, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+def test_dropped_places_give_no_gradient_whatever_they_were(device, dtype, rows):
+    """A place whose value and gate overflow to infinities, dropped: its output is 0, and so are its gradients."""
+    d, n = 8, 16
+    keep = fo.keep_scale(rows, n, 0.5, **RNG) != 0
+    row, col = (int(v) for v in (~keep).nonzero()[0])
+    x, w = _rand(device, rows, d, dtype=dtype, seed=1), _rand(device, 2 * n, d, dtype=dtype, seed=2)
+    x[:, 0] = 0
+    w[:, 0] = 0
+    x[row, 0], w[col, 0], w[n + col, 0] = 1e20, 1e20, 1e20
+    t = {"x": x, "w": w, "b": torch.zeros(2 * n, dtype=dtype, device=device), "dy": torch.ones(rows, n, dtype=dtype, device=device)}
+    calm = dict(t, w=w.clone())
+    calm["w"][col, 0] = calm["w"][n + col, 0] = 0
+    got, want = _run("gated", t, "gelu", 0.5), _run("gated", calm, "gelu", 0.5)
+    got[1], want[1] = got[1].clone(), want[1].clone()
+    assert bool((got[1][row, 0] == 0).all())
+    got[1][:, 0] = want[1][:, 0] = 0  # the other rows' dx there goes by the weight that was taken out
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
