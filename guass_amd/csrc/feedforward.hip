@@ -805,16 +805,20 @@ __global__ __launch_bounds__(256) void k_join(Shape sh, Epilogue e) {
 // rows are not whole, aligned groups of 16 bytes into rows that are.  Columns past the matrix become zero.  Bound by
 // memory: 4096 x 640 and 5120 x 640 of 32 bits 12 us (59 MB, 4.9 TB/s).
 
-// x = its 3 x 8 leading bits, by truncation: x - a0 and x - a0 - a1 are exact.  An infinity or a NaN stays in a0, and a
-// product with it becomes a NaN where the other operand's later planes are zero: what is not finite stays so, but an
-// infinity may come out as a NaN.
+// x = its 3 x 8 leading bits, by truncation: x - a0 and x - a0 - a1 are exact.  All have x's sign.  An infinity or a NaN
+// stays in a0.  Planes that would be zero hold the smallest normal number instead, of x's sign, unless x is below 2^-100: an
+// infinity times 0 would be a NaN where the product is infinite.  That adds 2^-25 of x at most.
 __device__ inline void split(float x, bf16 out[3]) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, x), size = bits & 0x7fffffffu;
+  const uint32_t least = size >= 0x0d800000u ? (bits & 0x80000000u) | 0x00800000u : 0u;
+  const bool finite = size < 0x7f800000u;
+  out[0] = __builtin_bit_cast(bf16, (uint16_t)((size > 0x7f800000u ? bits | 0x10000u : bits) >> 16));
+  float left = finite ? x - __builtin_bit_cast(float, bits & 0xffff0000u) : 0.0f;
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    const uint32_t top = __builtin_bit_cast(uint32_t, x) & 0xffff0000u;
-    const bool finite = (top & 0x7f800000u) != 0x7f800000u;
-    out[i] = __builtin_bit_cast(bf16, (uint16_t)((__builtin_bit_cast(uint32_t, x) | (finite ? 0u : (__builtin_bit_cast(uint32_t, x) & 0xffffu) ? 0x10000u : 0u)) >> 16));
-    x = finite ? x - __builtin_bit_cast(float, top) : 0.0f;
+  for (int i = 1; i < 3; ++i) {
+    const uint32_t top = __builtin_bit_cast(uint32_t, left) & 0xffff0000u;
+    out[i] = __builtin_bit_cast(bf16, (uint16_t)((left == 0.0f ? least : top) >> 16));
+    left -= __builtin_bit_cast(float, top);
   }
 }
 

@@ -11,8 +11,8 @@ Types: float32, bfloat16 and float16, one type for all of a call's tensors; sums
 bits.  Every call runs on torch's current stream of its tensors' device and does not synchronise.  A
 matrix whose last dimension is contiguous is read in place whatever its row stride is; others are copied.
 float32 products go through the matrix cores as three bfloat16 planes of each operand (errors as of float32
-sums; an infinity among the inputs makes what it reaches not finite, possibly NaN); of at most 64 rows the
-forward multiplies float32 as such.
+sums; an infinity times a number below 2^-100 may be a NaN); of at most 64 rows the forward multiplies
+float32 as such.
 
 Dropout draws from a counter-based generator, Philox4x32-10, keyed by ``seed``: element (row, col) takes 16
 bits of the block at counter (col // 8, row, ``offset``), the output seen as a matrix of its last dimension's

@@ -182,3 +182,24 @@ def test_dropped_places_give_no_gradient_whatever_they_were(device, dtype, rows)
     got[1][:, 0] = want[1][:, 0] = 0  # the other rows' dx there goes by the weight that was taken out
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows", [40, 200])
+def test_infinities_come_out_as_the_sums_have_them(device, dtype, rows):
+    """An infinity in x, in dy or in the weight makes infinities of its products' signs, and a NaN where it meets a zero,
+    in every type and at every number of rows.  The numbers that it meets have few bits (0.5, -1) and many (0.1)."""
+    d, n = 96, 64
+    t = _case(device, "linear", rows, d, n, dtype, 210)
+    t["x"][3, 17], t["x"][4, 17] = math.inf, -math.inf
+    t["w"][5, 17], t["w"][6, 17], t["w"][7, 17], t["w"][8, 17], t["w"][9, 18] = 0.0, 0.5, -1.0, 0.1, -math.inf
+    t["x"][10, 18], t["x"][11, 18], t["x"][12, 18] = 1.0, 0.0, -0.25
+    t["dy"][3, 20], t["dy"][4, 21], t["dy"][14, 9], t["dy"][15, 9] = 1.0, 0.0, 0.0, 2.0
+    t["dy"][16, 30] = math.inf
+    t["x"][16, 40], t["w"][30, 40] = -0.5, 2.0
+    for name, got, want in zip(("y", "dx", "dweight", "dbias"), _run("linear", t, None, 0.0), _exact("linear", t, None, 0.0)):
+        assert bool(torch.isinf(want).any()), name
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), name
+        assert torch.equal(torch.isinf(got), torch.isinf(want)), name
+        assert torch.equal(torch.sign(got[torch.isinf(want)]).double(), torch.sign(want[torch.isinf(want)])), name
