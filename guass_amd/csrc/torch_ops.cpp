@@ -3,6 +3,7 @@
 // backward runs on autograd's own thread, where the same work in Python took 40 us more (64 x 1280 dropout, forward and
 // backward: 96 us from Python, 48 us of them autograd's own).
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -123,6 +124,14 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
 bool wants(const Tensor& t) { return t.requires_grad(); }
 bool wants(const MaybeTensor& t) { return present(t) && t->requires_grad(); }
 
+// There is no forward-mode derivative: a tangent must not get lost, whether or not gradients are wanted too.
+template <typename... M>
+void check_no_tangent(const char* name, const Tensor& x, const M&... others) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  const bool tangent = x._fw_grad(0).defined() || (... || (present(others) && others->_fw_grad(0).defined()));
+  TORCH_CHECK_NOT_IMPLEMENTED(!tangent, name, " has no forward-mode derivative");
+}
+
 Tensor dropout_add(const Tensor& x, const MaybeTensor& residual, double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
   check_first(x);
   if (present(residual)) {
@@ -130,6 +139,7 @@ Tensor dropout_add(const Tensor& x, const MaybeTensor& residual, double p, int64
     TORCH_CHECK(residual->sizes() == x.sizes(), "residual must have x's shape ", x.sizes(), " (got ", residual->sizes(), ")");
   }
   check_seed(seed_tensor, x);
+  check_no_tangent("dropout_add", x, residual);
   if (at::GradMode::is_enabled() && (wants(x) || wants(residual))) return DropoutAdd::apply(x, residual, p, seed, seed_tensor, offset);
   return dropout_kernel(x, residual, make_dropout(p, seed, seed_tensor, offset));
 }
@@ -249,6 +259,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, co
               int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
   check_linear(x, weight, bias, residual, activation);
   check_seed(seed_tensor, x);
+  check_no_tangent(activation == GF_ACT_NONE ? "linear_dropout_add" : "gated_linear", x, MaybeTensor(weight), bias, residual);
   if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias) || wants(residual)))
     return Linear::apply(x, weight, bias, residual, activation, p, seed, seed_tensor, offset);
   return std::get<0>(linear_forward(x, weight, bias, residual, activation, make_dropout(p, seed, seed_tensor, offset), false));

@@ -1,0 +1,55 @@
+"""How the feed-forward operators take part in torch: derivatives that they do not have, gradients that nobody asks
+for, autocast, tracing.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from guass_amd import feedforward as ff
+
+
+def _say(*what):
+    print("[gpu-test] feedforward autograd", *what, flush=True)
+
+
+def _rand(device, *shape, dtype=torch.float32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).to(dtype).to(device)
+
+
+def _inputs(device, rows=4, d=8, n=16, dtype=torch.float32):
+    """x, a weight of 2 n rows, a bias of as many, a residual of the linear product's width."""
+    return {"x": _rand(device, rows, d, dtype=dtype, seed=1), "w": _rand(device, 2 * n, d, dtype=dtype, seed=2),
+            "b": _rand(device, 2 * n, dtype=dtype, seed=3), "r": _rand(device, rows, 2 * n, dtype=dtype, seed=4)}
+
+
+CALLS = {
+    "dropout_add": (lambda t: ff.dropout_add(t["x"], t["x2"], p=0.1, seed=1), ("x", "x2")),
+    "gated_linear": (lambda t: ff.gated_linear(t["x"], t["w"], t["b"], p=0.1, seed=1), ("x", "w", "b")),
+    "linear_dropout_add": (lambda t: ff.linear_dropout_add(t["x"], t["w"], t["b"], t["r"], p=0.1, seed=1), ("x", "w", "b", "r")),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", CALLS)
+def test_forward_mode_raises(device, op):
+    """A tangent on any input is refused, with gradients wanted, not wanted and switched off; not where forward mode is
+    switched off."""
+    _say("forward mode", op)
+    call, names = CALLS[op]
+    t = _inputs(device)
+    t["x2"] = t["x"].clone()
+    plain = call(t)
+    for name in names:
+        for grad in (False, True):
+            with fwd.dual_level():
+                dual = fwd.make_dual(t[name].clone().requires_grad_(grad), torch.ones_like(t[name]))
+                with pytest.raises(NotImplementedError, match=f"{op} has no forward-mode derivative"):
+                    call({**t, name: dual})
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call({**t, name: dual})
+                with fwd._set_fwd_grad_enabled(False):
+                    assert torch.equal(call({**t, name: dual}), plain)
