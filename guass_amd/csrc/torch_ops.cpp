@@ -248,7 +248,8 @@ struct Linear : torch::autograd::Function<Linear> {
     const auto [wx, ww, wb, wr] = ctx->saved_data["wants"].to<std::tuple<bool, bool, bool, bool>>();
     const auto saved = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
-    const bool again = dy.requires_grad() || saved[0].requires_grad() || saved[1].requires_grad();
+    // what the gradients depend on: a gated product's on the bias too, by value and gate
+    const bool again = dy.requires_grad() || saved[0].requires_grad() || saved[1].requires_grad() || (activation != GF_ACT_NONE && wb);
     auto [dx, dw, db] = linear_backward(saved[0], saved[1], saved[2], dy, activation, make_dropout(p, seed, saved[3], offset), wx, ww, wb);
     return once({dx, dw, db, wr ? dy : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()},
                 activation == GF_ACT_NONE ? "linear_dropout_add" : "gated_linear", again);

@@ -53,3 +53,30 @@ def test_forward_mode_raises(device, op):
                     call({**t, name: dual})
                 with fwd._set_fwd_grad_enabled(False):
                     assert torch.equal(call({**t, name: dual}), plain)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op,names", [
+    ("dropout_add", ("x",)), ("linear_dropout_add", ("x", "w")), ("gated_linear", ("x",)), ("gated_linear", ("w",)),
+    ("gated_linear", ("b",))])
+def test_a_second_derivative_raises(device, op, names):
+    """A gradient taken with a graph refuses to be differentiated, also where it depends on the bias alone."""
+    _say("second derivative", op, names)
+    t = _inputs(device)
+    t["x2"] = None
+    leaves = [t[n].requires_grad_(True) for n in names]
+    y = CALLS[op][0](t)
+    dy = torch.ones_like(y).requires_grad_(op == "dropout_add")
+    grad = torch.autograd.grad(y, leaves, dy, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match=f"{op} is differentiable once only"):
+        (grad**2).sum().backward()
+
+
+@pytest.mark.gpu
+def test_a_linear_bias_gradient_has_no_second_derivative(device):
+    """The linear product's bias gradient is a sum of dy: nothing of it depends on an input, and nothing raises."""
+    t = _inputs(device)
+    t["b"].requires_grad_(True)
+    y = ff.linear_dropout_add(t["x"], t["w"], t["b"])
+    grad, = torch.autograd.grad(y.sum(), t["b"], create_graph=True)
+    assert not grad.requires_grad and bool((grad == 4).all())
