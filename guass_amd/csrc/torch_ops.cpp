@@ -105,13 +105,13 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& residual, double p, int64_t seed,
                         const MaybeTensor& seed_tensor, int64_t offset) {
     ctx->saved_data["rng"] = std::make_tuple(p, seed, offset);
-    ctx->saved_data["wants"] = std::make_tuple(x.requires_grad(), present(residual) && residual->requires_grad());
+    ctx->saved_data["residual"] = present(residual);
     if (present(seed_tensor)) ctx->save_for_backward({*seed_tensor});
     return dropout_kernel(x, residual, make_dropout(p, seed, seed_tensor, offset));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto [p, seed, offset] = ctx->saved_data["rng"].to<std::tuple<double, int64_t, int64_t>>();
-    const auto [want_x, want_r] = ctx->saved_data["wants"].to<std::tuple<bool, bool>>();
+    const bool want_x = ctx->needs_input_grad(0), want_r = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1);
     const auto saved = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
     const bool again = dy.requires_grad();
@@ -236,20 +236,23 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x, const Tensor
 struct Linear : torch::autograd::Function<Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual,
                         int64_t activation, double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
-    const bool wx = wants(x), ww = wants(weight), wb = wants(bias);
-    auto [y, saved] = linear_forward(x, weight, bias, residual, activation, make_dropout(p, seed, seed_tensor, offset), wx || ww || wb);
+    const bool save = wants(x) || wants(weight) || wants(bias);
+    auto [y, saved] = linear_forward(x, weight, bias, residual, activation, make_dropout(p, seed, seed_tensor, offset), save);
     ctx->save_for_backward({x, weight, saved, present(seed_tensor) ? *seed_tensor : Tensor()});
     ctx->saved_data["call"] = std::make_tuple(activation, p, seed, offset);
-    ctx->saved_data["wants"] = std::make_tuple(wx, ww, wb, wants(residual));
+    ctx->saved_data["inputs"] = std::make_tuple(present(bias), present(residual), wants(bias));
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto [activation, p, seed, offset] = ctx->saved_data["call"].to<std::tuple<int64_t, double, int64_t, int64_t>>();
-    const auto [wx, ww, wb, wr] = ctx->saved_data["wants"].to<std::tuple<bool, bool, bool, bool>>();
+    const auto [has_bias, has_residual, trains_bias] = ctx->saved_data["inputs"].to<std::tuple<bool, bool, bool>>();
+    // what this backward is for: of the inputs that train, those that it was asked for (edges are the tensors that are there)
+    const bool wx = ctx->needs_input_grad(0), ww = ctx->needs_input_grad(1), wb = has_bias && ctx->needs_input_grad(2),
+               wr = has_residual && ctx->needs_input_grad(2 + has_bias);
     const auto saved = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
     // what the gradients depend on: a gated product's on the bias too, by value and gate
-    const bool again = dy.requires_grad() || saved[0].requires_grad() || saved[1].requires_grad() || (activation != GF_ACT_NONE && wb);
+    const bool again = dy.requires_grad() || saved[0].requires_grad() || saved[1].requires_grad() || (activation != GF_ACT_NONE && trains_bias);
     auto [dx, dw, db] = linear_backward(saved[0], saved[1], saved[2], dy, activation, make_dropout(p, seed, saved[3], offset), wx, ww, wb);
     return once({dx, dw, db, wr ? dy : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()},
                 activation == GF_ACT_NONE ? "linear_dropout_add" : "gated_linear", again);

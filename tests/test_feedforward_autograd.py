@@ -80,3 +80,40 @@ def test_a_linear_bias_gradient_has_no_second_derivative(device):
     y = ff.linear_dropout_add(t["x"], t["w"], t["b"])
     grad, = torch.autograd.grad(y.sum(), t["b"], create_graph=True)
     assert not grad.requires_grad and bool((grad == 4).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_bias", [True, False])
+@pytest.mark.parametrize("op", CALLS)
+def test_gradients_asked_for_are_the_full_ones(device, op, with_bias):
+    """Every input alone, all of them training: the gradient that a full backward gives, with and without a bias."""
+    _say("asked for", op, with_bias)
+    call, names = CALLS[op]
+    t = _inputs(device)
+    t["x2"] = t["x"].clone()
+    if not with_bias:
+        t["b"] = None
+        names = [n for n in names if n != "b"]
+    leaves = {n: t[n].requires_grad_(True) for n in names}
+    y = call(t)
+    dy = _rand(device, *y.shape, seed=9)
+    full = torch.autograd.grad(y, list(leaves.values()), dy, retain_graph=True)
+    for (name, leaf), want in zip(leaves.items(), full):
+        got, = torch.autograd.grad(y, leaf, dy, retain_graph=True)
+        assert torch.equal(got, want), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["gated_linear", "linear_dropout_add"])
+def test_gradients_not_asked_for_are_not_computed(device, op):
+    """dx alone of a weight that trains too: the backward takes less memory than dweight would."""
+    _say("not asked for", op)
+    x, w = _rand(device, 65, 4096, dtype=torch.bfloat16), torch.zeros(16384, 4096, dtype=torch.bfloat16, device=device)
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = ff.gated_linear(x, w) if op == "gated_linear" else ff.linear_dropout_add(x, w)
+    dy = torch.ones_like(y)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    torch.autograd.grad(y, x, dy)
+    assert torch.cuda.max_memory_allocated() - before < w.numel() * w.element_size()
