@@ -254,8 +254,10 @@ class GaussianLinear(nn.Linear):
 
     def forward(self, input: Tensor) -> Tensor:
         pending = self._batched_delta
-        if self.adapter_config.delta_apply == "merged" or (pending is not None and pending[2] == "merged_weight"):
+        if pending is not None and pending[2] == "merged_weight":
             return F.linear(input, self.merged_weight(), self._parameters["bias"])
+        if self.adapter_config.delta_apply == "merged":
+            return F.linear(input, self.merged_weight(), self.bias)
         delta_weight = self.compute_delta_weight().to(dtype=self.weight.dtype)
         base = F.linear(input, self.weight, self.bias)
         chunk = self._delta_apply_row_chunk()

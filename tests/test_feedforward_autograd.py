@@ -117,3 +117,22 @@ def test_gradients_not_asked_for_are_not_computed(device, op):
     before = torch.cuda.memory_allocated()
     torch.autograd.grad(y, x, dy)
     assert torch.cuda.max_memory_allocated() - before < w.numel() * w.element_size()
+
+
+def test_merged_layer_takes_a_parametrized_bias():
+    """GaussianLinear's merged forward reads the bias as an attribute: a parametrization or an override makes it."""
+    from torch.nn.utils import parametrize
+
+    from guass_amd.layers import GaussianAdapterConfig, GaussianLinear
+
+    class Twice(torch.nn.Module):
+        def forward(self, v):
+            return 2 * v
+
+    layer = GaussianLinear(8, 6, adapter_config=GaussianAdapterConfig(init_num_gaussians=4, delta_apply="merged"))
+    layer.compute_delta_weight = lambda: torch.ones(6, 8)  # the render needs a GPU
+    layer.last_forward_metadata = {}
+    bias = layer.bias.detach().clone()
+    parametrize.register_parametrization(layer, "bias", Twice())
+    x = torch.randn(3, 8)
+    assert torch.equal(layer(x), torch.nn.functional.linear(x, layer.weight + 1, 2 * bias))
