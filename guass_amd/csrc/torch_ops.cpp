@@ -3,6 +3,7 @@
 // backward runs on autograd's own thread, where the same work in Python took 40 us more (64 x 1280 dropout, forward and
 // backward: 96 us from Python, 48 us of them autograd's own).
 #include <ATen/ATen.h>
+#include <ATen/autocast_mode.h>
 #include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -269,7 +270,34 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, co
   return std::get<0>(linear_forward(x, weight, bias, residual, activation, make_dropout(p, seed, seed_tensor, offset), false));
 }
 
+// ------------------------------------------------------------------------------ autocast
+
+// As torch's linear: the operands in autocast's type.  A residual of that type is added by the kernels; another one after them,
+// by torch's rules (a float32 residual stream stays one).
+Tensor linear_autocast(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual, int64_t activation,
+                       double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
+  const c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::Autocast);
+  const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
+  auto cast = [&](const Tensor& t) { return at::autocast::cached_cast(type, t, at::kCUDA); };
+  const bool fused = !present(residual) || residual->scalar_type() == type;
+  const Tensor y = linear(cast(x), cast(weight), present(bias) ? MaybeTensor(cast(*bias)) : bias, fused ? residual : MaybeTensor(), activation, p,
+                          seed, seed_tensor, offset);
+  return fused ? y : *residual + y;
+}
+
+// As torch's dropout: in x's own type, and the sum by torch's rules where the residual's is another.
+Tensor dropout_add_autocast(const Tensor& x, const MaybeTensor& residual, double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
+  const c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::Autocast);
+  if (!present(residual) || residual->scalar_type() == x.scalar_type()) return dropout_add(x, residual, p, seed, seed_tensor, offset);
+  return *residual + dropout_add(x, std::nullopt, p, seed, seed_tensor, offset);
+}
+
 }  // namespace
+
+TORCH_LIBRARY_IMPL(guass_amd, Autocast, m) {
+  m.impl("dropout_add", dropout_add_autocast);
+  m.impl("linear", linear_autocast);
+}
 
 TORCH_LIBRARY(guass_amd, m) {
   m.def("dropout_add(Tensor x, Tensor? residual, float p, int seed, Tensor? seed_tensor, int offset) -> Tensor", dropout_add);

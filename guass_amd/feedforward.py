@@ -7,8 +7,8 @@
 each with its gradients.  W may be what an adapted layer renders (weight + delta-W): its gradient is then
 the field's dL/d(delta-W), and ``guass_amd.layers.GaussianFeedForward`` runs the three that way.
 
-Types: float32, bfloat16 and float16, one type for all of a call's tensors; sums are accumulated in 32
-bits.  Every call runs on torch's current stream of its tensors' device and does not synchronise.  A
+Types: float32, bfloat16 and float16, one type for all of a call's tensors (under ``torch.autocast`` the products
+take its type, and a residual of another type is added by torch's rules); sums are accumulated in 32 bits.  Every call runs on torch's current stream of its tensors' device and does not synchronise.  A
 matrix whose last dimension is contiguous is read in place whatever its row stride is; others are copied.
 float32 products go through the matrix cores as three bfloat16 planes of each operand (errors as of float32
 sums; an infinity times a number below 2^-100 may be a NaN); of at most 64 rows the forward multiplies

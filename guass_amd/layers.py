@@ -277,6 +277,8 @@ class GaussianFeedForward(nn.Module):
     reference's target model): residual + out_dropout(out(dropout(value * act(gate)))), (value, gate) the two halves
     of proj(x).  Both layers' weights are taken merged (from GaussianFieldBatch's render where that ran, else rendered
     here) by the kernels of guass_amd.feedforward; nothing of the inner width is kept but what the backward reads.
+    Autocast reaches the products as it reaches nn.Linear's.  The layers' own forward is not called, so neither are hooks
+    on it.
 
     In training mode ``forward`` needs a ``seed`` where something is dropped: an int, or an int64 tensor on the device that
     a captured graph can be given anew.  The two dropouts draw at counters 2 ``offset`` and 2 ``offset`` + 1, so give

@@ -136,3 +136,63 @@ def test_merged_layer_takes_a_parametrized_bias():
     parametrize.register_parametrization(layer, "bias", Twice())
     x = torch.randn(3, 8)
     assert torch.equal(layer(x), torch.nn.functional.linear(x, layer.weight + 1, 2 * bias))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16], ids=str)
+def test_autocast_takes_its_type(device, kind):
+    """Under autocast: the same as casting by hand; a residual of another type is added after; float32 leaves get their
+    gradients; dropout alone stays in its own type."""
+    _say("autocast", kind)
+    t = _inputs(device, rows=70, d=40, n=24)
+    rng = dict(p=0.2, seed=5)
+    leaves = [t[n].requires_grad_(True) for n in ("x", "w", "b", "r")]
+    x, w, b, r = leaves
+    low = lambda v: v.to(kind)  # noqa: E731
+    cases = [(lambda: ff.gated_linear(x, w, b, **rng), lambda: ff.gated_linear(low(x), low(w), low(b), **rng), kind),
+             (lambda: ff.gated_linear(low(x), w, None, **rng), lambda: ff.gated_linear(low(x), low(w), None, **rng), kind),
+             (lambda: ff.linear_dropout_add(x, w, b, r, **rng), lambda: r + ff.linear_dropout_add(low(x), low(w), low(b), **rng), torch.float32),
+             (lambda: ff.linear_dropout_add(low(x), w, b, low(r), **rng), lambda: ff.linear_dropout_add(low(x), low(w), low(b), low(r), **rng), kind),
+             (lambda: ff.dropout_add(x, x, **rng), lambda: ff.dropout_add(x, x, **rng), torch.float32),
+             (lambda: ff.dropout_add(low(x), x, **rng), lambda: x + ff.dropout_add(low(x), **rng), torch.float32)]
+    for call, by_hand, want_type in cases:
+        with torch.autocast("cuda", dtype=kind):
+            y = call()
+        want = by_hand()
+        assert y.dtype == want.dtype == want_type and torch.equal(y, want)
+        dy = _rand(device, *y.shape, dtype=y.dtype, seed=9)
+        for got, ref in zip(torch.autograd.grad(y, leaves, dy, allow_unused=True), torch.autograd.grad(want, leaves, dy, allow_unused=True)):
+            assert (got is None) == (ref is None)
+            assert got is None or torch.equal(got, ref)
+    with torch.autocast("cuda", dtype=kind), torch.autocast("cuda", enabled=False):
+        assert ff.gated_linear(x, w, b).dtype == torch.float32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("input_type", [torch.float32, torch.bfloat16], ids=str)
+def test_block_under_autocast(device, input_type):
+    """The adapted block with float32 weights in bfloat16 autocast, as its parts by torch: types, output and the Gaussians'
+    gradients (the composition rounds the inner activation and its parts, about eight roundings of 2^-9: 2% of
+    the norm is beyond four times their sum)."""
+    from guass_amd.layers import GaussianAdapterConfig, GaussianFeedForward, GaussianLinear
+
+    _say("block autocast", input_type)
+    torch.manual_seed(0)
+    cfg = GaussianAdapterConfig(init_num_gaussians=48, init_amp_scale=0.05, tile_out=16, tile_in=16, delta_apply="merged")
+    block = GaussianFeedForward(GaussianLinear(64, 192, adapter_config=cfg, device=device),
+                                GaussianLinear(96, 64, adapter_config=cfg, device=device))
+    x, r = _rand(device, 130, 64, dtype=input_type, seed=1), _rand(device, 130, 64, seed=2)
+    params = [p for ly in (block.proj, block.out) for p in ly.get_gaussian_parameters().values()]
+    dy = _rand(device, 130, 64, seed=3)
+    results = []
+    for fused in (True, False):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            if fused:
+                y = block(x, r)
+            else:
+                value, gate = block.proj(x).chunk(2, dim=-1)
+                y = block.out(value * torch.nn.functional.gelu(gate)) + r
+        results.append([y.detach(), *torch.autograd.grad(y, params, dy)])
+    for a, b in zip(*results):
+        assert a.dtype == b.dtype
+        assert float((a.double() - b.double()).norm() / b.double().norm()) < 2e-2
