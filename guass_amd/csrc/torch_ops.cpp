@@ -4,6 +4,7 @@
 // backward: 96 us from Python, 48 us of them autograd's own).
 #include <ATen/ATen.h>
 #include <ATen/autocast_mode.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -80,7 +81,18 @@ gf_dropout make_dropout(double p, int64_t seed, const MaybeTensor& seed_tensor, 
 
 // ------------------------------------------------------------------------------- dropout
 
-Tensor dropout_kernel(const Tensor& x, const MaybeTensor& residual, const gf_dropout& d) {
+void check_dropout(const Tensor& x, const MaybeTensor& residual, const MaybeTensor& seed) {
+  check_first(x);
+  if (present(residual)) {
+    check_like(*residual, "residual", x);
+    TORCH_CHECK(residual->sym_sizes() == x.sym_sizes(), "residual must have x's shape ", x.sym_sizes(), " (got ", residual->sym_sizes(), ")");
+  }
+  check_seed(seed, x);
+}
+
+Tensor dropout_forward(const Tensor& x, const MaybeTensor& residual, double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
+  check_dropout(x, residual, seed_tensor);
+  const gf_dropout d = make_dropout(p, seed, seed_tensor, offset);
   Tensor y = at::empty_like(x, at::MemoryFormat::Contiguous);
   if (y.numel() == 0) return y;
   const c10::DeviceGuard guard(x.device());
@@ -91,6 +103,11 @@ Tensor dropout_kernel(const Tensor& x, const MaybeTensor& residual, const gf_dro
                           stream_of(x)),
            "gf_dropout_add");
   return y;
+}
+
+Tensor call_dropout_forward(const Tensor& x, const MaybeTensor& residual, double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("guass_amd::dropout_forward", "").typed<decltype(dropout_forward)>();
+  return op.call(x, residual, p, seed, seed_tensor, offset);
 }
 
 // Gradients of a first backward that refuse a second one.
@@ -108,7 +125,7 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     ctx->saved_data["rng"] = std::make_tuple(p, seed, offset);
     ctx->saved_data["residual"] = present(residual);
     if (present(seed_tensor)) ctx->save_for_backward({*seed_tensor});
-    return dropout_kernel(x, residual, make_dropout(p, seed, seed_tensor, offset));
+    return call_dropout_forward(x, residual, p, seed, seed_tensor, offset);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto [p, seed, offset] = ctx->saved_data["rng"].to<std::tuple<double, int64_t, int64_t>>();
@@ -117,7 +134,7 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     const Tensor& dy = grads[0];
     const bool again = dy.requires_grad();
     Tensor dx;
-    if (want_x) dx = dropout_kernel(dy, std::nullopt, make_dropout(p, seed, saved.empty() ? MaybeTensor() : saved[0], offset));
+    if (want_x) dx = call_dropout_forward(dy, std::nullopt, p, seed, saved.empty() ? MaybeTensor() : saved[0], offset);
     return once({dx, want_r ? dy : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, "dropout_add", again);
   }
 };
@@ -134,37 +151,35 @@ void check_no_tangent(const char* name, const Tensor& x, const M&... others) {
 }
 
 Tensor dropout_add(const Tensor& x, const MaybeTensor& residual, double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
-  check_first(x);
-  if (present(residual)) {
-    check_like(*residual, "residual", x);
-    TORCH_CHECK(residual->sizes() == x.sizes(), "residual must have x's shape ", x.sizes(), " (got ", residual->sizes(), ")");
-  }
-  check_seed(seed_tensor, x);
+  check_dropout(x, residual, seed_tensor);
   check_no_tangent("dropout_add", x, residual);
   if (at::GradMode::is_enabled() && (wants(x) || wants(residual))) return DropoutAdd::apply(x, residual, p, seed, seed_tensor, offset);
-  return dropout_kernel(x, residual, make_dropout(p, seed, seed_tensor, offset));
+  return call_dropout_forward(x, residual, p, seed, seed_tensor, offset);
 }
 
 // ------------------------------------------------------------------------ linear and gated
 
-void check_linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual, int64_t activation) {
+void check_linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual, int64_t activation,
+                  const MaybeTensor& seed) {
   check_first(x);
   check_like(weight, "weight", x);
   TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2, "x must have shape [..., in_features] and weight two dimensions");
-  const int64_t rows = weight.size(0), cols = weight.size(1);
+  const auto rows = weight.sym_size(0), cols = weight.sym_size(1);  // symbolic in a trace
   TORCH_CHECK(rows != 0 && cols != 0, "weight must not be empty");
   TORCH_CHECK(activation == GF_ACT_NONE || rows % 2 == 0, "a gated weight must have an even number of rows: the value's, then the gate's");
-  TORCH_CHECK(x.size(-1) == cols, "x has ", x.size(-1), " features, weight takes ", cols);
+  TORCH_CHECK(x.sym_size(-1) == cols, "x has ", x.sym_size(-1), " features, weight takes ", cols);
   if (present(bias)) {
     check_like(*bias, "bias", x);
-    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == rows, "bias must have shape [", rows, "]");
+    TORCH_CHECK(bias->dim() == 1 && bias->sym_size(0) == rows, "bias must have shape [", rows, "]");
   }
   if (present(residual)) {
     check_like(*residual, "residual", x);
-    auto want = x.sizes().vec();
+    auto want = x.sym_sizes().vec();
     want.back() = rows;
-    TORCH_CHECK(residual->sizes() == at::IntArrayRef(want), "residual must have shape ", at::IntArrayRef(want), " (got ", residual->sizes(), ")");
+    TORCH_CHECK(residual->sym_sizes() == c10::SymIntArrayRef(want), "residual must have shape ", c10::SymIntArrayRef(want), " (got ",
+                residual->sym_sizes(), ")");
   }
+  check_seed(seed, x);
 }
 
 struct Products {
@@ -193,7 +208,10 @@ struct Products {
 
 // y, and what the backward needs of the products (undefined for a linear product or if not to be saved)
 std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual,
-                                          int64_t activation, const gf_dropout& d, bool save) {
+                                          int64_t activation, double p_drop, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset,
+                                          bool save) {
+  check_linear(x, weight, bias, residual, activation, seed_tensor);
+  const gf_dropout d = make_dropout(p_drop, seed, seed_tensor, offset);
   auto shape = x.sizes().vec();
   shape.back() = weight.size(0) / (activation == GF_ACT_NONE ? 1 : 2);
   Tensor y = at::empty(shape, x.options()), saved, b;
@@ -212,9 +230,23 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight,
   return {y, saved};
 }
 
+std::tuple<Tensor, Tensor> call_linear_forward(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual,
+                                               int64_t activation, double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset,
+                                               bool save) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("guass_amd::linear_forward", "").typed<decltype(linear_forward)>();
+  return op.call(x, weight, bias, residual, activation, p, seed, seed_tensor, offset, save);
+}
+
 // The gradients of x, weight and bias that are wanted.
-std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x, const Tensor& weight, const Tensor& saved, const Tensor& dy,
-                                                   int64_t activation, const gf_dropout& d, bool want_x, bool want_w, bool want_b) {
+std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x, const Tensor& weight, const MaybeTensor& saved, const Tensor& dy,
+                                                   int64_t activation, double p_drop, int64_t seed, const MaybeTensor& seed_tensor,
+                                                   int64_t offset, bool want_x, bool want_w, bool want_b) {
+  check_linear(x, weight, std::nullopt, std::nullopt, activation, seed_tensor);
+  check_like(dy, "dy", x);
+  auto want = x.sizes().vec();
+  want.back() = weight.size(0) / (activation == GF_ACT_NONE ? 1 : 2);
+  TORCH_CHECK(dy.sizes() == at::IntArrayRef(want), "dy must have shape ", at::IntArrayRef(want), " (got ", dy.sizes(), ")");
+  const gf_dropout d = make_dropout(p_drop, seed, seed_tensor, offset);
   const bool some = dy.numel() != 0;  // no rows: every sum is empty
   auto make = [&](at::IntArrayRef shape) { return some ? at::empty(shape, x.options()) : at::zeros(shape, x.options()); };
   Tensor dx, dw, db;
@@ -226,7 +258,11 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x, const Tensor
   Products p(x, weight, activation, d);
   const Rows g(dy);
   p.args.dy = g.data(), p.args.lddy = g.ld;
-  if (saved.defined()) p.args.saved = saved.data_ptr();
+  if (activation != GF_ACT_NONE) {
+    TORCH_CHECK(present(saved) && saved->is_cuda() && saved->is_contiguous() && saved->nbytes() >= gf_ff_saved_bytes(&p.args),
+                "saved must be what the forward with save=True returned");
+    p.args.saved = saved->data_ptr();
+  }
   if (want_x) p.args.dx = dx.data_ptr();
   if (want_w) p.args.dweight = dw.data_ptr();
   if (want_b) p.args.dbias = db.data_ptr();
@@ -234,11 +270,20 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x, const Tensor
   return {dx, dw, db};
 }
 
+std::tuple<Tensor, Tensor, Tensor> call_linear_backward(const Tensor& x, const Tensor& weight, const MaybeTensor& saved, const Tensor& dy,
+                                                        int64_t activation, double p, int64_t seed, const MaybeTensor& seed_tensor,
+                                                        int64_t offset, bool want_x, bool want_w, bool want_b) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("guass_amd::linear_backward", "").typed<decltype(linear_backward)>();
+  return op.call(x, weight, saved, dy, activation, p, seed, seed_tensor, offset, want_x, want_w, want_b);
+}
+
+MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
+
 struct Linear : torch::autograd::Function<Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual,
                         int64_t activation, double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
     const bool save = wants(x) || wants(weight) || wants(bias);
-    auto [y, saved] = linear_forward(x, weight, bias, residual, activation, make_dropout(p, seed, seed_tensor, offset), save);
+    auto [y, saved] = call_linear_forward(x, weight, bias, residual, activation, p, seed, seed_tensor, offset, save);
     ctx->save_for_backward({x, weight, saved, present(seed_tensor) ? *seed_tensor : Tensor()});
     ctx->saved_data["call"] = std::make_tuple(activation, p, seed, offset);
     ctx->saved_data["inputs"] = std::make_tuple(present(bias), present(residual), wants(bias));
@@ -254,7 +299,7 @@ struct Linear : torch::autograd::Function<Linear> {
     const Tensor& dy = grads[0];
     // what the gradients depend on: a gated product's on the bias too, by value and gate
     const bool again = dy.requires_grad() || saved[0].requires_grad() || saved[1].requires_grad() || (activation != GF_ACT_NONE && trains_bias);
-    auto [dx, dw, db] = linear_backward(saved[0], saved[1], saved[2], dy, activation, make_dropout(p, seed, saved[3], offset), wx, ww, wb);
+    auto [dx, dw, db] = call_linear_backward(saved[0], saved[1], maybe(saved[2]), dy, activation, p, seed, maybe(saved[3]), offset, wx, ww, wb);
     return once({dx, dw, db, wr ? dy : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()},
                 activation == GF_ACT_NONE ? "linear_dropout_add" : "gated_linear", again);
   }
@@ -262,12 +307,11 @@ struct Linear : torch::autograd::Function<Linear> {
 
 Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual, int64_t activation, double p,
               int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
-  check_linear(x, weight, bias, residual, activation);
-  check_seed(seed_tensor, x);
+  check_linear(x, weight, bias, residual, activation, seed_tensor);
   check_no_tangent(activation == GF_ACT_NONE ? "linear_dropout_add" : "gated_linear", x, MaybeTensor(weight), bias, residual);
   if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias) || wants(residual)))
     return Linear::apply(x, weight, bias, residual, activation, p, seed, seed_tensor, offset);
-  return std::get<0>(linear_forward(x, weight, bias, residual, activation, make_dropout(p, seed, seed_tensor, offset), false));
+  return std::get<0>(call_linear_forward(x, weight, bias, residual, activation, p, seed, seed_tensor, offset, false));
 }
 
 // ------------------------------------------------------------------------------ autocast
@@ -300,34 +344,24 @@ TORCH_LIBRARY_IMPL(guass_amd, Autocast, m) {
 }
 
 TORCH_LIBRARY(guass_amd, m) {
+  // what a user calls: checks and autograd around the operators below
   m.def("dropout_add(Tensor x, Tensor? residual, float p, int seed, Tensor? seed_tensor, int offset) -> Tensor", dropout_add);
   m.def("linear(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int activation, float p, int seed, Tensor? seed_tensor, "
         "int offset) -> Tensor", linear);
-  // the phases by themselves, without autograd: what a HIP graph captures
+  // the launches by themselves, without autograd: what a HIP graph captures, and what a trace (torch.compile) holds
+  m.def("dropout_forward(Tensor x, Tensor? residual, float p, int seed, Tensor? seed_tensor, int offset) -> Tensor");
   m.def("linear_forward(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int activation, float p, int seed, Tensor? seed_tensor, "
-        "int offset, bool save) -> (Tensor, Tensor)",
-        [](const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual, int64_t activation, double p,
-           int64_t seed, const MaybeTensor& seed_tensor, int64_t offset, bool save) {
-          check_linear(x, weight, bias, residual, activation);
-          check_seed(seed_tensor, x);
-          return linear_forward(x, weight, bias, residual, activation, make_dropout(p, seed, seed_tensor, offset), save);
-        });
+        "int offset, bool save) -> (Tensor, Tensor)");
   m.def("linear_backward(Tensor x, Tensor weight, Tensor? saved, Tensor dy, int activation, float p, int seed, Tensor? seed_tensor, "
-        "int offset, bool want_x, bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor)",
-        [](const Tensor& x, const Tensor& weight, const MaybeTensor& saved, const Tensor& dy, int64_t activation, double p, int64_t seed,
-           const MaybeTensor& seed_tensor, int64_t offset, bool want_x, bool want_weight, bool want_bias) {
-          check_linear(x, weight, std::nullopt, std::nullopt, activation);
-          check_like(dy, "dy", x);
-          auto want = x.sizes().vec();
-          want.back() = weight.size(0) / (activation == GF_ACT_NONE ? 1 : 2);
-          TORCH_CHECK(dy.sizes() == at::IntArrayRef(want), "dy must have shape ", at::IntArrayRef(want), " (got ", dy.sizes(), ")");
-          check_seed(seed_tensor, x);
-          const gf_dropout d = make_dropout(p, seed, seed_tensor, offset);
-          if (activation != GF_ACT_NONE && dy.numel() != 0) {
-            const Products sizes(x, weight, activation, d);
-            TORCH_CHECK(present(saved) && saved->is_cuda() && saved->is_contiguous() && saved->nbytes() >= gf_ff_saved_bytes(&sizes.args),
-                        "saved must be what the forward with save=True returned");
-          }
-          return linear_backward(x, weight, present(saved) ? *saved : Tensor(), dy, activation, d, want_x, want_weight, want_bias);
-        });
+        "int offset, bool want_x, bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(guass_amd, CUDA, m) {
+  m.impl("dropout_forward", dropout_forward);
+  m.impl("linear_forward", linear_forward);
+  m.impl("linear_backward", linear_backward);
+}
+
+TORCH_LIBRARY_IMPL(guass_amd, Autograd, m) {
+  for (const char* name : {"dropout_forward", "linear_forward", "linear_backward"}) m.impl(name, torch::CppFunction::makeFallthrough());
 }

@@ -25,8 +25,6 @@ captured graph draws anew at every replay if the program changes it between them
 
 from __future__ import annotations
 
-from functools import lru_cache
-
 import torch
 from torch import Tensor
 
@@ -37,8 +35,18 @@ ACTIVATIONS = tuple(a for a in N.GF_ACTIVATIONS if a is not None)
 __all__ = ["ACTIVATIONS", "dropout_add", "gated_linear", "linear_dropout_add"]
 
 
-@lru_cache(maxsize=1)
-def _ops():
+_OPS = None
+
+
+def _ops() -> tuple:
+    """What _load found, once a process (a global: a trace reads it as it is)."""
+    global _OPS
+    if _OPS is None:
+        _OPS = _load()
+    return _OPS
+
+
+def _load() -> tuple:
     """torch.ops.guass_amd: the operators of libguass_torch.so (csrc/torch_ops.cpp), which checks the tensors, makes
     outputs and workspaces and carries the gradients."""
     N.lib()  # raises if the kernels' library is not built
@@ -46,8 +54,36 @@ def _ops():
     if not path.exists():
         raise RuntimeError(f"{path} is not built; run `python -m guass_amd.build`")
     torch.ops.load_library(str(path))
+    _register_shapes()
     ops = torch.ops.guass_amd
     return ops.dropout_add.default, ops.linear.default, ops.linear_forward.default, ops.linear_backward.default
+
+
+def _register_shapes() -> None:
+    """The operators' outputs without data: what a trace (torch.compile, FakeTensorMode) runs instead of the kernels."""
+    fake = torch.library.register_fake
+
+    @fake("guass_amd::dropout_forward")
+    def _(x, residual, p, seed, seed_tensor, offset):
+        return x.new_empty(x.shape)
+
+    @fake("guass_amd::linear_forward")
+    def _(x, weight, bias, residual, activation, p, seed, seed_tensor, offset, save):
+        out = weight.shape[0] // (2 if activation else 1)
+        y = x.new_empty((*x.shape[:-1], out))
+        if not (save and activation):
+            return y, None
+        return y, x.new_empty((y.numel() // out * _saved_bytes(x.dtype, out),), dtype=torch.uint8)
+
+    @fake("guass_amd::linear_backward")
+    def _(x, weight, saved, dy, activation, p, seed, seed_tensor, offset, want_x, want_weight, want_bias):
+        return (x.new_empty(x.shape) if want_x else None, x.new_empty(weight.shape) if want_weight else None,
+                x.new_empty(weight.shape[:1]) if want_bias else None)
+
+
+def _saved_bytes(dtype: torch.dtype, out: int) -> int:
+    """What gf_ff_saved_bytes says of one row: whole groups of 8 elements, value and gate together."""
+    return (out + 7) // 8 * 8 * {torch.float32: 8, torch.float16: 6, torch.bfloat16: 5}[dtype]
 
 
 def _signed(v: int, name: str) -> int:

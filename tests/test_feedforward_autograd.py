@@ -196,3 +196,64 @@ def test_block_under_autocast(device, input_type):
     for a, b in zip(*results):
         assert a.dtype == b.dtype
         assert float((a.double() - b.double()).norm() / b.double().norm()) < 2e-2
+
+
+@pytest.mark.parametrize("dtype,code", [(torch.float32, 0), (torch.bfloat16, 1), (torch.float16, 2)], ids=str)
+def test_traced_size_of_what_is_saved(dtype, code):
+    import ctypes
+
+    from guass_amd import _native as N
+
+    for rows, out in ((1, 1), (3, 8), (7, 9), (64, 5120), (1001, 777)):
+        a = N.GfFfArgs()
+        a.dtype, a.activation, a.rows, a.in_features, a.out_features = code, 1, rows, 16, out
+        assert N.lib().gf_ff_saved_bytes(ctypes.byref(a)) == rows * ff._saved_bytes(dtype, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", CALLS)
+def test_compiled_as_eager(device, op):
+    """A compiled function that calls an operator: outputs and gradients as without, also with other sizes after."""
+    _say("compiled", op)
+    call, names = CALLS[op]
+    torch._dynamo.reset()  # one code object, compiled for each operator anew
+    ff._ops()  # loading the operators' library is not traced
+    compiled = torch.compile(lambda t: call(t) * 2, backend="aot_eager", fullgraph=True)
+    for rows in (4, 4, 9, 70):
+        t = _inputs(device, rows=rows)
+        t["x2"] = t["x"].clone()
+        with torch.no_grad():
+            assert torch.equal(compiled(t), call(t) * 2)
+        leaves = [t[n].requires_grad_(True) for n in names]
+        got, want = compiled(t), call(t) * 2
+        assert torch.equal(got, want)
+        dy = _rand(device, *want.shape, seed=9)
+        for a, b in zip(torch.autograd.grad(got, leaves, dy), torch.autograd.grad(want, leaves, dy)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_operators_hold_to_their_schemas(device):
+    """torch's own check: no input is written, outputs have the traced shapes, types and strides."""
+    _say("schemas")
+    ops = torch.ops.guass_amd
+    ff._ops()
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        t = _inputs(device, rows=5, dtype=dtype)
+        seed = torch.ones(1, dtype=torch.int64, device=device)
+        utils = ("test_schema", "test_faketensor")
+        torch.library.opcheck(ops.dropout_forward, (t["x"], None, 0.1, 3, None, 0), test_utils=utils)
+        torch.library.opcheck(ops.dropout_forward, (t["x"].t(), t["x"].t(), 0.1, 0, seed, 0), test_utils=utils)
+        for act in (0, 1):
+            torch.library.opcheck(ops.linear_forward, (t["x"], t["w"], t["b"], None, act, 0.1, 3, None, 0, True), test_utils=utils)
+            y, saved = ops.linear_forward(t["x"], t["w"], t["b"], None, act, 0.1, 3, None, 0, True)
+            for want in ((True, True, True), (False, True, False)):
+                torch.library.opcheck(ops.linear_backward, (t["x"], t["w"], saved, y, act, 0.1, 3, None, 0, *want), test_utils=utils)
+
+
+@pytest.mark.gpu
+def test_phases_by_themselves_carry_no_gradient(device):
+    t = _inputs(device)
+    t["x"].requires_grad_(True)
+    y, saved = ff._linear_forward(t["x"], t["w"], None, None, "gelu", 0.0, 0, 0, True)
+    assert not y.requires_grad and not saved.requires_grad
