@@ -1065,9 +1065,13 @@ Drop make_drop(const gf_dropout& d) {
 }
 
 constexpr int64_t kMaxSize = INT32_MAX;
+// Elements of a matrix, its row stride's gaps among them: more than a memory has, and 64 bits hold the bytes of all that is
+// made of one (planes, parts: at most 2^7 bytes an element).
+constexpr int64_t kMaxElements = int64_t(1) << 48;
 
-int check_matrix(const char* name, const void* p, int64_t ld, int64_t width, int size) {
+int check_matrix(const char* name, const void* p, int64_t rows, int64_t ld, int64_t width, int size) {
   if (p == nullptr) return fail(GF_E_INVALID_ARGUMENT, "%s must not be NULL", name);
+  if (rows > 1 && ld > kMaxElements / rows) return fail(GF_E_INVALID_ARGUMENT, "%s: too large", name);
   if (ld < width) return fail(GF_E_INVALID_ARGUMENT, "%s: row stride %lld is below its width %lld", name, (long long)ld, (long long)width);
   if ((uintptr_t)p % size != 0) return fail(GF_E_INVALID_ARGUMENT, "%s is not aligned to its type", name);
   return GF_OK;
@@ -1099,6 +1103,11 @@ int check_shape(const gf_ff_args* a) {
     return fail(GF_E_INVALID_ARGUMENT, "rows must not be negative and in_features and out_features must be positive");
   if (a->rows > kMaxSize || a->in_features > kMaxSize / 2 || a->out_features > kMaxSize / 4)
     return fail(GF_E_INVALID_ARGUMENT, "rows, in_features or out_features too large");
+  const int64_t weight_rows = a->out_features * (a->activation == GF_ACT_NONE ? 1 : 2);
+  if (std::max(a->rows, weight_rows) * a->in_features > kMaxElements || a->rows * weight_rows > kMaxElements)
+    return fail(GF_E_INVALID_ARGUMENT, "rows, in_features or out_features too large");
+  for (const int64_t ld : {a->ldx, a->ldw, a->ldr, a->lddy})
+    if (ld > kMaxElements || ld < -kMaxElements) return fail(GF_E_INVALID_ARGUMENT, "row stride too large");
   return check_dropout(&a->dropout);
 }
 
@@ -1376,9 +1385,9 @@ int gf_dropout_add(int32_t dtype, const gf_dropout* dropout, int64_t rows, int64
   FF_CHECK(check_dropout(dropout));
   if (rows < 0 || cols < 0 || rows > kMaxSize || cols > kMaxSize) return fail(GF_E_INVALID_ARGUMENT, "rows or cols negative or too large");
   if (rows == 0 || cols == 0) return GF_OK;
-  FF_CHECK(check_matrix("x", x, ldx, cols, size_of(dtype)));
-  FF_CHECK(check_matrix("y", y, ldy, cols, size_of(dtype)));
-  if (residual != nullptr) FF_CHECK(check_matrix("residual", residual, ldr, cols, size_of(dtype)));
+  FF_CHECK(check_matrix("x", x, rows, ldx, cols, size_of(dtype)));
+  FF_CHECK(check_matrix("y", y, rows, ldy, cols, size_of(dtype)));
+  if (residual != nullptr) FF_CHECK(check_matrix("residual", residual, rows, ldr, cols, size_of(dtype)));
   const Drop d = make_drop(*dropout);
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
@@ -1408,14 +1417,14 @@ int gf_ff_forward(const gf_ff_args* args, void* workspace, size_t workspace_byte
   const gf_ff_args& a = *args;
   if (a.rows == 0) return GF_OK;
   const int size = size_of(a.dtype);
-  FF_CHECK(check_matrix("x", a.x, a.ldx, a.in_features, size));
-  FF_CHECK(check_matrix("weight", a.weight, a.ldw, a.in_features, size));
-  FF_CHECK(check_matrix("y", a.y, a.out_features, a.out_features, size));
+  FF_CHECK(check_matrix("x", a.x, a.rows, a.ldx, a.in_features, size));
+  FF_CHECK(check_matrix("weight", a.weight, weight_rows(&a), a.ldw, a.in_features, size));
+  FF_CHECK(check_matrix("y", a.y, a.rows, a.out_features, a.out_features, size));
   if (a.residual != nullptr) {
     if (a.activation != GF_ACT_NONE) return fail(GF_E_INVALID_ARGUMENT, "a gated product takes no residual");
-    FF_CHECK(check_matrix("residual", a.residual, a.ldr, a.out_features, size));
+    FF_CHECK(check_matrix("residual", a.residual, a.rows, a.ldr, a.out_features, size));
   }
-  if (a.saved != nullptr) FF_CHECK(check_matrix("saved", a.saved, 1, 1, 16));
+  if (a.saved != nullptr) FF_CHECK(check_matrix("saved", a.saved, 1, 1, 1, 16));
   Arena count{nullptr}, ws{(uint8_t*)workspace};
   FF_CHECK(forward(a, count, false, nullptr));
   FF_CHECK(check_workspace(count.used, workspace, workspace_bytes));
@@ -1426,10 +1435,10 @@ int gf_ff_backward(const gf_ff_args* args, void* workspace, size_t workspace_byt
   FF_CHECK(check_shape(args));
   const gf_ff_args& a = *args;
   const int size = size_of(a.dtype);
-  FF_CHECK(check_matrix("x", a.x, a.ldx, a.in_features, size));
-  FF_CHECK(check_matrix("weight", a.weight, a.ldw, a.in_features, size));
-  FF_CHECK(check_matrix("dy", a.dy, a.lddy, a.out_features, size));
-  if (a.activation != GF_ACT_NONE) FF_CHECK(check_matrix("saved", a.saved, 1, 1, 16));
+  FF_CHECK(check_matrix("x", a.x, a.rows, a.ldx, a.in_features, size));
+  FF_CHECK(check_matrix("weight", a.weight, weight_rows(&a), a.ldw, a.in_features, size));
+  FF_CHECK(check_matrix("dy", a.dy, a.rows, a.lddy, a.out_features, size));
+  if (a.activation != GF_ACT_NONE) FF_CHECK(check_matrix("saved", a.saved, 1, 1, 1, 16));
   if (a.rows == 0) return fail(GF_E_INVALID_ARGUMENT, "a backward needs rows");
   Arena count{nullptr}, ws{(uint8_t*)workspace};
   FF_CHECK(backward(a, count, false, nullptr));

@@ -25,6 +25,8 @@ captured graph draws anew at every replay if the program changes it between them
 
 from __future__ import annotations
 
+from pathlib import Path
+
 import torch
 from torch import Tensor
 
@@ -50,7 +52,7 @@ def _load() -> tuple:
     """torch.ops.guass_amd: the operators of libguass_torch.so (csrc/torch_ops.cpp), which checks the tensors, makes
     outputs and workspaces and carries the gradients."""
     N.lib()  # raises if the kernels' library is not built
-    path = N.LIB_PATH.with_name("libguass_torch.so")
+    path = Path(__file__).with_name("libguass_torch.so")  # it takes the library that is loaded, wherever that lies
     if not path.exists():
         raise RuntimeError(f"{path} is not built; run `python -m guass_amd.build`")
     torch.ops.load_library(str(path))

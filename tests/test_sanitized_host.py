@@ -81,3 +81,26 @@ def test_sanitizer_reports_a_host_overflow(libs):
     assert proc.returncode != 0
     assert "AddressSanitizer: heap-buffer-overflow" in proc.stderr and "gf_batch_plan" in proc.stderr, \
         proc.stderr[-3000:]
+
+
+FEEDFORWARD_TESTS = ["tests/test_feedforward.py", "tests/test_feedforward_precision.py", "tests/test_feedforward_autograd.py",
+                     "tests/test_feedforward_abi.py"]
+
+
+def test_feedforward_cpu_tests_under_asan_and_ubsan(libs):
+    """The feed-forward entries' host code: argument checks, workspace counting at the sizes' limits, the choice of a cut."""
+    env = dict(os.environ)
+    env.update({
+        "LD_PRELOAD": str(build.asan_runtime()),
+        "ASAN_OPTIONS": "detect_leaks=0:abort_on_error=1:halt_on_error=1:symbolize=1",
+        "UBSAN_OPTIONS": "halt_on_error=1:print_stacktrace=1",
+        "GUASS_AMD_LIB": str(libs["lib"]),
+        "GUASS_AMD_HOST_LIB": str(libs["host_lib"]),
+    })
+    proc = subprocess.run([sys.executable, "-m", "pytest", "-q", "-m", "not gpu", "-p", "no:cacheprovider",
+                           *FEEDFORWARD_TESTS], cwd=ROOT, env=env, capture_output=True, text=True, timeout=900)
+    out = proc.stdout[-6000:] + "\n" + proc.stderr[-6000:]
+    assert proc.returncode == 0, out
+    for marker in ("ERROR: AddressSanitizer", "runtime error:", "SUMMARY: UndefinedBehaviorSanitizer"):
+        assert marker not in proc.stdout + proc.stderr, out
+    assert " passed" in proc.stdout, out
