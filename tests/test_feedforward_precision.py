@@ -95,7 +95,7 @@ def _check(device, kind, rows, d, n, dtype, act="gelu", p=0.0, seed=200, change=
         assert off <= limit, f"{name}: {off:.3e}, limit {limit:.3e}"
 
 
-# every tile shape of every operand layout, few rows, splits along k, odd sizes
+# few rows, splits along k, odd sizes
 SIZES = [(48, 320, 264), (300, 640, 1000), (1025, 2560, 640), (4089, 331, 2037), (8100, 328, 1279), (4089, 2037, 331)]
 
 
@@ -203,3 +203,116 @@ def test_infinities_come_out_as_the_sums_have_them(device, dtype, rows):
         assert torch.equal(torch.isnan(got), torch.isnan(want)), name
         assert torch.equal(torch.isinf(got), torch.isinf(want)), name
         assert torch.equal(torch.sign(got[torch.isinf(want)]).double(), torch.sign(want[torch.isinf(want)])), name
+
+
+# ------------------------------------------------------------------------------ what the limits tell apart, on the CPU
+
+
+def _planes(t):
+    """Three bfloat16 planes of float32 numbers, by truncation, in 64 bits."""
+    out, left = [], t.clone()
+    for _ in range(3):
+        top = (left.view(torch.int32) & -65536).view(torch.float32)
+        out.append(top.double())
+        left = left - top
+    return out
+
+
+@pytest.mark.parametrize("inner", [40, 320, 1279, 4089])
+def test_limits_see_a_lost_plane(inner):
+    """Six products of planes keep the float32 limit; without the three small ones, or without either operand's third plane,
+    the result lies beyond it."""
+    g = torch.Generator().manual_seed(inner)
+    a, b = torch.randn(64, inner, generator=g), torch.randn(96, inner, generator=g)
+    want = a.double() @ b.double().t()
+    p, q = _planes(a), _planes(b)
+    limit = _limits("linear", torch.float32, [want], (inner,))[0]
+    terms = {(i, j): p[i] @ q[j].t() for i in range(3) for j in range(3) if i + j <= 2}
+    assert _rms(sum(terms.values()), want) <= limit
+    for lost in ([(2, 0), (0, 2), (1, 1)], [(2, 0)], [(0, 2)]):
+        assert _rms(sum(v for k, v in terms.items() if k not in lost), want) > limit, lost
+
+
+@pytest.mark.parametrize("act", ff.ACTIVATIONS)
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 12), (torch.float16, 16)], ids=str)
+def test_limits_see_value_and_gate_lose_their_low_bits(dtype, bits, act):
+    """Value and gate in the bits that are kept meet a gated product's limits for dx and dweight; rounded to the tensors'
+    own type they do not."""
+    t = _case("cpu", "gated", 300, 72, 104, dtype, 220)
+    want = _exact("gated", t, act, 0.0)
+    limits = _limits("gated", dtype, want, (72, 208, 300, 300))
+
+    def gradients(keep):
+        x, w, b, dy = (t[k].double() for k in ("x", "w", "b", "dy"))
+        z = keep(x @ w.t() + b)
+        a, slope = fo.activation(z[:, 104:], act)
+        dz = torch.cat((dy * a, dy * z[:, :104] * slope), dim=1).to(dtype).double()
+        return [(dz @ w).to(dtype), (dz.t() @ x).to(dtype)]
+
+    def short(z):  # to `bits` significant ones
+        m, e = torch.frexp(z)
+        return torch.ldexp((m * 2**bits).round() / 2**bits, e)
+
+    assert all(_rms(g, v) <= limit for g, v, limit in zip(gradients(short), want[1:3], limits[1:3]))
+    assert any(_rms(g, v) > limit for g, v, limit in zip(gradients(lambda z: z.to(dtype).double()), want[1:3], limits[1:3]))
+
+
+# ------------------------------------------------------------------------------ large tiles; dy as dz
+
+
+# sizes at which the products take each of the large tiles, in each operand layout: odd ones, and ones that are read in place
+LARGE = [("gated", 4089, 331, 2037), ("linear", 4089, 331, 4075), ("linear", 8100, 328, 1279), ("linear", 4089, 4075, 331),
+         ("linear", 331, 4075, 4089), ("gated", 1030, 1031, 2090), ("gated", 4000, 2201, 600), ("linear", 331, 1279, 8100)]
+WHOLE = [("linear", 8104, 328, 1280), ("linear", 4088, 4072, 328), ("linear", 328, 4072, 4088), ("linear", 328, 1280, 8104)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("kind,rows,d,n", LARGE)
+def test_large_tiles_keep_the_limits(device, kind, rows, d, n, dtype):
+    _check(device, kind, rows, d, n, dtype, p=0.1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=ids)
+@pytest.mark.parametrize("kind,rows,d,n", WHOLE)
+def test_large_tiles_of_dy_itself(device, kind, rows, d, n, dtype):
+    _check(device, kind, rows, d, n, dtype, p=0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows", [1, 5, 40, 64, 65, 300])
+@pytest.mark.parametrize("n", [64, 72, 61])
+def test_nothing_dropped_takes_dy_as_it_lies(device, rows, n, dtype):
+    """Without dropout the products of a linear backward read dy in place where they can: a contiguous one, rows of a larger
+    matrix (aligned and not), an odd base, a broadcast one, a transposed one.  Each gives the contiguous one's gradients to
+    the bit, element by element within the oracle's bounds, with every gradient or the bias's alone."""
+    d = 56
+    t = _case(device, "linear", rows, d, n, dtype, 230)
+    leaves = [t[k].requires_grad_(True) for k in ("x", "w", "b")]
+    y = ff.linear_dropout_add(*leaves)
+
+    def layouts(dy):
+        yield "contiguous", dy
+        for left, right in ((8, 8), (8, 3), (1, 2)):
+            big = torch.full((rows + 1, left + n + right), math.nan, dtype=dtype, device=device)
+            big[:-1, left:left + n] = dy
+            yield f"rows {left} {right}", big[:-1, left:left + n]
+        yield "odd base", torch.empty(rows * n + 1, dtype=dtype, device=device)[1:].view(rows, n).copy_(dy)
+        yield "transposed", dy.t().contiguous().t()
+
+    for dy in (t["dy"], torch.full((1, 1), 0.75, dtype=dtype, device=device).expand(rows, n)):
+        want = fo.linear(t["x"], t["w"], t["b"], None, dy, dtype=dtype)[1:]
+        first = None
+        for name, view in layouts(dy.contiguous()):
+            _say("dy as it lies", rows, n, ids(dtype), name)
+            got = torch.autograd.grad(y, leaves, view, retain_graph=True)
+            for g, (value, bound) in zip(got, want):
+                assert bool(((g.cpu().double() - value).abs() <= bound).all()), name
+            first = first or got
+            assert all(torch.equal(a, b) for a, b in zip(got, first)), name
+            alone, = torch.autograd.grad(y, leaves[2], view, retain_graph=True)
+            assert torch.equal(alone, first[2]), name
+        got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
