@@ -197,7 +197,10 @@ __device__ inline float activation(float g, float* slope) {
   } else {  // (1 + tanh u) / 2 = 1 / (1 + e^-2u), u = sqrt(2/pi) (g + 0.044715 g^3)
     constexpr float c = 1.5957691216057308f;
     const float s = rcp_fast(1.0f + exp2_fast(-c * kLog2e * g * __builtin_fmaf(0.044715f * g, g, 1.0f)));
-    if (slope != nullptr) *slope = __builtin_fmaf(g * s * (1.0f - s), c * __builtin_fmaf(3.0f * 0.044715f * g, g, 1.0f), s);
+    if (slope != nullptr) {  // the square may overflow where s (1 - s) is 0
+      const float du = fminf(c * __builtin_fmaf(3.0f * 0.044715f * g, g, 1.0f), 3.4028234664e38f);
+      *slope = __builtin_fmaf(g * s * (1.0f - s), du, s);
+    }
     return g * s;
   }
 }

@@ -316,3 +316,22 @@ def test_nothing_dropped_takes_dy_as_it_lies(device, rows, n, dtype):
             assert torch.equal(alone, first[2]), name
         got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
         assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("act", ff.ACTIVATIONS)
+def test_gates_far_past_where_the_activations_are_flat(device, act, dtype, rows):
+    """Gates whose squares overflow: the activation is the gate or 0 there, its slope 1 or 0."""
+    gates = [1e15, -1e15, 1e19, -1e19, 1e20, -1e20, 1e30, -1e30]
+    n = len(gates)
+    x = torch.zeros(rows, 8)
+    x[:, :2] = 1.0
+    w = torch.zeros(2 * n, 8)
+    w[:n, 0] = 1.0
+    w[n:, 1] = torch.tensor(gates)
+    t = {"x": x.to(dtype).to(device), "w": w.to(dtype).to(device), "b": None, "dy": torch.ones(rows, n, dtype=dtype, device=device)}
+    want = _exact("gated", t, act, 0.0)
+    for got, v in zip(_run("gated", t, act, 0.0), want):
+        assert bool(((got.double() - v).abs() <= 2.0**-7 * v.abs() + 1e-30).all())
