@@ -42,7 +42,6 @@ GF_PHASE_BIN, GF_PHASE_EMIT, GF_PHASE_RENDER = 0x1, 0x2, 0x4
 GF_PHASE_REDUCE, GF_PHASE_FINISH = 0x1, 0x2
 GF_PHASE_ALL = 0xFF
 
-GF_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 GF_ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}
 
 
