@@ -167,7 +167,8 @@ __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // Phi(-a) e^(a^2/2) for a >= 0 as t Q(t), t = 1 / (1 + p a): p and Q fitted (least squares reweighted to the largest
-// relative error) over a in [0, 14], where it is good to 9e-8; past that Phi(-a) is below the smallest float.
+// relative error) over a in [0, 14]: good to 1.4e-7 with p and Q as floats, and to 3.7e-7 as evaluated in 32 bits (7.4e-7 if
+// the reciprocal is a unit off); past that Phi(-a) is below the smallest float.
 __device__ inline float normal_tail(float a) {
   const float t = rcp_fast(__builtin_fmaf(0.3045656383f, a, 1.0f));
   float q = 0.0367617272f;
@@ -224,9 +225,11 @@ using ActTag = std::integral_constant<int, ACT>;
 // Q's rows are the matrix instruction's rows, of which a lane holds 4 consecutive ones of each 8; they are assigned
 // so that a lane ends up with 8 consecutive n of one m.
 //
-// Bound by the matrix cores at the clock that the chip's power leaves them: 4096 x 4096 x 8192 in bfloat16 takes 203 us
-// (1.35 PFLOP/s) from operands the caches hold, in all three layouts, and 173 us of zeros; 223 us from memory.  Of
-// 8192 x 1280 -> 5120 gated the forward takes 241 us (0.89 PFLOP/s; 294 MB written), dx 202 us, dW 184 us.  32 bits:
+// 4096 x 4096 x 8192 in bfloat16 takes 203 us (1.35 PFLOP/s) from operands the caches hold, in all three layouts, and 173 us of
+// zeros, whose power leaves a higher clock; 223 us from memory.  Of 8192 x 1280 -> 5120 gated the forward takes 241 to 248 us
+// (0.89 PFLOP/s; 294 MB written), dx 202 to 211, dW 184 to 193, by the card.  There the matrix cores are busy for 43, 51 and
+// 58% of the cycles, at 1.8 to 1.9 GHz: what fills the rest (each round's first loads, operands from memory, the rounds' stores at
+// the same time) was not taken apart.  32 bits:
 // 4096 x 4096 x 2048 284 to 344 us by the layouts (0.20 to 0.24 PFLOP/s, six times that on the matrix cores).
 
 using half8 = short __attribute__((ext_vector_type(8)));
@@ -246,7 +249,7 @@ __device__ inline f32x16 mfma(half8 a, half8 b, f32x16 c) {
 }
 
 // A matrix in memory: rows of `ld` elements, 16-byte aligned, `width` (a multiple of 8) of them readable.  32-bit
-// matrices come as three such planes of bfloat16 (k_split), `plane` elements apart.
+// matrices come as three such planes of bfloat16 (k_pack, k_dz), `plane` elements apart.
 struct Matrix {
   const void* p;
   int64_t ld, plane;
@@ -486,8 +489,9 @@ struct Stage {
   }
 };
 
-// Planes of a 32-bit matrix times planes of another: a = a0 + a1 + a2 exactly, 8 bits each, so the six products down to
-// 2^-16 of a0 b0 leave out 3 2^-24 of a b.  Smallest first.
+// Planes of a 32-bit matrix times planes of another: a = a0 + a1 + a2 exactly, 8 bits each by truncation, so a1 is up to
+// 2^-7 of a and a2 up to 2^-15.  The six products that are taken leave out a1 b2 + a2 b1 + a2 b2: at most 8 2^-24 of a b,
+// 0.7 2^-24 on average, always towards zero.  Smallest first.
 constexpr int kPlaneP[6] = {2, 0, 1, 1, 0, 0}, kPlaneQ[6] = {0, 2, 1, 0, 1, 0};
 
 // This wave's LDS reads are done and its loads are in LDS; then all waves'.
@@ -675,7 +679,9 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / (kStageBytes<T, PKC, QKC, A
 // output columns (gated: 16 of the value's and of the gate's), its waves interleaved chunks of 64 bytes along k; a lane
 // loads 16 bytes of W's row (lane % 16) and of x's straight into the matrix instruction's operands, at whatever
 // alignment.  32-bit operands are multiplied as such (16 x 16 x 4).  The waves' sums meet in LDS.  One row of
-// 1280 -> 5120 gated in bfloat16: 9.3 us for 26 MB, 5120 -> 1280 8.9 us for 13 MB (a launch, and one trip to memory).
+// 1280 -> 5120 gated in bfloat16: 9.4 us for 26 MB (320 workgroups; 5 chunks a wave, four of them asked for together: two trips
+// to memory one after the other), 5120 -> 1280 8.8 us for 13 MB (80 workgroups on 256 units; 10 chunks a wave: up to four
+// trips).  The weights come from the last cache where the same call repeats.
 template <typename T, int ACT, int G>
 __global__ __launch_bounds__(1024) void k_few(int64_t M, int64_t N, int64_t K, const T* __restrict__ x, int64_t ldx,
                                               const T* __restrict__ w, int64_t ldw, Epilogue e) {
@@ -1215,7 +1221,9 @@ struct TileKind {
 // (8192 x 1280 x 10240, one round: 191 us, against 208 us in 160 tiles of 256 x 256) and 0.98 us with two of 128 x 128
 // (250 us for the first: twice the bytes from L2 for each operation).  Where not all units work, those that do run faster
 // (160 tiles: 1.30 us a step): the chip is held by its power.  A round costs about 7, 7 and 3 us besides, and split
-// parts are written and read back at about 4 TB/s, by one more launch.  In 32 bits a step of 32 takes 2.35 us with 256 x 128 and 1.25 us with
+// parts are written and read back at about 4 TB/s, by one more launch.  What the epilogue writes is not in it, so a gated
+// forward that keeps value and gate takes longer than it says, by whatever cut: 16384 x 320 -> 1280 72 us where it says 40,
+// 8192 x 1280 -> 5120 241 where it says 194, 4096 x 640 -> 2560 in 32 bits 172 where it says 145.  In 32 bits a step of 32 takes 2.35 us with 256 x 128 and 1.25 us with
 // 128 x 128 on each unit (4096 x 4096 x 2048: 284 to 329 us and 302 to 344 us, by the operands' layouts).
 constexpr TileKind kTiles16[] = {{Tile::k256x256, 256, 256, kUnits, 1.59, 7.0}, {Tile::k256x160, 256, 160, kUnits, 1.18, 7.0}, {Tile::k128x128, 128, 128, 2 * kUnits, 0.98, 3.0}};
 constexpr TileKind kTiles32[] = {{Tile::k256x128, 256, 128, kUnits, 2.35, 7.0}, {Tile::k128x128, 128, 128, kUnits, 1.25, 4.0}};

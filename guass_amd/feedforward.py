@@ -9,7 +9,9 @@ the field's dL/d(delta-W), and ``guass_amd.layers.GaussianFeedForward`` runs the
 
 Types: float32, bfloat16 and float16, one type for all of a call's tensors (under ``torch.autocast`` the products
 take its type, and a residual of another type is added by torch's rules); sums are accumulated in 32 bits.  Every call runs on torch's current stream of its tensors' device and does not synchronise.  A
-matrix whose last dimension is contiguous is read in place whatever its row stride is; others are copied.
+matrix whose last dimension is contiguous is taken whatever its row stride is; others are copied.  The products
+read 16-bit matrices in place whose rows begin at 16 bytes and are a multiple of 8 wide, and lay others out in the
+workspace first, as they do float32; of at most 64 rows the forward reads everything in place.
 float32 products go through the matrix cores as three bfloat16 planes of each operand (errors as of float32
 sums; an infinity times a number below 2^-100 may be a NaN); of at most 64 rows the forward multiplies
 float32 as such.
@@ -133,7 +135,8 @@ def gated_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activ
                  seed: int | Tensor = 0, offset: int = 0) -> Tensor:
     """dropout(value * activation(gate)) of x [..., in]: the first half of weight's rows [2 out, in] (and of bias
     [2 out]) makes the value, the second the gate.  ``activation``: "gelu" (by the error function), "gelu_tanh"
-    or "silu".  Where a gradient is wanted, value and gate are kept in x's type for the backward."""
+    or "silu".  Where a gradient is wanted, value and gate are kept for the backward: of bfloat16 in 20 bits each, of
+    float16 in 24, of float32 as they are."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {ACTIVATIONS} (got {activation!r})")
     _check_tensors(x=x, weight=weight)

@@ -501,7 +501,7 @@ int gf_selftest_softplus(uint64_t* checksum_host, void* stream);
  * multiplied by 65536 / (65536 - t).  No mask is stored: the backward makes it again.
  *
  * Matrices are row-major with unit column stride and a row stride (ld*, in elements) of at least their
- * width; all are of one type, `dtype`; products and sums are accumulated in 32 bits.  bias, residual and
+ * width, and at most 2^48 elements; all are of one type, `dtype`; products and sums are accumulated in 32 bits.  bias, residual and
  * the outputs that are not wanted are NULL.  dx [rows, in], dweight and dbias (shaped as weight and bias)
  * are written whole, contiguous; the residual's gradient is dy itself. */
 #define GF_DTYPE_F32 0

@@ -3,12 +3,13 @@
 Test infrastructure only.  ``linear`` and ``gated`` return every output with a bound, element by element, of
 the distance at which a right kernel can lie from it:
 
-* a sum of n products in 32 bits, each product to within 3 units of 2^-24 and taken in at most 6 parts, lies
-  within (6 n + 16) 2^-24 of its terms' absolute sum;
+* a sum of n products in 32 bits, each product to within 8 units of 2^-24 and taken in at most 6 parts, lies
+  within (6 n + 16) 2^-24 of its terms' absolute sum: 6 n additions, the 8 units, and 8 for the roundings after;
 * an activation or its slope is evaluated to within 2^-20 (1 + |gate|) absolutely, and moves by at most 1.2
   times its argument (the largest slope is 1.13, the largest second derivative 0.8);
 * a rounding to the tensors' type moves by u = eps / 2 of the value, or by half the smallest subnormal:
-  the outputs once, value, gate and dz (the products' gradient) once more each.
+  the outputs once, a gated dz (the products' gradient) once more.  The bounds allow one to value, gate and
+  a linear dz as well, more than a kernel needs that keeps value and gate in more bits and takes dy itself.
 """
 
 from __future__ import annotations
