@@ -215,7 +215,10 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight,
   auto shape = x.sizes().vec();
   shape.back() = weight.size(0) / (activation == GF_ACT_NONE ? 1 : 2);
   Tensor y = at::empty(shape, x.options()), saved, b;
-  if (y.numel() == 0) return {y, saved};
+  if (y.numel() == 0) {
+    if (save && activation != GF_ACT_NONE) saved = at::empty({0}, x.options().dtype(at::kByte));  // as a trace has it
+    return {y, saved};
+  }
   const c10::DeviceGuard guard(x.device());
   Products p(x, weight, activation, d);
   if (save && activation != GF_ACT_NONE) {

@@ -257,3 +257,30 @@ def test_phases_by_themselves_carry_no_gradient(device):
     t["x"].requires_grad_(True)
     y, saved = ff._linear_forward(t["x"], t["w"], None, None, "gelu", 0.0, 0, 0, True)
     assert not y.requires_grad and not saved.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", CALLS)
+def test_compiled_without_rows(device, op):
+    _say("compiled without rows", op)
+    call, names = CALLS[op]
+    torch._dynamo.reset()
+    ff._ops()
+    t = _inputs(device, rows=0)
+    t["x2"] = t["x"].clone()
+    leaves = [t[n].requires_grad_(True) for n in names]
+    y = torch.compile(lambda t: call(t) * 2, backend="aot_eager", fullgraph=True)(t)
+    assert y.shape[0] == 0
+    for leaf, grad in zip(leaves, torch.autograd.grad(y.sum(), leaves)):
+        assert grad.shape == leaf.shape and not bool(grad.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", CALLS)
+def test_inference_mode(device, op):
+    t = _inputs(device)
+    t["x2"] = t["x"].clone()
+    want = CALLS[op][0](t)
+    with torch.inference_mode():
+        u = {k: v * 1 for k, v in t.items()}
+        assert torch.equal(CALLS[op][0](u), want)
