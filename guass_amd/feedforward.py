@@ -27,6 +27,7 @@ captured graph draws anew at every replay if the program changes it between them
 
 from __future__ import annotations
 
+import threading
 from pathlib import Path
 
 import torch
@@ -40,13 +41,16 @@ __all__ = ["ACTIVATIONS", "dropout_add", "gated_linear", "linear_dropout_add"]
 
 
 _OPS = None
+_LOADING = threading.Lock()
 
 
 def _ops() -> tuple:
     """What _load found, once a process (a global: a trace reads it as it is)."""
     global _OPS
     if _OPS is None:
-        _OPS = _load()
+        with _LOADING:
+            if _OPS is None:
+                _OPS = _load()
     return _OPS
 
 

@@ -4,6 +4,10 @@ for, autocast, tracing.
 
 from __future__ import annotations
 
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -284,3 +288,30 @@ def test_inference_mode(device, op):
     with torch.inference_mode():
         u = {k: v * 1 for k, v in t.items()}
         assert torch.equal(CALLS[op][0](u), want)
+
+
+FIRST_CALLS = """
+import threading, time
+import torch
+from guass_amd import feedforward as ff
+load, results = torch.ops.load_library, []
+def slow(path):
+    time.sleep(0.2)
+    load(path)
+torch.ops.load_library = slow
+def call():
+    try:
+        results.append(ff._ops())
+    except Exception as e:
+        results.append(e)
+threads = [threading.Thread(target=call) for _ in range(8)]
+[t.start() for t in threads], [t.join() for t in threads]
+assert len(results) == 8 and all(r is results[0] for r in results), results
+"""
+
+
+def test_first_calls_from_many_threads():
+    """The operators are loaded and their shape functions registered once, whoever comes first."""
+    proc = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=Path(__file__).resolve().parent.parent, capture_output=True,
+                          text=True, timeout=300)
+    assert proc.returncode == 0, proc.stderr[-2000:]
