@@ -21,66 +21,9 @@
 #include <type_traits>
 #include <utility>
 
-#include "../../include/gaussfield.h"
-#include "error.h"
+#include "elements.h"
 
 namespace {
-
-using bf16 = __bf16;
-using f16 = _Float16;
-
-template <typename... A>
-int fail(int code, const char* fmt, A... a) {
-  char msg[512];
-  snprintf(msg, sizeof(msg), fmt, a...);
-  return gf_set_error(code, msg);
-}
-int fail(int code, const char* msg) { return gf_set_error(code, msg); }
-
-#define FF_LAUNCH_CHECK(name)                                                                    \
-  do {                                                                                           \
-    hipError_t e_ = hipGetLastError();                                                           \
-    if (e_ != hipSuccess) return fail(GF_E_HIP, "launch of %s failed: %s", name, hipGetErrorString(e_)); \
-  } while (0)
-
-// 8 consecutive elements in 32 bits: 16 bytes (two times 16) a lane at whatever alignment, which global memory takes,
-// or where they are not `all` there the first n, one by one.
-template <typename T, int N>
-using Vec = T __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-
-template <typename T>
-__device__ inline void load8(float v[8], const T* p, bool all, int n) {
-  constexpr int W = 16 / sizeof(T);
-  if (all) {
-#pragma unroll
-    for (int i = 0; i < 8; i += W) {
-      const Vec<T, W> t = *(const Vec<T, W>*)(p + i);
-#pragma unroll
-      for (int j = 0; j < W; ++j) v[i + j] = (float)t[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.0f;
-  }
-}
-
-template <typename T>
-__device__ inline void store8(T* p, const float v[8], bool all, int n) {
-  constexpr int W = 16 / sizeof(T);
-  if (all) {
-#pragma unroll
-    for (int i = 0; i < 8; i += W) {
-      Vec<T, W> t;
-#pragma unroll
-      for (int j = 0; j < W; ++j) t[j] = (T)v[i + j];
-      *(Vec<T, W>*)(p + i) = t;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = (T)v[j];
-  }
-}
 
 // ------------------------------------------------------------------------------------------
 // Dropout.
@@ -159,53 +102,6 @@ __global__ __launch_bounds__(256) void k_dropout(Drop d, int64_t rows, int64_t c
     if (group >= groups) group -= groups, ++row;
   }
 }
-
-// ------------------------------------------------------------------------------------------
-// Activations: act(g), and with it act'(g).  Exponentials and reciprocals are the hardware's (1 unit in the last place).
-
-__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ inline float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
-
-// Phi(-a) e^(a^2/2) for a >= 0 as t Q(t), t = 1 / (1 + p a): p and Q fitted (least squares reweighted to the largest
-// relative error) over a in [0, 14]: good to 1.4e-7 with p and Q as floats, and to 3.7e-7 as evaluated in 32 bits (7.4e-7 if
-// the reciprocal is a unit off); past that Phi(-a) is below the smallest float.
-__device__ inline float normal_tail(float a) {
-  const float t = rcp_fast(__builtin_fmaf(0.3045656383f, a, 1.0f));
-  float q = 0.0367617272f;
-  q = __builtin_fmaf(q, t, -0.153960079f);
-  q = __builtin_fmaf(q, t, 0.188459948f);
-  q = __builtin_fmaf(q, t, -0.0401414931f);
-  q = __builtin_fmaf(q, t, 0.122078776f);
-  q = __builtin_fmaf(q, t, 0.103001416f);
-  q = __builtin_fmaf(q, t, 0.122335792f);
-  q = __builtin_fmaf(q, t, 0.121463954f);
-  return q * t;
-}
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-template <int ACT>
-__device__ inline float activation(float g, float* slope) {
-  if constexpr (ACT == GF_ACT_GELU) {  // g Phi(g); Phi' = e^(-g^2/2) / sqrt(2 pi)
-    const float e = exp2_fast(-0.5f * kLog2e * g * g), tail = normal_tail(fabsf(g)) * e;
-    const float cdf = g < 0.0f ? tail : 1.0f - tail;
-    if (slope != nullptr) *slope = __builtin_fmaf(0.39894228040143268f * g, e, cdf);
-    return g * cdf;
-  } else if constexpr (ACT == GF_ACT_SILU) {  // g s, s = 1 / (1 + e^-g); s' = s (1 - s)
-    const float s = rcp_fast(1.0f + exp2_fast(-kLog2e * g));
-    if (slope != nullptr) *slope = __builtin_fmaf(g * s, 1.0f - s, s);
-    return g * s;
-  } else {  // (1 + tanh u) / 2 = 1 / (1 + e^-2u), u = sqrt(2/pi) (g + 0.044715 g^3)
-    constexpr float c = 1.5957691216057308f;
-    const float sq = fminf(0.044715f * g * g, 1e30f);  // finite: where it would not be, s (1 - s) is 0
-    const float s = rcp_fast(1.0f + exp2_fast(-c * kLog2e * g * (1.0f + sq)));
-    if (slope != nullptr) *slope = __builtin_fmaf(g * s * (1.0f - s), c * __builtin_fmaf(3.0f, sq, 1.0f), s);
-    return g * s;
-  }
-}
-
-template <int ACT>
-using ActTag = std::integral_constant<int, ACT>;
 
 // ------------------------------------------------------------------------------------------
 // Products.  C[m, n] = sum over k of P(m, k) Q(n, k) on the matrix cores, accumulated in 32 bits.
@@ -1062,10 +958,6 @@ __global__ __launch_bounds__(256) void k_join_sums(int64_t chunks, int64_t cols,
 // ------------------------------------------------------------------------------------------
 // Host.
 
-int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-
-int size_of(int32_t dtype) { return dtype == GF_DTYPE_F32 ? 4 : 2; }
-
 int check_dropout(const gf_dropout* d) {
   if (d == nullptr) return fail(GF_E_INVALID_ARGUMENT, "dropout must not be NULL");
   if (!(d->p >= 0.0 && d->p <= 1.0)) return fail(GF_E_INVALID_ARGUMENT, "dropout p must lie in [0, 1]");
@@ -1082,39 +974,9 @@ Drop make_drop(const gf_dropout& d) {
   return r;
 }
 
-constexpr int64_t kMaxSize = INT32_MAX;
-// Elements of a matrix, its row stride's gaps among them: more than a memory has, and 64 bits hold the bytes of all that is
-// made of one (planes, parts: at most 2^7 bytes an element).
-constexpr int64_t kMaxElements = int64_t(1) << 48;
-
-int check_matrix(const char* name, const void* p, int64_t rows, int64_t ld, int64_t width, int size) {
-  if (p == nullptr) return fail(GF_E_INVALID_ARGUMENT, "%s must not be NULL", name);
-  if (rows > 1 && ld > kMaxElements / rows) return fail(GF_E_INVALID_ARGUMENT, "%s: too large", name);
-  if (ld < width) return fail(GF_E_INVALID_ARGUMENT, "%s: row stride %lld is below its width %lld", name, (long long)ld, (long long)width);
-  if ((uintptr_t)p % size != 0) return fail(GF_E_INVALID_ARGUMENT, "%s is not aligned to its type", name);
-  return GF_OK;
-}
-
-int check_workspace(size_t need, const void* workspace, size_t bytes) {
-  if (bytes < need || (need != 0 && workspace == nullptr))
-    return fail(GF_E_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? bytes : size_t(0), need);
-  if ((uintptr_t)workspace % 16 != 0) return fail(GF_E_INVALID_ARGUMENT, "workspace is not 16-byte aligned");
-  return GF_OK;
-}
-
-#define FF_CHECK(expr)                 \
-  do {                                 \
-    if (int rc_ = (expr)) return rc_;  \
-  } while (0)
-
-int check_dtype(int32_t dtype) {
-  if (dtype < GF_DTYPE_F32 || dtype > GF_DTYPE_F16) return fail(GF_E_INVALID_ARGUMENT, "unknown dtype %d", (int)dtype);
-  return GF_OK;
-}
-
 int check_shape(const gf_ff_args* a) {
   if (a == nullptr) return fail(GF_E_INVALID_ARGUMENT, "args must not be NULL");
-  FF_CHECK(check_dtype(a->dtype));
+  GF_TRY(check_dtype(a->dtype));
   if (a->activation < GF_ACT_NONE || a->activation > GF_ACT_SILU)
     return fail(GF_E_INVALID_ARGUMENT, "unknown activation %d", (int)a->activation);
   if (a->rows < 0 || a->in_features <= 0 || a->out_features <= 0)
@@ -1132,46 +994,12 @@ int check_shape(const gf_ff_args* a) {
 int64_t weight_rows(const gf_ff_args* a) { return a->out_features * (a->activation == GF_ACT_NONE ? 1 : 2); }
 int64_t saved_ld(const gf_ff_args* a) { return round_up(a->out_features, 8); }
 
-template <typename F>
-int with_dtype(int32_t dtype, F f) {
-  switch (dtype) {
-    case GF_DTYPE_F32: return f(float());
-    case GF_DTYPE_BF16: return f(bf16());
-    default: return f(f16());
-  }
-}
-
-template <typename F>
-int with_activation(int32_t act, F f) {
-  switch (act) {
-    case GF_ACT_NONE: return f(ActTag<GF_ACT_NONE>());
-    case GF_ACT_GELU: return f(ActTag<GF_ACT_GELU>());
-    case GF_ACT_GELU_TANH: return f(ActTag<GF_ACT_GELU_TANH>());
-    default: return f(ActTag<GF_ACT_SILU>());
-  }
-}
-
-unsigned blocks_for(int64_t threads) { return (unsigned)std::min<int64_t>(std::max<int64_t>((threads + 255) / 256, 1), 8192); }
-
 bool aligned(const void* p, int64_t ld, int size) { return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0; }
-
-// Hands out a workspace from its start; without one it only counts.
-struct Arena {
-  uint8_t* base;
-  size_t used = 0;
-  void* take(int64_t bytes) {
-    void* p = base ? base + used : nullptr;
-    used += (size_t)round_up(bytes, 256);
-    return p;
-  }
-};
 
 template <typename T>
 bool reads_in_place(const void* x, int64_t cols, int64_t ld) {
   return !std::is_same_v<T, float> && aligned(x, ld, 2) && cols % 8 == 0;
 }
-
-#define FF_RUN if (run)  // nothing is launched while the workspace is counted
 
 // The matrices that have to be packed, and their launch.
 struct Packs {
@@ -1192,11 +1020,11 @@ Matrix operand(Arena& ws, Packs& packs, const void* x, int64_t rows, int64_t col
 
 template <typename T>
 int pack(bool run, const Packs& packs, hipStream_t s) {
-  FF_RUN if (packs.n != 0) {
+  GF_RUN if (packs.n != 0) {
     unsigned blocks[2] = {};
     for (int i = 0; i < packs.n; ++i) blocks[i] = blocks_for(packs.job[i].rows * packs.job[i].ld / 8);
     k_pack<T><<<blocks[0] + blocks[1], 256, 0, s>>>(packs.job[0], packs.job[packs.n - 1], blocks[0]);
-    FF_LAUNCH_CHECK("k_pack");
+    GF_LAUNCH_CHECK("k_pack");
   }
   return GF_OK;
 }
@@ -1262,12 +1090,12 @@ int product_tiled(Arena& ws, bool run, int64_t M, int64_t N, int64_t K, const Ma
   const bool join = sh.splits > 1;
   e.partial = nullptr;
   if (join) e.partial = (float*)ws.take(sh.splits * M * round_up(N, 8) * (ACT == GF_ACT_NONE ? 1 : 2) * 4);
-  FF_RUN {
+  GF_RUN {
     k_product<T, PKC, QKC, ACT, WM, WN, TM, TN><<<dim3((unsigned)(tm * tn), (unsigned)sh.splits), WM * WN * 64, 0, s>>>(sh, p, q, second, e);
-    FF_LAUNCH_CHECK("k_product");
+    GF_LAUNCH_CHECK("k_product");
     if (join) {
       k_join<T, ACT><<<blocks_for(M * ((N + 7) / 8)), 256, 0, s>>>(sh, e);
-      FF_LAUNCH_CHECK("k_join");
+      GF_LAUNCH_CHECK("k_join");
     }
   }
   return GF_OK;
@@ -1303,7 +1131,7 @@ int few(const gf_ff_args& a, const Epilogue& e, hipStream_t s) {
   const unsigned threads = a.in_features * (int64_t)sizeof(T) >= 16 * 4 * 64 ? 1024 : 512;
   auto* kernel = a.rows <= 16 ? k_few<T, ACT, 1> : a.rows <= 32 ? k_few<T, ACT, 2> : k_few<T, ACT, 4>;
   kernel<<<grid, threads, 0, s>>>(a.rows, a.out_features, a.in_features, (const T*)a.x, a.ldx, (const T*)a.weight, a.ldw, e);
-  FF_LAUNCH_CHECK("k_few");
+  GF_LAUNCH_CHECK("k_few");
   return GF_OK;
 }
 
@@ -1314,13 +1142,13 @@ int forward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
     return with_activation(a.activation, [&](auto act) {
       const Epilogue e{a.y, a.bias, a.residual, a.ldr, a.saved, saved_ld(&a), nullptr, make_drop(a.dropout)};
       if (a.rows <= 64) {
-        FF_RUN return few<T, act.value>(a, e, s);
+        GF_RUN return few<T, act.value>(a, e, s);
         return (int)GF_OK;
       }
       Packs packs;
       const Matrix x = operand<T>(ws, packs, a.x, a.rows, a.in_features, a.ldx);
       const Matrix w = operand<T>(ws, packs, a.weight, weight_rows(&a), a.in_features, a.ldw);
-      FF_CHECK(pack<T>(run, packs, s));
+      GF_TRY(pack<T>(run, packs, s));
       return product<T, true, true, act.value>(ws, run, a.rows, a.out_features, a.in_features, x, w, a.out_features, e, s);
     });
   });
@@ -1358,37 +1186,37 @@ int backward(const gf_ff_args& a, Arena& ws, bool run, hipStream_t s) {
         const int peak_blocks = (int)std::min<int64_t>((a.rows * ((out + 7) / 8) + 255) / 256, kPeaks);
         if (kScaledDz<T, ACT> && make) {
           peaks = (float*)ws.take((kPeaks + 1) * 4);
-          FF_RUN e.scale_at = peaks + kPeaks;
+          GF_RUN e.scale_at = peaks + kPeaks;
         }
         float* sums = a.dbias != nullptr && chunks > 1 ? (float*)ws.take(chunks * wr * 4) : nullptr;
-        FF_RUN {
+        GF_RUN {
           if constexpr (kScaledDz<T, ACT>) {
             if (make) {
               k_peak<T, ACT><<<peak_blocks, 256, 0, s>>>(drop, a.rows, out, (const T*)a.dy, a.lddy, a.saved, saved_ld(&a), peaks);
-              FF_LAUNCH_CHECK("k_peak");
+              GF_LAUNCH_CHECK("k_peak");
             }
           }
           k_dz<T, ACT><<<dim3((unsigned)across, (unsigned)chunks), 256, 0, s>>>(
               drop, a.rows, out, chunk, (const T*)a.dy, a.lddy, a.saved, saved_ld(&a), make ? (void*)dz.p : nullptr, dz.ld, dz.plane, sums,
               sums == nullptr ? (T*)a.dbias : nullptr, e.scale, peaks, peak_blocks);
-          FF_LAUNCH_CHECK("k_dz");
+          GF_LAUNCH_CHECK("k_dz");
           if (sums != nullptr) {
             k_join_sums<T><<<(unsigned)((wr + 31) / 32), 256, 0, s>>>(chunks, wr, sums, (T*)a.dbias);
-            FF_LAUNCH_CHECK("k_join_sums");
+            GF_LAUNCH_CHECK("k_join_sums");
           }
         }
       }
       Matrix w{}, x{};
       if (a.dx != nullptr) w = operand<T>(ws, packs, a.weight, wr, a.in_features, a.ldw);
       if (a.dweight != nullptr) x = operand<T>(ws, packs, a.x, a.rows, a.in_features, a.ldx);
-      FF_CHECK(pack<T>(run, packs, s));
+      GF_TRY(pack<T>(run, packs, s));
       if (a.dx != nullptr) {
         e.out = a.dx;
-        FF_CHECK((product<T, true, false, GF_ACT_NONE>(ws, run, a.rows, a.in_features, wr, dz, w, 0, e, s)));
+        GF_TRY((product<T, true, false, GF_ACT_NONE>(ws, run, a.rows, a.in_features, wr, dz, w, 0, e, s)));
       }
       if (a.dweight != nullptr) {
         e.out = a.dweight;
-        FF_CHECK((product<T, false, false, GF_ACT_NONE>(ws, run, wr, a.in_features, a.rows, dz, x, 0, e, s)));
+        GF_TRY((product<T, false, false, GF_ACT_NONE>(ws, run, wr, a.in_features, a.rows, dz, x, 0, e, s)));
       }
       return (int)GF_OK;
     });
@@ -1401,20 +1229,20 @@ extern "C" {
 
 int gf_dropout_add(int32_t dtype, const gf_dropout* dropout, int64_t rows, int64_t cols, const void* x, int64_t ldx,
                    const void* residual, int64_t ldr, void* y, int64_t ldy, void* stream) {
-  FF_CHECK(check_dtype(dtype));
-  FF_CHECK(check_dropout(dropout));
+  GF_TRY(check_dtype(dtype));
+  GF_TRY(check_dropout(dropout));
   if (rows < 0 || cols < 0 || rows > kMaxSize || cols > kMaxSize) return fail(GF_E_INVALID_ARGUMENT, "rows or cols negative or too large");
   if (rows == 0 || cols == 0) return GF_OK;
-  FF_CHECK(check_matrix("x", x, rows, ldx, cols, size_of(dtype)));
-  FF_CHECK(check_matrix("y", y, rows, ldy, cols, size_of(dtype)));
-  if (residual != nullptr) FF_CHECK(check_matrix("residual", residual, rows, ldr, cols, size_of(dtype)));
+  GF_TRY(check_matrix("x", x, rows, ldx, cols, size_of(dtype)));
+  GF_TRY(check_matrix("y", y, rows, ldy, cols, size_of(dtype)));
+  if (residual != nullptr) GF_TRY(check_matrix("residual", residual, rows, ldr, cols, size_of(dtype)));
   const Drop d = make_drop(*dropout);
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     auto* kernel = residual != nullptr ? k_dropout<T, true> : k_dropout<T, false>;
     kernel<<<blocks_for(rows * ((cols + 7) / 8)), 256, 0, (hipStream_t)stream>>>(d, rows, cols, (const T*)x, ldx, (const T*)residual, ldr, (T*)y,
                                                                                  ldy);
-    FF_LAUNCH_CHECK("k_dropout");
+    GF_LAUNCH_CHECK("k_dropout");
     return (int)GF_OK;
   });
 }
@@ -1433,36 +1261,36 @@ size_t gf_ff_workspace_bytes(const gf_ff_args* args, int32_t is_backward) {
 }
 
 int gf_ff_forward(const gf_ff_args* args, void* workspace, size_t workspace_bytes, void* stream) {
-  FF_CHECK(check_shape(args));
+  GF_TRY(check_shape(args));
   const gf_ff_args& a = *args;
   if (a.rows == 0) return GF_OK;
   const int size = size_of(a.dtype);
-  FF_CHECK(check_matrix("x", a.x, a.rows, a.ldx, a.in_features, size));
-  FF_CHECK(check_matrix("weight", a.weight, weight_rows(&a), a.ldw, a.in_features, size));
-  FF_CHECK(check_matrix("y", a.y, a.rows, a.out_features, a.out_features, size));
+  GF_TRY(check_matrix("x", a.x, a.rows, a.ldx, a.in_features, size));
+  GF_TRY(check_matrix("weight", a.weight, weight_rows(&a), a.ldw, a.in_features, size));
+  GF_TRY(check_matrix("y", a.y, a.rows, a.out_features, a.out_features, size));
   if (a.residual != nullptr) {
     if (a.activation != GF_ACT_NONE) return fail(GF_E_INVALID_ARGUMENT, "a gated product takes no residual");
-    FF_CHECK(check_matrix("residual", a.residual, a.rows, a.ldr, a.out_features, size));
+    GF_TRY(check_matrix("residual", a.residual, a.rows, a.ldr, a.out_features, size));
   }
-  if (a.saved != nullptr) FF_CHECK(check_matrix("saved", a.saved, 1, 1, 1, 16));
+  if (a.saved != nullptr) GF_TRY(check_matrix("saved", a.saved, 1, 1, 1, 16));
   Arena count{nullptr}, ws{(uint8_t*)workspace};
-  FF_CHECK(forward(a, count, false, nullptr));
-  FF_CHECK(check_workspace(count.used, workspace, workspace_bytes));
+  GF_TRY(forward(a, count, false, nullptr));
+  GF_TRY(check_workspace(count.used, workspace, workspace_bytes));
   return forward(a, ws, true, (hipStream_t)stream);
 }
 
 int gf_ff_backward(const gf_ff_args* args, void* workspace, size_t workspace_bytes, void* stream) {
-  FF_CHECK(check_shape(args));
+  GF_TRY(check_shape(args));
   const gf_ff_args& a = *args;
   const int size = size_of(a.dtype);
-  FF_CHECK(check_matrix("x", a.x, a.rows, a.ldx, a.in_features, size));
-  FF_CHECK(check_matrix("weight", a.weight, weight_rows(&a), a.ldw, a.in_features, size));
-  FF_CHECK(check_matrix("dy", a.dy, a.rows, a.lddy, a.out_features, size));
-  if (a.activation != GF_ACT_NONE) FF_CHECK(check_matrix("saved", a.saved, 1, 1, 1, 16));
+  GF_TRY(check_matrix("x", a.x, a.rows, a.ldx, a.in_features, size));
+  GF_TRY(check_matrix("weight", a.weight, weight_rows(&a), a.ldw, a.in_features, size));
+  GF_TRY(check_matrix("dy", a.dy, a.rows, a.lddy, a.out_features, size));
+  if (a.activation != GF_ACT_NONE) GF_TRY(check_matrix("saved", a.saved, 1, 1, 1, 16));
   if (a.rows == 0) return fail(GF_E_INVALID_ARGUMENT, "a backward needs rows");
   Arena count{nullptr}, ws{(uint8_t*)workspace};
-  FF_CHECK(backward(a, count, false, nullptr));
-  FF_CHECK(check_workspace(count.used, workspace, workspace_bytes));
+  GF_TRY(backward(a, count, false, nullptr));
+  GF_TRY(check_workspace(count.used, workspace, workspace_bytes));
   return backward(a, ws, true, (hipStream_t)stream);
 }
 
