@@ -36,6 +36,8 @@ EXPORTED = (
     "gf_forward_grads_offset", "gf_backward_direct_launches", "gf_fwd_bwd_fused", "gf_fwd_bwd_fused_supported",
     "gf_forward_kcap", "gf_backward_direct_kcap", "gf_forward_bin_info", "gf_read_bin_info", "gf_backward_train",
     "gf_dropout_add", "gf_ff_saved_bytes", "gf_ff_workspace_bytes", "gf_ff_forward", "gf_ff_backward",
+    "gf_norm_forward", "gf_norm_workspace_bytes", "gf_norm_backward",
+    "gf_q4_quantize", "gf_q4_dequantize", "gf_q4_saved_bytes", "gf_q4_workspace_bytes", "gf_q4_forward", "gf_q4_backward",
 )
 
 GF_PHASE_BIN, GF_PHASE_EMIT, GF_PHASE_RENDER = 0x1, 0x2, 0x4
@@ -43,6 +45,7 @@ GF_PHASE_REDUCE, GF_PHASE_FINISH = 0x1, 0x2
 GF_PHASE_ALL = 0xFF
 
 GF_ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}
+GF_NORMS = {None: 0, "layer": 1, "rms": 2}
 
 
 class GfFieldConfig(ctypes.Structure):
@@ -106,6 +109,32 @@ class GfFfArgs(ctypes.Structure):
         ("bias", c_void_p), ("residual", c_void_p), ("ldr", c_int64), ("y", c_void_p), ("saved", c_void_p),
         ("dy", c_void_p), ("lddy", c_int64), ("dx", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p),
         ("dropout", GfDropout),
+    ]
+
+
+class GfNormArgs(ctypes.Structure):
+    """``gf_norm_args``: the norms before and after a block (device pointers)."""
+
+    _fields_ = [
+        ("dtype", c_int32), ("kind", c_int32), ("next_kind", c_int32), ("reserved", c_int32), ("rows", c_int64), ("cols", c_int64),
+        ("group_rows", c_int64), ("eps", c_double), ("next_eps", c_double), ("gate_value", c_double),
+        ("residual_scale", c_double), ("x", c_void_p), ("ldx", c_int64), ("residual", c_void_p), ("ldr", c_int64),
+        ("weight", c_void_p), ("bias", c_void_p), ("gate", c_void_p), ("ld_gate", c_int64), ("next_weight", c_void_p),
+        ("next_bias", c_void_p), ("scale", c_void_p), ("ld_scale", c_int64), ("shift", c_void_p), ("ld_shift", c_int64),
+        ("stream", c_void_p), ("normed", c_void_p), ("dstream", c_void_p), ("ld_dstream", c_int64), ("dnormed", c_void_p),
+        ("ld_dnormed", c_int64), ("dx", c_void_p), ("dresidual", c_void_p), ("dweight", c_void_p), ("dbias", c_void_p),
+        ("dgate", c_void_p), ("dnext_weight", c_void_p), ("dnext_bias", c_void_p), ("dscale", c_void_p), ("dshift", c_void_p),
+    ]
+
+
+class GfQ4Args(ctypes.Structure):
+    """``gf_q4_args``: a product with a 4-bit weight (device pointers)."""
+
+    _fields_ = [
+        ("dtype", c_int32), ("activation", c_int32), ("rows", c_int64), ("in_features", c_int64), ("out_features", c_int64),
+        ("x", c_void_p), ("ldx", c_int64), ("codes", c_void_p), ("scales", c_void_p), ("bias", c_void_p),
+        ("residual", c_void_p), ("ldr", c_int64), ("y", c_void_p), ("saved", c_void_p), ("dy", c_void_p), ("lddy", c_int64),
+        ("dx", c_void_p), ("dbias", c_void_p),
     ]
 
 
@@ -187,13 +216,26 @@ def lib() -> ctypes.CDLL:
     L.gf_ff_workspace_bytes.restype = c_size_t
     L.gf_ff_forward.argtypes = [POINTER(GfFfArgs), _P, c_size_t, _P]
     L.gf_ff_backward.argtypes = [POINTER(GfFfArgs), _P, c_size_t, _P]
+    L.gf_norm_forward.argtypes = [POINTER(GfNormArgs), _P]
+    L.gf_norm_workspace_bytes.argtypes = [POINTER(GfNormArgs)]
+    L.gf_norm_workspace_bytes.restype = c_size_t
+    L.gf_norm_backward.argtypes = [POINTER(GfNormArgs), _P, c_size_t, _P]
+    L.gf_q4_quantize.argtypes = [c_int32, c_int64, c_int64, _P, c_int64, _P, _P, _P]
+    L.gf_q4_dequantize.argtypes = [c_int32, c_int64, c_int64, _P, _P, _P, _P]
+    L.gf_q4_saved_bytes.argtypes = [POINTER(GfQ4Args)]
+    L.gf_q4_saved_bytes.restype = c_size_t
+    L.gf_q4_workspace_bytes.argtypes = [POINTER(GfQ4Args), c_int32]
+    L.gf_q4_workspace_bytes.restype = c_size_t
+    L.gf_q4_forward.argtypes = [POINTER(GfQ4Args), _P, c_size_t, _P]
+    L.gf_q4_backward.argtypes = [POINTER(GfQ4Args), _P, c_size_t, _P]
     for name in ("gf_tile_grid", "gf_forward_bin", "gf_forward_emit", "gf_forward_render",
                  "gf_backward", "gf_backward_reduce", "gf_backward_finish", "gf_read_status",
                  "gf_selftest_softplus", "gf_batch_plan", "gf_batch_forward", "gf_batch_backward",
                  "gf_batch_set_grads", "gf_batch_read", "gf_backward_noalloc", "gf_forward",
                  "gf_backward_direct", "gf_fwd_bwd_fused", "gf_forward_kcap", "gf_backward_direct_kcap",
                  "gf_forward_bin_info", "gf_read_bin_info", "gf_backward_train",
-                 "gf_dropout_add", "gf_ff_forward", "gf_ff_backward"):
+                 "gf_dropout_add", "gf_ff_forward", "gf_ff_backward", "gf_norm_forward", "gf_norm_backward",
+                 "gf_q4_quantize", "gf_q4_dequantize", "gf_q4_forward", "gf_q4_backward"):
         getattr(L, name).restype = c_int
     _LIB = L
     return L

@@ -1,8 +1,9 @@
 """Builds the native libraries in-tree.
 
 * ``guass_amd/libgaussfield.so``       gfx950 kernels + C ABI (hipcc, --offload-arch=gfx950): the fields'
-                                       (gaussfield.hip) and the feed-forward block's (feedforward.hip)
-* ``guass_amd/libguass_torch.so``       the feed-forward operators as torch operators over it (g++)
+                                       (gaussfield.hip), the feed-forward block's (feedforward.hip), the norms
+                                       around a block (norms.hip) and 4-bit weights (quantized.hip)
+* ``guass_amd/libguass_torch.so``       the block's operators as torch operators over it (g++)
 * ``guass_amd/libgaussfield_host.so``  host build of the per-Gaussian geometry (g++), used by
                                        CPU tests to pin the exact arithmetic the GPU runs
 * ``oracle/_build/libm_sweep``         exhaustive libm check (test infrastructure)
@@ -26,7 +27,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
-GPU_SOURCES = [CSRC / "gaussfield.hip", CSRC / "feedforward.hip"]
+GPU_SOURCES = [CSRC / "gaussfield.hip", CSRC / "norms.hip", CSRC / "feedforward.hip", CSRC / "quantized.hip"]
+TORCH_SOURCES = [CSRC / "torch_ops.cpp", CSRC / "torch_block_ops.cpp"]
 LIB = PKG / "libgaussfield.so"
 HOST_LIB = PKG / "libgaussfield_host.so"
 TORCH_LIB = PKG / "libguass_torch.so"
@@ -83,13 +85,16 @@ def build_torch_lib() -> Path:
 
     home = Path(torch.__file__).parent
     rocm = Path(hipcc()).resolve().parent.parent
-    tmp = TORCH_LIB.with_suffix(".so.tmp")
-    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{home / 'include'}",
-          f"-I{home / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{rocm / 'include'}", str(CSRC / "torch_ops.cpp"),
-          "-o", str(tmp), f"-L{home / 'lib'}", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
-          str(LIB), "-Wl,-rpath,$ORIGIN"])
-    os.replace(tmp, TORCH_LIB)
+    new = TORCH_LIB.with_suffix(".so.tmp")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{home / 'include'}",
+             f"-I{home / 'include' / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{rocm / 'include'}"]
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor() as pool:
+        objects = [Path(tmp) / f"{src.stem}.o" for src in TORCH_SOURCES]
+        list(pool.map(lambda so: _run(["g++", *flags, "-c", str(so[0]), "-o", str(so[1])]), zip(TORCH_SOURCES, objects)))
+        _run(["g++", "-shared", *map(str, objects), "-o", str(new), f"-L{home / 'lib'}", "-ltorch_cpu", "-ltorch_hip", "-lc10",
+              "-lc10_hip", str(LIB), "-Wl,-rpath,$ORIGIN"])
+    os.replace(new, TORCH_LIB)
     return TORCH_LIB
 
 

@@ -2,78 +2,15 @@
 // workspaces and autograd around the C ABI of libgaussfield.so.  In C++ because a small call is all latency: the
 // backward runs on autograd's own thread, where the same work in Python took 40 us more (64 x 1280 dropout, forward and
 // backward: 96 us from Python, 48 us of them autograd's own).
-#include <ATen/ATen.h>
-#include <ATen/autocast_mode.h>
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <c10/core/AutogradState.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/library.h>
-
-#include <optional>
-#include <tuple>
-
-#include "../../include/gaussfield.h"
+#include "torch_common.h"
 
 namespace {
-
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-using MaybeTensor = std::optional<Tensor>;
-
-void check_rc(int rc, const char* what) { TORCH_CHECK(rc == GF_OK, what, ": ", gf_last_error(), " (code ", rc, ")"); }
-
-const char* type_name(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return "torch.float32";
-    case at::kBFloat16: return "torch.bfloat16";
-    case at::kHalf: return "torch.float16";
-    default: return c10::toString(t);
-  }
-}
-
-int dtype_of(const Tensor& x) {
-  return x.scalar_type() == at::kFloat ? GF_DTYPE_F32 : x.scalar_type() == at::kBFloat16 ? GF_DTYPE_BF16 : GF_DTYPE_F16;
-}
-
-void check_first(const Tensor& x) {
-  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
-  const auto t = x.scalar_type();
-  TORCH_CHECK(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "x must be float32, bfloat16 or float16 (got ", type_name(t), ")");
-}
-
-void check_like(const Tensor& t, const char* name, const Tensor& x) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-  TORCH_CHECK(t.scalar_type() == x.scalar_type(), name, " must be ", type_name(x.scalar_type()), " like x (got ", type_name(t.scalar_type()), ")");
-  TORCH_CHECK(t.device() == x.device(), "all tensors must be on the same device (got ", x.device(), " and ", t.device(), ")");
-}
-
-bool present(const MaybeTensor& t) { return t.has_value() && t->defined(); }
 
 void check_seed(const MaybeTensor& seed, const Tensor& x) {
   if (present(seed))
     TORCH_CHECK(seed->scalar_type() == at::kLong && seed->numel() == 1 && seed->device() == x.device(),
                 "a seed tensor must be one int64 element on x's device");
 }
-
-// A tensor as a matrix of its last dimension's rows with unit column stride: itself wherever it can be read so.
-struct Rows {
-  Tensor t;
-  int64_t rows, cols, ld;
-  explicit Rows(const Tensor& x) : t(x), rows(0), cols(x.size(-1)), ld(cols) {
-    if (!t.is_contiguous()) {
-      if (t.dim() != 2) t = t.reshape({-1, cols});
-      if ((t.stride(1) != 1 && cols > 1) || (t.stride(0) < cols && t.size(0) > 1)) t = t.contiguous();
-      if (t.size(0) > 1) ld = t.stride(0);
-    }
-    rows = cols ? t.numel() / cols : 0;
-  }
-  const void* data() const { return t.data_ptr(); }
-};
-
-void* stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().index()).stream(); }
 
 gf_dropout make_dropout(double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
   return {p, (uint64_t)seed, present(seed_tensor) ? (const uint64_t*)seed_tensor->data_ptr() : nullptr, (uint64_t)offset};
@@ -110,15 +47,6 @@ Tensor call_dropout_forward(const Tensor& x, const MaybeTensor& residual, double
   return op.call(x, residual, p, seed, seed_tensor, offset);
 }
 
-// Gradients of a first backward that refuse a second one.
-variable_list once(variable_list grads, const char* name, bool again) {
-  if (!at::GradMode::is_enabled() || !again) return grads;
-  for (auto& g : grads)
-    if (g.defined()) g = g.detach().set_requires_grad(true);
-  const auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once only", grads.size());
-  return (*error)(std::move(grads));
-}
-
 struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& residual, double p, int64_t seed,
                         const MaybeTensor& seed_tensor, int64_t offset) {
@@ -138,17 +66,6 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     return once({dx, want_r ? dy : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, "dropout_add", again);
   }
 };
-
-bool wants(const Tensor& t) { return t.requires_grad(); }
-bool wants(const MaybeTensor& t) { return present(t) && t->requires_grad(); }
-
-// There is no forward-mode derivative: a tangent must not get lost, whether or not gradients are wanted too.
-template <typename... M>
-void check_no_tangent(const char* name, const Tensor& x, const M&... others) {
-  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-  const bool tangent = x._fw_grad(0).defined() || (... || (present(others) && others->_fw_grad(0).defined()));
-  TORCH_CHECK_NOT_IMPLEMENTED(!tangent, name, " has no forward-mode derivative");
-}
 
 Tensor dropout_add(const Tensor& x, const MaybeTensor& residual, double p, int64_t seed, const MaybeTensor& seed_tensor, int64_t offset) {
   check_dropout(x, residual, seed_tensor);
@@ -279,8 +196,6 @@ std::tuple<Tensor, Tensor, Tensor> call_linear_backward(const Tensor& x, const T
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("guass_amd::linear_backward", "").typed<decltype(linear_backward)>();
   return op.call(x, weight, saved, dy, activation, p, seed, seed_tensor, offset, want_x, want_w, want_b);
 }
-
-MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
 
 struct Linear : torch::autograd::Function<Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual,

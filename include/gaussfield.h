@@ -549,6 +549,98 @@ size_t gf_ff_workspace_bytes(const gf_ff_args* args, int32_t backward);
 int gf_ff_forward(const gf_ff_args* args, void* workspace, size_t workspace_bytes, void* stream);
 int gf_ff_backward(const gf_ff_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Norms before and after a block (csrc/norms.hip).  No counterpart in the reference.
+ *
+ *   s = residual_scale * residual + gate * (n(x) * weight + bias)              the branch's half
+ *   h = (n'(s) * next_weight + next_bias) * (1 + scale) + shift                the next norm's half
+ *
+ * n(x) = (x - mean) / sqrt(variance + eps) (GF_NORM_LAYER), x / sqrt(mean of squares + eps) (GF_NORM_RMS) or x (GF_NORM_NONE), a
+ * row at a time.  residual NULL: the next norm alone, of x.  next_kind GF_NORM_NONE: the branch alone.  Both in one call: h is that of
+ * the unrounded s.
+ *
+ * Matrices are [rows, cols], cols at most 16384, of one type, `dtype`, with unit column stride and a row stride (ld*, in elements) of at
+ * least cols; outputs are contiguous.  weight, bias, next_weight, next_bias: [cols], or NULL (1, 0).  gate, scale, shift: a row for
+ * each group of group_rows consecutive rows (ld* apart), or one for all rows (ld* = 0), or NULL (gate_value, 0, 0).  Sums and statistics are
+ * held in 32 bits: squares of rows beyond 10^19 / sqrt(cols) leave their range.
+ *
+ * Backward: dstream and dnormed are the gradients of s and h (dstream NULL: zero, where there is a next norm); the gradients that are not NULL are
+ * written whole, contiguous, shaped as their parameter ([rows / group_rows, cols] or [cols]).  gate_value has none. */
+#define GF_NORM_NONE 0
+#define GF_NORM_LAYER 1
+#define GF_NORM_RMS 2
+
+typedef struct gf_norm_args {
+  int32_t dtype, kind, next_kind, reserved;
+  int64_t rows, cols, group_rows;
+  double eps, next_eps, gate_value, residual_scale;
+  const void* x;           int64_t ldx;
+  const void* residual;    int64_t ldr;
+  const void* weight;
+  const void* bias;
+  const void* gate;        int64_t ld_gate;
+  const void* next_weight;
+  const void* next_bias;
+  const void* scale;       int64_t ld_scale;
+  const void* shift;       int64_t ld_shift;
+  void* stream;                               /* s; with a next norm it may be NULL: not written */
+  void* normed;                               /* h                                               */
+  const void* dstream;     int64_t ld_dstream;
+  const void* dnormed;     int64_t ld_dnormed;
+  void* dx;
+  void* dresidual;
+  void* dweight;
+  void* dbias;
+  void* dgate;
+  void* dnext_weight;
+  void* dnext_bias;
+  void* dscale;
+  void* dshift;
+} gf_norm_args;
+
+int gf_norm_forward(const gf_norm_args* args, void* stream);
+/* Bytes of the workspace of a backward with these arguments; 0 on invalid arguments too (gf_last_error tells). */
+size_t gf_norm_workspace_bytes(const gf_norm_args* args);
+int gf_norm_backward(const gf_norm_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Weights in 4 bits (csrc/quantized.hip): a frozen weight, or a trained and merged one, as the OCP microscaling
+ * format's MXFP4 (Open Compute Project, "Microscaling Formats (MX) Specification", 2023).  No counterpart in the reference.
+ *
+ * Of a weight [rows, cols], groups of 32 consecutive elements of a row share a scale: a byte holding e + 127 for 2^e (255: NaN), scales [rows,
+ * ceil(cols / 32)].  An element is 4 bits, a sign and the place of its magnitude among 0, 0.5, 1, 1.5, 2, 3, 4, 6: two a byte, the first
+ * in the low half, codes [rows, 16 ceil(cols / 32)], 16-byte aligned, zero past the row.  Both contiguous.
+ *
+ * gf_q4_quantize: e is the least integer with the group's largest magnitude <= 7 * 2^e, in [-125, 125]; elements go to the nearest
+ * value, of two as near to the one with an even place; a group with an infinity or a NaN gets the scale NaN.  gf_q4_dequantize: value
+ * times scale in 32 bits, rounded to dtype.
+ *
+ * gf_q4_forward, gf_q4_backward: the linear and gated products above with such a weight [out, in] ([2 out, in]), no dropout; dx [rows,
+ * in] and dbias as there.  The products are of the weight's values in dtype. */
+typedef struct gf_q4_args {
+  int32_t dtype, activation;
+  int64_t rows, in_features, out_features;
+  const void* x;        int64_t ldx;  /* forward                                                */
+  const void* codes;
+  const void* scales;
+  const void* bias;
+  const void* residual; int64_t ldr;  /* linear only                                            */
+  void* y;                            /* [rows, out], contiguous                                */
+  void* saved;                        /* gated: gf_q4_saved_bytes, written by a forward that a
+                                         backward follows (NULL: none) and read by it           */
+  const void* dy;       int64_t lddy; /* backward                                               */
+  void* dx;
+  void* dbias;
+} gf_q4_args;
+
+int gf_q4_quantize(int32_t dtype, int64_t rows, int64_t cols, const void* weight, int64_t ldw, void* codes, void* scales, void* stream);
+int gf_q4_dequantize(int32_t dtype, int64_t rows, int64_t cols, const void* codes, const void* scales, void* weight, void* stream);
+
+size_t gf_q4_saved_bytes(const gf_q4_args* args);
+size_t gf_q4_workspace_bytes(const gf_q4_args* args, int32_t backward);
+int gf_q4_forward(const gf_q4_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int gf_q4_backward(const gf_q4_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
