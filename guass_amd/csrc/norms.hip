@@ -27,182 +27,320 @@ struct Norms {
   T *dx, *dresidual, *dweight, *dbias, *dgate, *dnext_weight, *dnext_bias, *dscale, *dshift;
 };
 
-// The sum of v over the L lanes of a row.  Past a wave the waves' sums meet in LDS: `slot` alternates between two places, so that
-// one barrier a sum is enough (whoever writes a place again has passed the next sum's barrier, as have all that read it).
-template <int L>
-struct Sum {
-  float (*part)[L > 64 ? L / 64 : 1];
-  int slot = 0;
-  __device__ float operator()(float v) {
-#pragma unroll
-    for (int i = (L < 64 ? L : 64) / 2; i > 0; i /= 2) v += __shfl_xor(v, i);
-    if constexpr (L > 64) {
-      if ((threadIdx.x & 63) == 0) part[slot][threadIdx.x / 64] = v;
-      __syncthreads();
-      v = 0.0f;
-#pragma unroll
-      for (int i = 0; i < L / 64; ++i) v += part[slot][i];
-      slot ^= 1;
-    }
-    return v;
-  }
-};
+// Rows and lanes.  A lane holds G groups of 8 consecutive columns of a row.  A row takes 16 lanes (up to 128 columns), a wave (up to 512),
+// or several waves of a workgroup; a workgroup takes several rows at a time.
+//
+// Sums go over a row's lanes by cross-lane instructions, no LDS; past a wave the waves' sums meet in LDS, two numbers at once, at one
+// barrier: the places alternate, and whoever writes one again has passed the barrier behind which all have read it.
+constexpr int kMaxWaves = 16;
 
-// A row of L lanes: lane `lane` holds the groups of 8 columns (g L + lane).  Elements past the row are zero.
-template <int L, int G>
+template <int CTRL, int ROWS = 0xf>
+__device__ inline float lanes_moved(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, ROWS == 0xf));
+}
+
+// The sum over 16 consecutive lanes (WIDE: over the wave), the same bits in each.
+template <bool WIDE>
+__device__ inline float lanes_sum(float v) {
+  v += lanes_moved<0xB1>(v);   // lane ^ 1
+  v += lanes_moved<0x4E>(v);   // lane ^ 2
+  v += lanes_moved<0x141>(v);  // the other four of eight
+  v += lanes_moved<0x140>(v);  // the other eight of sixteen
+  if constexpr (WIDE) {
+    v += lanes_moved<0x142, 0xa>(v);  // lane 15's to the second sixteen, lane 47's to the fourth
+    v += lanes_moved<0x143, 0xc>(v);  // lane 31's to the upper half
+    v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+  }
+  return v;
+}
+
+enum class Row { kPart, kWave, kWaves };  // a row of 16 lanes, of a wave, of several waves
+
+template <Row R, int G>
 struct Place {
-  int lane, cols;
-  __device__ int col(int g) const { return (g * L + lane) * 8; }
+  int cols, lane, wave, waves, sub;  // lane of the row's wave (or part of one); which of the row's waves; which of the workgroup's rows
+  float2 (*meet)[kMaxWaves][kMaxWaves];
+  float inverse_last;  // 1 / the columns of the row's last wave
+  int slot = 0;
+
+  __device__ Place(int cols, int waves, float2 (*meet)[kMaxWaves][kMaxWaves]) : cols(cols), waves(waves), meet(meet) {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if constexpr (R == Row::kPart) {
+      lane = threadIdx.x & 15, wave = 0, sub = threadIdx.x >> 4;
+    } else {
+      lane = threadIdx.x & 63, sub = R == Row::kWave ? w : w / waves, wave = R == Row::kWave ? 0 : w % waves;
+    }
+    inverse_last = R == Row::kWaves ? 1.0f / (float)(cols - (waves - 1) * 512 * G) : 0.0f;
+  }
+  static __host__ __device__ int rows_at_once(int threads, int waves) {
+    return R == Row::kPart ? threads / 16 : R == Row::kWave ? threads / 64 : threads / 64 / waves;
+  }
+
+  __device__ int col(int g) const { return ((wave * G + g) * (R == Row::kPart ? 16 : 64) + lane) * 8; }
   __device__ int count(int g) const {
     const int n = cols - col(g);
     return n < 0 ? 0 : n < 8 ? n : 8;
   }
-  template <typename T>
-  __device__ void load(float v[G][8], const T* row) const {
+
+  // a and b summed over the row
+  __device__ float2 sum2(float a, float b) {
+    float2 v{lanes_sum<R != Row::kPart>(a), lanes_sum<R != Row::kPart>(b)};
+    if constexpr (R == Row::kWaves) {
+      v = exchange(v);
+      v = {lanes_sum<false>(v.x), lanes_sum<false>(v.y)};
+    }
+    return v;
+  }
+
+  // Each wave's v to the lane of its number in every sixteen lanes of the row, zero to the others.
+  __device__ float2 exchange(float2 v) {
+    if (lane == 0) meet[slot][sub][wave] = v;
+    __syncthreads();
+    const int i = threadIdx.x & 15;
+    v = meet[slot][sub][i];
+    slot ^= 1;
+    return i < waves ? v : float2{0.0f, 0.0f};
+  }
+
+  // s / n, one step from s times the rounded 1 / n: exact where the quotient is, so a row of one value has it for a mean.
+  static __device__ float quotient(float s, float n, float inverse) {
+    const float q = s * inverse;
+    return __builtin_fmaf(__builtin_fmaf(-q, n, s), inverse, q);
+  }
+
+  // The mean and the sum of squares about it.  Each wave takes its own about its own mean, from registers, and the waves' are joined
+  // (Chan, Golub, LeVeque: "Updating formulae and a pairwise algorithm for computing sample variances", 1979): nothing cancels, at
+  // one barrier.
+  __device__ float2 spread(const float x[G][8], float inverse) {
+    float s = 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; ++g) load8(v[g], row + col(g), count(g) == 8, count(g));
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += x[g][j];
+    s = lanes_sum<R != Row::kPart>(s);
+    constexpr int kWhole = 512 * G;
+    const float mean = R != Row::kWaves ? quotient(s, (float)cols, inverse) : s * (wave + 1 < waves ? 1.0f / kWhole : inverse_last);
+    float d[G][8], m = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[g][j] = x[g][j] - mean;
+    clear(d);
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = __builtin_fmaf(d[g][j], d[g][j], m);
+    m = lanes_sum<R != Row::kPart>(m);
+    if constexpr (R != Row::kWaves) return {mean, m};
+    const float2 v = exchange({s, m});
+    const float total = quotient(lanes_sum<false>(v.x), (float)cols, inverse);
+    const int i = threadIdx.x & 15;
+    const float size = i + 1 < waves ? (float)kWhole : i + 1 == waves ? (float)(cols - (waves - 1) * kWhole) : 0.0f;
+    const float off = v.x * (i + 1 < waves ? 1.0f / kWhole : inverse_last) - total;
+    return {total, lanes_sum<false>(__builtin_fmaf(size * off, off, v.y))};
+  }
+
+  // 8 elements a group, zero past the row.
+  template <typename T>
+  __device__ void load(Vec<T, 8> v[G], const T* row) const {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int n = count(g);
+      v[g] = (T)0.0f;
+      if (n == 8) {
+        v[g] = *(const Vec<T, 8>*)(row + col(g));
+      } else if (n > 0) {
+#pragma unroll
+        for (int j = 0; j < 7; ++j)
+          if (j < n) v[g][j] = row[col(g) + j];
+      }
+    }
   }
   template <typename T>
   __device__ void store(T* row, const float v[G][8]) const {
 #pragma unroll
-    for (int g = 0; g < G; ++g) store8(row + col(g), v[g], count(g) == 8, count(g));
+    for (int g = 0; g < G; ++g)
+      if (count(g) > 0) store8(row + col(g), v[g], count(g) == 8, count(g));
   }
-  // v times (plus) a vector of parameters
-  template <typename T, typename F>
-  __device__ void apply(float v[G][8], const T* p, F f) const {
-    if (p == nullptr) return;
+  // Past the row, zero.
+  __device__ void clear(float v[G][8]) const {
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      float w[8];
-      load8(w, p + col(g), count(g) == 8, count(g));
+      const int n = count(g);
+      if (n < 8) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[g][j] = f(v[g][j], w[j]);
+        for (int j = 0; j < 8; ++j)
+          if (j >= n) v[g][j] = 0.0f;
+      }
     }
   }
 };
 
-// x becomes n(x), zero past the row; returns 1 / deviation (rms: 1 / root mean square).  The mean first, then the squares of what is
-// left: both from registers, so nothing cancels.
-template <int L, int G>
-__device__ inline float normalise(float x[G][8], int kind, float eps, float inverse, const Place<L, G>& at, Sum<L>& sum) {
-  float v = 0.0f;
-  if (kind == GF_NORM_LAYER) {
+template <typename T, int G>
+__device__ inline void widen(float v[G][8], const Vec<T, 8> from[G]) {
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[g][j] = (float)from[g][j];
+}
+
+// v[] = f(v[], p[]) with a row of parameters, or with `without` where there is none.
+template <typename T, int G, typename P, typename F>
+__device__ inline void with_row(float v[G][8], const P& at, const T* p, float without, F f) {
+  if (p == nullptr) {
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v += x[g][j];
-    const float mean = sum(v) / (float)at.cols;  // a row of one value has that mean
-    v = 0.0f;
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const int n = at.count(g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[g][j] -= mean;
-      if (n < 8) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j >= n) x[g][j] = 0.0f;
-      }
-    }
+      for (int j = 0; j < 8; ++j) v[g][j] = f(v[g][j], without);
+    return;
   }
+  Vec<T, 8> w[G];
+  at.load(w, p);
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v = __builtin_fmaf(x[g][j], x[g][j], v);
-  const float rstd = 1.0f / sqrtf(__builtin_fmaf(sum(v), inverse, eps));
+    for (int j = 0; j < 8; ++j) v[g][j] = f(v[g][j], (float)w[g][j]);
+}
+
+// A half's affine map n -> n times[] + plus[] for a group of rows.  The branch's: gate * weight, gate * bias.  The next norm's:
+// (1 + scale) * weight, (1 + scale) * bias + shift.
+template <int G>
+struct Affine {
+  float times[G][8], plus[G][8];
+};
+
+template <typename T, int G, typename P>
+__device__ inline void branch_affine(Affine<G>& m, const Norms<T>& a, const P& at, int64_t group) {
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[g][j] *= rstd;
+    for (int j = 0; j < 8; ++j) m.times[g][j] = 1.0f, m.plus[g][j] = 0.0f;
+  with_row<T, G>(m.times, at, a.gate ? a.gate + group * a.ld_gate : nullptr, a.gate_value, [](float v, float w) { return w; });
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m.plus[g][j] = m.times[g][j];
+  with_row<T, G>(m.plus, at, a.bias, 0.0f, [](float v, float w) { return v * w; });
+  with_row<T, G>(m.times, at, a.weight, 1.0f, [](float v, float w) { return v * w; });
+}
+
+template <typename T, int G, typename P>
+__device__ inline void next_affine(Affine<G>& m, const Norms<T>& a, const P& at, int64_t group) {
+  with_row<T, G>(m.times, at, a.scale ? a.scale + group * a.ld_scale : nullptr, 0.0f, [](float v, float w) { return 1.0f + w; });
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m.plus[g][j] = m.times[g][j];
+  with_row<T, G>(m.plus, at, a.next_bias, 0.0f, [](float v, float w) { return v * w; });
+  with_row<T, G>(m.plus, at, a.shift ? a.shift + group * a.ld_shift : nullptr, 0.0f, [](float v, float w) { return v + w; });
+  with_row<T, G>(m.times, at, a.next_weight, 1.0f, [](float v, float w) { return v * w; });
+}
+
+// 1 / sqrt(v) by the hardware's (1 unit in the last place), which takes a subnormal number for zero.
+__device__ inline float inverse_root(float v) {
+  const bool low = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_rsqf(low ? v * 0x1p64f : v);
+  return low ? r * 0x1p32f : r;
+}
+
+// x becomes n(x), zero past the row; returns 1 / deviation (rms: 1 / root mean square).
+template <int G, typename P>
+__device__ inline float normalise(float x[G][8], int kind, float eps, float inverse, P& at) {
+  float rstd;
+  if (kind == GF_NORM_LAYER) {
+    const float2 s = at.spread(x, inverse);
+    rstd = inverse_root(__builtin_fmaf(s.y, inverse, eps));
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[g][j] = (x[g][j] - s.x) * rstd;
+    at.clear(x);
+  } else {
+    float v = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v = __builtin_fmaf(x[g][j], x[g][j], v);
+    rstd = inverse_root(__builtin_fmaf(at.sum2(v, 0.0f).x, inverse, eps));
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[g][j] *= rstd;
+  }
   return rstd;
 }
 
 // The gradient of x from that of n(x), in place: rstd (g - mean g - n(x) mean(g n(x))), without mean g for rms; zero past the row.
-template <int L, int G>
-__device__ inline void through_norm(float g_[G][8], const float n_[G][8], int kind, float rstd, float inverse, const Place<L, G>& at,
-                                    Sum<L>& sum) {
+template <int G, typename P>
+__device__ inline void through_norm(float g_[G][8], const float n_[G][8], int kind, float rstd, float inverse, P& at) {
   float a = 0.0f, b = 0.0f;
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
     for (int j = 0; j < 8; ++j) a += g_[g][j], b = __builtin_fmaf(g_[g][j], n_[g][j], b);
-  a = kind == GF_NORM_LAYER ? sum(a) * inverse : 0.0f;
-  b = sum(b) * inverse;
+  const float2 s = at.sum2(a, b);
+  a = kind == GF_NORM_LAYER ? s.x * inverse : 0.0f;
+  b = s.y * inverse;
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int n = at.count(g);
+  for (int g = 0; g < G; ++g)
 #pragma unroll
     for (int j = 0; j < 8; ++j) g_[g][j] = rstd * (g_[g][j] - __builtin_fmaf(n_[g][j], b, a));
-    if (n < 8) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j >= n) g_[g][j] = 0.0f;
-    }
-  }
+  if (kind == GF_NORM_LAYER) at.clear(g_);
 }
 
-constexpr auto kTimes = [](float v, float w) { return v * w; };
-constexpr auto kPlus = [](float v, float w) { return v + w; };
-constexpr auto kTimesOnePlus = [](float v, float w) { return __builtin_fmaf(v, w, v); };
+// Chunks of rows, each of one group: `chunks` a group of `rows` rows, `all` together.
+struct Chunks {
+  int64_t rows, chunks, all;
+};
 
-// v (n(x), or x itself) becomes g (v w + b).
-template <typename T, int L, int G>
-__device__ inline void branch(const Norms<T>& a, const Place<L, G>& at, float v[G][8], int64_t group) {
-  at.apply(v, a.weight, kTimes);
-  at.apply(v, a.bias, kPlus);
-  if (a.gate != nullptr) {
-    at.apply(v, a.gate + group * a.ld_gate, kTimes);
-  } else {
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[g][j] *= a.gate_value;
-  }
-}
+template <Row R, int G>
+constexpr int kForwardThreads = R != Row::kWaves ? 256 : G == 1 ? 768 : 1024;
 
-// The gradient of g (v w + b), in place, into that of v.
-template <typename T, int L, int G>
-__device__ inline void through_branch(const Norms<T>& a, const Place<L, G>& at, float v[G][8], int64_t group) {
-  at.apply(v, a.weight, kTimes);
-  if (a.gate != nullptr) {
-    at.apply(v, a.gate + group * a.ld_gate, kTimes);
-  } else {
+// Forward.  BRANCH: s from x and the residual; NEXT: h from s (without BRANCH, from x).  A group's maps stay in registers for a chunk, and the
+// next row is on its way while one is worked on.
+template <typename T, Row R, int G, bool BRANCH, bool NEXT>
+__global__ __launch_bounds__((kForwardThreads<R, G>)) void k_norm_forward(Norms<T> a, Chunks cut, int waves) {
+  __shared__ float2 meet[2][kMaxWaves][kMaxWaves];
+  Place<R, G> at(a.cols, waves, meet);
+  const int at_once = at.rows_at_once(blockDim.x, waves);
+  for (int64_t chunk = blockIdx.x; chunk < cut.all; chunk += gridDim.x) {
+    const int64_t group = chunk / cut.chunks, first = chunk % cut.chunks * cut.rows;
+    const int64_t begin = group * a.group_rows + first, end = group * a.group_rows + (first + cut.rows < a.group_rows ? first + cut.rows : a.group_rows);
+    Affine<BRANCH ? G : 1> mb;
+    Affine<NEXT ? G : 1> mn;
+    if constexpr (BRANCH) branch_affine<T, G>(mb, a, at, group);
+    if constexpr (NEXT) next_affine<T, G>(mn, a, at, group);
+    Vec<T, 8> vx[G], vr[BRANCH ? G : 1];
+    auto fetch = [&](int64_t row) {
+      at.load(vx, a.x + row * a.ldx);
+      if constexpr (BRANCH) at.load(vr, a.residual + row * a.ldr);
+    };
+    // all of a workgroup's rows take part in every turn (there are barriers): past the chunk the last row again, not stored
+    int64_t row = begin + at.sub;
+    fetch(row < end ? row : end - 1);
+    for (int64_t turn = begin; turn < end; turn += at_once, row += at_once) {
+      float v[G][8], r[BRANCH ? G : 1][8];
+      widen<T, G>(v, vx);
+      if constexpr (BRANCH) widen<T, G>(r, vr);
+      if (turn + at_once < end) fetch(row + at_once < end ? row + at_once : end - 1);
+      const bool mine = row < end;
+      if constexpr (BRANCH) {
+        if (a.kind != GF_NORM_NONE) normalise<G>(v, a.kind, a.eps, a.inverse, at);
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[g][j] *= a.gate_value;
-  }
-}
-
-// Forward, L lanes a row.  BRANCH: s from x and the residual; NEXT: h from s (without BRANCH, from x).
-template <typename T, int L, int G, bool BRANCH, bool NEXT>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_forward(Norms<T> a) {
-  constexpr int kAtOnce = L < 256 ? 256 / L : 1;
-  __shared__ float part[2][L > 64 ? L / 64 : 1];
-  Sum<L> sum{part};
-  const Place<L, G> at{(int)threadIdx.x % L, a.cols};
-  for (int64_t row = (int64_t)blockIdx.x * kAtOnce + threadIdx.x / L; row < a.rows; row += (int64_t)gridDim.x * kAtOnce) {
-    const int64_t group = (uint32_t)row / (uint32_t)a.group_rows;
-    float v[G][8];
-    at.load(v, a.x + row * a.ldx);
-    if constexpr (BRANCH) {
-      float r[G][8];
-      at.load(r, a.residual + row * a.ldr);
-      if (a.kind != GF_NORM_NONE) normalise<L, G>(v, a.kind, a.eps, a.inverse, at, sum);
-      branch(a, at, v, group);
+          for (int j = 0; j < 8; ++j)
+            v[g][j] = __builtin_fmaf(a.residual_scale, r[g][j], __builtin_fmaf(v[g][j], mb.times[g][j], mb.plus[g][j]));
+        if (a.stream != nullptr && mine) at.store(a.stream + row * a.cols, v);
+      }
+      if constexpr (NEXT) {
+        normalise<G>(v, a.next_kind, a.next_eps, a.inverse, at);
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[g][j] = __builtin_fmaf(a.residual_scale, r[g][j], v[g][j]);
-      if (a.stream != nullptr) at.store(a.stream + row * a.cols, v);
-    }
-    if constexpr (NEXT) {
-      normalise<L, G>(v, a.next_kind, a.next_eps, a.inverse, at, sum);
-      at.apply(v, a.next_weight, kTimes);
-      at.apply(v, a.next_bias, kPlus);
-      if (a.scale != nullptr) at.apply(v, a.scale + group * a.ld_scale, kTimesOnePlus);
-      if (a.shift != nullptr) at.apply(v, a.shift + group * a.ld_shift, kPlus);
-      at.store(a.normed + row * a.cols, v);
+          for (int j = 0; j < 8; ++j) v[g][j] = __builtin_fmaf(v[g][j], mn.times[g][j], mn.plus[g][j]);
+        if (mine) at.store(a.normed + row * a.cols, v);
+      }
     }
   }
 }
@@ -210,73 +348,86 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_forward(Norms<T> a) 
 // Column sums of a chunk of rows, per element: of ds, ds n(x), dh, dh n'(s).
 constexpr int kSums = 4;
 
-// Backward, by chunks of rows of one group each (`chunks` a group, `all` together).  SUMS: the column sums too, into parts [chunk][kSums][width].
-template <typename T, int L, int G, bool BRANCH, bool NEXT, bool SUMS>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_backward(Norms<T> a, int64_t chunk_rows, int64_t chunks, int64_t all, float* parts,
-                                                                      int64_t width) {
-  constexpr int kAtOnce = L < 256 ? 256 / L : 1;
-  __shared__ float part[2][L > 64 ? L / 64 : 1];
-  __shared__ float meet[SUMS && kAtOnce > 1 ? kAtOnce : 1][SUMS && kAtOnce > 1 ? L * G * 8 : 1];
-  Sum<L> sum{part};
-  const int sub = threadIdx.x / L;
-  const Place<L, G> at{(int)threadIdx.x % L, a.cols};
-  for (int64_t chunk = blockIdx.x; chunk < all; chunk += gridDim.x) {
-    const int64_t group = chunk / chunks, first = (chunk % chunks) * chunk_rows;
-    const int64_t begin = group * a.group_rows + first;
-    const int64_t end = group * a.group_rows + (first + chunk_rows < a.group_rows ? first + chunk_rows : a.group_rows);
+template <Row R, int G>
+constexpr int kBackwardThreads = R == Row::kPart ? 256 : R == Row::kWave ? 512 : G == 1 ? 768 : 1024;
+
+// Backward, by chunks of rows.  SUMS: the column sums too, into parts [chunk][kSums][width].
+template <typename T, Row R, int G, bool BRANCH, bool NEXT, bool SUMS>
+__global__ __launch_bounds__((kBackwardThreads<R, G>)) void k_norm_backward(Norms<T> a, Chunks cut, int waves, float* parts, int64_t width) {
+  __shared__ float2 meet[2][kMaxWaves][kMaxWaves];
+  constexpr int kThreads = kBackwardThreads<R, G>;
+  __shared__ float together[SUMS && G == 1 ? kThreads * 8 : 1];  // with two groups a lane a workgroup has one row
+  Place<R, G> at(a.cols, waves, meet);
+  const int at_once = at.rows_at_once(blockDim.x, waves);
+  for (int64_t chunk = blockIdx.x; chunk < cut.all; chunk += gridDim.x) {
+    const int64_t group = chunk / cut.chunks, first = chunk % cut.chunks * cut.rows;
+    const int64_t begin = group * a.group_rows + first, end = group * a.group_rows + (first + cut.rows < a.group_rows ? first + cut.rows : a.group_rows);
+    Affine<BRANCH ? G : 1> mb;
+    Affine<NEXT ? G : 1> mn;
+    if constexpr (BRANCH) branch_affine<T, G>(mb, a, at, group);
+    if constexpr (NEXT) next_affine<T, G>(mn, a, at, group);
     float sums[SUMS ? kSums : 1][G][8] = {};
-    auto add = [&](int k, const float d[G][8], const float n[G][8]) {
-      if constexpr (SUMS) {
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) sums[k][g][j] += d[g][j], sums[k + 1][g][j] = __builtin_fmaf(d[g][j], n[g][j], sums[k + 1][g][j]);
+    const bool needs_x = NEXT || SUMS || a.kind != GF_NORM_NONE;
+    Vec<T, 8> vx[G] = {}, vr[BRANCH && NEXT ? G : 1], vs[BRANCH ? G : 1] = {}, vh[NEXT ? G : 1];
+    auto fetch = [&](int64_t row) {
+      if (needs_x) at.load(vx, a.x + row * a.ldx);
+      if constexpr (BRANCH && NEXT) at.load(vr, a.residual + row * a.ldr);
+      if constexpr (BRANCH) {
+        if (a.dstream != nullptr) at.load(vs, a.dstream + row * a.ld_dstream);
       }
+      if constexpr (NEXT) at.load(vh, a.dnormed + row * a.ld_dnormed);
     };
-    for (int64_t row = begin + sub; row < end; row += kAtOnce) {
-      float x[G][8], d[G][8];
-      if (NEXT || SUMS || a.kind != GF_NORM_NONE) at.load(x, a.x + row * a.ldx);
-      float rstd = 1.0f;
-      if constexpr (BRANCH && !NEXT) {
-        at.load(d, a.dstream + row * a.ld_dstream);
-        if (a.kind != GF_NORM_NONE) rstd = normalise<L, G>(x, a.kind, a.eps, a.inverse, at, sum);
-      }
-      if constexpr (NEXT) {
-        at.load(d, a.dnormed + row * a.ld_dnormed);
-        float s[BRANCH ? G : 1][8], ds[BRANCH ? G : 1][8];
-        if constexpr (BRANCH) {
-          float r[G][8];
-          at.load(r, a.residual + row * a.ldr);
-          if (a.dstream != nullptr) at.load(ds, a.dstream + row * a.ld_dstream);
-          if (a.kind != GF_NORM_NONE) rstd = normalise<L, G>(x, a.kind, a.eps, a.inverse, at, sum);
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[g][j] = x[g][j];
-          branch(a, at, s, group);
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[g][j] = __builtin_fmaf(a.residual_scale, r[g][j], s[g][j]);
-        }
-        float(*n)[8] = BRANCH ? s : x;
-        const float next_rstd = normalise<L, G>(n, a.next_kind, a.next_eps, a.inverse, at, sum);
-        add(2, d, n);
-        at.apply(d, a.next_weight, kTimes);
-        if (a.scale != nullptr) at.apply(d, a.scale + group * a.ld_scale, kTimesOnePlus);
-        through_norm<L, G>(d, n, a.next_kind, next_rstd, a.inverse, at, sum);
-        if constexpr (BRANCH) {
-          if (a.dstream != nullptr) {
+    int64_t row = begin + at.sub;
+    fetch(row < end ? row : end - 1);
+    for (int64_t turn = begin; turn < end; turn += at_once, row += at_once) {
+      const bool mine = row < end;
+      // past the chunk the last row again, neither stored nor added
+      auto add = [&](int k, const float d[G][8], const float n[G][8]) {
+        if constexpr (SUMS) {
+          if (mine) {
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
-              for (int j = 0; j < 8; ++j) d[g][j] += ds[g][j];
+              for (int j = 0; j < 8; ++j) sums[k][g][j] += d[g][j], sums[k + 1][g][j] = __builtin_fmaf(d[g][j], n[g][j], sums[k + 1][g][j]);
           }
         }
+      };
+      float x[G][8], r[BRANCH && NEXT ? G : 1][8], d[G][8], ds[BRANCH ? G : 1][8];
+      widen<T, G>(x, vx);
+      if constexpr (BRANCH && NEXT) widen<T, G>(r, vr);
+      if constexpr (BRANCH) widen<T, G>(ds, vs);
+      if constexpr (NEXT) widen<T, G>(d, vh);
+      if (turn + at_once < end) fetch(row + at_once < end ? row + at_once : end - 1);
+      float rstd = 1.0f;
+      if constexpr (BRANCH) {
+        if (a.kind != GF_NORM_NONE) rstd = normalise<G>(x, a.kind, a.eps, a.inverse, at);
+      }
+      if constexpr (NEXT) {
+        float s[G][8];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if constexpr (BRANCH)
+              s[g][j] = __builtin_fmaf(a.residual_scale, r[g][j], __builtin_fmaf(x[g][j], mb.times[g][j], mb.plus[g][j]));
+            else
+              s[g][j] = x[g][j];
+          }
+        const float next_rstd = normalise<G>(s, a.next_kind, a.next_eps, a.inverse, at);
+        add(2, d, s);
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[g][j] *= mn.times[g][j];
+        through_norm<G>(d, s, a.next_kind, next_rstd, a.inverse, at);
       }
       if constexpr (BRANCH) {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[g][j] = NEXT ? d[g][j] + ds[g][j] : ds[g][j];
         add(0, d, x);
-        if (a.dresidual != nullptr) {
+        if (a.dresidual != nullptr && mine) {
           float t[G][8];
 #pragma unroll
           for (int g = 0; g < G; ++g)
@@ -285,34 +436,37 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_backward(Norms<T> a,
           at.store(a.dresidual + row * a.cols, t);
         }
         if (a.dx != nullptr) {
-          through_branch(a, at, d, group);
-          if (a.kind != GF_NORM_NONE) through_norm<L, G>(d, x, a.kind, rstd, a.inverse, at, sum);
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[g][j] *= mb.times[g][j];
+          if (a.kind != GF_NORM_NONE) through_norm<G>(d, x, a.kind, rstd, a.inverse, at);
         }
       }
-      if (a.dx != nullptr) at.store(a.dx + row * a.cols, d);
+      if (a.dx != nullptr && mine) at.store(a.dx + row * a.cols, d);
     }
     if constexpr (SUMS) {
+      const int span = R == Row::kPart ? 128 : 512 * G * (R == Row::kWave ? 1 : waves);  // columns that a row's lanes hold
 #pragma unroll
       for (int k = BRANCH ? 0 : 2; k < (NEXT ? kSums : 2); ++k) {
-        float* const out = parts + ((int64_t)chunk * kSums + k) * width;
-        if constexpr (kAtOnce == 1) {
+        float* const out = parts + (chunk * kSums + k) * width;
+        if (at_once == 1) {
+#pragma unroll
           for (int g = 0; g < G; ++g)
             if (at.count(g) > 0) store8(out + at.col(g), sums[k][g], true, 8);
-        } else {
-          __syncthreads();
+          continue;
+        }
+        __syncthreads();
 #pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) meet[sub][at.col(g) + j] = sums[k][g][j];
-          __syncthreads();
-          for (int c = threadIdx.x; c < a.cols; c += 256) {
-            float v = meet[0][c];
-#pragma unroll
-            for (int i = 1; i < kAtOnce; ++i) v += meet[i][c];
-            out[c] = v;
-          }
+        for (int g = 0; g < G; ++g) store8(together + at.sub * span + at.col(g), sums[k][g], true, 8);
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+          float v = together[c];
+          for (int i = 1; i < at_once; ++i) v += together[i * span + c];
+          out[c] = v;
         }
       }
+      __syncthreads();
     }
   }
 }
@@ -320,8 +474,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_backward(Norms<T> a,
 // The chunks' sums into gradients: 32 columns a workgroup, the branch's (z = 0) or the next norm's.  With S0 = sum d, S1 = sum d n of a
 // group, w, b the half's weight and bias and f its factor (the gate; 1 + scale):
 //   of the factor  w S1 + b S0;   of the shift  S0;   of w  sum over groups of f S1;   of b  sum over groups of f S0.
-// 32 half-waves share out the groups, several of them one group where there are fewer; a slab (y) is a range of groups, and what is shared
-// by all groups goes to `partial` [slab][half][4][width] (of the weight, the bias, the factor, the shift) where there are several slabs.
+// 8 lanes take 32 columns, 128 such members of a workgroup share out the groups, `team` of them (a power of two) one group: all chunks of
+// it are asked for at once.  A slab (y) is a range of groups, and what is shared by all groups goes to `partial` [slab][half][4][width]
+// (of the weight, the bias, the factor, the shift) where there are several slabs.
 template <typename T>
 struct Half {
   const T *weight, *bias, *factor;
@@ -330,62 +485,93 @@ struct Half {
   T *dweight, *dbias, *dfactor, *dshift;
 };
 
+using f32x4 = float __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ inline f32x4 load4(const T* p, int64_t c, int n, float without) {
+  f32x4 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = p != nullptr && j < n ? (float)p[c + j] : without;
+  return v;
+}
+
+template <typename T>
+__device__ inline void store4(T* p, int64_t c, int n, f32x4 v) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < n) p[c + j] = (T)v[j];
+}
+
+__device__ inline f32x4 from_lane(f32x4 v, int mask) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = __shfl_xor(v[j], mask);
+  return v;
+}
+
 template <typename T>
 __global__ __launch_bounds__(1024) void k_norm_finish(Half<T> branch, Half<T> next, int half0, int32_t cols, int64_t groups, int64_t chunks,
                                                       const float* parts, int64_t width, int team, float* partial) {
-  __shared__ float meet[4][32][32];
-  const int lane = threadIdx.x & 31, member = threadIdx.x >> 5, half = half0 + blockIdx.z;
+  __shared__ f32x4 meet[4][16][8];
+  const int lane = threadIdx.x & 7, member = threadIdx.x >> 3, wave = threadIdx.x >> 6, half = half0 + blockIdx.z;
+  const bool first_of_wave = (threadIdx.x & 63) < 8;
   const Half<T>& h = half == 0 ? branch : next;
-  const int64_t c = blockIdx.x * 32ll + lane;
-  const bool in = c < cols;
+  const int64_t c = blockIdx.x * 32ll + lane * 4;
+  const int n = cols - c < 0 ? 0 : cols - c < 4 ? (int)(cols - c) : 4;
   const int64_t slab = (groups + gridDim.y - 1) / gridDim.y, g0 = blockIdx.y * slab, g1 = g0 + slab < groups ? g0 + slab : groups;
-  const int teams = 32 / team, of = member % team;
-  const float w = in && h.weight != nullptr ? (float)h.weight[c] : 1.0f, b = in && h.bias != nullptr ? (float)h.bias[c] : 0.0f;
-  float dw = 0.0f, db = 0.0f, df = 0.0f, dsh = 0.0f;
+  const int teams = 128 / team, of = member & (team - 1);
+  const f32x4 w = load4(h.weight, c, n, 1.0f), b = load4(h.bias, c, n, 0.0f);
+  f32x4 shared[4] = {};
   for (int64_t base = g0; base < g1; base += teams) {
     const int64_t g = base + member / team;
-    float s0 = 0.0f, s1 = 0.0f;
-    if (in && g < g1) {
+    f32x4 s0 = 0.0f, s1 = 0.0f;
+    if (n > 0 && g < g1) {
 #pragma unroll 4
       for (int64_t i = of; i < chunks; i += team) {
-        const float* p = parts + ((g * chunks + i) * kSums + 2 * half) * width + c;
-        s0 += p[0], s1 += p[width];
+        const float* p = parts + ((g * chunks + i) * kSums + 2 * half) * width + c;  // 4 of them: width is a multiple of 8
+        s0 += *(const f32x4*)p, s1 += *(const f32x4*)(p + width);
       }
     }
-    if (team > 1) {
+    for (int i = 1; i < team && i < 8; i *= 2) s0 += from_lane(s0, 8 * i), s1 += from_lane(s1, 8 * i);
+    if (team > 8) {
       __syncthreads();
-      meet[0][member][lane] = s0, meet[1][member][lane] = s1;
+      if (first_of_wave) meet[0][wave][lane] = s0, meet[1][wave][lane] = s1;
       __syncthreads();
-      if (of == 0) {
-        for (int i = 1; i < team; ++i) s0 += meet[0][member + i][lane], s1 += meet[1][member + i][lane];
-      }
+      s0 = 0.0f, s1 = 0.0f;
+      const int w0 = wave & ~(team / 8 - 1);
+      for (int i = 0; i < team / 8; ++i) s0 += meet[0][w0 + i][lane], s1 += meet[1][w0 + i][lane];
     }
-    if (in && g < g1 && of == 0) {
-      const float f = h.factor != nullptr ? h.one + (float)h.factor[g * h.ld_factor + c] : h.value;
-      dw = __builtin_fmaf(f, s1, dw), db = __builtin_fmaf(f, s0, db);
-      const float own = __builtin_fmaf(w, s1, b * s0);
+    if (n > 0 && g < g1 && of == 0) {
+      const f32x4 f = h.factor != nullptr ? h.one + load4(h.factor + g * h.ld_factor, c, n, 0.0f) : f32x4(h.value);
+      shared[0] += f * s1, shared[1] += f * s0;
+      const f32x4 own = w * s1 + b * s0;
       if (h.dfactor != nullptr) {
-        if (h.ld_factor != 0) h.dfactor[g * cols + c] = (T)own;
-        else df += own;
+        if (h.ld_factor != 0) store4(h.dfactor + g * cols, c, n, own);
+        else shared[2] += own;
       }
       if (h.dshift != nullptr) {
-        if (h.ld_shift != 0) h.dshift[g * cols + c] = (T)s0;
-        else dsh += s0;
+        if (h.ld_shift != 0) store4(h.dshift + g * cols, c, n, s0);
+        else shared[3] += s0;
       }
     }
   }
   __syncthreads();
-  meet[0][member][lane] = dw, meet[1][member][lane] = db, meet[2][member][lane] = df, meet[3][member][lane] = dsh;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+#pragma unroll
+    for (int i = 1; i < 8; i *= 2) shared[k] += from_lane(shared[k], 8 * i);
+    if (first_of_wave) meet[k][wave][lane] = shared[k];
+  }
   __syncthreads();
-  if (member >= 4 || !in) return;
-  float v = 0.0f;
-  for (int i = 0; i < 32; i += team) v += meet[member][i][lane];
+  if (member >= 4 || n == 0) return;
+  f32x4 v = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v += meet[member][i][lane];
   if (partial != nullptr) {
-    partial[((int64_t)blockIdx.y * 2 + half) * 4 * width + member * width + c] = v;
+    *(f32x4*)(partial + ((int64_t)blockIdx.y * 2 + half) * 4 * width + member * width + c) = v;
     return;
   }
   T* const out = member == 0 ? h.dweight : member == 1 ? h.dbias : member == 2 ? (h.ld_factor == 0 ? h.dfactor : nullptr) : h.ld_shift == 0 ? h.dshift : nullptr;
-  if (out != nullptr) out[c] = (T)v;
+  if (out != nullptr) store4(out, c, n, v);
 }
 
 template <typename T>
@@ -457,22 +643,37 @@ Norms<T> make_norms(const gf_norm_args& a) {
   return n;
 }
 
-template <int L, int G>
-struct Lanes {
-  static constexpr int lanes = L, groups = G;
+template <Row R, int G>
+struct Form {
+  static constexpr Row row = R;
+  static constexpr int groups = G;
 };
 
-// How many lanes take a row, and how many groups of 8 columns each.
+// How a row is held: 16 lanes up to 128 columns, a wave up to 512, else a wave for each 512, or (16 are a workgroup's limit) each 1024.
 template <typename F>
-int with_lanes(int64_t cols, F f) {
-  if (cols <= 128) return f(Lanes<16, 1>());
-  if (cols <= 512) return f(Lanes<64, 1>());
-  if (cols <= 1024) return f(Lanes<64, 2>());
-  if (cols <= 1536) return f(Lanes<64, 3>());
-  if (cols <= 2048) return f(Lanes<256, 1>());
-  if (cols <= 4096) return f(Lanes<256, 2>());
-  if (cols <= 6144) return f(Lanes<256, 3>());
-  return f(Lanes<1024, 2>());
+int with_form(int64_t cols, F f) {
+  if (cols <= 128) return f(Form<Row::kPart, 1>(), 1);
+  if (cols <= 512) return f(Form<Row::kWave, 1>(), 1);
+  if (cols <= 512 * 12) return f(Form<Row::kWaves, 1>(), (int)((cols + 511) / 512));
+  return f(Form<Row::kWaves, 2>(), (int)((cols + 1023) / 1024));
+}
+
+// Threads of a workgroup: as many rows at a time as `most` waves hold, but no more than there are in a group.
+template <Row R>
+int threads_of(int waves, int64_t group_rows, int most) {
+  if (R == Row::kPart) return (int)std::min<int64_t>(round_up(group_rows * 16, 64), most * 64);
+  return waves * 64 * (int)std::max<int64_t>(std::min<int64_t>(group_rows, most / waves), 1);
+}
+
+// Each group in chunks of whole turns of a workgroup, until there are about `want` chunks.
+Chunks cut_rows(int64_t rows, int64_t group_rows, int at_once, int64_t want) {
+  const int64_t groups = rows / group_rows, turns = (group_rows + at_once - 1) / at_once;
+  const int64_t each = std::max<int64_t>((turns * groups + want - 1) / want, 1);
+  Chunks c;
+  c.rows = std::min(each, turns) * at_once;
+  c.chunks = (group_rows + c.rows - 1) / c.rows;
+  c.all = groups * c.chunks;
+  return c;
 }
 
 template <typename F>
@@ -491,30 +692,31 @@ int backward(const gf_norm_args& a, Arena& ws, bool run, hipStream_t s) {
   const int64_t groups = a.rows / a.group_rows, width = round_up(a.cols, 8);
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return with_lanes(a.cols, [&](auto lanes) {
-      constexpr int L = lanes.lanes, G = lanes.groups, kThreads = L < 256 ? 256 : L, kAtOnce = kThreads / L;
+    return with_form(a.cols, [&](auto form, int waves) {
+      constexpr Row R = form.row;
+      constexpr int G = form.groups;
       return with_halves(a, [&](auto branch, auto next) {
         constexpr bool kBranch = branch.value, kNext = next.value;
         const bool sums = wants_sums(a);
-        const int64_t want = std::max<int64_t>((sums ? 512 : 4096) / groups, 1);
-        const int64_t cut = std::min(want, (a.group_rows + kAtOnce - 1) / kAtOnce), chunk_rows = (a.group_rows + cut - 1) / cut;
-        const int64_t chunks = (a.group_rows + chunk_rows - 1) / chunk_rows, all = groups * chunks;
-        const int64_t slabs = groups <= 256 ? 1 : std::min<int64_t>((groups + 127) / 128, 64);
+        const int threads = threads_of<R>(waves, a.group_rows, G == 1 ? kBackwardThreads<R, G> / 64 : waves), at_once = Place<R, G>::rows_at_once(threads, waves);
+        const Chunks cut = cut_rows(a.rows, a.group_rows, at_once, sums ? 256 : 2048);
+        const int64_t chunks = cut.chunks, all = cut.all;
+        const int64_t slabs = groups <= 1024 ? 1 : std::min<int64_t>((groups + 511) / 512, 64);
         float* const parts = sums ? (float*)ws.take(all * kSums * width * 4) : nullptr;
         float* const partial = sums && slabs > 1 ? (float*)ws.take(slabs * 8 * width * 4) : nullptr;
         GF_RUN {
           const Norms<T> n = make_norms<T>(a);
           const unsigned grid = (unsigned)std::min<int64_t>(all, 1 << 20);
           if (sums)
-            k_norm_backward<T, L, G, kBranch, kNext, true><<<grid, kThreads, 0, s>>>(n, chunk_rows, chunks, all, parts, width);
+            k_norm_backward<T, R, G, kBranch, kNext, true><<<grid, threads, 0, s>>>(n, cut, waves, parts, width);
           else
-            k_norm_backward<T, L, G, kBranch, kNext, false><<<grid, kThreads, 0, s>>>(n, chunk_rows, chunks, all, nullptr, 0);
+            k_norm_backward<T, R, G, kBranch, kNext, false><<<grid, threads, 0, s>>>(n, cut, waves, nullptr, 0);
           GF_LAUNCH_CHECK("k_norm_backward");
           if (sums) {
             const Half<T> b{n.weight, n.bias, n.gate, n.ld_gate, 0, 0.0f, n.gate_value, n.dweight, n.dbias, n.dgate, nullptr};
             const Half<T> f{n.next_weight, n.next_bias, n.scale, n.ld_scale, n.ld_shift, 1.0f, 1.0f, n.dnext_weight, n.dnext_bias, n.dscale, n.dshift};
             int team = 1;
-            while (team < 32 && team * 2 * groups <= 32) team *= 2;
+            while (team < 128 && team * 2 * groups <= 128) team *= 2;
             const int half0 = kBranch ? 0 : 1, halves = (kBranch ? 1 : 0) + (kNext ? 1 : 0);
             k_norm_finish<T><<<dim3((unsigned)((a.cols + 31) / 32), (unsigned)slabs, halves), 1024, 0, s>>>(b, f, half0, n.cols, groups, chunks, parts,
                                                                                                          width, team, partial);
@@ -549,11 +751,14 @@ int gf_norm_forward(const gf_norm_args* args, void* stream) {
     return fail(GF_E_INVALID_ARGUMENT, "stream must not be NULL");
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return with_lanes(a.cols, [&](auto lanes) {
-      constexpr int L = lanes.lanes, G = lanes.groups, kThreads = L < 256 ? 256 : L, kAtOnce = kThreads / L;
+    return with_form(a.cols, [&](auto form, int waves) {
+      constexpr Row R = form.row;
+      constexpr int G = form.groups;
       return with_halves(a, [&](auto branch, auto next) {
-        const unsigned grid = (unsigned)std::min<int64_t>((a.rows + kAtOnce - 1) / kAtOnce, 8192);
-        k_norm_forward<T, L, G, branch.value, next.value><<<grid, kThreads, 0, (hipStream_t)stream>>>(make_norms<T>(a));
+        const int threads = threads_of<R>(waves, a.group_rows, 4), at_once = Place<R, G>::rows_at_once(threads, waves);
+        const Chunks cut = cut_rows(a.rows, a.group_rows, at_once, 2048);
+        const unsigned grid = (unsigned)std::min<int64_t>(cut.all, 1 << 20);
+        k_norm_forward<T, R, G, branch.value, next.value><<<grid, threads, 0, (hipStream_t)stream>>>(make_norms<T>(a), cut, waves);
         GF_LAUNCH_CHECK("k_norm_forward");
         return (int)GF_OK;
       });
