@@ -12,8 +12,6 @@
 
 namespace {
 
-constexpr int kGroup = 32;  // elements of a scale
-
 using f32x2 = float __attribute__((ext_vector_type(2)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
 using bf16x2 = bf16 __attribute__((ext_vector_type(2)));
@@ -29,16 +27,29 @@ __device__ inline float scale_of(uint32_t byte) {
 }
 
 // ------------------------------------------------------------------------------------------
-// 4 lanes a group, 8 elements each.  The scale 2^e: e the least with max <= 7 * 2^e, so that what lies between 6 and 7 goes to 6, as near
-// as a next value 8 would let it; from the bits of the largest magnitude m 2^p, 1 <= m < 2: e = p - 2 up to m = 1.75, else p - 1.  Within
-// [-125, 125], where every value is a normal number of 32 bits.  A group with an infinity or a NaN gets the scale NaN.
+// The layout: tiles of 16 rows x 128 columns, a band of 16 rows after another, a tile as k_q4_few's lanes take it.  A word holds 8 codes,
+// the first lowest; lane q * 16 + row of a tile has the four words of columns 32 j + 8 q (j = 0..3) side by side: what it multiplies by in
+// four matrix instructions, whose operands are 8 columns from each sixteen lanes.  So a wave reads a tile as 1024 bytes in a row.  The
+// tile's scales: a word a row, a byte for each group of 32.  Codes past the matrix are zero.
+
+constexpr int kTileCodes = 1024, kTileScales = 64;
+
+// Where word `w` (columns 8 w..) of a row lies within its tile, in words.
+__device__ inline int word_of(int row, int w) { return ((w & 3) * 16 + row) * 4 + (w >> 2); }
+
+// A tile a workgroup and turn: 16 lanes a row, 8 elements each, four lanes a group.  The scale 2^e: e the least with max <= 7 * 2^e, so that
+// what lies between 6 and 7 goes to 6, as near as a next value 8 would let it; from the bits of the largest magnitude m 2^p, 1 <= m < 2:
+// e = p - 2 up to m = 1.75, else p - 1.  Within [-125, 125], where every value is a normal number of 32 bits.  A group with an infinity or a
+// NaN gets the scale NaN.  The words change places in LDS, so that both sides of memory are read and written in a row.
 template <typename T>
-__global__ __launch_bounds__(256) void k_quantize(int64_t rows, int64_t cols, int64_t groups, const T* __restrict__ w, int64_t ldw,
-                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const int64_t all = rows * groups * 4;
-  for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < all; t += gridDim.x * 256ll) {  // whole groups: 256 and `all` are multiples of 4
-    const int64_t row = t / (groups * 4), q = t % (groups * 4), c = q * 8;
-    const int n = cols - c >= 8 ? 8 : cols - c > 0 ? (int)(cols - c) : 0;
+__global__ __launch_bounds__(256) void k_quantize(int64_t rows, int64_t cols, int64_t across, int64_t tiles, const T* __restrict__ w, int64_t ldw,
+                                                  uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  __shared__ uint32_t words[2][256];
+  const int r = threadIdx.x >> 4, q = threadIdx.x & 15;
+  int slot = 0;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, slot ^= 1) {
+    const int64_t row = tile / across * 16 + r, c = tile % across * 128 + q * 8;
+    const int n = row >= rows || cols <= c ? 0 : cols - c >= 8 ? 8 : (int)(cols - c);
     float v[8];
     load8(v, w + row * ldw + c, n == 8, n);
     uint32_t most = 0;
@@ -57,21 +68,27 @@ __global__ __launch_bounds__(256) void k_quantize(int64_t rows, int64_t cols, in
       code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[4] * inverse, v[5] * inverse, 1.0f, 2);
       code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, v[6] * inverse, v[7] * inverse, 1.0f, 3);
     }
-    *(uint32_t*)(codes + row * groups * 16 + q * 4) = code;
-    if ((q & 3) == 0) scales[row * groups + q / 4] = finite ? (uint8_t)(e + 127) : (uint8_t)255;
+    words[slot][word_of(r, q)] = code;  // the other half is read in the turn before, whose barrier lies behind
+    if ((q & 3) == 0) scales[tile * kTileScales + r * 4 + q / 4] = finite ? (uint8_t)(e + 127) : (uint8_t)255;
+    __syncthreads();
+    codes[tile * (kTileCodes / 4) + threadIdx.x] = words[slot][threadIdx.x];
   }
 }
 
-// 8 values a thread, times their scale in 32 bits and rounded to T.
+// A tile a workgroup and turn, 8 values a thread, times their scale in 32 bits and rounded to T.
 template <typename T>
-__global__ __launch_bounds__(256) void k_dequantize(int64_t rows, int64_t cols, int64_t groups, const uint8_t* __restrict__ codes,
+__global__ __launch_bounds__(256) void k_dequantize(int64_t rows, int64_t cols, int64_t across, int64_t tiles, const uint32_t* __restrict__ codes,
                                                     const uint8_t* __restrict__ scales, T* __restrict__ w) {
-  const int64_t across = (cols + 7) / 8, all = rows * across;
-  for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < all; t += gridDim.x * 256ll) {
-    const int64_t row = t / across, q = t % across, c = q * 8;
-    const int n = cols - c >= 8 ? 8 : (int)(cols - c);
-    const uint32_t code = *(const uint32_t*)(codes + row * groups * 16 + q * 4);
-    const float scale = scale_of(scales[row * groups + q / 4]);
+  __shared__ uint32_t words[2][256];
+  const int r = threadIdx.x >> 4, q = threadIdx.x & 15;
+  int slot = 0;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, slot ^= 1) {
+    const int64_t row = tile / across * 16 + r, c = tile % across * 128 + q * 8;
+    const int n = row >= rows || cols <= c ? 0 : cols - c >= 8 ? 8 : (int)(cols - c);
+    words[slot][threadIdx.x] = codes[tile * (kTileCodes / 4) + threadIdx.x];
+    const float scale = scale_of(scales[tile * kTileScales + r * 4 + q / 4]);
+    __syncthreads();
+    const uint32_t code = words[slot][word_of(r, q)];
     const f32x2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 1),
                         __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 3)};
     float v[8];
@@ -108,92 +125,150 @@ __device__ inline Vec<T, 8> operand8(uint32_t code, float scale) {
 
 template <typename T>
 struct Few {
-  int64_t M, N, K, groups;
+  int64_t M, N, K, across;  // across: tiles of a band
   const T* x;
   int64_t ldx;
   const uint8_t *codes, *scales;
   const T *bias, *residual;
   int64_t ldr;
   T* y;
+  int act;
 };
 
-// The product of at most 16 G rows.  A workgroup takes 16 output columns (gated: 16 of the value's and of the gate's), its waves
-// interleaved chunks of 4 groups along k.  A lane loads 16 bytes, one group of W's row (lane % 16), which are the operands of 4
-// matrix instructions 16 x 16 x 32: k may be summed in any order as long as x's operands have the same one, so lane / 16 chooses a group
-// of the chunk and the instruction 8 elements in each.  32-bit operands are multiplied as such (16 x 16 x 4).  The waves' sums meet in LDS.
-template <typename T, int ACT, int G>
-__global__ __launch_bounds__(1024) void k_q4_few(Few<T> a) {
-  constexpr int H = ACT == GF_ACT_NONE ? 1 : 2;
-  __shared__ float sums[16][H][G][16][16 + 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int64_t n0 = blockIdx.x * 16ll;
-  const int64_t n = n0 + (lane & 15) < a.N ? n0 + (lane & 15) : a.N - 1;
-  const uint8_t *pc[H], *ps[H];
-  const T* px[G];
+// The product of at most 16 G rows.  A workgroup takes 16 NT output columns (gated: as many of the value's and of the gate's), its waves
+// the tiles along k in turn, and the waves' sums meet in LDS.  Bound by reading the codes, so two tiles of them are under way at a time, and by x,
+// which every workgroup reads: NT halves that where there are columns enough.
+//
+// x's operands are 8 columns of row lane % 16 from each sixteen lanes.  Loaded as such, neighbouring lanes would ask for different lines
+// of memory, 64 a load.  Of more than 4 rows a wave loads them row by row, 16 lanes and 256 bytes each, and passes them through its own
+// piece of LDS (no barrier: a wave's LDS operations keep their order), 16 bytes at a time, at place p ^ row of a row's 16 so that neither side's
+// lanes meet in a bank.  Up to 4 rows (DIRECT) the lanes that have one load it themselves.  32-bit operands are multiplied as such
+// (16 x 16 x 4).
+template <typename T, int G>
+constexpr int kFewWaves = G == 1 ? 16 : G * (int)sizeof(T) >= 16 ? 4 : 8;  // as registers allow
+
+template <typename T, int H, int G, int NT, bool DIRECT>
+__global__ __launch_bounds__((kFewWaves<T, G> * 64)) void k_q4_few(Few<T> a) {
+  constexpr int R = H * NT, W = kFewWaves<T, G>, S = (int)sizeof(T), E = 16 / S, P = 8 * S;  // P pieces of E elements in a row of a tile
+  constexpr int kSums = W * R * G * 16 * 17 * 4, kStage = DIRECT ? 0 : W * G * 16 * P * 16;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kSums > kStage ? kSums : kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, quarter = lane >> 4;
+  const int64_t n0 = blockIdx.x * (16ll * NT);
+  using Piece = Vec<T, E>;
+  const uint8_t *pc[R], *ps[R];
 #pragma unroll
-  for (int h = 0; h < H; ++h) pc[h] = a.codes + (n + h * a.N) * a.groups * 16, ps[h] = a.scales + (n + h * a.N) * a.groups;
+  for (int r = 0; r < R; ++r) {
+    const int64_t n = n0 + r / H * 16 + (lane & 15);
+    const int64_t row = (n < a.N ? n : a.N - 1) + r % H * a.N;
+    pc[r] = a.codes + row / 16 * a.across * kTileCodes + (quarter * 16 + row % 16) * 16;
+    ps[r] = a.scales + row / 16 * a.across * kTileScales + row % 16 * 4;
+  }
+  const int64_t whole = a.K / 128;  // tiles
+  f32x4 acc[R][G] = {};
+  struct Codes {
+    u32x4 words[R];
+    uint32_t scales[R];  // of the four groups, a byte each
+  };
+  auto load = [&](Codes& c, int64_t at) {
 #pragma unroll
-  for (int g = 0; g < G; ++g) px[g] = a.x + (16 * g + (lane & 15) < a.M ? 16 * g + (lane & 15) : a.M - 1) * a.ldx;
-  f32x4 acc[H][G] = {};
-  for (int64_t at = (int64_t)wave * 4 + (lane >> 4); at - (lane >> 4) < a.groups; at += waves * 4) {
-    const bool in = at < a.groups;
-    u32x4 code[H];
-    float scale[H];
+    for (int r = 0; r < R; ++r) c.words[r] = *(const u32x4*)(pc[r] + at * kTileCodes), c.scales[r] = *(const uint32_t*)(ps[r] + at * kTileScales);
+  };
+  // x's part of a tile: 16 G rows of P pieces, 64 / P rows a load
+  constexpr int kLoads = DIRECT ? 4 * 8 / E : G * P / 4;
+  struct Part {
+    Piece x[kLoads];
+  };
+  auto x_row = [&](int i) { return DIRECT ? lane & 15 : i * (64 / P) + lane / P; };
+  auto x_col = [&](int i) { return DIRECT ? i / (8 / E) * 32 + quarter * 8 + i % (8 / E) * E : lane % P * E; };
+  auto load_x = [&](Part& c, int64_t at) {
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      code[h] = in ? *(const u32x4*)(pc[h] + at * 16) : u32x4{0, 0, 0, 0};
-      scale[h] = in ? scale_of(ps[h][at]) : 0.0f;
+    for (int i = 0; i < kLoads; ++i) {
+      c.x[i] = (T)0.0f;
+      if (x_row(i) < a.M) c.x[i] = *(const Piece*)(a.x + x_row(i) * a.ldx + at * 128 + x_col(i));
     }
+  };
+  uint8_t* const stage = lds + wave * (kStage / W);
+  // the next tile's part of x is asked for once this one's has left its registers
+  auto multiply = [&](const Codes& c, Part& part, int64_t next) {
+    const Part here = part;
+    if constexpr (!DIRECT) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        *(Piece*)__builtin_assume_aligned(stage + (x_row(i) * P + ((lane % P) ^ (x_row(i) % 16 * (P / 16)))) * 16, 16) = here.x[i];
+    }
+    if (next < whole) load_x(part, next);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t k = at * 32 + j * 8;
-      const int left = a.K - k >= 8 ? 8 : a.K - k > 0 ? (int)(a.K - k) : 0;
-      Vec<T, 8> x[G];
+      Vec<T, 8> b[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        if (left == 8) {
-          x[g] = *(const Vec<T, 8>*)(px[g] + k);
-        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[g][i] = i < left ? px[g][k + i] : (T)0.0f;
+        for (int h = 0; h < 8 / E; ++h) {
+          const int m = g * 16 + (lane & 15), p = (j * 4 + quarter) * (8 / E) + h;
+          const Piece v = DIRECT ? here.x[j * (8 / E) + h] : *(const Piece*)__builtin_assume_aligned(stage + (m * P + (p ^ (m % 16 * (P / 16)))) * 16, 16);
+#pragma unroll
+          for (int e = 0; e < E; ++e) b[g][h * E + e] = v[e];
         }
       }
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        const Vec<T, 8> w = operand8<T>(code[h][j], scale[h]);
+      for (int r = 0; r < R; ++r) {
+        const Vec<T, 8> w = operand8<T>(c.words[r][j], scale_of(c.scales[r] >> 8 * j & 255u));
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[h][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i], x[g][i], acc[h][g], 0, 0, 0);
+            for (int i = 0; i < 8; ++i) acc[r][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i], b[g][i], acc[r][g], 0, 0, 0);
           } else if constexpr (std::is_same_v<T, f16>) {
-            acc[h][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, x[g]), acc[h][g], 0, 0, 0);
+            acc[r][g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, b[g]), acc[r][g], 0, 0, 0);
           } else {
-            acc[h][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x[g]), acc[h][g], 0, 0, 0);
+            acc[r][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, b[g]), acc[r][g], 0, 0, 0);
           }
         }
       }
     }
+  };
+  Codes c[2];
+  Part part;
+  if (wave < a.across) load(c[0], wave);
+  if (wave + waves < a.across) load(c[1], wave + waves);
+  if (wave < whole) load_x(part, wave);
+  int64_t at = wave;
+  for (; at < whole; at += waves) {
+    multiply(c[0], part, at + waves);
+    c[0] = c[1];
+    if (at + 2 * waves < a.across) load(c[1], at + 2 * waves);
+  }
+  if (at < a.across) {  // the part of a tile, at the wave whose turn it is
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      for (int e = 0; e < E; ++e) {
+        const int64_t k = at * 128 + x_col(i) + e;
+        part.x[i][e] = x_row(i) < a.M && k < a.K ? a.x[x_row(i) * a.ldx + k] : (T)0.0f;
+      }
+    multiply(c[0], part, whole);
   }
   // Lane l has row l % 16 of each 16 and columns 4 (l / 16) .. + 4.
+  auto sums = (float(*)[R][G][16][17])lds;
+  if constexpr (!DIRECT) __syncthreads();  // the staged rows are read
 #pragma unroll
-  for (int h = 0; h < H; ++h)
+  for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sums[wave][h][g][lane & 15][4 * (lane >> 4) + r] = acc[h][g][r];
+      for (int i = 0; i < 4; ++i) sums[wave][r][g][lane & 15][4 * quarter + i] = acc[r][g][i];
   __syncthreads();
-  for (int t = threadIdx.x; t < G * 256; t += blockDim.x) {
-    const int64_t m = t / 16, col = n0 + t % 16;
+  for (int t = threadIdx.x; t < NT * G * 256; t += blockDim.x) {
+    const int64_t m = t / 16 % (16 * G), col = n0 + t / (256 * G) * 16 + t % 16;
     if (m >= a.M || col >= a.N) continue;
     float v[H];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       v[h] = 0.0f;
-      for (int i = 0; i < waves; ++i) v[h] += sums[i][h][t / 256][t / 16 % 16][t % 16];
+      for (int i = 0; i < waves; ++i) v[h] += sums[i][t / (256 * G) * H + h][m / 16][m % 16][t % 16];
       if (a.bias != nullptr) v[h] += (float)a.bias[col + h * a.N];
     }
-    if constexpr (H == 2) v[0] *= activation<ACT>(v[1], nullptr);
+    if constexpr (H == 2)
+      v[0] *= a.act == GF_ACT_GELU ? activation<GF_ACT_GELU>(v[1], nullptr) : a.act == GF_ACT_SILU ? activation<GF_ACT_SILU>(v[1], nullptr) : activation<GF_ACT_GELU_TANH>(v[1], nullptr);
     if (a.residual != nullptr) v[0] += (float)a.residual[m * a.ldr + col];
     a.y[m * a.N + col] = (T)v[0];
   }
@@ -202,15 +277,18 @@ __global__ __launch_bounds__(1024) void k_q4_few(Few<T> a) {
 // ------------------------------------------------------------------------------------------
 // Host.
 
-int64_t groups_of(int64_t cols) { return (cols + kGroup - 1) / kGroup; }
+int64_t bands_of(int64_t rows) { return (rows + 15) / 16; }
+int64_t across_of(int64_t cols) { return (cols + 127) / 128; }
+unsigned tile_blocks(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, 16384); }
 int64_t weight_rows(const gf_q4_args& a) { return a.out_features * (a.activation == GF_ACT_NONE ? 1 : 2); }
 
 int check_weight(int64_t rows, int64_t cols, const void* codes, const void* scales) {
   if (rows < 0 || cols <= 0 || rows > kMaxSize || cols > kMaxSize / 2) return fail(GF_E_INVALID_ARGUMENT, "rows or cols of the weight negative or too large");
-  if (rows != 0 && round_up(cols, kGroup) > kMaxElements / rows) return fail(GF_E_INVALID_ARGUMENT, "weight: too large");
+  if (rows != 0 && round_up(cols, 128) > kMaxElements / rows) return fail(GF_E_INVALID_ARGUMENT, "weight: too large");
   if (rows == 0) return GF_OK;
   if (codes == nullptr || scales == nullptr) return fail(GF_E_INVALID_ARGUMENT, "codes and scales must not be NULL");
-  if ((uintptr_t)codes % 16 != 0) return fail(GF_E_INVALID_ARGUMENT, "codes must be 16-byte aligned");
+  if ((uintptr_t)codes % 16 != 0 || (uintptr_t)scales % 4 != 0)
+    return fail(GF_E_INVALID_ARGUMENT, "codes must be 16-byte aligned, scales 4-byte");
   return GF_OK;
 }
 
@@ -222,7 +300,7 @@ int check_args(const gf_q4_args* a) {
     return fail(GF_E_INVALID_ARGUMENT, "rows must not be negative and in_features and out_features must be positive");
   if (a->rows > kMaxSize || a->in_features > kMaxSize / 2 || a->out_features > kMaxSize / 4)
     return fail(GF_E_INVALID_ARGUMENT, "rows, in_features or out_features too large");
-  if (std::max(a->rows, weight_rows(*a)) * round_up(a->in_features, kGroup) > kMaxElements || a->rows * weight_rows(*a) > kMaxElements)
+  if (std::max(a->rows, weight_rows(*a)) * round_up(a->in_features, 128) > kMaxElements || a->rows * weight_rows(*a) > kMaxElements)
     return fail(GF_E_INVALID_ARGUMENT, "rows, in_features or out_features too large");
   for (const int64_t ld : {a->ldx, a->ldr, a->lddy})
     if (ld > kMaxElements || ld < -kMaxElements) return fail(GF_E_INVALID_ARGUMENT, "row stride too large");
@@ -242,8 +320,8 @@ bool few(const gf_q4_args& a) { return a.rows <= 64 && a.saved == nullptr; }
 
 template <typename T>
 int dequantize(int64_t rows, int64_t cols, const void* codes, const void* scales, void* out, hipStream_t s) {
-  const int64_t groups = groups_of(cols);
-  k_dequantize<T><<<blocks_for(rows * ((cols + 7) / 8)), 256, 0, s>>>(rows, cols, groups, (const uint8_t*)codes, (const uint8_t*)scales, (T*)out);
+  const int64_t across = across_of(cols), tiles = bands_of(rows) * across;
+  k_dequantize<T><<<tile_blocks(tiles), 256, 0, s>>>(rows, cols, across, tiles, (const uint32_t*)codes, (const uint8_t*)scales, (T*)out);
   GF_LAUNCH_CHECK("k_dequantize");
   return GF_OK;
 }
@@ -261,21 +339,39 @@ int through_dense(const gf_q4_args& a, bool is_backward, Arena& ws, bool run, hi
   return GF_OK;
 }
 
+template <typename T, int H, int G, bool DIRECT>
+int launch_few(const Few<T>& f, bool wide, hipStream_t s) {
+  // 32 columns a workgroup where that still makes one for each of 256 compute units: of 8192 -> 8192 in bfloat16 one row takes 10.6 us
+  // (16 columns: 11.8), 64 rows 22.6 (36).  16 waves up to a workgroup a unit, else 8, of which two are at work on a unit: 5120 -> 1280 4.5 us
+  // (8 waves: 5.3), 4096 -> 14336 9.6 (16: 11.3), 1280 -> 5120 gated 5.1 (16: 5.9).
+  const int64_t cols = wide ? 32 : 16, groups = (f.N + cols - 1) / cols;
+  const unsigned waves = (unsigned)std::min<int64_t>(f.across, std::min(kFewWaves<T, G>, groups <= 256 ? 16 : 8));
+  if constexpr (H == 1) {
+    if (wide) {
+      k_q4_few<T, 1, G, 2, DIRECT><<<(unsigned)groups, waves * 64, 0, s>>>(f);
+      GF_LAUNCH_CHECK("k_q4_few");
+      return GF_OK;
+    }
+  }
+  k_q4_few<T, H, G, 1, DIRECT><<<(unsigned)groups, waves * 64, 0, s>>>(f);
+  GF_LAUNCH_CHECK("k_q4_few");
+  return GF_OK;
+}
+
 int run_few(const gf_q4_args& a, hipStream_t s) {
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return with_activation(a.activation, [&](auto act) {
-      constexpr int ACT = act.value;
-      const int64_t groups = groups_of(a.in_features);
-      const Few<T> f{a.rows, a.out_features, a.in_features, groups, (const T*)a.x, a.ldx, (const uint8_t*)a.codes, (const uint8_t*)a.scales, (const T*)a.bias,
-                     (const T*)a.residual, a.ldr, (T*)a.y};
-      const dim3 grid((unsigned)((a.out_features + 15) / 16));
-      const unsigned threads = groups >= 16 * 4 ? 1024 : 512;
-      auto* kernel = a.rows <= 16 ? k_q4_few<T, ACT, 1> : a.rows <= 32 ? k_q4_few<T, ACT, 2> : k_q4_few<T, ACT, 4>;
-      kernel<<<grid, threads, 0, s>>>(f);
-      GF_LAUNCH_CHECK("k_q4_few");
-      return (int)GF_OK;
-    });
+    const Few<T> f{a.rows, a.out_features, a.in_features, across_of(a.in_features), (const T*)a.x, a.ldx, (const uint8_t*)a.codes, (const uint8_t*)a.scales,
+                   (const T*)a.bias, (const T*)a.residual, a.ldr, (T*)a.y, a.activation};
+    const bool wide = a.activation == GF_ACT_NONE && f.N >= 32 * 256;
+    auto run = [&](auto halves) {
+      constexpr int H = halves.value;
+      if (f.M <= 4) return launch_few<T, H, 1, true>(f, wide, s);
+      if (f.M <= 16) return launch_few<T, H, 1, false>(f, wide, s);
+      if (f.M <= 32) return launch_few<T, H, 2, false>(f, wide, s);
+      return launch_few<T, H, 4, false>(f, wide, s);
+    };
+    return a.activation == GF_ACT_NONE ? run(std::integral_constant<int, 1>()) : run(std::integral_constant<int, 2>());
   });
 }
 
@@ -290,9 +386,8 @@ int gf_q4_quantize(int32_t dtype, int64_t rows, int64_t cols, const void* weight
   GF_TRY(check_matrix("weight", weight, rows, ldw, cols, size_of(dtype)));
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const int64_t groups = groups_of(cols);
-    k_quantize<T><<<blocks_for(rows * groups * 4), 256, 0, (hipStream_t)stream>>>(rows, cols, groups, (const T*)weight, ldw, (uint8_t*)codes,
-                                                                                 (uint8_t*)scales);
+    const int64_t across = across_of(cols), tiles = bands_of(rows) * across;
+    k_quantize<T><<<tile_blocks(tiles), 256, 0, (hipStream_t)stream>>>(rows, cols, across, tiles, (const T*)weight, ldw, (uint32_t*)codes, (uint8_t*)scales);
     GF_LAUNCH_CHECK("k_quantize");
     return (int)GF_OK;
   });

@@ -224,20 +224,20 @@ std::tuple<Tensor, Tensor> block_norm_autocast(NORM_PARAMETERS) {
 
 // ------------------------------------------------------------------------ 4-bit weights
 
+constexpr int64_t kTileCodes = 1024, kTileScales = 64;  // bytes of a tile of 16 rows x 128 columns
+
 // codes and scales as the kernels read them
 struct Packed {
   Tensor codes, scales;
-  int64_t rows;
-  Packed(const Tensor& c, const Tensor& s, int64_t cols, c10::Device device) : codes(c), scales(s), rows(0) {
+  Packed(const Tensor& c, const Tensor& s, int64_t rows, int64_t cols, c10::Device device) : codes(c), scales(s) {
     TORCH_CHECK(c.scalar_type() == at::kByte && s.scalar_type() == at::kByte, "codes and scales must be uint8");
     TORCH_CHECK(c.device() == device && s.device() == device, "all tensors must be on the same device (got ", device, ", ", c.device(), " and ",
                 s.device(), ")");
-    const int64_t groups = (cols + 31) / 32;
-    TORCH_CHECK(c.dim() == 2 && s.dim() == 2 && c.size(0) == s.size(0) && c.size(1) == 16 * groups && s.size(1) == groups, "a weight of ", cols,
-                " features has codes [rows, ", 16 * groups, "] and scales [rows, ", groups, "] (got ", c.sizes(), " and ", s.sizes(), ")");
-    rows = c.size(0);
+    const int64_t bands = (rows + 15) / 16, across = (cols + 127) / 128, codes_of[] = {bands, across, kTileCodes}, scales_of[] = {bands, across, kTileScales};
+    TORCH_CHECK(rows >= 0 && cols > 0 && c.sizes() == at::IntArrayRef(codes_of) && s.sizes() == at::IntArrayRef(scales_of), "a weight [", rows, ", ", cols,
+                "] has tiles of codes [", bands, ", ", across, ", 1024] and scales [", bands, ", ", across, ", 64] (got ", c.sizes(), " and ", s.sizes(), ")");
     if (!codes.is_contiguous() || (uintptr_t)codes.data_ptr() % 16 != 0) codes = codes.clone(at::MemoryFormat::Contiguous);
-    scales = scales.contiguous();
+    if (!scales.is_contiguous() || (uintptr_t)scales.data_ptr() % 4 != 0) scales = scales.clone(at::MemoryFormat::Contiguous);
   }
 };
 
@@ -247,22 +247,23 @@ std::tuple<Tensor, Tensor> q4_quantize(const Tensor& weight) {
   TORCH_CHECK(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "weight must be float32, bfloat16 or float16 (got ", type_name(t), ")");
   TORCH_CHECK(weight.dim() == 2 && weight.size(1) > 0, "weight must have two dimensions, the second not empty");
   const c10::DeviceGuard guard(weight.device());
-  const int64_t rows = weight.size(0), cols = weight.size(1), groups = (cols + 31) / 32;
+  const int64_t rows = weight.size(0), cols = weight.size(1), bands = (rows + 15) / 16, across = (cols + 127) / 128;
   const auto bytes = weight.options().dtype(at::kByte);
-  Tensor codes = at::empty({rows, groups * 16}, bytes), scales = at::empty({rows, groups}, bytes);
+  Tensor codes = at::empty({bands, across, kTileCodes}, bytes), scales = at::empty({bands, across, kTileScales}, bytes);
+  if (rows == 0) return {codes, scales};
   const Rows w(weight);
   check_rc(gf_q4_quantize(dtype_of(weight), rows, cols, w.data(), w.ld, codes.data_ptr(), scales.data_ptr(), stream_of(weight)), "gf_q4_quantize");
   return {codes, scales};
 }
 
-Tensor q4_dequantize(const Tensor& codes, const Tensor& scales, int64_t cols, at::ScalarType dtype) {
+Tensor q4_dequantize(const Tensor& codes, const Tensor& scales, int64_t rows, int64_t cols, at::ScalarType dtype) {
   TORCH_CHECK(codes.is_cuda(), "codes must be a CUDA tensor");
   TORCH_CHECK(dtype == at::kFloat || dtype == at::kBFloat16 || dtype == at::kHalf, "dtype must be float32, bfloat16 or float16 (got ", type_name(dtype), ")");
-  TORCH_CHECK(cols > 0, "a weight has at least one feature");
   const c10::DeviceGuard guard(codes.device());
-  const Packed p(codes, scales, cols, codes.device());
-  Tensor weight = at::empty({p.rows, cols}, codes.options().dtype(dtype));
-  check_rc(gf_q4_dequantize(dtype_of(weight), p.rows, cols, p.codes.data_ptr(), p.scales.data_ptr(), weight.data_ptr(), stream_of(codes)),
+  const Packed p(codes, scales, rows, cols, codes.device());
+  Tensor weight = at::empty({rows, cols}, codes.options().dtype(dtype));
+  if (rows == 0) return weight;
+  check_rc(gf_q4_dequantize(dtype_of(weight), rows, cols, p.codes.data_ptr(), p.scales.data_ptr(), weight.data_ptr(), stream_of(codes)),
            "gf_q4_dequantize");
   return weight;
 }
@@ -270,10 +271,10 @@ Tensor q4_dequantize(const Tensor& codes, const Tensor& scales, int64_t cols, at
 struct Q4Call {
   Packed w;
   gf_q4_args a{};
-  Q4Call(const Tensor& like, const Tensor& codes, const Tensor& scales, int64_t cols, int64_t rows, int64_t activation)
-      : w(codes, scales, cols, like.device()) {
+  Q4Call(const Tensor& like, const Tensor& codes, const Tensor& scales, int64_t out, int64_t cols, int64_t rows, int64_t activation)
+      : w(codes, scales, out, cols, like.device()) {
     a.dtype = dtype_of(like), a.activation = (int32_t)activation;
-    a.rows = rows, a.in_features = cols, a.out_features = w.rows / (activation == GF_ACT_NONE ? 1 : 2);
+    a.rows = rows, a.in_features = cols, a.out_features = out / (activation == GF_ACT_NONE ? 1 : 2);
     a.codes = w.codes.data_ptr(), a.scales = w.scales.data_ptr();
   }
   void run(bool backward, const Tensor& like) {
@@ -288,11 +289,10 @@ struct Q4Call {
   }
 };
 
-void check_q4(const Tensor& x, const Tensor& codes, const MaybeTensor& bias, const MaybeTensor& residual, int64_t cols, int64_t activation) {
+void check_q4(const Tensor& x, const MaybeTensor& bias, const MaybeTensor& residual, int64_t rows, int64_t cols, int64_t activation) {
   check_first(x);
-  TORCH_CHECK(x.dim() >= 1 && codes.dim() == 2, "x must have shape [..., in_features] and codes two dimensions");
-  TORCH_CHECK(cols > 0 && codes.sym_size(0) != 0, "weight must not be empty");
-  const auto rows = codes.sym_size(0);
+  TORCH_CHECK(x.dim() >= 1, "x must have shape [..., in_features]");
+  TORCH_CHECK(cols > 0 && rows > 0, "weight must not be empty");
   TORCH_CHECK(activation == GF_ACT_NONE || rows % 2 == 0, "a gated weight must have an even number of rows: the value's, then the gate's");
   TORCH_CHECK(x.sym_size(-1) == cols, "x has ", x.sym_size(-1), " features, weight takes ", cols);
   if (present(bias)) {
@@ -310,11 +310,11 @@ void check_q4(const Tensor& x, const Tensor& codes, const MaybeTensor& bias, con
 
 // y, and what the backward needs of a gated product (undefined for a linear one or if not to be saved)
 std::tuple<Tensor, Tensor> q4_forward(const Tensor& x, const Tensor& codes, const Tensor& scales, const MaybeTensor& bias, const MaybeTensor& residual,
-                                      int64_t cols, int64_t activation, bool save) {
-  check_q4(x, codes, bias, residual, cols, activation);
+                                      int64_t rows, int64_t cols, int64_t activation, bool save) {
+  check_q4(x, bias, residual, rows, cols, activation);
   const c10::DeviceGuard guard(x.device());
   const Rows r(x);
-  Q4Call c(x, codes, scales, cols, r.rows, activation);
+  Q4Call c(x, codes, scales, rows, cols, r.rows, activation);
   auto shape = x.sizes().vec();
   shape.back() = c.a.out_features;
   Tensor y = at::empty(shape, x.options()), saved, b;
@@ -331,21 +331,20 @@ std::tuple<Tensor, Tensor> q4_forward(const Tensor& x, const Tensor& codes, cons
 }
 
 // The gradients of x and bias that are wanted.
-std::tuple<Tensor, Tensor> q4_backward(const Tensor& dy, const Tensor& codes, const Tensor& scales, const MaybeTensor& saved, int64_t cols,
+std::tuple<Tensor, Tensor> q4_backward(const Tensor& dy, const Tensor& codes, const Tensor& scales, const MaybeTensor& saved, int64_t rows, int64_t cols,
                                        int64_t activation, bool want_x, bool want_b) {
   check_first(dy);
   TORCH_CHECK(dy.dim() >= 1, "dy must have at least one dimension");
   const c10::DeviceGuard guard(dy.device());
-  TORCH_CHECK(codes.dim() == 2 && dy.size(-1) == codes.size(0) / (activation == GF_ACT_NONE ? 1 : 2), "dy has ", dy.size(-1), " features, codes ",
-              codes.sizes());
+  TORCH_CHECK(rows > 0 && dy.size(-1) == rows / (activation == GF_ACT_NONE ? 1 : 2), "dy has ", dy.size(-1), " features, weight ", rows, " rows");
   const Rows g(dy);
-  Q4Call c(dy, codes, scales, cols, g.rows, activation);
+  Q4Call c(dy, codes, scales, rows, cols, g.rows, activation);
   auto shape = dy.sizes().vec();
   shape.back() = cols;
   auto make = [&](at::IntArrayRef s) { return g.rows ? at::empty(s, dy.options()) : at::zeros(s, dy.options()); };
   Tensor dx, db;
   if (want_x) dx = make(shape);
-  if (want_b) db = make({codes.size(0)});
+  if (want_b) db = make({rows});
   if (g.rows == 0 || !(want_x || want_b)) return {dx, db};
   c.a.dy = g.data(), c.a.lddy = g.ld;
   if (activation != GF_ACT_NONE) {
@@ -360,57 +359,58 @@ std::tuple<Tensor, Tensor> q4_backward(const Tensor& dy, const Tensor& codes, co
 }
 
 std::tuple<Tensor, Tensor> call_q4_forward(const Tensor& x, const Tensor& codes, const Tensor& scales, const MaybeTensor& bias,
-                                           const MaybeTensor& residual, int64_t cols, int64_t activation, bool save) {
+                                           const MaybeTensor& residual, int64_t rows, int64_t cols, int64_t activation, bool save) {
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("guass_amd::q4_forward", "").typed<decltype(q4_forward)>();
-  return op.call(x, codes, scales, bias, residual, cols, activation, save);
+  return op.call(x, codes, scales, bias, residual, rows, cols, activation, save);
 }
 
-std::tuple<Tensor, Tensor> call_q4_backward(const Tensor& dy, const Tensor& codes, const Tensor& scales, const MaybeTensor& saved, int64_t cols,
+std::tuple<Tensor, Tensor> call_q4_backward(const Tensor& dy, const Tensor& codes, const Tensor& scales, const MaybeTensor& saved, int64_t rows, int64_t cols,
                                             int64_t activation, bool want_x, bool want_b) {
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("guass_amd::q4_backward", "").typed<decltype(q4_backward)>();
-  return op.call(dy, codes, scales, saved, cols, activation, want_x, want_b);
+  return op.call(dy, codes, scales, saved, rows, cols, activation, want_x, want_b);
 }
 
 const char* q4_name(int64_t activation) { return activation == GF_ACT_NONE ? "quantized_linear" : "quantized_gated_linear"; }
 
 struct Q4Linear : torch::autograd::Function<Q4Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& codes, const Tensor& scales, const MaybeTensor& bias,
-                        const MaybeTensor& residual, int64_t cols, int64_t activation) {
-    auto [y, saved] = call_q4_forward(x, codes, scales, bias, residual, cols, activation, wants(x) || wants(bias));
+                        const MaybeTensor& residual, int64_t rows, int64_t cols, int64_t activation) {
+    auto [y, saved] = call_q4_forward(x, codes, scales, bias, residual, rows, cols, activation, wants(x) || wants(bias));
     ctx->save_for_backward({codes, scales, saved});
-    ctx->saved_data["call"] = std::make_tuple(cols, activation, present(bias), present(residual), wants(x) || wants(bias));
+    ctx->saved_data["call"] = std::make_tuple(rows, cols, activation, present(bias), present(residual), wants(x) || wants(bias));
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const auto [cols, activation, has_bias, has_residual, trains] = ctx->saved_data["call"].to<std::tuple<int64_t, int64_t, bool, bool, bool>>();
+    const auto [rows, cols, activation, has_bias, has_residual, trains] =
+        ctx->saved_data["call"].to<std::tuple<int64_t, int64_t, int64_t, bool, bool, bool>>();
     // edges are the tensors that are there: x, codes, scales, bias, residual
     const bool wx = ctx->needs_input_grad(0), wb = has_bias && ctx->needs_input_grad(3), wr = has_residual && ctx->needs_input_grad(3 + has_bias);
     const auto saved = ctx->get_saved_variables();
     const Tensor& dy = grads[0];
     // what the gradients depend on: of a gated product x and bias too, by value and gate
     const bool again = dy.requires_grad() || (activation != GF_ACT_NONE && trains);
-    auto [dx, db] = call_q4_backward(dy, saved[0], saved[1], maybe(saved[2]), cols, activation, wx, wb);
-    return once({dx, Tensor(), Tensor(), db, wr ? dy : Tensor(), Tensor(), Tensor()}, q4_name(activation), again);
+    auto [dx, db] = call_q4_backward(dy, saved[0], saved[1], maybe(saved[2]), rows, cols, activation, wx, wb);
+    return once({dx, Tensor(), Tensor(), db, wr ? dy : Tensor(), Tensor(), Tensor(), Tensor()}, q4_name(activation), again);
   }
 };
 
-Tensor q4_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, const MaybeTensor& bias, const MaybeTensor& residual, int64_t cols,
+Tensor q4_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, const MaybeTensor& bias, const MaybeTensor& residual, int64_t rows, int64_t cols,
                  int64_t activation) {
-  check_q4(x, codes, bias, residual, cols, activation);
+  check_q4(x, bias, residual, rows, cols, activation);
   check_no_tangent(q4_name(activation), x, bias, residual);
   if (at::GradMode::is_enabled() && (wants(x) || wants(bias) || wants(residual)))
-    return Q4Linear::apply(x, codes, scales, bias, residual, cols, activation);
-  return std::get<0>(call_q4_forward(x, codes, scales, bias, residual, cols, activation, false));
+    return Q4Linear::apply(x, codes, scales, bias, residual, rows, cols, activation);
+  return std::get<0>(call_q4_forward(x, codes, scales, bias, residual, rows, cols, activation, false));
 }
 
 // As torch's linear: x and bias in autocast's type, and a residual of another type added by torch's rules.
 Tensor q4_linear_autocast(const Tensor& x, const Tensor& codes, const Tensor& scales, const MaybeTensor& bias, const MaybeTensor& residual,
-                          int64_t cols, int64_t activation) {
+                          int64_t rows, int64_t cols, int64_t activation) {
   const c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::Autocast);
   const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
   auto cast = [&](const Tensor& t) { return at::autocast::cached_cast(type, t, at::kCUDA); };
   const bool fused = !present(residual) || residual->scalar_type() == type;
-  const Tensor y = q4_linear(cast(x), codes, scales, present(bias) ? MaybeTensor(cast(*bias)) : bias, fused ? residual : MaybeTensor(), cols, activation);
+  const Tensor y = q4_linear(cast(x), codes, scales, present(bias) ? MaybeTensor(cast(*bias)) : bias, fused ? residual : MaybeTensor(), rows, cols, activation);
   return fused ? y : *residual + y;
 }
 
@@ -428,15 +428,15 @@ TORCH_LIBRARY_IMPL(guass_amd, Autocast, m) {
 TORCH_LIBRARY_FRAGMENT(guass_amd, m) {
   // what a user calls: checks and autograd around the operators below
   m.def("block_norm(" NORM_SCHEMA ") -> (Tensor, Tensor)", block_norm);
-  m.def("q4_linear(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor? residual, int cols, int activation) -> Tensor", q4_linear);
+  m.def("q4_linear(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor? residual, int rows, int cols, int activation) -> Tensor", q4_linear);
   // the launches by themselves, without autograd: what a HIP graph captures, and what a trace (torch.compile) holds
   m.def("block_norm_forward(" NORM_SCHEMA ", bool want_stream) -> (Tensor, Tensor)");
   m.def("block_norm_backward(" NORM_SCHEMA ", Tensor? dstream, Tensor? dnormed, int wants) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, "
         "Tensor, Tensor)");
   m.def("q4_quantize(Tensor weight) -> (Tensor, Tensor)");
-  m.def("q4_dequantize(Tensor codes, Tensor scales, int cols, ScalarType dtype) -> Tensor");
-  m.def("q4_forward(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor? residual, int cols, int activation, bool save) -> (Tensor, Tensor)");
-  m.def("q4_backward(Tensor dy, Tensor codes, Tensor scales, Tensor? saved, int cols, int activation, bool want_x, bool want_b) -> (Tensor, Tensor)");
+  m.def("q4_dequantize(Tensor codes, Tensor scales, int rows, int cols, ScalarType dtype) -> Tensor");
+  m.def("q4_forward(Tensor x, Tensor codes, Tensor scales, Tensor? bias, Tensor? residual, int rows, int cols, int activation, bool save) -> (Tensor, Tensor)");
+  m.def("q4_backward(Tensor dy, Tensor codes, Tensor scales, Tensor? saved, int rows, int cols, int activation, bool want_x, bool want_b) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(guass_amd, CUDA, m) {

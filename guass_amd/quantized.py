@@ -52,33 +52,41 @@ def _register_shapes() -> None:
 
     @fake("guass_amd::q4_quantize")
     def _(weight):
-        groups = (weight.shape[1] + GROUP - 1) // GROUP
-        return (weight.new_empty((weight.shape[0], 16 * groups), dtype=torch.uint8),
-                weight.new_empty((weight.shape[0], groups), dtype=torch.uint8))
+        tiles = (weight.shape[0] + 15) // 16, (weight.shape[1] + 127) // 128
+        return weight.new_empty((*tiles, 1024), dtype=torch.uint8), weight.new_empty((*tiles, 64), dtype=torch.uint8)
 
     @fake("guass_amd::q4_dequantize")
-    def _(codes, scales, cols, dtype):
-        return codes.new_empty((codes.shape[0], cols), dtype=dtype)
+    def _(codes, scales, rows, cols, dtype):
+        return codes.new_empty((rows, cols), dtype=dtype)
 
     @fake("guass_amd::q4_forward")
-    def _(x, codes, scales, bias, residual, cols, activation, save):
-        out = codes.shape[0] // (2 if activation else 1)
+    def _(x, codes, scales, bias, residual, rows, cols, activation, save):
+        out = rows // (2 if activation else 1)
         y = x.new_empty((*x.shape[:-1], out))
         if not (save and activation):
             return y, None
         return y, x.new_empty((y.numel() // out * feedforward._saved_bytes(x.dtype, out),), dtype=torch.uint8)
 
     @fake("guass_amd::q4_backward")
-    def _(dy, codes, scales, saved, cols, activation, want_x, want_b):
-        return (dy.new_empty((*dy.shape[:-1], cols)) if want_x else None, dy.new_empty(codes.shape[:1]) if want_b else None)
+    def _(dy, codes, scales, saved, rows, cols, activation, want_x, want_b):
+        return dy.new_empty((*dy.shape[:-1], cols)) if want_x else None, dy.new_empty((rows,)) if want_b else None
+
+
+def _fill(t: Tensor, rows: int, cols: int) -> Tensor:
+    """t with zeros below and right of it."""
+    return torch.nn.functional.pad(t, (0, cols - t.shape[1], 0, rows - t.shape[0]))
 
 
 class QuantizedWeight:
-    """A weight [rows, in_features] in 4 bits.  ``codes`` uint8 [rows, 16 ceil(in_features / 32)]: two elements a byte, the first in the
-    low half, each a sign (8) and the place of its magnitude among 0, 0.5, 1, 1.5, 2, 3, 4, 6; zero past the row.  ``scales``
-    uint8 [rows, ceil(in_features / 32)]: e + 127 of a group's 2^e, 255 for NaN."""
+    """A weight [rows, in_features] in 4 bits, made of ``codes`` uint8 [rows, 16 ceil(in_features / 32)] (two elements a byte, the first in
+    the low half, each a sign (8) and the place of its magnitude among 0, 0.5, 1, 1.5, 2, 3, 4, 6; zero past the row) and ``scales`` uint8
+    [rows, ceil(in_features / 32)] (e + 127 of a group's 2^e, 255 for NaN).
 
-    __slots__ = ("codes", "scales", "in_features")
+    Held as the kernels read it, in tiles of 16 rows and 128 columns: ``tile_codes`` uint8 [ceil(rows / 16), ceil(in_features / 128), 1024]
+    and ``tile_scales`` [..., 64].  Of the words of 8 codes of a tile's row, word 4 j + q lies at (16 q + row) * 4 + j; the scale of
+    group j at 4 row + j."""
+
+    __slots__ = ("tile_codes", "tile_scales", "rows", "in_features")
 
     def __init__(self, codes: Tensor, scales: Tensor, in_features: int):
         for name, t in (("codes", codes), ("scales", scales)):
@@ -94,24 +102,53 @@ class QuantizedWeight:
                              f"(got {list(codes.shape)} and {list(scales.shape)})")
         if codes.device != scales.device:
             raise ValueError(f"codes and scales must be on the same device (got {codes.device} and {scales.device})")
-        self.codes, self.scales, self.in_features = codes, scales, in_features
+        bands, across = (codes.shape[0] + 15) // 16, (in_features + 127) // 128
+        words = _fill(codes, 16 * bands, 64 * across).view(bands, 16, across, 4, 4, 4)  # row, tile, j, q, byte
+        self.tile_codes = words.permute(0, 2, 4, 1, 3, 5).reshape(bands, across, 1024)
+        self.tile_scales = _fill(scales, 16 * bands, 4 * across).view(bands, 16, across, 4).permute(0, 2, 1, 3).reshape(bands, across, 64)
+        self.rows, self.in_features = codes.shape[0], in_features
+
+    @classmethod
+    def from_tiles(cls, tile_codes: Tensor, tile_scales: Tensor, rows: int, in_features: int) -> "QuantizedWeight":
+        """Of tiles as another one holds them."""
+        tiles = (rows + 15) // 16, (in_features + 127) // 128
+        for name, t, size in (("tile_codes", tile_codes, 1024), ("tile_scales", tile_scales, 64)):
+            if t.dtype != torch.uint8 or t.shape != (*tiles, size):
+                raise ValueError(f"{name} of a weight [{rows}, {in_features}] must be uint8 {[*tiles, size]} (got {t.dtype} {list(t.shape)})")
+        if tile_codes.device != tile_scales.device:
+            raise ValueError(f"tiles must be on the same device (got {tile_codes.device} and {tile_scales.device})")
+        self = cls.__new__(cls)
+        self.tile_codes, self.tile_scales, self.rows, self.in_features = tile_codes, tile_scales, rows, in_features
+        return self
+
+    @property
+    def codes(self) -> Tensor:
+        bands, across, _ = self.tile_codes.shape
+        words = self.tile_codes.reshape(bands, across, 4, 16, 4, 4).permute(0, 3, 1, 4, 2, 5)
+        return words.reshape(16 * bands, 64 * across)[:self.rows, :(self.in_features + GROUP - 1) // GROUP * 16].contiguous()
+
+    @property
+    def scales(self) -> Tensor:
+        bands, across, _ = self.tile_scales.shape
+        groups = self.tile_scales.reshape(bands, across, 16, 4).permute(0, 2, 1, 3)
+        return groups.reshape(16 * bands, 4 * across)[:self.rows, :(self.in_features + GROUP - 1) // GROUP].contiguous()
 
     @property
     def shape(self) -> torch.Size:
-        return torch.Size((self.codes.shape[0], self.in_features))
+        return torch.Size((self.rows, self.in_features))
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.tile_codes.device
 
     def to(self, device) -> "QuantizedWeight":
-        return QuantizedWeight(self.codes.to(device), self.scales.to(device), self.in_features)
+        return QuantizedWeight.from_tiles(self.tile_codes.to(device), self.tile_scales.to(device), self.rows, self.in_features)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> Tensor:
         """The values that it stands for, [rows, in_features], rounded to ``dtype``."""
-        if not self.codes.is_cuda:
+        if not self.tile_codes.is_cuda:
             raise RuntimeError("codes must be a CUDA tensor")
-        return _ops()[2](self.codes, self.scales, self.in_features, dtype)
+        return _ops()[2](self.tile_codes, self.tile_scales, self.rows, self.in_features, dtype)
 
     def __repr__(self) -> str:
         return f"QuantizedWeight({list(self.shape)}, device={str(self.device)!r})"
@@ -127,7 +164,7 @@ def quantize(weight: Tensor) -> QuantizedWeight:
     if weight.dim() != 2:
         raise ValueError(f"weight must have two dimensions (got {list(weight.shape)})")
     weight = weight.detach()
-    return QuantizedWeight(*_ops()[1](weight), weight.shape[1])
+    return QuantizedWeight.from_tiles(*_ops()[1](weight), *weight.shape)
 
 
 def _check(x, weight) -> None:
@@ -140,7 +177,7 @@ def _check(x, weight) -> None:
 def quantized_linear(x: Tensor, weight: QuantizedWeight, bias: Tensor | None = None, residual: Tensor | None = None) -> Tensor:
     """residual + x W^T + bias of x [..., in], weight [out, in], bias [out], residual [..., out]."""
     _check(x, weight)
-    return _ops()[0](x, weight.codes, weight.scales, bias, residual, weight.in_features, 0)
+    return _ops()[0](x, weight.tile_codes, weight.tile_scales, bias, residual, weight.rows, weight.in_features, 0)
 
 
 def quantized_gated_linear(x: Tensor, weight: QuantizedWeight, bias: Tensor | None = None, *, activation: str = "gelu") -> Tensor:
@@ -149,4 +186,4 @@ def quantized_gated_linear(x: Tensor, weight: QuantizedWeight, bias: Tensor | No
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {ACTIVATIONS} (got {activation!r})")
     _check(x, weight)
-    return _ops()[0](x, weight.codes, weight.scales, bias, None, weight.in_features, N.GF_ACTIVATIONS[activation])
+    return _ops()[0](x, weight.tile_codes, weight.tile_scales, bias, None, weight.rows, weight.in_features, N.GF_ACTIVATIONS[activation])

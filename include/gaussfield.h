@@ -607,9 +607,11 @@ int gf_norm_backward(const gf_norm_args* args, void* workspace, size_t workspace
  * Weights in 4 bits (csrc/quantized.hip): a frozen weight, or a trained and merged one, as the OCP microscaling
  * format's MXFP4 (Open Compute Project, "Microscaling Formats (MX) Specification", 2023).  No counterpart in the reference.
  *
- * Of a weight [rows, cols], groups of 32 consecutive elements of a row share a scale: a byte holding e + 127 for 2^e (255: NaN), scales [rows,
- * ceil(cols / 32)].  An element is 4 bits, a sign and the place of its magnitude among 0, 0.5, 1, 1.5, 2, 3, 4, 6: two a byte, the first
- * in the low half, codes [rows, 16 ceil(cols / 32)], 16-byte aligned, zero past the row.  Both contiguous.
+ * Of a weight [rows, cols], groups of 32 consecutive elements of a row share a scale: a byte holding e + 127 for 2^e (255: NaN).  An element
+ * is 4 bits, a sign and the place of its magnitude among 0, 0.5, 1, 1.5, 2, 3, 4, 6.  Both are held in tiles of 16 rows and 128 columns,
+ * [ceil(rows / 16)][ceil(cols / 128)], codes 16-byte aligned, scales 4-byte.  A tile's codes are 1024 bytes: 8 consecutive elements of a row are a
+ * 32-bit word, the first lowest, and word 4 j + q (j, q in 0..3) of row r lies at word (16 q + r) * 4 + j; codes past the matrix are zero.  Its
+ * scales are 64 bytes: that of group j of row r at 4 r + j.
  *
  * gf_q4_quantize: e is the least integer with the group's largest magnitude <= 7 * 2^e, in [-125, 125]; elements go to the nearest
  * value, of two as near to the one with an even place; a group with an infinity or a NaN gets the scale NaN.  gf_q4_dequantize: value

@@ -397,8 +397,8 @@ def test_captured_phases_replay(device):
 
     def step():
         codes, scales = ops.q4_quantize(w)
-        y, saved = ops.q4_forward(many, codes, scales, None, None, 200, 1, True)
-        return [codes, scales, ops.q4_forward(few, codes, scales, None, None, 200, 0, False)[0], y, *ops.q4_backward(dy, codes, scales, saved, 200, 1, True, True)]
+        y, saved = ops.q4_forward(many, codes, scales, None, None, 96, 200, 1, True)
+        return [codes, scales, ops.q4_forward(few, codes, scales, None, None, 96, 200, 0, False)[0], y, *ops.q4_backward(dy, codes, scales, saved, 96, 200, 1, True, True)]
 
     step()
     torch.cuda.synchronize()
