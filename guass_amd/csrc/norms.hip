@@ -13,6 +13,8 @@
 
 namespace {
 
+using f32x4 = float __attribute__((ext_vector_type(4)));
+
 // What the kernels read and write; a matrix as in gf_norm_args.
 template <typename T>
 struct Norms {
@@ -27,21 +29,21 @@ struct Norms {
   T *dx, *dresidual, *dweight, *dbias, *dgate, *dnext_weight, *dnext_bias, *dscale, *dshift;
 };
 
-// Rows and lanes.  A lane holds G groups of 8 consecutive columns of a row.  A row takes 16 lanes (up to 128 columns), a wave (up to 512),
-// or several waves of a workgroup; a workgroup takes several rows at a time.
+// Rows and lanes.  A lane holds G groups of 8 consecutive columns of a row.  A row takes 16 lanes (up to 128 columns), a wave (up to 1536),
+// or all waves of a workgroup; else a workgroup takes several rows at a time.
 //
 // Sums go over a row's lanes by cross-lane instructions, no LDS; past a wave the waves' sums meet in LDS, two numbers at once, at one
 // barrier: the places alternate, and whoever writes one again has passed the barrier behind which all have read it.
 constexpr int kMaxWaves = 16;
 
 template <int CTRL, int ROWS = 0xf>
-__device__ inline float lanes_moved(float v) {
+__device__ __attribute__((always_inline)) inline float lanes_moved(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, ROWS == 0xf));
 }
 
 // The sum over 16 consecutive lanes (WIDE: over the wave), the same bits in each.
 template <bool WIDE>
-__device__ inline float lanes_sum(float v) {
+__device__ __attribute__((always_inline)) inline float lanes_sum(float v) {
   v += lanes_moved<0xB1>(v);   // lane ^ 1
   v += lanes_moved<0x4E>(v);   // lane ^ 2
   v += lanes_moved<0x141>(v);  // the other four of eight
@@ -54,27 +56,25 @@ __device__ inline float lanes_sum(float v) {
   return v;
 }
 
-enum class Row { kPart, kWave, kWaves };  // a row of 16 lanes, of a wave, of several waves
+enum class Row { kPart, kWave, kWaves };  // a row of 16 lanes, of a wave, of the workgroup's waves
 
 template <Row R, int G>
 struct Place {
   int cols, lane, wave, waves, sub;  // lane of the row's wave (or part of one); which of the row's waves; which of the workgroup's rows
-  float2 (*meet)[kMaxWaves][kMaxWaves];
+  float2 (*meet)[kMaxWaves];
   float inverse_last;  // 1 / the columns of the row's last wave
   int slot = 0;
 
-  __device__ Place(int cols, int waves, float2 (*meet)[kMaxWaves][kMaxWaves]) : cols(cols), waves(waves), meet(meet) {
+  __device__ Place(int cols, float2 (*meet)[kMaxWaves]) : cols(cols), waves(R == Row::kWaves ? blockDim.x >> 6 : 1), meet(meet) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if constexpr (R == Row::kPart) {
       lane = threadIdx.x & 15, wave = 0, sub = threadIdx.x >> 4;
     } else {
-      lane = threadIdx.x & 63, sub = R == Row::kWave ? w : w / waves, wave = R == Row::kWave ? 0 : w % waves;
+      lane = threadIdx.x & 63, sub = R == Row::kWave ? w : 0, wave = R == Row::kWave ? 0 : w;
     }
     inverse_last = R == Row::kWaves ? 1.0f / (float)(cols - (waves - 1) * 512 * G) : 0.0f;
   }
-  static __host__ __device__ int rows_at_once(int threads, int waves) {
-    return R == Row::kPart ? threads / 16 : R == Row::kWave ? threads / 64 : threads / 64 / waves;
-  }
+  static __host__ __device__ int rows_at_once(int threads) { return R == Row::kPart ? threads / 16 : R == Row::kWave ? threads / 64 : 1; }
 
   __device__ int col(int g) const { return ((wave * G + g) * (R == Row::kPart ? 16 : 64) + lane) * 8; }
   __device__ int count(int g) const {
@@ -94,10 +94,10 @@ struct Place {
 
   // Each wave's v to the lane of its number in every sixteen lanes of the row, zero to the others.
   __device__ float2 exchange(float2 v) {
-    if (lane == 0) meet[slot][sub][wave] = v;
+    if (lane == 0) meet[slot][wave] = v;
     __syncthreads();
     const int i = threadIdx.x & 15;
-    v = meet[slot][sub][i];
+    v = meet[slot][i];
     slot ^= 1;
     return i < waves ? v : float2{0.0f, 0.0f};
   }
@@ -177,67 +177,108 @@ struct Place {
 };
 
 template <typename T, int G>
-__device__ inline void widen(float v[G][8], const Vec<T, 8> from[G]) {
+__device__ __attribute__((always_inline)) inline void widen(float v[G][8], const Vec<T, 8> from[G]) {
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[g][j] = (float)from[g][j];
 }
 
-// v[] = f(v[], p[]) with a row of parameters, or with `without` where there is none.
-template <typename T, int G, typename P, typename F>
-__device__ inline void with_row(float v[G][8], const P& at, const T* p, float without, F f) {
-  if (p == nullptr) {
+// A half's map n -> n times + plus for a group of rows.  The branch's: gate * weight, gate * bias.  The next norm's: (1 + scale) * weight,
+// (1 + scale) * bias + shift.  It is in registers for a chunk of rows where a lane has one group of columns; where it has more, in LDS, a
+// copy for all rows, so that registers are left for two rows on their way.
+template <int G, bool SHARED>
+struct Maps {
+  float own[SHARED ? 1 : 4][SHARED ? 1 : G][8];
+  f32x4 (*shared)[G][2][64];  // [4][group][half][lane]
+  int lane;
+  __device__ void put(int which, int g, const float v[8]) {
+    if constexpr (!SHARED) {
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+      for (int j = 0; j < 8; ++j) own[which][g][j] = v[j];
+    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[g][j] = f(v[g][j], without);
-    return;
+      for (int h = 0; h < 2; ++h) shared[which][g][h][lane] = f32x4{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
+    }
   }
-  Vec<T, 8> w[G];
-  at.load(w, p);
+  __device__ void get(int which, int g, float v[8]) const {
+    if constexpr (!SHARED) {
 #pragma unroll
-  for (int g = 0; g < G; ++g)
+      for (int j = 0; j < 8; ++j) v[j] = own[which][g][j];
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[g][j] = f(v[g][j], (float)w[g][j]);
-}
-
-// A half's affine map n -> n times[] + plus[] for a group of rows.  The branch's: gate * weight, gate * bias.  The next norm's:
-// (1 + scale) * weight, (1 + scale) * bias + shift.
-template <int G>
-struct Affine {
-  float times[G][8], plus[G][8];
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 q = shared[which][g][h][lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * h + j] = q[j];
+      }
+    }
+  }
 };
+enum { kBranchTimes, kBranchPlus, kNextTimes, kNextPlus };
 
-template <typename T, int G, typename P>
-__device__ inline void branch_affine(Affine<G>& m, const Norms<T>& a, const P& at, int64_t group) {
+// 8 of a row of parameters, or of what stands for it where there is none.
+template <typename T, typename P>
+__device__ __attribute__((always_inline)) inline Vec<T, 8> row8(const P& at, int g, const T* p, float without) {
+  const int n = at.count(g);
+  Vec<T, 8> v = (T)(p == nullptr ? without : 0.0f);
+  if (p != nullptr && n == 8) {
+    v = *(const Vec<T, 8>*)(p + at.col(g));
+  } else if (n < 8) {
 #pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m.times[g][j] = 1.0f, m.plus[g][j] = 0.0f;
-  with_row<T, G>(m.times, at, a.gate ? a.gate + group * a.ld_gate : nullptr, a.gate_value, [](float v, float w) { return w; });
-#pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m.plus[g][j] = m.times[g][j];
-  with_row<T, G>(m.plus, at, a.bias, 0.0f, [](float v, float w) { return v * w; });
-  with_row<T, G>(m.times, at, a.weight, 1.0f, [](float v, float w) { return v * w; });
+    for (int j = 0; j < 8; ++j)
+      if (j >= n) v[j] = (T)0.0f;
+      else if (p != nullptr) v[j] = p[at.col(g) + j];
+  }
+  return v;
 }
 
-template <typename T, int G, typename P>
-__device__ inline void next_affine(Affine<G>& m, const Norms<T>& a, const P& at, int64_t group) {
-  with_row<T, G>(m.times, at, a.scale ? a.scale + group * a.ld_scale : nullptr, 0.0f, [](float v, float w) { return 1.0f + w; });
+// Everything is asked for before anything is used.  In LDS the waves share out the groups.
+template <typename T, int G, bool BRANCH, bool NEXT, bool SHARED, typename P>
+__device__ __attribute__((always_inline)) inline void make_maps(Maps<G, SHARED>& m, const Norms<T>& a, const P& at, int64_t group, int wave, int waves) {
+  auto one = [&](int g) __attribute__((always_inline)) {
+    Vec<T, 8> f, w, b, f2, w2, b2, s2;
+    if constexpr (BRANCH) {
+      f = row8(at, g, a.gate ? a.gate + group * a.ld_gate : nullptr, 1.0f);
+      w = row8(at, g, a.weight, 1.0f);
+      b = row8(at, g, a.bias, 0.0f);
+    }
+    if constexpr (NEXT) {
+      f2 = row8(at, g, a.scale ? a.scale + group * a.ld_scale : nullptr, 0.0f);
+      w2 = row8(at, g, a.next_weight, 1.0f);
+      b2 = row8(at, g, a.next_bias, 0.0f);
+      s2 = row8(at, g, a.shift ? a.shift + group * a.ld_shift : nullptr, 0.0f);
+    }
+    float times[8], plus[8];
+    if constexpr (BRANCH) {
+      const float value = a.gate ? 1.0f : a.gate_value;
 #pragma unroll
-  for (int g = 0; g < G; ++g)
+      for (int j = 0; j < 8; ++j) times[j] = value * (float)f[j] * (float)w[j], plus[j] = value * (float)f[j] * (float)b[j];
+      m.put(kBranchTimes, g, times), m.put(kBranchPlus, g, plus);
+    }
+    if constexpr (NEXT) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m.plus[g][j] = m.times[g][j];
-  with_row<T, G>(m.plus, at, a.next_bias, 0.0f, [](float v, float w) { return v * w; });
-  with_row<T, G>(m.plus, at, a.shift ? a.shift + group * a.ld_shift : nullptr, 0.0f, [](float v, float w) { return v + w; });
-  with_row<T, G>(m.times, at, a.next_weight, 1.0f, [](float v, float w) { return v * w; });
+      for (int j = 0; j < 8; ++j) {
+        const float factor = 1.0f + (float)f2[j];
+        times[j] = factor * (float)w2[j], plus[j] = __builtin_fmaf(factor, (float)b2[j], (float)s2[j]);
+      }
+      m.put(kNextTimes, g, times), m.put(kNextPlus, g, plus);
+    }
+  };
+  if constexpr (SHARED) {
+    for (int g = wave; g < G; g += waves) one(g);
+  } else {
+#pragma unroll
+    for (int g = 0; g < G; ++g) one(g);
+  }
 }
+
+// Whether they are in LDS: where a wave has a row of several groups.
+template <Row R, int G>
+constexpr bool kMapsShared = R == Row::kWave && G > 1;
 
 // 1 / sqrt(v) by the hardware's (1 unit in the last place), which takes a subnormal number for zero.
-__device__ inline float inverse_root(float v) {
+__device__ __attribute__((always_inline)) inline float inverse_root(float v) {
   const bool low = v < 0x1p-96f;
   const float r = __builtin_amdgcn_rsqf(low ? v * 0x1p64f : v);
   return low ? r * 0x1p32f : r;
@@ -245,7 +286,7 @@ __device__ inline float inverse_root(float v) {
 
 // x becomes n(x), zero past the row; returns 1 / deviation (rms: 1 / root mean square).
 template <int G, typename P>
-__device__ inline float normalise(float x[G][8], int kind, float eps, float inverse, P& at) {
+__device__ __attribute__((always_inline)) inline float normalise(float x[G][8], int kind, float eps, float inverse, P& at) {
   float rstd;
   if (kind == GF_NORM_LAYER) {
     const float2 s = at.spread(x, inverse);
@@ -272,7 +313,7 @@ __device__ inline float normalise(float x[G][8], int kind, float eps, float inve
 
 // The gradient of x from that of n(x), in place: rstd (g - mean g - n(x) mean(g n(x))), without mean g for rms; zero past the row.
 template <int G, typename P>
-__device__ inline void through_norm(float g_[G][8], const float n_[G][8], int kind, float rstd, float inverse, P& at) {
+__device__ __attribute__((always_inline)) inline void through_norm(float g_[G][8], const float n_[G][8], int kind, float rstd, float inverse, P& at) {
   float a = 0.0f, b = 0.0f;
 #pragma unroll
   for (int g = 0; g < G; ++g)
@@ -293,53 +334,63 @@ struct Chunks {
   int64_t rows, chunks, all;
 };
 
-template <Row R, int G>
-constexpr int kForwardThreads = R != Row::kWaves ? 256 : G == 1 ? 768 : 1024;
+// The maps' LDS of a kernel, and a barrier around its filling.
+#define GF_MAPS(BRANCH, NEXT)                                                                                            \
+  constexpr bool kShared = kMapsShared<R, G>;                                                                            \
+  __shared__ f32x4 map_words[kShared ? 4 : 1][kShared ? G : 1][2][64];                                                   \
+  Maps<G, kShared> maps;                                                                                                 \
+  maps.lane = at.lane, maps.shared = (f32x4(*)[G][2][64])map_words;                                                      \
+  auto set_maps = [&](int64_t group) {                                                                                   \
+    if (kShared) __syncthreads();                                                                                        \
+    make_maps<T, G, BRANCH, NEXT, kShared>(maps, a, at, group, kShared ? at.sub : 0, kShared ? (int)blockDim.x >> 6 : 1); \
+    if (kShared) __syncthreads();                                                                                        \
+  }
 
-// Forward.  BRANCH: s from x and the residual; NEXT: h from s (without BRANCH, from x).  A group's maps stay in registers for a chunk, and the
-// next row is on its way while one is worked on.
-template <typename T, Row R, int G, bool BRANCH, bool NEXT>
-__global__ __launch_bounds__((kForwardThreads<R, G>)) void k_norm_forward(Norms<T> a, Chunks cut, int waves) {
-  __shared__ float2 meet[2][kMaxWaves][kMaxWaves];
-  Place<R, G> at(a.cols, waves, meet);
-  const int at_once = at.rows_at_once(blockDim.x, waves);
+// Forward.  BRANCH: s from x and the residual; NEXT: h from s (without BRANCH, from x).  The next row is on its way while one is worked on.
+template <typename T, Row R, int G, int THREADS, bool BRANCH, bool NEXT>
+__global__ __launch_bounds__(THREADS) void k_norm_forward(Norms<T> a, Chunks cut) {
+  __shared__ float2 meet[2][kMaxWaves];
+  Place<R, G> at(a.cols, meet);
+  GF_MAPS(BRANCH, NEXT);
+  const int at_once = at.rows_at_once(blockDim.x);
   for (int64_t chunk = blockIdx.x; chunk < cut.all; chunk += gridDim.x) {
     const int64_t group = chunk / cut.chunks, first = chunk % cut.chunks * cut.rows;
     const int64_t begin = group * a.group_rows + first, end = group * a.group_rows + (first + cut.rows < a.group_rows ? first + cut.rows : a.group_rows);
-    Affine<BRANCH ? G : 1> mb;
-    Affine<NEXT ? G : 1> mn;
-    if constexpr (BRANCH) branch_affine<T, G>(mb, a, at, group);
-    if constexpr (NEXT) next_affine<T, G>(mn, a, at, group);
     Vec<T, 8> vx[G], vr[BRANCH ? G : 1];
     auto fetch = [&](int64_t row) {
       at.load(vx, a.x + row * a.ldx);
       if constexpr (BRANCH) at.load(vr, a.residual + row * a.ldr);
     };
-    // all of a workgroup's rows take part in every turn (there are barriers): past the chunk the last row again, not stored
     int64_t row = begin + at.sub;
-    fetch(row < end ? row : end - 1);
-    for (int64_t turn = begin; turn < end; turn += at_once, row += at_once) {
+    if (row < end) fetch(row);
+    set_maps(group);
+    for (; row < end; row += at_once) {
+      asm volatile("" ::: "memory");  // what LDS holds of the maps stays there
       float v[G][8], r[BRANCH ? G : 1][8];
       widen<T, G>(v, vx);
       if constexpr (BRANCH) widen<T, G>(r, vr);
-      if (turn + at_once < end) fetch(row + at_once < end ? row + at_once : end - 1);
-      const bool mine = row < end;
+      if (row + at_once < end) fetch(row + at_once);
       if constexpr (BRANCH) {
         if (a.kind != GF_NORM_NONE) normalise<G>(v, a.kind, a.eps, a.inverse, at);
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+          float w[8], b[8];
+          maps.get(kBranchTimes, g, w), maps.get(kBranchPlus, g, b);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            v[g][j] = __builtin_fmaf(a.residual_scale, r[g][j], __builtin_fmaf(v[g][j], mb.times[g][j], mb.plus[g][j]));
-        if (a.stream != nullptr && mine) at.store(a.stream + row * a.cols, v);
+          for (int j = 0; j < 8; ++j) v[g][j] = __builtin_fmaf(a.residual_scale, r[g][j], __builtin_fmaf(v[g][j], w[j], b[j]));
+        }
+        if (a.stream != nullptr) at.store(a.stream + row * a.cols, v);
       }
       if constexpr (NEXT) {
         normalise<G>(v, a.next_kind, a.next_eps, a.inverse, at);
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+          float w[8], b[8];
+          maps.get(kNextTimes, g, w), maps.get(kNextPlus, g, b);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[g][j] = __builtin_fmaf(v[g][j], mn.times[g][j], mn.plus[g][j]);
-        if (mine) at.store(a.normed + row * a.cols, v);
+          for (int j = 0; j < 8; ++j) v[g][j] = __builtin_fmaf(v[g][j], w[j], b[j]);
+        }
+        at.store(a.normed + row * a.cols, v);
       }
     }
   }
@@ -348,56 +399,59 @@ __global__ __launch_bounds__((kForwardThreads<R, G>)) void k_norm_forward(Norms<
 // Column sums of a chunk of rows, per element: of ds, ds n(x), dh, dh n'(s).
 constexpr int kSums = 4;
 
-template <Row R, int G>
-constexpr int kBackwardThreads = R == Row::kPart ? 256 : R == Row::kWave ? 512 : G == 1 ? 768 : 1024;
-
 // Backward, by chunks of rows.  SUMS: the column sums too, into parts [chunk][kSums][width].
-template <typename T, Row R, int G, bool BRANCH, bool NEXT, bool SUMS>
-__global__ __launch_bounds__((kBackwardThreads<R, G>)) void k_norm_backward(Norms<T> a, Chunks cut, int waves, float* parts, int64_t width) {
-  __shared__ float2 meet[2][kMaxWaves][kMaxWaves];
-  constexpr int kThreads = kBackwardThreads<R, G>;
-  __shared__ float together[SUMS && G == 1 ? kThreads * 8 : 1];  // with two groups a lane a workgroup has one row
-  Place<R, G> at(a.cols, waves, meet);
-  const int at_once = at.rows_at_once(blockDim.x, waves);
+template <typename T, Row R, int G, int THREADS, bool BRANCH, bool NEXT, bool SUMS>
+__global__ __launch_bounds__(THREADS) void k_norm_backward(Norms<T> a, Chunks cut, float* parts, int64_t width) {
+  __shared__ float2 meet[2][kMaxWaves];
+  constexpr int kSpan = (R == Row::kPart ? 128 : 512) * G, kRows = R == Row::kPart ? 16 : 8;  // columns that a row's lanes hold; rows at a time
+  __shared__ f32x4 together[2][SUMS && R != Row::kWaves ? kRows : 1][SUMS && R != Row::kWaves ? kSpan / 4 : 1];
+  Place<R, G> at(a.cols, meet);
+  GF_MAPS(BRANCH, NEXT);
+  const int at_once = at.rows_at_once(blockDim.x);
   for (int64_t chunk = blockIdx.x; chunk < cut.all; chunk += gridDim.x) {
     const int64_t group = chunk / cut.chunks, first = chunk % cut.chunks * cut.rows;
     const int64_t begin = group * a.group_rows + first, end = group * a.group_rows + (first + cut.rows < a.group_rows ? first + cut.rows : a.group_rows);
-    Affine<BRANCH ? G : 1> mb;
-    Affine<NEXT ? G : 1> mn;
-    if constexpr (BRANCH) branch_affine<T, G>(mb, a, at, group);
-    if constexpr (NEXT) next_affine<T, G>(mn, a, at, group);
-    float sums[SUMS ? kSums : 1][G][8] = {};
     const bool needs_x = NEXT || SUMS || a.kind != GF_NORM_NONE;
+    // The next row is on its way while one is worked on: x and the residual, and the gradients too where registers are left (else those
+    // come while the row's statistics are made).
+    constexpr bool kAhead = G == 1 || !(BRANCH && NEXT);
     Vec<T, 8> vx[G] = {}, vr[BRANCH && NEXT ? G : 1], vs[BRANCH ? G : 1] = {}, vh[NEXT ? G : 1];
-    auto fetch = [&](int64_t row) {
-      if (needs_x) at.load(vx, a.x + row * a.ldx);
-      if constexpr (BRANCH && NEXT) at.load(vr, a.residual + row * a.ldr);
+    auto fetch_gradients = [&](int64_t row) {
       if constexpr (BRANCH) {
         if (a.dstream != nullptr) at.load(vs, a.dstream + row * a.ld_dstream);
       }
       if constexpr (NEXT) at.load(vh, a.dnormed + row * a.ld_dnormed);
     };
+    auto fetch = [&](int64_t row) {
+      if (needs_x) at.load(vx, a.x + row * a.ldx);
+      if constexpr (BRANCH && NEXT) at.load(vr, a.residual + row * a.ldr);
+      if constexpr (kAhead) fetch_gradients(row);
+    };
     int64_t row = begin + at.sub;
-    fetch(row < end ? row : end - 1);
-    for (int64_t turn = begin; turn < end; turn += at_once, row += at_once) {
-      const bool mine = row < end;
-      // past the chunk the last row again, neither stored nor added
-      auto add = [&](int k, const float d[G][8], const float n[G][8]) {
-        if constexpr (SUMS) {
-          if (mine) {
+    if (row < end) fetch(row);
+    set_maps(group);
+    float sums[SUMS ? kSums : 1][G][8] = {};
+    auto add = [&](int k, const float d[G][8], const float n[G][8]) {
+      if constexpr (SUMS) {
 #pragma unroll
-            for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-              for (int j = 0; j < 8; ++j) sums[k][g][j] += d[g][j], sums[k + 1][g][j] = __builtin_fmaf(d[g][j], n[g][j], sums[k + 1][g][j]);
-          }
-        }
-      };
-      float x[G][8], r[BRANCH && NEXT ? G : 1][8], d[G][8], ds[BRANCH ? G : 1][8];
+          for (int j = 0; j < 8; ++j) sums[k][g][j] += d[g][j], sums[k + 1][g][j] = __builtin_fmaf(d[g][j], n[g][j], sums[k + 1][g][j]);
+      }
+    };
+    for (; row < end; row += at_once) {
+      asm volatile("" ::: "memory");  // what LDS holds of the maps stays there
+      if constexpr (!kAhead) fetch_gradients(row);
+      float x[G][8], r[BRANCH && NEXT ? G : 1][8], d[G][8];
       widen<T, G>(x, vx);
       if constexpr (BRANCH && NEXT) widen<T, G>(r, vr);
-      if constexpr (BRANCH) widen<T, G>(ds, vs);
-      if constexpr (NEXT) widen<T, G>(d, vh);
-      if (turn + at_once < end) fetch(row + at_once < end ? row + at_once : end - 1);
+      Vec<T, 8> ws[BRANCH ? G : 1], wh[NEXT ? G : 1];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if constexpr (BRANCH) ws[g] = vs[g];
+        if constexpr (NEXT) wh[g] = vh[g];
+      }
+      if (row + at_once < end) fetch(row + at_once);
       float rstd = 1.0f;
       if constexpr (BRANCH) {
         if (a.kind != GF_NORM_NONE) rstd = normalise<G>(x, a.kind, a.eps, a.inverse, at);
@@ -405,29 +459,36 @@ __global__ __launch_bounds__((kBackwardThreads<R, G>)) void k_norm_backward(Norm
       if constexpr (NEXT) {
         float s[G][8];
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+          float w[8], b[8];
+          if constexpr (BRANCH) maps.get(kBranchTimes, g, w), maps.get(kBranchPlus, g, b);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             if constexpr (BRANCH)
-              s[g][j] = __builtin_fmaf(a.residual_scale, r[g][j], __builtin_fmaf(x[g][j], mb.times[g][j], mb.plus[g][j]));
+              s[g][j] = __builtin_fmaf(a.residual_scale, r[g][j], __builtin_fmaf(x[g][j], w[j], b[j]));
             else
               s[g][j] = x[g][j];
           }
+        }
         const float next_rstd = normalise<G>(s, a.next_kind, a.next_eps, a.inverse, at);
+        widen<T, G>(d, wh);
         add(2, d, s);
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+          float w[8];
+          maps.get(kNextTimes, g, w);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[g][j] *= mn.times[g][j];
+          for (int j = 0; j < 8; ++j) d[g][j] *= w[j];
+        }
         through_norm<G>(d, s, a.next_kind, next_rstd, a.inverse, at);
       }
       if constexpr (BRANCH) {
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[g][j] = NEXT ? d[g][j] + ds[g][j] : ds[g][j];
+          for (int j = 0; j < 8; ++j) d[g][j] = NEXT ? d[g][j] + (float)ws[g][j] : (float)ws[g][j];
         add(0, d, x);
-        if (a.dresidual != nullptr && mine) {
+        if (a.dresidual != nullptr) {
           float t[G][8];
 #pragma unroll
           for (int g = 0; g < G; ++g)
@@ -437,33 +498,46 @@ __global__ __launch_bounds__((kBackwardThreads<R, G>)) void k_norm_backward(Norm
         }
         if (a.dx != nullptr) {
 #pragma unroll
-          for (int g = 0; g < G; ++g)
+          for (int g = 0; g < G; ++g) {
+            float w[8];
+            maps.get(kBranchTimes, g, w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) d[g][j] *= mb.times[g][j];
+            for (int j = 0; j < 8; ++j) d[g][j] *= w[j];
+          }
           if (a.kind != GF_NORM_NONE) through_norm<G>(d, x, a.kind, rstd, a.inverse, at);
         }
       }
-      if (a.dx != nullptr && mine) at.store(a.dx + row * a.cols, d);
+      if (a.dx != nullptr) at.store(a.dx + row * a.cols, d);
     }
     if constexpr (SUMS) {
-      const int span = R == Row::kPart ? 128 : 512 * G * (R == Row::kWave ? 1 : waves);  // columns that a row's lanes hold
 #pragma unroll
-      for (int k = BRANCH ? 0 : 2; k < (NEXT ? kSums : 2); ++k) {
+      for (int k = BRANCH ? 0 : 2; k < (NEXT ? kSums : 2); k += 2) {
         float* const out = parts + (chunk * kSums + k) * width;
-        if (at_once == 1) {
+        if (R == Row::kWaves || at_once == 1) {
 #pragma unroll
           for (int g = 0; g < G; ++g)
-            if (at.count(g) > 0) store8(out + at.col(g), sums[k][g], true, 8);
+            if (at.count(g) > 0) store8(out + at.col(g), sums[k][g], true, 8), store8(out + width + at.col(g), sums[k + 1][g], true, 8);
           continue;
         }
         __syncthreads();
 #pragma unroll
-        for (int g = 0; g < G; ++g) store8(together + at.sub * span + at.col(g), sums[k][g], true, 8);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float* const v = sums[k + i][g] + 4 * h;
+              together[i][at.sub][at.col(g) / 4 + h] = f32x4{v[0], v[1], v[2], v[3]};
+            }
         __syncthreads();
-        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
-          float v = together[c];
-          for (int i = 1; i < at_once; ++i) v += together[i * span + c];
-          out[c] = v;
+        for (int c = threadIdx.x; c < 2 * (kSpan / 4); c += blockDim.x) {
+          const int i = c / (kSpan / 4), q = c % (kSpan / 4);
+          if (q * 4 >= width) continue;
+          f32x4 v = together[i][0][q];
+#pragma unroll
+          for (int n = 1; n < kRows; ++n)
+            if (n < at_once) v += together[i][n][q];
+          *(f32x4*)(out + i * width + q * 4) = v;
         }
       }
       __syncthreads();
@@ -485,24 +559,35 @@ struct Half {
   T *dweight, *dbias, *dfactor, *dshift;
 };
 
-using f32x4 = float __attribute__((ext_vector_type(4)));
-
+// Asked for only: what needs it waits for it.
 template <typename T>
-__device__ inline f32x4 load4(const T* p, int64_t c, int n, float without) {
-  f32x4 v;
+__device__ __attribute__((always_inline)) inline Vec<T, 4> load4(const T* p, int64_t c, int n, float without) {
+  Vec<T, 4> v = (T)without;
+  if (p == nullptr) return v;
+  if (n == 4) return *(const Vec<T, 4>*)(p + c);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = p != nullptr && j < n ? (float)p[c + j] : without;
+  for (int j = 0; j < 3; ++j)
+    if (j < n) v[j] = p[c + j];
   return v;
 }
 
 template <typename T>
-__device__ inline void store4(T* p, int64_t c, int n, f32x4 v) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (j < n) p[c + j] = (T)v[j];
+__device__ __attribute__((always_inline)) inline f32x4 widen4(Vec<T, 4> v) {
+  return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
 }
 
-__device__ inline f32x4 from_lane(f32x4 v, int mask) {
+template <typename T>
+__device__ __attribute__((always_inline)) inline void store4(T* p, int64_t c, int n, f32x4 v) {
+  if (n == 4) {
+    *(Vec<T, 4>*)(p + c) = Vec<T, 4>{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < n) p[c + j] = (T)v[j];
+  }
+}
+
+__device__ __attribute__((always_inline)) inline f32x4 from_lane(f32x4 v, int mask) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = __shfl_xor(v[j], mask);
   return v;
@@ -519,11 +604,12 @@ __global__ __launch_bounds__(1024) void k_norm_finish(Half<T> branch, Half<T> ne
   const int n = cols - c < 0 ? 0 : cols - c < 4 ? (int)(cols - c) : 4;
   const int64_t slab = (groups + gridDim.y - 1) / gridDim.y, g0 = blockIdx.y * slab, g1 = g0 + slab < groups ? g0 + slab : groups;
   const int teams = 128 / team, of = member & (team - 1);
-  const f32x4 w = load4(h.weight, c, n, 1.0f), b = load4(h.bias, c, n, 0.0f);
+  const Vec<T, 4> w = load4(h.weight, c, n, 1.0f), b = load4(h.bias, c, n, 0.0f);
   f32x4 shared[4] = {};
   for (int64_t base = g0; base < g1; base += teams) {
     const int64_t g = base + member / team;
     f32x4 s0 = 0.0f, s1 = 0.0f;
+    const Vec<T, 4> factor = load4(h.factor != nullptr && g < g1 ? h.factor + g * h.ld_factor : nullptr, c, n, 0.0f);
     if (n > 0 && g < g1) {
 #pragma unroll 4
       for (int64_t i = of; i < chunks; i += team) {
@@ -541,9 +627,9 @@ __global__ __launch_bounds__(1024) void k_norm_finish(Half<T> branch, Half<T> ne
       for (int i = 0; i < team / 8; ++i) s0 += meet[0][w0 + i][lane], s1 += meet[1][w0 + i][lane];
     }
     if (n > 0 && g < g1 && of == 0) {
-      const f32x4 f = h.factor != nullptr ? h.one + load4(h.factor + g * h.ld_factor, c, n, 0.0f) : f32x4(h.value);
+      const f32x4 f = h.factor != nullptr ? h.one + widen4<T>(factor) : f32x4(h.value);
       shared[0] += f * s1, shared[1] += f * s0;
-      const f32x4 own = w * s1 + b * s0;
+      const f32x4 own = widen4<T>(w) * s1 + widen4<T>(b) * s0;
       if (h.dfactor != nullptr) {
         if (h.ld_factor != 0) store4(h.dfactor + g * cols, c, n, own);
         else shared[2] += own;
@@ -643,26 +729,39 @@ Norms<T> make_norms(const gf_norm_args& a) {
   return n;
 }
 
-template <Row R, int G>
+template <Row R, int G, int THREADS>
 struct Form {
   static constexpr Row row = R;
-  static constexpr int groups = G;
+  static constexpr int groups = G, threads = THREADS;
 };
 
-// How a row is held: 16 lanes up to 128 columns, a wave up to 512, else a wave for each 512, or (16 are a workgroup's limit) each 1024.
+// How a row is held: 16 lanes up to 128 columns, a wave up to `wave_cols`, else a workgroup's waves, 512 columns each, past 6144 (12 waves,
+// as many as have the registers) 1024.
 template <typename F>
-int with_form(int64_t cols, F f) {
-  if (cols <= 128) return f(Form<Row::kPart, 1>(), 1);
-  if (cols <= 512) return f(Form<Row::kWave, 1>(), 1);
-  if (cols <= 512 * 12) return f(Form<Row::kWaves, 1>(), (int)((cols + 511) / 512));
-  return f(Form<Row::kWaves, 2>(), (int)((cols + 1023) / 1024));
+int with_form(int64_t cols, int64_t wave_cols, F f) {
+  if (cols <= 128) return f(Form<Row::kPart, 1, 256>());
+  if (cols <= 512) return f(Form<Row::kWave, 1, 512>());
+  if (cols <= std::min<int64_t>(wave_cols, 1024)) return f(Form<Row::kWave, 2, 512>());
+  if (cols <= std::min<int64_t>(wave_cols, 1536)) return f(Form<Row::kWave, 3, 512>());
+  if (cols <= 6144) return f(Form<Row::kWaves, 1, 768>());
+  if (cols <= 8192) return f(Form<Row::kWaves, 2, 512>());
+  return f(Form<Row::kWaves, 2, 1024>());
+}
+
+// The widest row that a wave takes alone.  8192 x 1280 in bfloat16, gate_add_norm: 22 us forward (three waves a row: 26 to 29), 31 backward
+// without sums (33).  The sums of both halves leave a wave with three groups a lane no registers: 54 us by three waves, 66 by one.
+// With few rows a row's time counts: one of 1280 takes 3.2 us by three waves, 5.6 by one.
+int64_t wave_cols(const gf_norm_args& a, bool sums) {
+  if (a.rows < 2048) return 512;
+  return sums && a.residual != nullptr && a.next_kind != GF_NORM_NONE ? 1024 : 1536;
 }
 
 // Threads of a workgroup: as many rows at a time as `most` waves hold, but no more than there are in a group.
-template <Row R>
-int threads_of(int waves, int64_t group_rows, int most) {
+template <Row R, int G>
+int threads_of(int64_t cols, int64_t group_rows, int most) {
+  if (R == Row::kWaves) return 64 * (int)((cols + 512 * G - 1) / (512 * G));
   if (R == Row::kPart) return (int)std::min<int64_t>(round_up(group_rows * 16, 64), most * 64);
-  return waves * 64 * (int)std::max<int64_t>(std::min<int64_t>(group_rows, most / waves), 1);
+  return 64 * (int)std::min<int64_t>(group_rows, most);
 }
 
 // Each group in chunks of whole turns of a workgroup, until there are about `want` chunks.
@@ -690,16 +789,19 @@ bool wants_sums(const gf_norm_args& a) {
 
 int backward(const gf_norm_args& a, Arena& ws, bool run, hipStream_t s) {
   const int64_t groups = a.rows / a.group_rows, width = round_up(a.cols, 8);
+  const bool sums = wants_sums(a);
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return with_form(a.cols, [&](auto form, int waves) {
+    return with_form(a.cols, wave_cols(a, sums), [&](auto form) {
       constexpr Row R = form.row;
-      constexpr int G = form.groups;
+      constexpr int G = form.groups, kThreads = form.threads;
       return with_halves(a, [&](auto branch, auto next) {
-        constexpr bool kBranch = branch.value, kNext = next.value;
-        const bool sums = wants_sums(a);
-        const int threads = threads_of<R>(waves, a.group_rows, G == 1 ? kBackwardThreads<R, G> / 64 : waves), at_once = Place<R, G>::rows_at_once(threads, waves);
-        const Chunks cut = cut_rows(a.rows, a.group_rows, at_once, sums ? 256 : 2048);
+        constexpr bool kBranch = branch.value, kNext = next.value, kSumless = R == Row::kWave && G == 3 && kBranch && kNext;
+        // Workgroups for each of 256 compute units as their registers allow, and each of them its chunks' sums to write.  Without sums two, which
+        // the barriers or loads of one do not keep waiting (8192 x 1280 gate_add_norm: 31 us; one of 8 waves 37).
+        const int threads = threads_of<R, G>(a.cols, a.group_rows, R == Row::kPart || (!sums && G > 1) ? 4 : 8);
+        const int fit = R == Row::kWaves ? std::min(std::max(12 * 64 / threads, 1), 3) : 1;
+        const Chunks cut = cut_rows(a.rows, a.group_rows, Place<R, G>::rows_at_once(threads), 256 * (sums ? fit : 2));
         const int64_t chunks = cut.chunks, all = cut.all;
         const int64_t slabs = groups <= 1024 ? 1 : std::min<int64_t>((groups + 511) / 512, 64);
         float* const parts = sums ? (float*)ws.take(all * kSums * width * 4) : nullptr;
@@ -707,10 +809,11 @@ int backward(const gf_norm_args& a, Arena& ws, bool run, hipStream_t s) {
         GF_RUN {
           const Norms<T> n = make_norms<T>(a);
           const unsigned grid = (unsigned)std::min<int64_t>(all, 1 << 20);
-          if (sums)
-            k_norm_backward<T, R, G, kBranch, kNext, true><<<grid, threads, 0, s>>>(n, cut, waves, parts, width);
-          else
-            k_norm_backward<T, R, G, kBranch, kNext, false><<<grid, threads, 0, s>>>(n, cut, waves, nullptr, 0);
+          if (!sums) {
+            k_norm_backward<T, R, G, kThreads, kBranch, kNext, false><<<grid, threads, 0, s>>>(n, cut, nullptr, 0);
+          } else if constexpr (!kSumless) {
+            k_norm_backward<T, R, G, kThreads, kBranch, kNext, true><<<grid, threads, 0, s>>>(n, cut, parts, width);
+          }
           GF_LAUNCH_CHECK("k_norm_backward");
           if (sums) {
             const Half<T> b{n.weight, n.bias, n.gate, n.ld_gate, 0, 0.0f, n.gate_value, n.dweight, n.dbias, n.dgate, nullptr};
@@ -751,14 +854,16 @@ int gf_norm_forward(const gf_norm_args* args, void* stream) {
     return fail(GF_E_INVALID_ARGUMENT, "stream must not be NULL");
   return with_dtype(a.dtype, [&](auto t) {
     using T = decltype(t);
-    return with_form(a.cols, [&](auto form, int waves) {
+    return with_form(a.cols, wave_cols(a, false), [&](auto form) {
       constexpr Row R = form.row;
-      constexpr int G = form.groups;
+      constexpr int G = form.groups, kThreads = form.threads;
       return with_halves(a, [&](auto branch, auto next) {
-        const int threads = threads_of<R>(waves, a.group_rows, 4), at_once = Place<R, G>::rows_at_once(threads, waves);
-        const Chunks cut = cut_rows(a.rows, a.group_rows, at_once, 2048);
+        // enough workgroups to fill the units, each with rows enough that its maps and first row count for little (16384 x 2560 gate_add: 46 us,
+        // with 1024 workgroups 55)
+        const int threads = threads_of<R, G>(a.cols, a.group_rows, 4);
+        const Chunks cut = cut_rows(a.rows, a.group_rows, Place<R, G>::rows_at_once(threads), R == Row::kWaves ? 512 : 768);
         const unsigned grid = (unsigned)std::min<int64_t>(cut.all, 1 << 20);
-        k_norm_forward<T, R, G, branch.value, next.value><<<grid, threads, 0, (hipStream_t)stream>>>(make_norms<T>(a), cut, waves);
+        k_norm_forward<T, R, G, kThreads, branch.value, next.value><<<grid, threads, 0, (hipStream_t)stream>>>(make_norms<T>(a), cut);
         GF_LAUNCH_CHECK("k_norm_forward");
         return (int)GF_OK;
       });
