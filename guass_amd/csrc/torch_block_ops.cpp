@@ -190,12 +190,17 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     }
     variable_list out(15);
     if (!dstream.defined() && !dnormed.defined()) return out;
-    const NormGrads g = call_norm_backward(s[kX], maybe(s[kResidual]), maybe(s[kWeight]), maybe(s[kBias]), maybe(s[kGate]), gate_value, residual_scale,
+    // an unscaled residual that only gate_add has seen: its gradient is the stream's
+    const bool same = !next && residual_scale == 1.0 && (wants >> kResidual & 1);
+    if (same) wants &= ~(int64_t(1) << kResidual);
+    NormGrads g;
+    if (wants) g = call_norm_backward(s[kX], maybe(s[kResidual]), maybe(s[kWeight]), maybe(s[kBias]), maybe(s[kGate]), gate_value, residual_scale,
                                            kind, eps, maybe(s[kNextWeight]), maybe(s[kNextBias]), maybe(s[kScale]), maybe(s[kShift]), next_kind, next_eps,
                                            maybe(dstream), maybe(dnormed), wants);
     const auto& [g0, g1, g2, g3, g4, g5, g6, g7, g8] = g;
     const Tensor* const all[kWants] = {&g0, &g1, &g2, &g3, &g4, &g5, &g6, &g7, &g8};
     for (int i = 0; i < kWants; ++i) out[kAt[i]] = *all[i];
+    if (same) out[kAt[kResidual]] = dstream;
     return once(std::move(out), norm_name(branch, next), again);
   }
 };

@@ -322,6 +322,145 @@ class GaussianFeedForward(nn.Module):
                                   offset=2 * offset + 1)
 
 
+class BlockNorm(nn.Module):
+    """The norm before a block, on the kernels of guass_amd.norms: norm(x) * weight + bias, times (1 + scale) plus shift.  ``after``
+    ends one block and gives the next one its norm in one pass."""
+
+    def __init__(self, features: int, *, kind: str = "layer", eps: float = 1e-5, affine: bool = True, bias: bool = True, device=None,
+                 dtype=None) -> None:
+        super().__init__()
+        from guass_amd.norms import NORMS
+
+        if kind not in NORMS:
+            raise ValueError(f"kind must be one of {NORMS} (got {kind!r})")
+        if features < 1:
+            raise ValueError(f"features must be positive (got {features})")
+        self.features, self.kind, self.eps = features, kind, float(eps)
+        self.weight = nn.Parameter(torch.ones(features, device=device, dtype=dtype)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(features, device=device, dtype=dtype)) if affine and bias else None
+
+    @classmethod
+    def from_norm(cls, norm: nn.Module) -> "BlockNorm":
+        """Of a torch LayerNorm or RMSNorm over the last dimension, whose parameters it takes over."""
+        kinds = {nn.LayerNorm: "layer", nn.RMSNorm: "rms"}
+        if type(norm) not in kinds:
+            raise TypeError(f"norm must be a LayerNorm or an RMSNorm (got {type(norm).__name__})")
+        if len(norm.normalized_shape) != 1:
+            raise ValueError(f"norm must be over the last dimension (got normalized_shape {tuple(norm.normalized_shape)})")
+        if norm.eps is None:
+            raise ValueError("norm must have an eps")
+        made = cls(norm.normalized_shape[0], kind=kinds[type(norm)], eps=norm.eps, affine=False)
+        made.weight, made.bias = norm.weight, getattr(norm, "bias", None)
+        return made
+
+    def forward(self, input: Tensor, *, scale: Tensor | None = None, shift: Tensor | None = None) -> Tensor:
+        from guass_amd.norms import norm
+
+        return norm(input, self.weight, self.bias, kind=self.kind, scale=scale, shift=shift, eps=self.eps)
+
+    def after(self, branch: Tensor, residual: Tensor, *, branch_norm: "BlockNorm | None" = None, gate: float | Tensor = 1.0,
+              residual_scale: float = 1.0, scale: Tensor | None = None, shift: Tensor | None = None) -> tuple[Tensor, Tensor]:
+        """(stream, self(stream)) of stream = residual_scale * residual + gate * branch_norm(branch)."""
+        from guass_amd.norms import gate_add_norm
+
+        own = dict(kind=branch_norm.kind, eps=branch_norm.eps) if branch_norm is not None else {}
+        w, b = (branch_norm.weight, branch_norm.bias) if branch_norm is not None else (None, None)
+        return gate_add_norm(branch, residual, w, b, self.weight, self.bias, gate=gate, residual_scale=residual_scale, next_kind=self.kind,
+                             scale=scale, shift=shift, next_eps=self.eps, **own)
+
+
+class QuantizedLinear(nn.Module):
+    """nn.Linear with a weight in 4 bits that does not train (guass_amd.quantized): a frozen layer, or a trained GaussianLinear
+    merged (weight + adapter_scale * delta-W, rendered once)."""
+
+    def __init__(self, weight, bias: Tensor | None = None) -> None:
+        super().__init__()
+        from guass_amd.quantized import QuantizedWeight
+
+        if not isinstance(weight, QuantizedWeight):
+            raise TypeError("weight must be a QuantizedWeight")
+        self.out_features, self.in_features = weight.shape
+        self.register_buffer("tile_codes", weight.tile_codes)
+        self.register_buffer("tile_scales", weight.tile_scales)
+        self.bias = None if bias is None else nn.Parameter(bias.detach().clone(), requires_grad=False)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "QuantizedLinear":
+        from guass_amd.quantized import quantize
+
+        if not isinstance(linear, nn.Linear):
+            raise TypeError(f"linear must be an nn.Linear (got {type(linear).__name__})")
+        with torch.no_grad():
+            weight = linear.merged_weight() if isinstance(linear, GaussianLinear) else linear.weight
+            return cls(quantize(weight), linear.bias)
+
+    @property
+    def weight(self):
+        from guass_amd.quantized import QuantizedWeight
+
+        return QuantizedWeight.from_tiles(self.tile_codes, self.tile_scales, self.out_features, self.in_features)
+
+    def forward(self, input: Tensor, residual: Tensor | None = None) -> Tensor:
+        from guass_amd.quantized import quantized_linear
+
+        return quantized_linear(input, self.weight, self.bias, residual)
+
+
+class QuantizedFeedForward(nn.Module):
+    """GaussianFeedForward's inference form, both weights merged and in 4 bits: residual + out(value * act(gate)), (value, gate) the
+    halves of proj(x).  Nothing is dropped, and only inputs and biases can train."""
+
+    def __init__(self, proj: QuantizedLinear, out: QuantizedLinear, *, activation: str = "gelu") -> None:
+        super().__init__()
+        from guass_amd.feedforward import ACTIVATIONS
+
+        for name, ly in (("proj", proj), ("out", out)):
+            if not isinstance(ly, QuantizedLinear):
+                raise TypeError(f"{name} is not a QuantizedLinear")
+        if proj.out_features != 2 * out.in_features:
+            raise ValueError(f"proj must make value and gate of out's {out.in_features} features (got {proj.out_features})")
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation must be one of {ACTIVATIONS} (got {activation!r})")
+        self.proj, self.out, self.activation = proj, out, activation
+
+    @classmethod
+    def from_feed_forward(cls, ff: GaussianFeedForward) -> "QuantizedFeedForward":
+        return cls(QuantizedLinear.from_linear(ff.proj), QuantizedLinear.from_linear(ff.out), activation=ff.activation)
+
+    def forward(self, input: Tensor, residual: Tensor | None = None) -> Tensor:
+        from guass_amd.quantized import quantized_gated_linear
+
+        return self.out(quantized_gated_linear(input, self.proj.weight, self.proj.bias, activation=self.activation), residual)
+
+
+class FeedForwardBlock(nn.Module):
+    """A block's second half whole: stream + gate * out_norm(ff(norm(stream) * (1 + scale) + shift)).  ``ff`` is a
+    GaussianFeedForward (``forward`` then takes its seed and offset) or a QuantizedFeedForward; ``scale``, ``shift`` and ``gate`` are
+    a sample's or all rows' (guass_amd.norms).  Without gate and out_norm the sum is the last product's epilogue."""
+
+    def __init__(self, norm: BlockNorm, ff: nn.Module, out_norm: BlockNorm | None = None) -> None:
+        super().__init__()
+        if not isinstance(norm, BlockNorm) or not (out_norm is None or isinstance(out_norm, BlockNorm)):
+            raise TypeError("norm and out_norm must be BlockNorms")
+        if not isinstance(ff, (GaussianFeedForward, QuantizedFeedForward)):
+            raise TypeError("ff must be a GaussianFeedForward or a QuantizedFeedForward")
+        self.norm, self.ff, self.out_norm = norm, ff, out_norm
+
+    def forward(self, stream: Tensor, *, scale: Tensor | None = None, shift: Tensor | None = None, gate: float | Tensor | None = None,
+                seed: int | Tensor | None = None, offset: int = 0) -> Tensor:
+        from guass_amd.norms import gate_add
+
+        h = self.norm(stream, scale=scale, shift=shift)
+        rng = dict(seed=seed, offset=offset) if isinstance(self.ff, GaussianFeedForward) else {}
+        if gate is None and self.out_norm is None:
+            return self.ff(h, stream, **rng)
+        y, out = self.ff(h, **rng), self.out_norm
+        gate = 1.0 if gate is None else gate
+        if out is None:
+            return gate_add(y, stream, gate=gate)
+        return gate_add(y, stream, out.weight, out.bias, kind=out.kind, gate=gate, eps=out.eps)
+
+
 class _null:
     def __enter__(self):
         return None
