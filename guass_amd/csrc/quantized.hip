@@ -2,12 +2,12 @@
 //
 //   k_quantize    groups of 32 of a row: a power of two for a scale, and the nearest of the 16 values e2m1 has
 //   k_dequantize  the values that codes and scales stand for, in a type of 16 or 32 bits
-//   k_q4_few      the product of at most 64 rows: codes straight into the matrix instructions' operands
+//   k_q4_few      the product of few rows: codes straight into the matrix instructions' operands
 //   k_column_sums, k_column_join  a linear product's bias's gradient
 //
 // A group's scale being a power of two, a weight's value is exact in bfloat16 (sign, 2 bits of fraction), and in float16 as long as the
 // scale is not extreme: the matrix cores get it without a rounding of its own.  The hardware turns two codes into two values of a
-// scale in one instruction.  More rows than 64 go through k_dequantize and the feed-forward products (feedforward.hip), forward
+// scale in one instruction.  More rows go through k_dequantize and the feed-forward products (feedforward.hip), forward
 // and backward: the weight is frozen, so a backward has the inputs' gradient only.
 #include "elements.h"
 
@@ -136,7 +136,7 @@ struct Few {
   int act;
 };
 
-// The product of at most 16 G rows.  A workgroup takes 16 NT output columns (gated: as many of the value's and of the gate's), its waves
+// The product of 16 G rows a workgroup (y).  It takes 16 NT output columns (gated: as many of the value's and of the gate's), its waves
 // the tiles along k in turn, and the waves' sums meet in LDS.  Bound by reading the codes, so two tiles of them are under way at a time, and by x,
 // which every workgroup reads: NT halves that where there are columns enough.
 //
@@ -154,7 +154,8 @@ __global__ __launch_bounds__((kFewWaves<T, G> * 64)) void k_q4_few(Few<T> a) {
   constexpr int kSums = W * R * G * 16 * 17 * 4, kStage = DIRECT ? 0 : W * G * 16 * P * 16;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kSums > kStage ? kSums : kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, quarter = lane >> 4;
-  const int64_t n0 = blockIdx.x * (16ll * NT);
+  const int64_t n0 = blockIdx.x * (16ll * NT), m0 = blockIdx.y * (16ll * G);
+  a.M -= m0, a.x += m0 * a.ldx, a.y += m0 * a.N, a.residual += a.residual != nullptr ? m0 * a.ldr : 0;
   using Piece = Vec<T, E>;
   const uint8_t *pc[R], *ps[R];
 #pragma unroll
@@ -277,7 +278,7 @@ __global__ __launch_bounds__((kFewWaves<T, G> * 64)) void k_q4_few(Few<T> a) {
 
 // ------------------------------------------------------------------------------------------
 // The bias's gradient of a linear product, the columns' sums of dy: 8 columns a thread, a chunk of rows a workgroup (y), then the chunks in
-// their order.  Bound by reading dy: 8192 x 10240 in bfloat16 TIME us.
+// their order.  Bound by reading dy: 8192 x 10240 in bfloat16 40 us (4.1 TB/s), and 5 to join.
 template <typename T>
 __global__ __launch_bounds__(256) void k_column_sums(int64_t rows, int64_t cols, int64_t chunk, const T* __restrict__ dy, int64_t ld, float* __restrict__ sums,
                                                      int64_t width) {
@@ -370,7 +371,9 @@ gf_ff_args dense(const gf_q4_args& a, const void* weight) {
   return f;
 }
 
-bool few(const gf_q4_args& a) { return a.rows <= 64 && a.saved == nullptr; }
+// By the codes: in 16 bits up to 128 rows, 64 at a time (8192 -> 8192: 65 rows 40 us, through the values 64; 1280 -> 5120 gated 26 and 30), in 32
+// bits up to 64 (of 128, 1280 -> 5120 gated takes 88 us by the codes, 64 through the values).
+bool few(const gf_q4_args& a) { return a.rows <= (a.dtype == GF_DTYPE_F32 ? 64 : 128) && a.saved == nullptr; }
 
 template <typename T>
 int dequantize(int64_t rows, int64_t cols, const void* codes, const void* scales, void* out, hipStream_t s) {
@@ -427,14 +430,15 @@ int launch_few(const Few<T>& f, bool wide, hipStream_t s) {
   // (8 waves: 5.3), 4096 -> 14336 9.6 (16: 11.3), 1280 -> 5120 gated 5.1 (16: 5.9).
   const int64_t cols = wide ? 32 : 16, groups = (f.N + cols - 1) / cols;
   const unsigned waves = (unsigned)std::min<int64_t>(f.across, std::min(kFewWaves<T, G>, groups <= 256 ? 16 : 8));
+  const unsigned blocks = (unsigned)((f.M + 16 * G - 1) / (16 * G));
   if constexpr (H == 1) {
     if (wide) {
-      k_q4_few<T, 1, G, 2, DIRECT><<<(unsigned)groups, waves * 64, 0, s>>>(f);
+      k_q4_few<T, 1, G, 2, DIRECT><<<dim3((unsigned)groups, blocks), waves * 64, 0, s>>>(f);
       GF_LAUNCH_CHECK("k_q4_few");
       return GF_OK;
     }
   }
-  k_q4_few<T, H, G, 1, DIRECT><<<(unsigned)groups, waves * 64, 0, s>>>(f);
+  k_q4_few<T, H, G, 1, DIRECT><<<dim3((unsigned)groups, blocks), waves * 64, 0, s>>>(f);
   GF_LAUNCH_CHECK("k_q4_few");
   return GF_OK;
 }

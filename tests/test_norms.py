@@ -466,3 +466,39 @@ def test_captured_phases_replay(device):
         got = [c.clone() for c in captured]
         for a, b in zip(got, step()):
             assert torch.equal(a, b), f"replay {k}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_dimensions(device, dtype):
+    """One dimension, two, four; the same tensor as both inputs and as both weights."""
+    _say("dimensions", dtype)
+    for shape in ((72,), (5, 72), (2, 3, 4, 72)):
+        t = _tensors(device, shape, dtype, op="gate_add_norm")
+        _check("gate_add_norm", t, _kw("gate_add_norm", "layer", "rms"), dtype, f"{shape}")
+        t["residual"], t["next_weight"] = t["x"], t["weight"]
+        _check("gate_add_norm", t, _kw("gate_add_norm", "layer", "rms"), dtype, f"{shape} alike")
+    x = _rand(device, 6, 72, dtype=torch.float32, seed=1).requires_grad_(True)
+    dy = _rand(device, 6, 72, dtype=torch.float32, seed=2)
+    both, = torch.autograd.grad(norms.gate_add(x, x, kind="rms"), x, dy)
+    u, v = (x.detach().clone().requires_grad_(True) for _ in range(2))
+    assert torch.equal(both, sum(torch.autograd.grad(norms.gate_add(u, v, kind="rms"), (u, v), dy)))
+
+
+@pytest.mark.gpu
+def test_more_elements_than_32_bits_count(device):
+    """Rows behind the first 2^32 bytes and 2^31 elements: as the same rows by themselves."""
+    _say("large")
+    rows, cols = 2**31 // 6144 + 40, 6144
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=device)
+    x[-7:] = _rand(device, 7, cols, dtype=torch.bfloat16, seed=1)
+    x[:-7] = x[-1]
+    w = _rand(device, cols, dtype=torch.bfloat16, seed=2)
+    stream, normed = norms.gate_add_norm(x, x, w, None, w, kind="rms")
+    want = norms.gate_add_norm(x[-7:], x[-7:], w, None, w, kind="rms")
+    assert torch.equal(stream[-7:], want[0]) and torch.equal(normed[-7:], want[1])
+    del stream, normed
+    norms._ops()
+    back = torch.ops.guass_amd.block_norm_backward
+    args = lambda x, g: (x, None, None, None, None, 1.0, 1.0, 0, 0.0, w, None, None, None, 1, 1e-5, None, g, 1)  # noqa: E731
+    assert torch.equal(back(*args(x, x))[0][-7:], back(*args(x[-7:], x[-7:]))[0])

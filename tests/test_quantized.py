@@ -124,7 +124,7 @@ def test_abi_refuses_by_phase():
     assert fwd(residual=4096, ldr=8) == 1 and "takes no residual" in err()
     assert fwd(activation=0, residual=4096, ldr=7) == 1 and "residual: row stride 7" in err()
     assert fwd() == 2 and "workspace" in err()  # it saves, so it goes through the weight's values
-    assert fwd(rows=65, saved=None) == 2
+    assert fwd(rows=129, saved=None) == 2 and fwd(rows=65, saved=None, dtype=0) == 2
     assert fwd(rows=0, x=None) == 0
     back = lambda **kw: lib.gf_q4_backward(ctypes.byref(_args(**kw)), 4096, 2**40, None)  # noqa: E731
     assert back(rows=0) == 1 and "needs rows" in err()
@@ -146,8 +146,9 @@ def test_abi_workspaces(dtype, size):
     """None for few rows that save nothing; else the weight's values at least, without overflow up to the limits."""
     lib = N.lib()
     ws = lambda back, **kw: lib.gf_q4_workspace_bytes(ctypes.byref(_args(dtype=dtype, **kw)), back)  # noqa: E731
-    assert ws(0, saved=None) == 0 and ws(0, saved=None, rows=64) == 0
-    for rows, d, n in ((1, 40, 8), (64, 8, 8), (65, 8, 8), (2**31 - 1, 8, 2**10), (1, 2**21, 2**20), (2**20, 2**21, 2**19)):
+    most = 64 if dtype == 0 else 128
+    assert ws(0, saved=None) == 0 and ws(0, saved=None, rows=most) == 0 and ws(0, saved=None, rows=most + 1) > 0
+    for rows, d, n in ((1, 40, 8), (64, 8, 8), (65, 8, 8), (129, 8, 8), (2**31 - 1, 8, 2**10), (1, 2**21, 2**20), (2**20, 2**21, 2**19)):
         for back in (0, 1):
             got = ws(back, rows=rows, in_features=d, out_features=n, ldx=d, lddy=n)
             assert 2 * n * d * size <= got < 2**62
@@ -265,7 +266,7 @@ def _products(device, kind, rows, d, n, dtype, act="gelu", bias=True, residual=T
 
 
 # one token; tiny and odd; groups and tiles by one each way; a long contraction; more rows than go by the codes
-SHAPES = [(1, 64, 64), (1, 1, 1), (2, 3, 5), (5, 33, 7), (16, 32, 16), (17, 31, 17), (33, 320, 96), (48, 129, 15), (64, 127, 33), (65, 128, 40), (130, 200, 136),
+SHAPES = [(1, 64, 64), (1, 1, 1), (2, 3, 5), (5, 33, 7), (16, 32, 16), (17, 31, 17), (33, 320, 96), (48, 129, 15), (64, 127, 33), (65, 128, 40), (127, 129, 50), (128, 40, 8200), (130, 200, 136),
           (3, 2056, 16), (1, 8200, 40), (40, 8, 1288), (300, 77, 100)]
 
 
@@ -280,7 +281,7 @@ def test_products(device, kind, shape, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
-@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 32, 33, 63, 64])
+@pytest.mark.parametrize("rows", [1, 2, 4, 5, 15, 16, 17, 32, 33, 63, 64, 65, 100, 128, 129])
 def test_rows_at_a_wide_block(device, rows, dtype):
     _say("rows", rows, dtype)
     _products(device, "linear", rows, 1280, 320, dtype, seed=20)
@@ -301,7 +302,7 @@ def test_activations(device, act, dtype):
 def test_layouts(device, dtype):
     """Rows of larger matrices beside which NaN lies, odd bases, three dimensions; codes that are slices or not aligned."""
     _say("layouts", dtype)
-    for rows in (5, 80):
+    for rows in (5, 80, 150):
         d, n = 72, 40
         w, values = _weight(device, n, d, seed=3)
         x, b, r = (_rand(device, *s, dtype=dtype, seed=60 + i) for i, s in enumerate(((rows, d), (n,), (rows, n))))
@@ -331,18 +332,19 @@ def test_layouts(device, dtype):
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_a_bad_row_stays_in_its_row(device, bad, dtype):
     """Also behind an odd width, where the kernels read past nothing; an infinity times the code 0 is a NaN, times another infinite."""
-    for rows, d in ((20, 50), (100, 50)):
+    for rows, d in ((3, 50), (20, 50), (100, 50), (150, 50)):
         w, values = _weight(device, 24, d, seed=4)
         x = _rand(device, rows, d, dtype=dtype, seed=5)
         want = q4.quantized_linear(x, w)
-        x[7, 49] = bad
+        at = rows - 1 - rows // 3
+        x[at, 49] = bad
         got = q4.quantized_linear(x, w)
-        keep = torch.arange(rows, device=device) != 7
+        keep = torch.arange(rows, device=device) != at
         assert torch.equal(got[keep], want[keep])
-        row = got[7].cpu()
+        row = got[at].cpu()
         if math.isnan(bad):
             assert bool(torch.isnan(row).all())
-        elif rows <= 64:
+        elif rows <= 64 or (rows <= 128 and dtype != torch.float32):
             exact = values[:, 49].float() * bad
             assert torch.equal(torch.isnan(row), torch.isnan(exact)) and torch.equal(row.float().nan_to_num(0.0, 1.0, -1.0), exact.nan_to_num(0.0, 1.0, -1.0))
 
@@ -413,3 +415,22 @@ def test_captured_phases_replay(device):
         got = [c.clone() for c in captured]
         for a, b in zip(got, step()):
             assert torch.equal(a, b), f"replay {k}"
+
+
+@pytest.mark.gpu
+def test_more_elements_than_32_bits_count(device):
+    """A weight of more than 2^31 elements: its last rows as by themselves."""
+    _say("large")
+    rows, cols = 2**31 // 16384 + 40, 16384
+    w = torch.empty(rows, cols, dtype=torch.bfloat16, device=device)
+    w[-19:] = _rand(device, 19, cols, dtype=torch.bfloat16, seed=1)
+    w[:-19] = w[-1]
+    big, last = q4.quantize(w), q4.quantize(w[-19:])
+    del w
+    values = big.dequantize(torch.bfloat16)
+    assert torch.equal(values[-19:], last.dequantize(torch.bfloat16))
+    for m in (1, 20):
+        x = _rand(device, m, cols, dtype=torch.bfloat16, seed=2)
+        y = q4.quantized_linear(x, big)[:, -19:].double()
+        want = x.double() @ values[-19:].double().t()
+        assert float((y - want).norm() / want.norm()) < 2.0**-8
