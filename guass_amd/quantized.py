@@ -10,7 +10,7 @@ A weight that does not train is kept so: the frozen base of an adapted layer, or
 bfloat16, and in float16 where the scale lies in [2^-23, 2^13] (past that, it is rounded to float16).
 
 The products' other tensors are of one type, float32, bfloat16 or float16; sums are accumulated in 32 bits.  Under ``torch.autocast``
-x and the bias take its type, as in nn.Linear.  Few rows (128; in float32 64) read the codes as they are; more, and
+x and the bias take its type, as in nn.Linear.  At most 128 rows read the codes as they are; more, and
 a gated product's training pass, write the weight's values out for the call and run the products of ``guass_amd.feedforward``, backward too: the gradients of
 x, bias and residual, none of the weight.  Every call runs on torch's current stream of its tensors' device and does not synchronise.
 """
