@@ -552,10 +552,10 @@ __global__ __launch_bounds__(THREADS) void k_norm_backward(Norms<T> a, Chunks cu
 // The chunks' sums into gradients: 32 columns a workgroup, the branch's (z = 0) or the next norm's.  With S0 = sum d, S1 = sum d n of a
 // group, w, b the half's weight and bias and f its factor (the gate; 1 + scale):
 //   of the factor  w S1 + b S0;   of the shift  S0;   of w  sum over groups of f S1;   of b  sum over groups of f S0.
-// 8 lanes take 32 columns, 128 such members of a workgroup share out the groups, `team` of them (a power of two) one group: all chunks of
+// 8 lanes take 32 columns, 64 such members of a workgroup share out the groups, `team` of them (a power of two) one group: all chunks of
 // it are asked for at once.  A slab (y) is a range of groups, and what is shared by all groups goes to `partial` [slab][half][4][width]
-// (of the weight, the bias, the factor, the shift) where there are several slabs.  8 to 10 us whatever its size: a launch and the trips to memory
-// of sums that other dies have written.
+// (of the weight, the bias, the factor, the shift) where there are several slabs.  7 to 11 us: a launch and the
+// trips to memory of sums that other dies have written (with 1024 threads 8 to 10, with 256 7 to 18).
 template <typename T>
 struct Half {
   const T *weight, *bias, *factor;
@@ -598,17 +598,19 @@ __device__ __attribute__((always_inline)) inline f32x4 from_lane(f32x4 v, int ma
   return v;
 }
 
+constexpr int kFinishThreads = 512;
+
 template <typename T>
-__global__ __launch_bounds__(1024) void k_norm_finish(Half<T> branch, Half<T> next, int half0, int32_t cols, int64_t groups, int64_t chunks,
+__global__ __launch_bounds__(kFinishThreads) void k_norm_finish(Half<T> branch, Half<T> next, int half0, int32_t cols, int64_t groups, int64_t chunks,
                                                       const float* parts, int64_t width, int team, float* partial) {
-  __shared__ f32x4 meet[4][16][8];
+  __shared__ f32x4 meet[4][kFinishThreads / 64][8];
   const int lane = threadIdx.x & 7, member = threadIdx.x >> 3, wave = threadIdx.x >> 6, half = half0 + blockIdx.z;
   const bool first_of_wave = (threadIdx.x & 63) < 8;
   const Half<T>& h = half == 0 ? branch : next;
   const int64_t c = blockIdx.x * 32ll + lane * 4;
   const int n = cols - c < 0 ? 0 : cols - c < 4 ? (int)(cols - c) : 4;
   const int64_t slab = (groups + gridDim.y - 1) / gridDim.y, g0 = blockIdx.y * slab, g1 = g0 + slab < groups ? g0 + slab : groups;
-  const int teams = 128 / team, of = member & (team - 1);
+  const int teams = kFinishThreads / 8 / team, of = member & (team - 1);
   const Vec<T, 4> w = load4(h.weight, c, n, 1.0f), b = load4(h.bias, c, n, 0.0f);
   f32x4 shared[4] = {};
   for (int64_t base = g0; base < g1; base += teams) {
@@ -616,7 +618,7 @@ __global__ __launch_bounds__(1024) void k_norm_finish(Half<T> branch, Half<T> ne
     f32x4 s0 = 0.0f, s1 = 0.0f;
     const Vec<T, 4> factor = load4(h.factor != nullptr && g < g1 ? h.factor + g * h.ld_factor : nullptr, c, n, 0.0f);
     if (n > 0 && g < g1) {
-#pragma unroll 4
+#pragma unroll 8
       for (int64_t i = of; i < chunks; i += team) {
         const float* p = parts + ((g * chunks + i) * kSums + 2 * half) * width + c;  // 4 of them: width is a multiple of 8
         s0 += *(const f32x4*)p, s1 += *(const f32x4*)(p + width);
@@ -656,7 +658,7 @@ __global__ __launch_bounds__(1024) void k_norm_finish(Half<T> branch, Half<T> ne
   if (member >= 4 || n == 0) return;
   f32x4 v = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v += meet[member][i][lane];
+  for (int i = 0; i < kFinishThreads / 64; ++i) v += meet[member][i][lane];
   if (partial != nullptr) {
     *(f32x4*)(partial + ((int64_t)blockIdx.y * 2 + half) * 4 * width + member * width + c) = v;
     return;
@@ -824,9 +826,9 @@ int backward(const gf_norm_args& a, Arena& ws, bool run, hipStream_t s) {
             const Half<T> b{n.weight, n.bias, n.gate, n.ld_gate, 0, 0.0f, n.gate_value, n.dweight, n.dbias, n.dgate, nullptr};
             const Half<T> f{n.next_weight, n.next_bias, n.scale, n.ld_scale, n.ld_shift, 1.0f, 1.0f, n.dnext_weight, n.dnext_bias, n.dscale, n.dshift};
             int team = 1;
-            while (team < 128 && team * 2 * groups <= 128) team *= 2;
+            while (team < kFinishThreads / 8 && team * 2 * groups <= kFinishThreads / 8) team *= 2;
             const int half0 = kBranch ? 0 : 1, halves = (kBranch ? 1 : 0) + (kNext ? 1 : 0);
-            k_norm_finish<T><<<dim3((unsigned)((a.cols + 31) / 32), (unsigned)slabs, halves), 1024, 0, s>>>(b, f, half0, n.cols, groups, chunks, parts,
+            k_norm_finish<T><<<dim3((unsigned)((a.cols + 31) / 32), (unsigned)slabs, halves), kFinishThreads, 0, s>>>(b, f, half0, n.cols, groups, chunks, parts,
                                                                                                          width, team, partial);
             GF_LAUNCH_CHECK("k_norm_finish");
             if (partial != nullptr) {
