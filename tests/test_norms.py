@@ -227,7 +227,7 @@ def test_abi_workspace():
 # ------------------------------------------------------------------------------------ the GPU
 
 # a width on each side of every way of holding a row, odd ones among them
-WIDTHS = [1, 7, 8, 64, 127, 128, 129, 320, 512, 513, 640, 1000, 1025, 1280, 1536, 1537, 2048, 2055, 4096, 4104, 6144, 6150, 16384]
+WIDTHS = [1, 7, 8, 64, 127, 128, 129, 320, 512, 513, 640, 1000, 1025, 1280, 1536, 1537, 2048, 2055, 4096, 4104, 6144, 6150, 8192, 8200, 12001, 16384]
 
 
 @pytest.mark.gpu
@@ -502,3 +502,22 @@ def test_more_elements_than_32_bits_count(device):
     back = torch.ops.guass_amd.block_norm_backward
     args = lambda x, g: (x, None, None, None, None, 1.0, 1.0, 0, 0.0, w, None, None, None, 1, 1e-5, None, g, 1)  # noqa: E731
     assert torch.equal(back(*args(x, x))[0][-7:], back(*args(x[-7:], x[-7:]))[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [65, 300, 513, 1000, 1024, 1025, 1280, 1536, 1537])
+@pytest.mark.parametrize("op", ["norm", "gate_add", "gate_add_norm"])
+def test_many_rows(device, op, cols):
+    """Rows enough for a wave to take one alone; with the parameters' sums and without, whose kernels hold a row otherwise."""
+    for dtype, shape, per in ((torch.bfloat16, (3, 700, cols), 1), (torch.float32, (2053, cols), None), (torch.float16, (700, 3, cols), 1)):
+        _say("many rows", op, cols, dtype)
+        t = _tensors(device, shape, dtype, op=op, per=per, seed=cols)
+        kw = _kw(op, "layer", "rms" if dtype == torch.float16 else "layer")
+        _check(op, t, kw, dtype, f"{op} {shape}")
+        some = {k: v.detach().requires_grad_(k in ("x", "residual")) for k, v in t.items()}
+        out = _call(op, some, kw)
+        dy = {n: _rand(device, *shape, dtype=dtype, seed=90 + i, std=0.5) for i, n in enumerate(out)}
+        names = [n for n in ("x", "residual") if n in some]
+        want = bo.norms(t, dtype=dtype, **{"d" + n: g for n, g in dy.items()}, **kw)
+        for n, g in zip(names, torch.autograd.grad(list(out.values()), [some[n] for n in names], list(dy.values()))):
+            _close(g, want["d" + n], f"{op} {shape} d{n} alone")

@@ -231,6 +231,9 @@ def test_every_code_and_scale(device, dtype):
     y = q4.quantized_linear(eye, w).cpu()
     assert torch.equal(y[:, sane], want[sane].t())
     assert bool(torch.isnan(y[:, 255]).all())
+    if dtype == torch.float16:  # past the scales at which values are exact: as they are rounded to the type
+        sane = slice(127 - 30, 127 + 14)
+        assert torch.equal(y[:, sane], want[sane].t())
 
 
 def _products(device, kind, rows, d, n, dtype, act="gelu", bias=True, residual=True, seed=0, x=None):
@@ -266,7 +269,7 @@ def _products(device, kind, rows, d, n, dtype, act="gelu", bias=True, residual=T
 
 # one token; tiny and odd; groups and tiles by one each way; a long contraction; more rows than go by the codes
 SHAPES = [(1, 64, 64), (1, 1, 1), (2, 3, 5), (5, 33, 7), (16, 32, 16), (17, 31, 17), (33, 320, 96), (48, 129, 15), (64, 127, 33), (65, 128, 40), (127, 129, 50), (128, 40, 8200), (130, 200, 136),
-          (3, 2056, 16), (1, 8200, 40), (40, 8, 1288), (300, 77, 100)]
+          (3, 2056, 16), (1, 8200, 40), (40, 8, 1288), (300, 77, 100), (1, 40, 8200), (4, 129, 8192), (5, 1100, 8200), (20, 96, 8208), (33, 300, 8195)]
 
 
 @pytest.mark.gpu
