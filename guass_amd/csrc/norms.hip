@@ -348,7 +348,7 @@ struct Chunks {
 
 // Forward.  BRANCH: s from x and the residual; NEXT: h from s (without BRANCH, from x).  The next row is on its way while one is worked on.
 // In bfloat16: gate_add of 16384 x 2560 46 us (5.4 TB/s: memory), gate_add_norm of 8192 x 1280 22 us (3.8 TB/s: two statistics a row one after
-// the other, 8 waves a unit), norm of 16384 x 320 10 us (2 TB/s: 24 of 64 lanes idle, a launch and six turns); one row of 1280 3 to 4 us.
+// the other), norm of 16384 x 320 10 us (2 TB/s: 24 of 64 lanes idle, a launch and six turns); one row of 1280 3 to 4 us.
 template <typename T, Row R, int G, int THREADS, bool BRANCH, bool NEXT>
 __global__ __launch_bounds__(THREADS) void k_norm_forward(Norms<T> a, Chunks cut) {
   __shared__ float2 meet[2][kMaxWaves];
@@ -402,8 +402,8 @@ __global__ __launch_bounds__(THREADS) void k_norm_forward(Norms<T> a, Chunks cut
 constexpr int kSums = 4;
 
 // Backward, by chunks of rows.  SUMS: the column sums too, into parts [chunk][kSums][width].  In bfloat16: gate_add of 16384 x 2560 64 us (3.9
-// TB/s), gate_add_norm of 8192 x 1280 43 us (2.9 TB/s; 31 us, 4.1 TB/s, without sums, whose 32 registers a lane leave 9 waves a unit for 15), norm of
-// 16384 x 320 15 us (2.1 TB/s).
+// TB/s), gate_add_norm of 8192 x 1280 43 us (2.9 TB/s, nine waves a unit; 31 us, 4.1 TB/s, without sums), norm of 16384 x 320 15 us
+// (2.1 TB/s).
 template <typename T, Row R, int G, int THREADS, bool BRANCH, bool NEXT, bool SUMS>
 __global__ __launch_bounds__(THREADS) void k_norm_backward(Norms<T> a, Chunks cut, float* parts, int64_t width) {
   __shared__ float2 meet[2][kMaxWaves];
