@@ -401,8 +401,8 @@ __global__ __launch_bounds__(THREADS) void k_norm_forward(Norms<T> a, Chunks cut
 // Column sums of a chunk of rows, per element: of ds, ds n(x), dh, dh n'(s).
 constexpr int kSums = 4;
 
-// Backward, by chunks of rows.  SUMS: the column sums too, into parts [chunk][kSums][width].  In bfloat16: gate_add of 16384 x 2560 64 us (3.9
-// TB/s), gate_add_norm of 8192 x 1280 43 us (2.9 TB/s, nine waves a unit; 31 us, 4.1 TB/s, without sums), norm of 16384 x 320 15 us
+// Backward, by chunks of rows.  SUMS: the column sums too, into parts [chunk][kSums][width].  In bfloat16: gate_add of 16384 x 2560 56 us (4.5
+// TB/s), gate_add_norm of 8192 x 1280 42 us (3.0 TB/s, nine waves a unit; 31 us, 4.1 TB/s, without sums), norm of 16384 x 320 15 us
 // (2.1 TB/s).
 template <typename T, Row R, int G, int THREADS, bool BRANCH, bool NEXT, bool SUMS>
 __global__ __launch_bounds__(THREADS) void k_norm_backward(Norms<T> a, Chunks cut, float* parts, int64_t width) {
@@ -549,13 +549,13 @@ __global__ __launch_bounds__(THREADS) void k_norm_backward(Norms<T> a, Chunks cu
   }
 }
 
-// The chunks' sums into gradients: 32 columns a workgroup, the branch's (z = 0) or the next norm's.  With S0 = sum d, S1 = sum d n of a
+// The chunks' sums into gradients: 16 columns a workgroup, the branch's (z = 0) or the next norm's.  With S0 = sum d, S1 = sum d n of a
 // group, w, b the half's weight and bias and f its factor (the gate; 1 + scale):
 //   of the factor  w S1 + b S0;   of the shift  S0;   of w  sum over groups of f S1;   of b  sum over groups of f S0.
-// 8 lanes take 32 columns, 64 such members of a workgroup share out the groups, `team` of them (a power of two) one group: all chunks of
-// it are asked for at once.  A slab (y) is a range of groups, and what is shared by all groups goes to `partial` [slab][half][4][width]
-// (of the weight, the bias, the factor, the shift) where there are several slabs.  7 to 11 us: a launch and the
-// trips to memory of sums that other dies have written (with 1024 threads 8 to 10, with 256 7 to 18).
+// 4 lanes take 16 columns, 128 such members of a workgroup share out the groups, `team` of them (a power of two) one group: all chunks of
+// it are asked for at once (sums of 16384 x 2560: 10.8 us; 32 columns a workgroup 12.8, 8, less than a line of memory, 18).  A slab (y) is a range of groups, and what is shared by all groups goes to `partial` [slab][half][4][width]
+// (of the weight, the bias, the factor, the shift) where there are several slabs.  7 to 11 us: a launch and
+// the trips to memory of sums that other dies have written.
 template <typename T>
 struct Half {
   const T *weight, *bias, *factor;
@@ -598,19 +598,19 @@ __device__ __attribute__((always_inline)) inline f32x4 from_lane(f32x4 v, int ma
   return v;
 }
 
-constexpr int kFinishThreads = 512;
+constexpr int kFinishThreads = 512, kFinishLanes = 4, kFinishMembers = 64 / kFinishLanes;  // lanes of 4 columns each; members of a wave
 
 template <typename T>
 __global__ __launch_bounds__(kFinishThreads) void k_norm_finish(Half<T> branch, Half<T> next, int half0, int32_t cols, int64_t groups, int64_t chunks,
                                                       const float* parts, int64_t width, int team, float* partial) {
-  __shared__ f32x4 meet[4][kFinishThreads / 64][8];
-  const int lane = threadIdx.x & 7, member = threadIdx.x >> 3, wave = threadIdx.x >> 6, half = half0 + blockIdx.z;
-  const bool first_of_wave = (threadIdx.x & 63) < 8;
+  __shared__ f32x4 meet[4][kFinishThreads / 64][kFinishLanes];
+  const int lane = threadIdx.x % kFinishLanes, member = threadIdx.x / kFinishLanes, wave = threadIdx.x >> 6, half = half0 + blockIdx.z;
+  const bool first_of_wave = (threadIdx.x & 63) < kFinishLanes;
   const Half<T>& h = half == 0 ? branch : next;
-  const int64_t c = blockIdx.x * 32ll + lane * 4;
+  const int64_t c = blockIdx.x * (4ll * kFinishLanes) + lane * 4;
   const int n = cols - c < 0 ? 0 : cols - c < 4 ? (int)(cols - c) : 4;
   const int64_t slab = (groups + gridDim.y - 1) / gridDim.y, g0 = blockIdx.y * slab, g1 = g0 + slab < groups ? g0 + slab : groups;
-  const int teams = kFinishThreads / 8 / team, of = member & (team - 1);
+  const int teams = kFinishThreads / kFinishLanes / team, of = member & (team - 1);
   const Vec<T, 4> w = load4(h.weight, c, n, 1.0f), b = load4(h.bias, c, n, 0.0f);
   f32x4 shared[4] = {};
   for (int64_t base = g0; base < g1; base += teams) {
@@ -624,14 +624,14 @@ __global__ __launch_bounds__(kFinishThreads) void k_norm_finish(Half<T> branch, 
         s0 += *(const f32x4*)p, s1 += *(const f32x4*)(p + width);
       }
     }
-    for (int i = 1; i < team && i < 8; i *= 2) s0 += from_lane(s0, 8 * i), s1 += from_lane(s1, 8 * i);
-    if (team > 8) {
+    for (int i = 1; i < team && i < kFinishMembers; i *= 2) s0 += from_lane(s0, kFinishLanes * i), s1 += from_lane(s1, kFinishLanes * i);
+    if (team > kFinishMembers) {
       __syncthreads();
       if (first_of_wave) meet[0][wave][lane] = s0, meet[1][wave][lane] = s1;
       __syncthreads();
       s0 = 0.0f, s1 = 0.0f;
-      const int w0 = wave & ~(team / 8 - 1);
-      for (int i = 0; i < team / 8; ++i) s0 += meet[0][w0 + i][lane], s1 += meet[1][w0 + i][lane];
+      const int w0 = wave & ~(team / kFinishMembers - 1);
+      for (int i = 0; i < team / kFinishMembers; ++i) s0 += meet[0][w0 + i][lane], s1 += meet[1][w0 + i][lane];
     }
     if (n > 0 && g < g1 && of == 0) {
       const f32x4 f = h.factor != nullptr ? h.one + widen4<T>(factor) : f32x4(h.value);
@@ -651,7 +651,7 @@ __global__ __launch_bounds__(kFinishThreads) void k_norm_finish(Half<T> branch, 
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
 #pragma unroll
-    for (int i = 1; i < 8; i *= 2) shared[k] += from_lane(shared[k], 8 * i);
+    for (int i = 1; i < kFinishMembers; i *= 2) shared[k] += from_lane(shared[k], kFinishLanes * i);
     if (first_of_wave) meet[k][wave][lane] = shared[k];
   }
   __syncthreads();
@@ -804,10 +804,11 @@ int backward(const gf_norm_args& a, Arena& ws, bool run, hipStream_t s) {
       constexpr int G = form.groups, kThreads = form.threads;
       return with_halves(a, [&](auto branch, auto next) {
         constexpr bool kBranch = branch.value, kNext = next.value, kSumless = R == Row::kWave && G == 3 && kBranch && kNext;
-        // Workgroups for each of 256 compute units as their registers allow, and each of them its chunks' sums to write.  Without sums two, which
-        // the barriers or loads of one do not keep waiting (8192 x 1280 gate_add_norm: 31 us; one of 8 waves 37).
+        // Workgroups for each of 256 compute units as their registers allow (12 waves for both halves' sums, 16 for one's), and each of them its
+        // chunks' sums to write and k_norm_finish to read: gate_add of 16384 x 2560 in 512 workgroups 63 and 10 us, 768 56 and 11, 1024 63 and
+        // 15.  Without sums two, which the barriers or loads of one do not keep waiting (8192 x 1280 gate_add_norm: 31 us; one of 8 waves 37).
         const int threads = threads_of<R, G>(a.cols, a.group_rows, R == Row::kPart || (!sums && G > 1) ? 4 : 8);
-        const int fit = R == Row::kWaves ? std::min(std::max(12 * 64 / threads, 1), 3) : 1;
+        const int fit = R == Row::kWaves ? std::min(std::max((kBranch && kNext ? 12 : 16) * 64 / threads, 1), 3) : 1;
         const Chunks cut = cut_rows(a.rows, a.group_rows, Place<R, G>::rows_at_once(threads), 256 * (sums ? fit : 2));
         const int64_t chunks = cut.chunks, all = cut.all;
         const int64_t slabs = groups <= 1024 ? 1 : std::min<int64_t>((groups + 511) / 512, 64);
@@ -826,9 +827,9 @@ int backward(const gf_norm_args& a, Arena& ws, bool run, hipStream_t s) {
             const Half<T> b{n.weight, n.bias, n.gate, n.ld_gate, 0, 0.0f, n.gate_value, n.dweight, n.dbias, n.dgate, nullptr};
             const Half<T> f{n.next_weight, n.next_bias, n.scale, n.ld_scale, n.ld_shift, 1.0f, 1.0f, n.dnext_weight, n.dnext_bias, n.dscale, n.dshift};
             int team = 1;
-            while (team < kFinishThreads / 8 && team * 2 * groups <= kFinishThreads / 8) team *= 2;
+            while (team < kFinishThreads / kFinishLanes && team * 2 * groups <= kFinishThreads / kFinishLanes) team *= 2;
             const int half0 = kBranch ? 0 : 1, halves = (kBranch ? 1 : 0) + (kNext ? 1 : 0);
-            k_norm_finish<T><<<dim3((unsigned)((a.cols + 31) / 32), (unsigned)slabs, halves), kFinishThreads, 0, s>>>(b, f, half0, n.cols, groups, chunks, parts,
+            k_norm_finish<T><<<dim3((unsigned)((a.cols + 4 * kFinishLanes - 1) / (4 * kFinishLanes)), (unsigned)slabs, halves), kFinishThreads, 0, s>>>(b, f, half0, n.cols, groups, chunks, parts,
                                                                                                          width, team, partial);
             GF_LAUNCH_CHECK("k_norm_finish");
             if (partial != nullptr) {
