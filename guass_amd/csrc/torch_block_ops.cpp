@@ -162,31 +162,54 @@ NormGrads call_norm_backward(NORM_PARAMETERS, const MaybeTensor& dstream, const 
 
 const char* norm_name(bool branch, bool next) { return !branch ? "norm" : next ? "gate_add_norm" : "gate_add"; }
 
+// A gradient's inputs, by Want's bits.  The branch's half alone needs neither the residual nor, without a norm and the gate's gradient, x.
+int64_t branch_needs(int i, bool normed) {
+  const int64_t row = normed ? 1 << kX : 0;
+  switch (i) {
+    case kX: return row | 1 << kWeight | 1 << kGate;
+    case kWeight: return row | 1 << kGate;
+    case kBias: return 1 << kGate;
+    case kGate: return 1 << kX | 1 << kWeight | 1 << kBias;
+    default: return 0;
+  }
+}
+
 struct BlockNorm : torch::autograd::Function<BlockNorm> {
   // the positions of the tensors among forward's arguments
   static constexpr int kAt[kWants] = {0, 1, 2, 3, 4, 9, 10, 11, 12};
   static variable_list forward(AutogradContext* ctx, NORM_PARAMETERS) {
     const bool branch = present(residual), next = next_kind != GF_NORM_NONE;
     auto [stream, normed] = call_norm_forward(NORM_ARGUMENTS, true);
-    auto keep = [](const MaybeTensor& t) { return present(t) ? *t : Tensor(); };
-    ctx->save_for_backward({x, keep(residual), keep(weight), keep(bias), keep(gate), keep(next_weight), keep(next_bias), keep(scale), keep(shift)});
-    ctx->saved_data["call"] = std::make_tuple(gate_value, residual_scale, kind, eps, next_kind, next_eps);
+    const MaybeTensor first(x);
+    const MaybeTensor* const inputs[kWants] = {&first, &residual, &weight, &bias, &gate, &next_weight, &next_bias, &scale, &shift};
+    // x and the residual only where a gradient is made of them: they are as large as the stream, and the caller may write them
+    int64_t there = 0, needs = next ? 1 << kX | 1 << kResidual : 0;
+    for (int i = 0; i < kWants; ++i) {
+      if (!present(*inputs[i])) continue;
+      there |= int64_t(1) << i;
+      if (!next && wants(*inputs[i])) needs |= branch_needs(i, kind != GF_NORM_NONE);
+    }
+    variable_list saved(kWants);
+    for (int i = 0; i < kWants; ++i)
+      if ((there >> i & 1) && (i > kResidual || (needs >> i & 1))) saved[i] = **inputs[i];
+    ctx->save_for_backward(std::move(saved));
+    ctx->saved_data["call"] = std::make_tuple(gate_value, residual_scale, kind, eps, next_kind, next_eps, there);
     ctx->set_materialize_grads(false);
     if (!branch) return {normed};
     return next ? variable_list{stream, normed} : variable_list{stream};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const auto [gate_value, residual_scale, kind, eps, next_kind, next_eps] =
-        ctx->saved_data["call"].to<std::tuple<double, double, int64_t, double, int64_t, double>>();
-    const auto s = ctx->get_saved_variables();
-    const bool branch = s[kResidual].defined(), next = next_kind != GF_NORM_NONE;
+    const auto [gate_value, residual_scale, kind, eps, next_kind, next_eps, there] =
+        ctx->saved_data["call"].to<std::tuple<double, double, int64_t, double, int64_t, double, int64_t>>();
+    auto s = ctx->get_saved_variables();
+    const bool branch = there >> kResidual & 1, next = next_kind != GF_NORM_NONE;
     const Tensor dstream = branch ? grads[0] : Tensor(), dnormed = next ? grads[branch ? 1 : 0] : Tensor();
     int64_t wants = 0;
     bool again = (dstream.defined() && dstream.requires_grad()) || (dnormed.defined() && dnormed.requires_grad());
     for (int i = 0, edge = 0; i < kWants; ++i) {
-      if (!s[i].defined()) continue;
+      if (!(there >> i & 1)) continue;
       if (ctx->needs_input_grad(edge++)) wants |= int64_t(1) << i;  // edges are the tensors that are there
-      again = again || s[i].requires_grad();
+      again = again || (s[i].defined() && s[i].requires_grad());
     }
     variable_list out(15);
     if (!dstream.defined() && !dnormed.defined()) return out;
@@ -194,9 +217,15 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     const bool same = !next && residual_scale == 1.0 && (wants >> kResidual & 1);
     if (same) wants &= ~(int64_t(1) << kResidual);
     NormGrads g;
-    if (wants) g = call_norm_backward(s[kX], maybe(s[kResidual]), maybe(s[kWeight]), maybe(s[kBias]), maybe(s[kGate]), gate_value, residual_scale,
-                                           kind, eps, maybe(s[kNextWeight]), maybe(s[kNextBias]), maybe(s[kScale]), maybe(s[kShift]), next_kind, next_eps,
-                                           maybe(dstream), maybe(dnormed), wants);
+    if (wants) {
+      if (!next) {  // what is not read needs a shape only
+        for (const int i : {kX, kResidual})
+          if (!s[i].defined()) s[i] = dstream;
+      }
+      g = call_norm_backward(s[kX], maybe(s[kResidual]), maybe(s[kWeight]), maybe(s[kBias]), maybe(s[kGate]), gate_value, residual_scale, kind, eps,
+                             maybe(s[kNextWeight]), maybe(s[kNextBias]), maybe(s[kScale]), maybe(s[kShift]), next_kind, next_eps, maybe(dstream),
+                             maybe(dnormed), wants);
+    }
     const auto& [g0, g1, g2, g3, g4, g5, g6, g7, g8] = g;
     const Tensor* const all[kWants] = {&g0, &g1, &g2, &g3, &g4, &g5, &g6, &g7, &g8};
     for (int i = 0; i < kWants; ++i) out[kAt[i]] = *all[i];

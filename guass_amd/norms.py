@@ -5,7 +5,8 @@
 * ``gate_add_norm``  both in one pass: the stream, and the norm that the next block gets
 
 each with its gradients.  A row is the last dimension; statistics and sums are held in 32 bits, and an output is rounded
-once: ``gate_add_norm``'s norm is that of the stream before its rounding.
+once: ``gate_add_norm``'s norm is that of the stream before its rounding.  For the backward they keep their inputs, and nothing else:
+``gate_add`` x where a norm or the gate's gradient needs it, and not the residual.
 
 Types: float32, bfloat16 and float16, one type for all of a call's tensors; under ``torch.autocast`` float32, as torch's
 layer_norm.  Rows of 1 to 16384 elements.  ``weight`` and ``bias`` have a row's shape.  ``gate``, ``scale`` and ``shift`` have it too, or
