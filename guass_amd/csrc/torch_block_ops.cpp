@@ -162,8 +162,19 @@ NormGrads call_norm_backward(NORM_PARAMETERS, const MaybeTensor& dstream, const 
 
 const char* norm_name(bool branch, bool next) { return !branch ? "norm" : next ? "gate_add_norm" : "gate_add"; }
 
-// A gradient's inputs, by Want's bits.  The branch's half alone needs neither the residual nor, without a norm and the gate's gradient, x.
-int64_t branch_needs(int i, bool normed) {
+// What a gradient is made of besides the outputs' gradients, by Want's bits, where the next norm has one (`next`) and where the stream has
+// alone: then the residual goes into none, and x only through a norm or into what is summed with it.
+int64_t made_of(int i, bool next, bool normed) {
+  if (next) {
+    const int64_t stream = 1 << kX | 1 << kResidual | 1 << kWeight | 1 << kBias | 1 << kGate;
+    switch (i) {
+      case kNextWeight: return stream | 1 << kScale;
+      case kNextBias: return 1 << kScale;
+      case kScale: return stream | 1 << kNextWeight | 1 << kNextBias;
+      case kShift: return 0;
+      default: return stream | 1 << kNextWeight | 1 << kScale;
+    }
+  }
   const int64_t row = normed ? 1 << kX : 0;
   switch (i) {
     case kX: return row | 1 << kWeight | 1 << kGate;
@@ -187,7 +198,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     for (int i = 0; i < kWants; ++i) {
       if (!present(*inputs[i])) continue;
       there |= int64_t(1) << i;
-      if (!next && wants(*inputs[i])) needs |= branch_needs(i, kind != GF_NORM_NONE);
+      if (!next && wants(*inputs[i])) needs |= made_of(i, false, kind != GF_NORM_NONE);
     }
     variable_list saved(kWants);
     for (int i = 0; i < kWants; ++i)
@@ -204,12 +215,11 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     auto s = ctx->get_saved_variables();
     const bool branch = there >> kResidual & 1, next = next_kind != GF_NORM_NONE;
     const Tensor dstream = branch ? grads[0] : Tensor(), dnormed = next ? grads[branch ? 1 : 0] : Tensor();
-    int64_t wants = 0;
-    bool again = (dstream.defined() && dstream.requires_grad()) || (dnormed.defined() && dnormed.requires_grad());
+    int64_t wants = 0, train = 0;
     for (int i = 0, edge = 0; i < kWants; ++i) {
       if (!(there >> i & 1)) continue;
       if (ctx->needs_input_grad(edge++)) wants |= int64_t(1) << i;  // edges are the tensors that are there
-      again = again || (s[i].defined() && s[i].requires_grad());
+      if (s[i].defined() && s[i].requires_grad()) train |= int64_t(1) << i;
     }
     variable_list out(15);
     if (!dstream.defined() && !dnormed.defined()) return out;
@@ -228,9 +238,20 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
     }
     const auto& [g0, g1, g2, g3, g4, g5, g6, g7, g8] = g;
     const Tensor* const all[kWants] = {&g0, &g1, &g2, &g3, &g4, &g5, &g6, &g7, &g8};
-    for (int i = 0; i < kWants; ++i) out[kAt[i]] = *all[i];
+    // those that depend on what trains refuse a second derivative
+    const bool linear = (dstream.defined() && dstream.requires_grad()) || (dnormed.defined() && dnormed.requires_grad());
+    variable_list refusing(kWants);
+    bool again = false;
+    for (int i = 0; i < kWants; ++i) {
+      const bool depends = all[i]->defined() && (linear || (made_of(i, dnormed.defined(), kind != GF_NORM_NONE) & train));
+      (depends ? refusing[i] : out[kAt[i]]) = *all[i];
+      again = again || depends;
+    }
+    refusing = once(std::move(refusing), norm_name(branch, next), again);
+    for (int i = 0; i < kWants; ++i)
+      if (refusing[i].defined()) out[kAt[i]] = refusing[i];
     if (same) out[kAt[kResidual]] = dstream;
-    return once(std::move(out), norm_name(branch, next), again);
+    return out;
   }
 };
 
@@ -424,7 +445,9 @@ struct Q4Linear : torch::autograd::Function<Q4Linear> {
     // what the gradients depend on: of a gated product x and bias too, by value and gate
     const bool again = dy.requires_grad() || (activation != GF_ACT_NONE && trains);
     auto [dx, db] = call_q4_backward(dy, saved[0], saved[1], maybe(saved[2]), rows, cols, activation, wx, wb);
-    return once({dx, Tensor(), Tensor(), db, wr ? dy : Tensor(), Tensor(), Tensor(), Tensor()}, q4_name(activation), again);
+    variable_list out = once({dx, Tensor(), Tensor(), db, Tensor(), Tensor(), Tensor(), Tensor()}, q4_name(activation), again);
+    if (wr) out[4] = dy;
+    return out;
   }
 };
 

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from guass_amd import norms
+from guass_amd import quantized as q4
 
 
 def _say(*what):
@@ -70,3 +71,71 @@ def test_what_a_gradient_is_made_of_may_not_be_written(device, name):
         own[name].zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         h.sum().backward()
+
+
+LINEAR = {  # calls whose gradients depend on no input that trains
+    "gate_add of a number": (lambda t: norms.gate_add(t["x"], t["r"], gate=0.5, residual_scale=0.25), "xr"),
+    "gate_add, a frozen gate": (lambda t: norms.gate_add(t["x"], t["r"], gate=t["g"].detach()), "xr"),
+    "gate_add's residual": (lambda t: norms.gate_add(t["x"].detach(), t["r"], t["w"], kind="layer", gate=t["g"], residual_scale=2.0), "r"),
+    "norm's shift": (lambda t: norms.norm(t["x"], t["w"], shift=t["g"]), "g"),
+    "norm's bias": (lambda t: norms.norm(t["x"], t["w"], t["b"]), "b"),
+    "gate_add_norm's shift": (lambda t: norms.gate_add_norm(t["x"], t["r"], next_weight=t["w"], shift=t["g"])[1], "g"),
+    "gate_add_norm's stream": (lambda t: norms.gate_add_norm(t["x"], t["r"], next_weight=t["w"], gate=0.5)[0], "xr"),
+    "quantized_linear": (lambda t: q4.quantized_linear(t["x"], _weight(t["x"].device), t["b"], t["r"]), "xbr"),
+}
+
+
+def _weight(device):
+    return q4.quantize(_rand(device, 40, 40, seed=50))
+
+
+def _inputs(device):
+    t = {k: _rand(device, 2, 5, 40, seed=i) for i, k in enumerate("xr")}
+    t.update(w=_rand(device, 40, seed=3), b=_rand(device, 40, seed=4), g=_rand(device, 40, seed=5))
+    return {k: v.requires_grad_(True) for k, v in t.items()}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", LINEAR)
+def test_a_constant_gradient_is_no_second_derivative(device, name):
+    """With create_graph such a gradient comes back as it is: a penalty on it, beside a loss, has a backward (and no say in it)."""
+    _say("constant", name)
+    call, train = LINEAR[name]
+    t = _inputs(device)
+    dy = _rand(device, 2, 5, 40, seed=9)
+    leaves = [t[k] for k in train]
+    want = torch.autograd.grad(call(t), leaves, dy)
+    got = torch.autograd.grad(call(t), leaves, dy, create_graph=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b) and not a.requires_grad
+    loss = sum((g**2).sum() for g in got) + t["x"].sum()
+    assert torch.equal(torch.autograd.grad(loss, t["x"])[0], torch.ones_like(t["x"]))
+
+
+@pytest.mark.gpu
+def test_an_unscaled_residuals_gradient_is_differentiable(device):
+    """It is the stream's (the product's) gradient itself, with that one's graph, also where others refuse a second derivative."""
+    for call in (lambda t: norms.gate_add(t["x"], t["r"], t["w"], kind="rms"), lambda t: q4.quantized_linear(t["x"], _weight(device), t["b"], t["r"])):
+        t = _inputs(device)
+        dy = _rand(device, 2, 5, 40, seed=9).requires_grad_(True)
+        dx, dr = torch.autograd.grad(call(t), (t["x"], t["r"]), dy, create_graph=True)
+        assert torch.equal(torch.autograd.grad((dr**2).sum(), dy)[0], 2 * dy)
+        with pytest.raises(RuntimeError, match="differentiable once only"):
+            (dx**2).sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which,train", [("x", "xw"), ("x", "xg"), ("w", "xw"), ("w", "wg"), ("b", "bg"), ("g", "xg"), ("g", "wg"), ("g", "bg")])
+def test_a_gradient_that_depends_refuses(device, which, train):
+    """gate_add's, each by an input that it is made of and that trains; and of the next norm by the stream's."""
+    t = {k: v.detach().requires_grad_(k in train) for k, v in _inputs(device).items()}
+    dy = _rand(device, 2, 5, 40, seed=9)
+    grad, = torch.autograd.grad(norms.gate_add(t["x"], t["r"], t["w"], t["b"], kind="layer", gate=t["g"]), t[which], dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="gate_add is differentiable once only"):
+        (grad**2).sum().backward()
+    t = _inputs(device)
+    calls = {"x": t["r"], "w": t["w"], "b": t["b"], "g": t["g"]}
+    _, h = norms.gate_add_norm(t["x"], t["r"], next_weight=t["w"], next_bias=t["b"], scale=t["g"])
+    grad, = torch.autograd.grad(h, calls[which], dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="gate_add_norm is differentiable once only"):
+        (grad**2).sum().backward()
