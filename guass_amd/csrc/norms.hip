@@ -398,10 +398,10 @@ __global__ __launch_bounds__(THREADS) void k_norm_forward(Norms<T> a, Chunks cut
   }
 }
 
-// Column sums of a chunk of rows, per element: of ds, ds n(x), dh, dh n'(s).
+// Column sums of a chunk of rows, per element: of ds, ds n(x), dh, dh n'(s).  A half that is not there has none in memory.
 constexpr int kSums = 4;
 
-// Backward, by chunks of rows.  SUMS: the column sums too, into parts [chunk][kSums][width].  In bfloat16: gate_add of 16384 x 2560 56 us (4.5
+// Backward, by chunks of rows.  SUMS: the column sums too, into parts [chunk][2 of each half][width].  In bfloat16: gate_add of 16384 x 2560 56 us (4.5
 // TB/s), gate_add_norm of 8192 x 1280 42 us (3.0 TB/s, nine waves a unit; 31 us, 4.1 TB/s, without sums), norm of 16384 x 320 15 us
 // (2.1 TB/s).
 template <typename T, Row R, int G, int THREADS, bool BRANCH, bool NEXT, bool SUMS>
@@ -516,7 +516,7 @@ __global__ __launch_bounds__(THREADS) void k_norm_backward(Norms<T> a, Chunks cu
     if constexpr (SUMS) {
 #pragma unroll
       for (int k = BRANCH ? 0 : 2; k < (NEXT ? kSums : 2); k += 2) {
-        float* const out = parts + (chunk * kSums + k) * width;
+        float* const out = parts + (BRANCH && NEXT ? chunk * kSums + k : chunk * 2) * width;
         if (R == Row::kWaves || at_once == 1) {
 #pragma unroll
           for (int g = 0; g < G; ++g)
@@ -553,9 +553,9 @@ __global__ __launch_bounds__(THREADS) void k_norm_backward(Norms<T> a, Chunks cu
 // group, w, b the half's weight and bias and f its factor (the gate; 1 + scale):
 //   of the factor  w S1 + b S0;   of the shift  S0;   of w  sum over groups of f S1;   of b  sum over groups of f S0.
 // 4 lanes take 16 columns, 128 such members of a workgroup share out the groups, `team` of them (a power of two) one group: all chunks of
-// it are asked for at once (sums of 16384 x 2560: 10.8 us; 32 columns a workgroup 12.8, 8, less than a line of memory, 18).  A slab (y) is a range of groups, and what is shared by all groups goes to `partial` [slab][half][4][width]
-// (of the weight, the bias, the factor, the shift) where there are several slabs.  7 to 11 us: a launch and
-// the trips to memory of sums that other dies have written.
+// it are asked for at once (sums of 16384 x 2560: 10.8 us; 32 columns a workgroup 12.8, 8, less than a line of memory, 18).  A slab (y) is
+// a range of groups, and what is shared by all groups goes to `partial` [slab][half][4][width] (of the weight, the bias, the factor, the
+// shift) where there are several slabs.  7 to 11 us: a launch and the trips to memory of sums that other dies have written.
 template <typename T>
 struct Half {
   const T *weight, *bias, *factor;
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(kFinishThreads) void k_norm_finish(Half<T> branch, 
     if (n > 0 && g < g1) {
 #pragma unroll 8
       for (int64_t i = of; i < chunks; i += team) {
-        const float* p = parts + ((g * chunks + i) * kSums + 2 * half) * width + c;  // 4 of them: width is a multiple of 8
+        const float* p = parts + ((g * chunks + i) * gridDim.z + blockIdx.z) * 2 * width + c;  // 4 of them: width is a multiple of 8
         s0 += *(const f32x4*)p, s1 += *(const f32x4*)(p + width);
       }
     }
@@ -660,7 +660,7 @@ __global__ __launch_bounds__(kFinishThreads) void k_norm_finish(Half<T> branch, 
 #pragma unroll
   for (int i = 0; i < kFinishThreads / 64; ++i) v += meet[member][i][lane];
   if (partial != nullptr) {
-    *(f32x4*)(partial + ((int64_t)blockIdx.y * 2 + half) * 4 * width + member * width + c) = v;
+    *(f32x4*)(partial + (((int64_t)blockIdx.y * gridDim.z + blockIdx.z) * 4 + member) * width + c) = v;
     return;
   }
   T* const out = member == 0 ? h.dweight : member == 1 ? h.dbias : member == 2 ? (h.ld_factor == 0 ? h.dfactor : nullptr) : h.ld_shift == 0 ? h.dshift : nullptr;
@@ -677,7 +677,7 @@ __global__ __launch_bounds__(256) void k_norm_join(Half<T> branch, Half<T> next,
   if (c >= cols || out == nullptr) return;
   float v = 0.0f;
 #pragma unroll 4
-  for (int64_t i = 0; i < slabs; ++i) v += partial[(i * 2 + half) * 4 * width + which * width + c];
+  for (int64_t i = 0; i < slabs; ++i) v += partial[((i * gridDim.z + blockIdx.z) * 4 + which) * width + c];
   out[c] = (T)v;
 }
 
@@ -812,8 +812,9 @@ int backward(const gf_norm_args& a, Arena& ws, bool run, hipStream_t s) {
         const Chunks cut = cut_rows(a.rows, a.group_rows, Place<R, G>::rows_at_once(threads), 256 * (sums ? fit : 2));
         const int64_t chunks = cut.chunks, all = cut.all;
         const int64_t slabs = groups <= 1024 ? 1 : std::min<int64_t>((groups + 511) / 512, 64);
-        float* const parts = sums ? (float*)ws.take(all * kSums * width * 4) : nullptr;
-        float* const partial = sums && slabs > 1 ? (float*)ws.take(slabs * 8 * width * 4) : nullptr;
+        const int half0 = kBranch ? 0 : 1, halves = (kBranch ? 1 : 0) + (kNext ? 1 : 0);
+        float* const parts = sums ? (float*)ws.take(all * 2 * halves * width * 4) : nullptr;
+        float* const partial = sums && slabs > 1 ? (float*)ws.take(slabs * halves * 4 * width * 4) : nullptr;
         GF_RUN {
           const Norms<T> n = make_norms<T>(a);
           const unsigned grid = (unsigned)std::min<int64_t>(all, 1 << 20);
@@ -828,9 +829,8 @@ int backward(const gf_norm_args& a, Arena& ws, bool run, hipStream_t s) {
             const Half<T> f{n.next_weight, n.next_bias, n.scale, n.ld_scale, n.ld_shift, 1.0f, 1.0f, n.dnext_weight, n.dnext_bias, n.dscale, n.dshift};
             int team = 1;
             while (team < kFinishThreads / kFinishLanes && team * 2 * groups <= kFinishThreads / kFinishLanes) team *= 2;
-            const int half0 = kBranch ? 0 : 1, halves = (kBranch ? 1 : 0) + (kNext ? 1 : 0);
-            k_norm_finish<T><<<dim3((unsigned)((a.cols + 4 * kFinishLanes - 1) / (4 * kFinishLanes)), (unsigned)slabs, halves), kFinishThreads, 0, s>>>(b, f, half0, n.cols, groups, chunks, parts,
-                                                                                                         width, team, partial);
+            const dim3 blocks((unsigned)((a.cols + 4 * kFinishLanes - 1) / (4 * kFinishLanes)), (unsigned)slabs, halves);
+            k_norm_finish<T><<<blocks, kFinishThreads, 0, s>>>(b, f, half0, n.cols, groups, chunks, parts, width, team, partial);
             GF_LAUNCH_CHECK("k_norm_finish");
             if (partial != nullptr) {
               k_norm_join<T><<<dim3((unsigned)((a.cols + 255) / 256), 4, halves), 256, 0, s>>>(b, f, half0, n.cols, slabs, partial, width);
