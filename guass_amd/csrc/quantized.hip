@@ -150,11 +150,18 @@ struct Few {
 //
 // x's operands are 8 columns of row lane % 16 from each sixteen lanes.  Loaded as such, neighbouring lanes would ask for different lines
 // of memory, 64 a load.  Of more than 4 rows a wave loads them row by row, 16 lanes and 256 bytes each, and passes them through its own
-// piece of LDS (no barrier: a wave's LDS operations keep their order), 16 bytes at a time, at place p ^ row of a row's 16 so that neither side's
-// lanes meet in a bank.  Up to 4 rows (DIRECT) the lanes that have one load it themselves.  32-bit operands are multiplied as such
-// (16 x 16 x 4).
+// piece of LDS, 16 bytes at a time, at place p ^ row of a row's 16 so that neither side's lanes meet in a bank.  The hardware keeps a wave's
+// LDS operations in their order, so it takes no barrier of the workgroup; that the compiler keeps it, a fence says.  Up to 4 rows (DIRECT)
+// the lanes that have one load it themselves.  32-bit operands are multiplied as such (16 x 16 x 4).
 template <typename T, int G>
 constexpr int kFewWaves = G == 1 ? 16 : G * (int)sizeof(T) >= 16 ? 4 : 8;  // as registers allow
+
+// What lanes of a wave have written to LDS before, others of it read after, and the other way round.  No instruction.
+__device__ __attribute__((always_inline)) inline void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
 
 template <typename T, int H, int G, int NT, bool DIRECT>
 __global__ __launch_bounds__((kFewWaves<T, G> * 64)) void k_q4_few(Few<T> a) {
@@ -202,9 +209,11 @@ __global__ __launch_bounds__((kFewWaves<T, G> * 64)) void k_q4_few(Few<T> a) {
   auto multiply = [&](const Codes& c, Part& part, int64_t next) {
     const Part here = part;
     if constexpr (!DIRECT) {
+      wave_fence();  // the tile before is read
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
         *(Piece*)__builtin_assume_aligned(stage + (x_row(i) * P + ((lane % P) ^ (x_row(i) % 16 * (P / 16)))) * 16, 16) = here.x[i];
+      wave_fence();
     }
     if (next < whole) load_x(part, next);
 #pragma unroll
