@@ -51,3 +51,42 @@ def test_sums_of_whole_numbers(device, rows, dtype):
             assert bool(((got.double() - want).abs() <= bound).all()), f"{rows} x {d} -> {n}"
             continue
         assert torch.equal(got, want), f"{rows} x {d} -> {n}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("rows", [3, 32, 100])
+def test_every_scale_whose_values_the_type_holds(device, rows, dtype):
+    """All 16 codes at 2^-125 to 2^125, picked out by a row of x with a single 1: exact, as the type has them (0.5 * 2^-125 is its smallest
+    normal number, 6 * 2^125 below its largest)."""
+    _say("scales", rows, dtype)
+    codes = torch.tensor([[2 * i | (2 * i + 1) << 4 for i in range(8)] * 2], dtype=torch.uint8).expand(251, 16).contiguous()
+    scales = torch.arange(2, 253, dtype=torch.uint8)[:, None].contiguous()
+    values = bo.dequantize(codes, scales, 32)
+    w = q4.QuantizedWeight(codes.to(device), scales.to(device), 32)
+    assert torch.equal(w.dequantize(dtype).cpu().double(), values)
+    for first in range(0, 32, rows):
+        x = torch.zeros(rows, 32, dtype=dtype)
+        at = torch.arange(rows)
+        x[at, (first + at) % 32] = 1.0
+        got = q4.quantized_linear(x.to(device), w).cpu().double()
+        assert torch.equal(got, values[:, (first + at) % 32].t())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows", [64, 128, 129, 200])
+def test_an_infinity_at_every_number_of_rows(device, rows, dtype):
+    """In x at a column of any code: infinite of the code's sign, a NaN where the code is zero, the other rows as without."""
+    _say("infinity", rows, dtype)
+    w, values = _weight(device, 48, 50, seed=4)
+    x = _whole(rows, 50, seed=5).to(dtype).to(device)
+    want = q4.quantized_linear(x, w)
+    at = rows - 1 - rows // 3
+    for bad in (math.inf, -math.inf):
+        x[at, 49] = bad
+        got = q4.quantized_linear(x, w)
+        keep = torch.arange(rows, device=device) != at
+        assert torch.equal(got[keep], want[keep])
+        exact = values[:, 49] * bad
+        assert bool(torch.isnan(exact).any()) and torch.equal(got[at].cpu().double().nan_to_num(0.5, 1.0, -1.0), exact.nan_to_num(0.5, 1.0, -1.0))
