@@ -253,14 +253,17 @@ __device__ __attribute__((always_inline)) inline void make_maps(Maps<G, SHARED>&
     if constexpr (BRANCH) {
       const float value = a.gate ? 1.0f : a.gate_value;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) times[j] = value * (float)f[j] * (float)w[j], plus[j] = value * (float)f[j] * (float)b[j];
+      for (int j = 0; j < 8; ++j) {
+        const float factor = value * (float)f[j];
+        times[j] = factor * (float)w[j], plus[j] = a.bias ? factor * (float)b[j] : 0.0f;  // an infinite gate times no bias is no NaN
+      }
       m.put(kBranchTimes, g, times), m.put(kBranchPlus, g, plus);
     }
     if constexpr (NEXT) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float factor = 1.0f + (float)f2[j];
-        times[j] = factor * (float)w2[j], plus[j] = __builtin_fmaf(factor, (float)b2[j], (float)s2[j]);
+        times[j] = factor * (float)w2[j], plus[j] = a.next_bias ? __builtin_fmaf(factor, (float)b2[j], (float)s2[j]) : (float)s2[j];
       }
       m.put(kNextTimes, g, times), m.put(kNextPlus, g, plus);
     }
@@ -636,7 +639,7 @@ __global__ __launch_bounds__(kFinishThreads) void k_norm_finish(Half<T> branch, 
     if (n > 0 && g < g1 && of == 0) {
       const f32x4 f = h.factor != nullptr ? h.one + widen4<T>(factor) : f32x4(h.value);
       shared[0] += f * s1, shared[1] += f * s0;
-      const f32x4 own = widen4<T>(w) * s1 + widen4<T>(b) * s0;
+      const f32x4 own = widen4<T>(w) * s1 + (h.bias != nullptr ? widen4<T>(b) * s0 : f32x4(0.0f));
       if (h.dfactor != nullptr) {
         if (h.ld_factor != 0) store4(h.dfactor + g * cols, c, n, own);
         else shared[2] += own;

@@ -13,7 +13,8 @@ layer_norm.  Rows of 1 to 16384 elements.  ``weight`` and ``bias`` have a row's 
 that of x with ones behind its first dimensions ([samples, 1, features] of x [samples, places, features]: one row a
 sample); those of a call that are not shared by all rows are shared by the same ones.  Rows of a larger matrix (slices of one
 modulation, say) are read in place.  Every call runs on torch's current stream of its tensors' device and does not synchronise.
-Squares are summed in 32 bits: a row with elements past about 10^19 has no statistics.
+Squares are summed in 32 bits: a row with elements past about 10^19 has no statistics.  A factor goes into weight and bias before the row does:
+an infinite gate or scale beside a bias gives a NaN where its two infinities differ in sign.
 """
 
 from __future__ import annotations
