@@ -63,3 +63,38 @@ def test_an_infinite_gradient_without_a_bias(device, dtype):
         f = factor.clone().requires_grad_(True)
         g, = torch.autograd.grad(call(f), f, dy)
         assert float(g[17]) == want and int(torch.isfinite(g).sum()) == 39
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op,shape", [("gate_add", (16, 1024, 2560)), ("gate_add_norm", (32, 256, 1280)), ("norm", (4, 4096, 320)), ("gate_add", (3, 701, 1333))])
+def test_pass_after_pass_the_same_bits(device, op, shape):
+    """Training passes on two sets of inputs in turn that nothing waits between, as many workgroups' sums joined as a card has units: every
+    output and gradient has the bits of a pass by itself."""
+    _say("again", op, shape)
+    cols, dtype = shape[-1], torch.bfloat16
+    sets = []
+    for k in range(2):
+        t = {"x": _rand(device, *shape, dtype=dtype, seed=10 * k), "r": _rand(device, *shape, dtype=dtype, seed=10 * k + 1)}
+        t.update({n: _rand(device, cols, dtype=dtype, seed=10 * k + 2 + i) for i, n in enumerate("wb")})
+        t.update({n: _rand(device, shape[0], 1, cols, dtype=dtype, seed=10 * k + 4 + i) for i, n in enumerate(("g", "s"))})
+        sets.append(({n: v.requires_grad_(True) for n, v in t.items()}, [_rand(device, *shape, dtype=dtype, seed=10 * k + 6 + i) for i in range(2)]))
+
+    def step(k):
+        t, dy = sets[k]
+        if op == "norm":
+            out, names = (norms.norm(t["x"], t["w"], t["b"], scale=t["g"], shift=t["s"]),), "xwbgs"
+        elif op == "gate_add":
+            out, names = (norms.gate_add(t["x"], t["r"], t["w"], t["b"], kind="layer", gate=t["g"]),), "xrwbg"
+        else:
+            out, names = norms.gate_add_norm(t["x"], t["r"], t["w"], t["b"], t["w"], t["b"], kind="layer", gate=t["g"], scale=t["s"]), "xrwbgs"
+        return [*(o.detach() for o in out), *torch.autograd.grad(out, [t[n] for n in names], dy[:len(out)])]
+
+    want = []
+    for k in range(2):
+        want.append(step(k))
+        torch.cuda.synchronize()
+    differ = torch.zeros((), dtype=torch.int64, device=device)
+    for i in range(24):
+        for a, b in zip(step(i % 2), want[i % 2]):
+            differ += (a != b).sum()
+    assert int(differ) == 0
