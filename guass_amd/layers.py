@@ -340,16 +340,19 @@ class BlockNorm(nn.Module):
         self.bias = nn.Parameter(torch.zeros(features, device=device, dtype=dtype)) if affine and bias else None
 
     @classmethod
-    def from_norm(cls, norm: nn.Module) -> "BlockNorm":
-        """Of a torch LayerNorm or RMSNorm over the last dimension, whose parameters it takes over."""
+    def from_norm(cls, norm: nn.Module, *, eps: float | None = None) -> "BlockNorm":
+        """Of a torch LayerNorm or RMSNorm over the last dimension, whose parameters it takes over, and eps where none is given.  A torch
+        RMSNorm made without one takes the machine epsilon of whatever type its input has: here it is to be given
+        (torch.finfo(torch.float32).eps, say)."""
         kinds = {nn.LayerNorm: "layer", nn.RMSNorm: "rms"}
         if type(norm) not in kinds:
             raise TypeError(f"norm must be a LayerNorm or an RMSNorm (got {type(norm).__name__})")
         if len(norm.normalized_shape) != 1:
             raise ValueError(f"norm must be over the last dimension (got normalized_shape {tuple(norm.normalized_shape)})")
-        if norm.eps is None:
-            raise ValueError("norm must have an eps")
-        made = cls(norm.normalized_shape[0], kind=kinds[type(norm)], eps=norm.eps, affine=False)
+        eps = norm.eps if eps is None else eps
+        if eps is None:
+            raise ValueError("norm must have an eps, or eps be given")
+        made = cls(norm.normalized_shape[0], kind=kinds[type(norm)], eps=eps, affine=False)
         made.weight, made.bias = norm.weight, getattr(norm, "bias", None)
         return made
 
