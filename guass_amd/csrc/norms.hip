@@ -760,7 +760,8 @@ int with_form(int64_t cols, int64_t wave_cols, F f) {
 
 // The widest row that a wave takes alone.  8192 x 1280 in bfloat16, gate_add_norm: 22 us forward (three waves a row: 26 to 29), 31 backward
 // without sums (33).  The sums of both halves leave a wave with three groups a lane no registers: 54 us by three waves, 66 by one.
-// With few rows a row's time counts: one of 1280 takes 3.2 us by three waves, 5.6 by one.
+// With few rows a row's time counts: one of 1280 takes 3.2 us by three waves, 5.6 by one.  2048 rows give each of 256
+// units eight waves; the border was not timed at other widths.
 int64_t wave_cols(const gf_norm_args& a, bool sums) {
   if (a.rows < 2048) return 512;
   return sums && a.residual != nullptr && a.next_kind != GF_NORM_NONE ? 1024 : 1536;

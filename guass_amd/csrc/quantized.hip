@@ -287,7 +287,9 @@ __global__ __launch_bounds__((kFewWaves<T, G> * 64)) void k_q4_few(Few<T> a) {
       if (a.bias != nullptr) v[h] += (float)a.bias[col + h * a.N];
     }
     if constexpr (H == 2)
-      v[0] *= a.act == GF_ACT_GELU ? activation<GF_ACT_GELU>(v[1], nullptr) : a.act == GF_ACT_SILU ? activation<GF_ACT_SILU>(v[1], nullptr) : activation<GF_ACT_GELU_TANH>(v[1], nullptr);
+      v[0] *= a.act == GF_ACT_GELU   ? activation<GF_ACT_GELU>(v[1], nullptr)
+              : a.act == GF_ACT_SILU ? activation<GF_ACT_SILU>(v[1], nullptr)
+                                     : activation<GF_ACT_GELU_TANH>(v[1], nullptr);
     if (a.residual != nullptr) v[0] += (float)a.residual[m * a.ldr + col];
     a.y[m * a.N + col] = (T)v[0];
   }
@@ -389,8 +391,9 @@ gf_ff_args dense(const gf_q4_args& a, const void* weight) {
   return f;
 }
 
-// By the codes up to 128 rows, 64 at a time.  128 rows, through the values first: in bfloat16 8192 -> 8192 66 and 40 us, 1280 -> 5120 gated 31 and
-// 19, 320 -> 2560 gated 12 and 16; in 32 bits 332 and 197, 62 and 66, 28 and 25.
+// By the codes up to 128 rows, 64 at a time, whatever the size: one border, where either way loses somewhere.  128 rows, through the values
+// and by the codes: in bfloat16 8192 -> 8192 66 and 40 us, 1280 -> 5120 gated 31 and 19, 320 -> 2560 gated 12 and 16; in 32 bits 332 and 197, 62
+// and 66, 28 and 25: of these six, small gated weights lose 4 us by the codes.
 bool few(const gf_q4_args& a) { return a.rows <= 128 && a.saved == nullptr; }
 
 template <typename T>

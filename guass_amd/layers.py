@@ -324,7 +324,8 @@ class GaussianFeedForward(nn.Module):
 
 class BlockNorm(nn.Module):
     """The norm before a block, on the kernels of guass_amd.norms: norm(x) * weight + bias, times (1 + scale) plus shift.  ``after``
-    ends one block and gives the next one its norm in one pass."""
+    ends one block and gives the next one its norm in one pass; it is no call of the layers, so no hooks run, on this one or on
+    ``branch_norm``."""
 
     def __init__(self, features: int, *, kind: str = "layer", eps: float = 1e-5, affine: bool = True, bias: bool = True, device=None,
                  dtype=None) -> None:
@@ -411,7 +412,8 @@ class QuantizedLinear(nn.Module):
 
 class QuantizedFeedForward(nn.Module):
     """GaussianFeedForward's inference form, both weights merged and in 4 bits: residual + out(value * act(gate)), (value, gate) the
-    halves of proj(x).  Nothing is dropped, and only inputs and biases can train."""
+    halves of proj(x).  Nothing is dropped, and only inputs and biases can train.  proj's own forward is not called (out's is), so neither
+    are hooks on it."""
 
     def __init__(self, proj: QuantizedLinear, out: QuantizedLinear, *, activation: str = "gelu") -> None:
         super().__init__()
@@ -439,7 +441,8 @@ class QuantizedFeedForward(nn.Module):
 class FeedForwardBlock(nn.Module):
     """A block's second half whole: stream + gate * out_norm(ff(norm(stream) * (1 + scale) + shift)).  ``ff`` is a
     GaussianFeedForward (``forward`` then takes its seed and offset) or a QuantizedFeedForward; ``scale``, ``shift`` and ``gate`` are
-    a sample's or all rows' (guass_amd.norms).  Without gate and out_norm the sum is the last product's epilogue."""
+    a sample's or all rows' (guass_amd.norms).  Without gate and out_norm the sum is the last product's epilogue.  out_norm's own
+    forward is not called, so neither are hooks on it."""
 
     def __init__(self, norm: BlockNorm, ff: nn.Module, out_norm: BlockNorm | None = None) -> None:
         super().__init__()

@@ -4,15 +4,18 @@
 * ``quantized_linear``        residual + x W^T + b
 * ``quantized_gated_linear``  value * act(gate), (value, gate) the two halves of x W^T + b
 
-A weight that does not train is kept so: the frozen base of an adapted layer, or what a trained adapter was merged into
-(``guass_amd.layers.QuantizedLinear``, ``QuantizedFeedForward``).  The format is the OCP microscaling formats' MXFP4: groups of
+A weight that does not train is kept so: what a trained adapter was merged into or a frozen layer (``guass_amd.layers.QuantizedLinear``,
+``QuantizedFeedForward``).  Gradients go through it to the inputs of these functions; a layer that trains an adapter beside a 4-bit base is not
+here (``GaussianLinear`` has a dense one).  The format is the OCP microscaling formats' MXFP4: groups of
 32 along a row share a scale 2^e, and an element is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  4.25 bits an element; its value is exact in
 bfloat16, and in float16 where the scale lies in [2^-23, 2^13] (past that, it is rounded to float16).
 
 The products' other tensors are of one type, float32, bfloat16 or float16; sums are accumulated in 32 bits.  Under ``torch.autocast``
 x and the bias take its type, as in nn.Linear.  At most 128 rows read the codes as they are; more, and
-a gated product's training pass, write the weight's values out for the call and run the products of ``guass_amd.feedforward``, backward too: the gradients of
-x, bias and residual, none of the weight.  Every call runs on torch's current stream of its tensors' device and does not synchronise.
+a gated product's training pass, write the weight's values out for the call and run the products of ``guass_amd.feedforward``, backward too: the
+gradients of x, bias and residual, none of the weight.  As there, a gated product's backward keeps value and gate in 20 (bfloat16) or 24
+bits (float16) and rounds dz, the products' gradient, to the tensors' type before dx = dz W: in 16 bits dx has two roundings, a
+linear product's one.  Every call runs on torch's current stream of its tensors' device and does not synchronise.
 """
 
 from __future__ import annotations

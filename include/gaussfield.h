@@ -618,7 +618,7 @@ int gf_norm_backward(const gf_norm_args* args, void* workspace, size_t workspace
  * times scale in 32 bits, rounded to dtype.
  *
  * gf_q4_forward, gf_q4_backward: the linear and gated products above with such a weight [out, in] ([2 out, in]), no dropout; dx [rows,
- * in] and dbias as there.  The products are of the weight's values in dtype. */
+ * in] and dbias as there (a gated dx of 16 bits with dz's rounding besides its own).  The products are of the weight's values in dtype. */
 typedef struct gf_q4_args {
   int32_t dtype, activation;
   int64_t rows, in_features, out_features;
