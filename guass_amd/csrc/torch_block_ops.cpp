@@ -58,20 +58,24 @@ void check_same(const MaybeTensor& t, const char* name, const Tensor& x) {
 #define NORM_ARGUMENTS \
   x, residual, weight, bias, gate, gate_value, residual_scale, kind, eps, next_weight, next_bias, scale, shift, next_kind, next_eps
 
-// The call as the C ABI takes it, with the tensors that it points into.
+// The call as the C ABI takes it, with the tensors that it points into.  A residual that is not read (a backward without a next norm) has x's
+// place.
 struct NormCall {
   Rows x;
   std::optional<Rows> residual;
   std::array<Tensor, 4> vectors;
   Shared gate, scale, shift;
   gf_norm_args a{};
-  explicit NormCall(NORM_PARAMETERS) : x(x) {
+  explicit NormCall(NORM_PARAMETERS, bool reads_residual = true) : x(x) {
     a.dtype = dtype_of(x), a.kind = (int32_t)kind, a.next_kind = (int32_t)next_kind;
     a.rows = this->x.rows, a.cols = this->x.cols;
     a.eps = eps, a.next_eps = next_eps, a.gate_value = gate_value, a.residual_scale = residual_scale;
     a.x = this->x.data(), a.ldx = this->x.ld;
     check_same(residual, "residual", x);
-    if (present(residual)) this->residual.emplace(*residual), a.residual = this->residual->data(), a.ldr = this->residual->ld;
+    if (present(residual) && reads_residual)
+      this->residual.emplace(*residual), a.residual = this->residual->data(), a.ldr = this->residual->ld;
+    else if (present(residual))
+      a.residual = a.x, a.ldr = a.ldx;
     const MaybeTensor* const from[] = {&weight, &bias, &next_weight, &next_bias};
     const void** const to[] = {&a.weight, &a.bias, &a.next_weight, &a.next_bias};
     const char* const names[] = {"weight", "bias", present(residual) ? "next_weight" : "weight", present(residual) ? "next_bias" : "bias"};
@@ -136,9 +140,9 @@ NormGrads block_norm_backward(NORM_PARAMETERS, const MaybeTensor& dstream, const
   if (x.numel() != 0 && (next || present(dstream))) {
     const MaybeTensor none;
     NormCall c(x, residual, weight, bias, gate, gate_value, residual_scale, kind, eps, next ? next_weight : none, next ? next_bias : none,
-               next ? scale : none, next ? shift : none, next ? next_kind : (int64_t)GF_NORM_NONE, next_eps);
+               next ? scale : none, next ? shift : none, next ? next_kind : (int64_t)GF_NORM_NONE, next_eps, next);
     std::optional<Rows> ds, dh;
-    if (present(dstream)) ds.emplace(*dstream), c.a.dstream = ds->data(), c.a.ld_dstream = ds->ld;
+    if (present(dstream)) ds = dstream->is_same(x) ? c.x : Rows(*dstream), c.a.dstream = ds->data(), c.a.ld_dstream = ds->ld;
     if (next) dh.emplace(*dnormed), c.a.dnormed = dh->data(), c.a.ld_dnormed = dh->ld;
     c.a.dx = at_[kX], c.a.dresidual = at_[kResidual], c.a.dweight = at_[kWeight], c.a.dbias = at_[kBias], c.a.dgate = at_[kGate];
     c.a.dnext_weight = at_[kNextWeight], c.a.dnext_bias = at_[kNextBias], c.a.dscale = at_[kScale], c.a.dshift = at_[kShift];

@@ -565,7 +565,8 @@ int gf_ff_backward(const gf_ff_args* args, void* workspace, size_t workspace_byt
  * held in 32 bits: squares of rows beyond 10^19 / sqrt(cols) leave their range.
  *
  * Backward: dstream and dnormed are the gradients of s and h (dstream NULL: zero, where there is a next norm); the gradients that are not NULL are
- * written whole, contiguous, shaped as their parameter ([rows / group_rows, cols] or [cols]).  gate_value has none. */
+ * written whole, contiguous, shaped as their parameter ([rows / group_rows, cols] or [cols]).  gate_value has none.  Without a next norm no
+ * gradient is made of the residual, and of x only those through the branch's norm and the gate's: any matrix of their size may stand there. */
 #define GF_NORM_NONE 0
 #define GF_NORM_LAYER 1
 #define GF_NORM_RMS 2

@@ -139,3 +139,21 @@ def test_a_gradient_that_depends_refuses(device, which, train):
     grad, = torch.autograd.grad(h, calls[which], dy, create_graph=True)
     with pytest.raises(RuntimeError, match="gate_add_norm is differentiable once only"):
         (grad**2).sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,gate", [(None, 0.5), ("layer", 1.0)])
+def test_a_broadcast_gradient_is_laid_out_once(device, kind, gate):
+    """gate_add's backward takes the gradient's place for x and the residual where it reads neither, with no copies of its own for them."""
+    _say("broadcast gradient", kind)
+    x, r = (_rand(device, 512, 1024, seed=i).requires_grad_(True) for i in range(2))
+    one = torch.full((1, 1), 3.0, device=device).expand(512, 1024)
+    want = torch.autograd.grad(norms.gate_add(x, r, kind=kind, gate=gate, residual_scale=0.25), (x, r), one.contiguous())
+    y = norms.gate_add(x, r * 1, kind=kind, gate=gate, residual_scale=0.25)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats(device)
+    before = torch.cuda.memory_allocated(device)
+    got = torch.autograd.grad(y, (x, r), one)
+    size = 4 * x.numel()  # the gradient laid out, dx, the residual's, and that times 1 behind it
+    assert torch.cuda.max_memory_allocated(device) - before < 4 * size + size // 2
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
