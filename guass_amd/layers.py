@@ -375,7 +375,8 @@ class BlockNorm(nn.Module):
 
 class QuantizedLinear(nn.Module):
     """nn.Linear with a weight in 4 bits that does not train (guass_amd.quantized): a frozen layer, or a trained GaussianLinear
-    merged (weight + adapter_scale * delta-W, rendered once)."""
+    merged (weight + adapter_scale * delta-W, rendered once).  A state dict holds the weight's size beside its tiles, which are alike for
+    several sizes; one without it loads too."""
 
     def __init__(self, weight, bias: Tensor | None = None) -> None:
         super().__init__()
@@ -397,6 +398,22 @@ class QuantizedLinear(nn.Module):
         with torch.no_grad():
             weight = linear.merged_weight() if isinstance(linear, GaussianLinear) else linear.weight
             return cls(quantize(weight), linear.bias)
+
+    def get_extra_state(self) -> Tensor:
+        return torch.tensor([self.out_features, self.in_features])
+
+    def set_extra_state(self, state: Tensor) -> None:
+        """Nothing: _load_from_state_dict has looked at it."""
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs) -> None:
+        size = state_dict.get(prefix + "_extra_state")
+        if size is not None and [int(n) for n in size] != [self.out_features, self.in_features]:
+            error_msgs.append(f"size mismatch for {prefix}weight: {[int(n) for n in size]} in the checkpoint, the layer's is "
+                              f"{[self.out_features, self.in_features]}")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if size is None and prefix + "_extra_state" in missing_keys:
+            missing_keys.remove(prefix + "_extra_state")
 
     @property
     def weight(self):

@@ -6,7 +6,8 @@ import pytest
 import torch
 from torch import nn
 
-from guass_amd.layers import BlockNorm
+from guass_amd.layers import BlockNorm, QuantizedFeedForward, QuantizedLinear
+from guass_amd.quantized import QuantizedWeight
 
 
 def test_a_norm_without_an_eps_takes_a_given_one():
@@ -18,6 +19,47 @@ def test_a_norm_without_an_eps_takes_a_given_one():
     assert BlockNorm.from_norm(nn.LayerNorm(8, eps=1e-3), eps=0.0).eps == 0.0
     with pytest.raises(ValueError, match="must have an eps, or eps be given"):
         BlockNorm.from_norm(rms)
+
+
+def _quantized(rows, cols, value, bias=False):
+    groups = -(-cols // 32)
+    weight = QuantizedWeight(torch.full((rows, 16 * groups), value, dtype=torch.uint8), torch.full((rows, groups), 120, dtype=torch.uint8), cols)
+    return QuantizedLinear(weight, torch.full((rows,), float(value)) if bias else None)
+
+
+def test_a_state_dict_of_another_size_is_refused():
+    """Also where the tiles, of 16 rows and 128 columns, are alike; the layer stays as it was."""
+    for rows, cols in ((20, 40), (24, 33), (17, 128)):
+        layer, other = _quantized(24, 40, 1), _quantized(rows, cols, 2)
+        assert layer.tile_codes.shape == other.tile_codes.shape
+        with pytest.raises(RuntimeError, match=rf"size mismatch for weight: \[{rows}, {cols}\] in the checkpoint, the layer's is \[24, 40\]"):
+            layer.load_state_dict(other.state_dict())
+        assert torch.equal(layer.weight.codes, _quantized(24, 40, 1).weight.codes)
+    ff, other = (QuantizedFeedForward(_quantized(2 * n, 40, n), _quantized(40, n, n)) for n in (20, 18))
+    with pytest.raises(RuntimeError, match="size mismatch for proj.weight"):
+        ff.load_state_dict(other.state_dict())
+
+
+def test_a_state_dict_loads():
+    """As saved and read back, without the size, and not strictly; what is missing or too much is said as ever."""
+    import io
+
+    whole = _quantized(24, 40, 2, bias=True)
+    file = io.BytesIO()
+    torch.save(whole.state_dict(), file)
+    file.seek(0)
+    state = torch.load(file, weights_only=True)
+    old = {k: v for k, v in state.items() if k != "_extra_state"}
+    for given in (state, old):
+        layer = _quantized(24, 40, 1, bias=True)
+        assert layer.load_state_dict(given) == ([], [])
+        assert torch.equal(layer.weight.codes, whole.weight.codes) and torch.equal(layer.weight.scales, whole.weight.scales)
+        assert torch.equal(layer.bias, whole.bias)
+    layer = _quantized(24, 40, 1)
+    with pytest.raises(RuntimeError, match="Unexpected key"):
+        layer.load_state_dict(state)
+    keys = layer.load_state_dict({"tile_codes": state["tile_codes"]}, strict=False)
+    assert keys.missing_keys == ["tile_scales"] and torch.equal(layer.tile_codes, whole.tile_codes)
 
 
 @pytest.mark.gpu
