@@ -9,6 +9,9 @@
 // A row is read once into registers, its statistics and all that follows are computed there in 32 bits, and each output is rounded
 // once: a fused pass gives h of the unrounded s.  Nothing is kept for the backward but the inputs: it makes s and both statistics
 // again from what it reads anyway.  No atomics: every sum has one order.
+//
+// Times at the kernels are medians within whole passes, forward and backward on two states in turn, under a profiler; times that compare two
+// forms or numbers of workgroups are of one kernel repeated, whose inputs the caches may partly hold.
 #include "elements.h"
 
 namespace {
@@ -350,8 +353,9 @@ struct Chunks {
   }
 
 // Forward.  BRANCH: s from x and the residual; NEXT: h from s (without BRANCH, from x).  The next row is on its way while one is worked on.
-// In bfloat16: gate_add of 16384 x 2560 46 us (5.4 TB/s: memory), gate_add_norm of 8192 x 1280 22 us (3.8 TB/s: two statistics a row one after
-// the other), norm of 16384 x 320 10 us (2 TB/s: 24 of 64 lanes idle, a launch and six turns); one row of 1280 3 to 4 us.
+// In bfloat16: gate_add of 16384 x 2560 51 us (5.0 TB/s: memory), gate_add_norm of 8192 x 1280 22 us (3.9 TB/s: two statistics a row one after
+// the other), norm of 16384 x 320 11 us (1.9 TB/s: 684 workgroups of four waves are 11 waves a unit, fewer than their registers let it hold, and
+// 24 of their 64 lanes are idle); one row of 1280 3.9 us.
 template <typename T, Row R, int G, int THREADS, bool BRANCH, bool NEXT>
 __global__ __launch_bounds__(THREADS) void k_norm_forward(Norms<T> a, Chunks cut) {
   __shared__ float2 meet[2][kMaxWaves];
@@ -404,9 +408,9 @@ __global__ __launch_bounds__(THREADS) void k_norm_forward(Norms<T> a, Chunks cut
 // Column sums of a chunk of rows, per element: of ds, ds n(x), dh, dh n'(s).  A half that is not there has none in memory.
 constexpr int kSums = 4;
 
-// Backward, by chunks of rows.  SUMS: the column sums too, into parts [chunk][2 of each half][width].  In bfloat16: gate_add of 16384 x 2560 56 us (4.5
-// TB/s), gate_add_norm of 8192 x 1280 42 us (3.0 TB/s, nine waves a unit; 31 us, 4.1 TB/s, without sums), norm of 16384 x 320 15 us
-// (2.1 TB/s).
+// Backward, by chunks of rows.  SUMS: the column sums too, into parts [chunk][2 of each half][width].  In bfloat16: gate_add of 16384 x 2560
+// 54 to 58 us (4.3 to 4.7 TB/s), gate_add_norm of 8192 x 1280 42 us (3.0 TB/s, nine waves a unit where the registers let it hold twelve;
+// repeated without sums 31 us, 4.1 TB/s), norm of 16384 x 320 15 us (2.1 TB/s, eight waves a unit).
 template <typename T, Row R, int G, int THREADS, bool BRANCH, bool NEXT, bool SUMS>
 __global__ __launch_bounds__(THREADS) void k_norm_backward(Norms<T> a, Chunks cut, float* parts, int64_t width) {
   __shared__ float2 meet[2][kMaxWaves];
@@ -556,9 +560,9 @@ __global__ __launch_bounds__(THREADS) void k_norm_backward(Norms<T> a, Chunks cu
 // group, w, b the half's weight and bias and f its factor (the gate; 1 + scale):
 //   of the factor  w S1 + b S0;   of the shift  S0;   of w  sum over groups of f S1;   of b  sum over groups of f S0.
 // 4 lanes take 16 columns, 128 such members of a workgroup share out the groups, `team` of them (a power of two) one group: all chunks of
-// it are asked for at once (sums of 16384 x 2560: 10.8 us; 32 columns a workgroup 12.8, 8, less than a line of memory, 18).  A slab (y) is
+// it are asked for at once (sums of 16384 x 2560, repeated: 10.8 us; 32 columns a workgroup 12.8, 8, less than a line of memory, 18).  A slab (y) is
 // a range of groups, and what is shared by all groups goes to `partial` [slab][half][4][width] (of the weight, the bias, the factor, the
-// shift) where there are several slabs.  7 to 11 us: a launch and the trips to memory of sums that other dies have written.
+// shift) where there are several slabs.  6 to 11 us: a launch and the trips to memory of sums that other dies have written.
 template <typename T>
 struct Half {
   const T *weight, *bias, *factor;
@@ -758,7 +762,7 @@ int with_form(int64_t cols, int64_t wave_cols, F f) {
   return f(Form<Row::kWaves, 2, 1024>());
 }
 
-// The widest row that a wave takes alone.  8192 x 1280 in bfloat16, gate_add_norm: 22 us forward (three waves a row: 26 to 29), 31 backward
+// The widest row that a wave takes alone.  8192 x 1280 in bfloat16, gate_add_norm, repeated: 22 us forward (three waves a row: 26 to 29), 31 backward
 // without sums (33).  The sums of both halves leave a wave with three groups a lane no registers: 54 us by three waves, 66 by one.
 // With few rows a row's time counts: one of 1280 takes 3.2 us by three waves, 5.6 by one.  2048 rows give each of 256
 // units eight waves; the border was not timed at other widths.
@@ -809,8 +813,8 @@ int backward(const gf_norm_args& a, Arena& ws, bool run, hipStream_t s) {
       return with_halves(a, [&](auto branch, auto next) {
         constexpr bool kBranch = branch.value, kNext = next.value, kSumless = R == Row::kWave && G == 3 && kBranch && kNext;
         // Workgroups for each of 256 compute units as their registers allow (12 waves for both halves' sums, 16 for one's), and each of them its
-        // chunks' sums to write and k_norm_finish to read: gate_add of 16384 x 2560 in 512 workgroups 63 and 10 us, 768 56 and 11, 1024 63 and
-        // 15.  Without sums two, which the barriers or loads of one do not keep waiting (8192 x 1280 gate_add_norm: 31 us; one of 8 waves 37).
+        // chunks' sums to write and k_norm_finish to read: gate_add of 16384 x 2560, repeated, in 512 workgroups 63 and 10 us, 768 56 and 11,
+        // 1024 63 and 15.  Without sums two, which the barriers or loads of one do not keep waiting (8192 x 1280 gate_add_norm: 31 us; one of 8 waves 37).
         const int threads = threads_of<R, G>(a.cols, a.group_rows, R == Row::kPart || (!sums && G > 1) ? 4 : 8);
         const int fit = R == Row::kWaves ? std::min(std::max((kBranch && kNext ? 12 : 16) * 64 / threads, 1), 3) : 1;
         const Chunks cut = cut_rows(a.rows, a.group_rows, Place<R, G>::rows_at_once(threads), 256 * (sums ? fit : 2));
@@ -870,8 +874,8 @@ int gf_norm_forward(const gf_norm_args* args, void* stream) {
       constexpr Row R = form.row;
       constexpr int G = form.groups, kThreads = form.threads;
       return with_halves(a, [&](auto branch, auto next) {
-        // enough workgroups to fill the units, each with rows enough that its maps and first row count for little (16384 x 2560 gate_add: 46 us,
-        // with 1024 workgroups 55)
+        // enough workgroups to fill the units, each with rows enough that its maps and first row count for little (16384 x 2560 gate_add,
+        // repeated: 46 us, with 1024 workgroups 55)
         const int threads = threads_of<R, G>(a.cols, a.group_rows, 4);
         const Chunks cut = cut_rows(a.rows, a.group_rows, Place<R, G>::rows_at_once(threads), R == Row::kWaves ? 512 : 768);
         const unsigned grid = (unsigned)std::min<int64_t>(cut.all, 1 << 20);

@@ -9,6 +9,9 @@
 // scale is not extreme: the matrix cores get it without a rounding of its own.  The hardware turns two codes into two values of a
 // scale in one instruction.  More rows go through k_dequantize and the feed-forward products (feedforward.hip), forward
 // and backward: the weight is frozen, so a backward has the inputs' gradient only.
+//
+// Times at the kernels are medians within whole passes on two states in turn, under a profiler; those that compare two forms are of one call
+// repeated, whose inputs the caches may partly hold.
 #include "elements.h"
 
 namespace {
@@ -42,7 +45,7 @@ __device__ inline int word_of(int row, int w) { return ((w & 3) * 16 + row) * 4 
 // what lies between 6 and 7 goes to 6, as near as a next value 8 would let it; from the bits of the largest magnitude m 2^p, 1 <= m < 2:
 // e = p - 2 up to m = 1.75, else p - 1.  Within [-125, 125], where every value is a normal number of 32 bits.  A group with an infinity or a
 // NaN gets the scale NaN.  The words change places in LDS, so that both sides of memory are read and written in a row.  Bound by memory: 10240 x
-// 1280 in 32 bits 11 us (5.3 TB/s), 8192 x 8192 in bfloat16 33 us (5.1 TB/s).
+// 1280 in 32 bits 11 us (5.4 TB/s); repeated, 8192 x 8192 in bfloat16 33 us (5.1 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void k_quantize(int64_t rows, int64_t cols, int64_t across, int64_t tiles, const T* __restrict__ w, int64_t ldw,
                                                   uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -78,7 +81,8 @@ __global__ __launch_bounds__(256) void k_quantize(int64_t rows, int64_t cols, in
 }
 
 // A tile a workgroup and turn, 8 values a thread, times their scale in 32 bits and rounded to T.  The next tile's words are on their way
-// while one is written.  Bound by memory: 10240 x 1280 into bfloat16 7.7 us (4.3 TB/s), 8192 x 8192 34 us (5.0 TB/s).
+// while one is written.  Bound by memory: 10240 x 1280 into bfloat16 9.0 us (3.7 TB/s), into 32 bits 13 us (4.5 TB/s); repeated, 8192 x 8192
+// into bfloat16 34 us (5.0 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void k_dequantize(int64_t rows, int64_t cols, int64_t across, int64_t tiles, const uint32_t* __restrict__ codes,
                                                     const uint8_t* __restrict__ scales, T* __restrict__ w) {
@@ -297,7 +301,7 @@ __global__ __launch_bounds__((kFewWaves<T, G> * 64)) void k_q4_few(Few<T> a) {
 
 // ------------------------------------------------------------------------------------------
 // The bias's gradient of a linear product, the columns' sums of dy: 8 columns a thread, a chunk of rows a workgroup (y), then the chunks in
-// their order.  Bound by reading dy: 8192 x 10240 in bfloat16 34 us in all (5.0 TB/s), 8192 x 1280 8.5.
+// their order.  Bound by reading dy: 8192 x 10240 in bfloat16 41 + 5 us in a training pass (3.7 TB/s), repeated 34 in all (5.0 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void k_column_sums(int64_t rows, int64_t cols, int64_t chunk, const T* __restrict__ dy, int64_t ld, float* __restrict__ sums,
                                                      int64_t width) {
@@ -353,7 +357,7 @@ __global__ __launch_bounds__(256) void k_column_join(int64_t chunks, int64_t col
 
 int64_t bands_of(int64_t rows) { return (rows + 15) / 16; }
 int64_t across_of(int64_t cols) { return (cols + 127) / 128; }
-// 8 workgroups a unit: 10240 x 1280 into bfloat16 7.7 us (16384 workgroups, a tile each: 8.2; 1024: 8.3)
+// 8 workgroups a unit: 10240 x 1280 into bfloat16, repeated, 7.7 us (16384 workgroups, a tile each: 8.2; 1024: 8.3)
 unsigned tile_blocks(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, 2048); }
 int64_t weight_rows(const gf_q4_args& a) { return a.out_features * (a.activation == GF_ACT_NONE ? 1 : 2); }
 
@@ -392,7 +396,7 @@ gf_ff_args dense(const gf_q4_args& a, const void* weight) {
 }
 
 // By the codes up to 128 rows, 64 at a time, whatever the size: one border, where either way loses somewhere.  128 rows, through the values
-// and by the codes: in bfloat16 8192 -> 8192 66 and 40 us, 1280 -> 5120 gated 31 and 19, 320 -> 2560 gated 12 and 16; in 32 bits 332 and 197, 62
+// and by the codes, repeated: in bfloat16 8192 -> 8192 66 and 40 us, 1280 -> 5120 gated 31 and 19, 320 -> 2560 gated 12 and 16; in 32 bits 332 and 197, 62
 // and 66, 28 and 25: of these six, small gated weights lose 4 us by the codes.
 bool few(const gf_q4_args& a) { return a.rows <= 128 && a.saved == nullptr; }
 
@@ -417,7 +421,8 @@ int through_dense(const gf_q4_args& a, bool is_backward, Arena& ws, bool run, hi
   return GF_OK;
 }
 
-// A workgroup a unit, since every chunk is read back to be joined: 8192 x 10240 34 us, 8192 x 1280 8.5 and 1000 x 5120 7.9; with four 35, 14 and 9.0.
+// A workgroup a unit, since every chunk is read back to be joined: repeated, 8192 x 10240 34 us, 8192 x 1280 8.4 and 1000 x 5120 7.9; with
+// four 35, 14 and 9.0.  Not compared within a training pass.
 int column_sums(const gf_q4_args& a, Arena& ws, bool run, hipStream_t s) {
   const int64_t across = (a.out_features + 2047) / 2048, width = round_up(a.out_features, 8);
   const int64_t want = std::max<int64_t>(std::min<int64_t>(256 / across, a.rows / 8), 1), chunk = (a.rows + want - 1) / want, chunks = (a.rows + chunk - 1) / chunk;
@@ -447,7 +452,7 @@ int backward(const gf_q4_args& a, Arena& ws, bool run, hipStream_t s) {
 
 template <typename T, int H, int G, bool DIRECT>
 int launch_few(const Few<T>& f, bool wide, hipStream_t s) {
-  // 32 columns a workgroup where that still makes one for each of 256 compute units: of 8192 -> 8192 in bfloat16 one row takes 10.6 us
+  // 32 columns a workgroup where that still makes one for each of 256 compute units: of 8192 -> 8192 in bfloat16, repeated, one row takes 10.6 us
   // (16 columns: 11.8), 64 rows 22.6 (36).  16 waves up to a workgroup a unit, else 8, of which two are at work on a unit: 5120 -> 1280 4.5 us
   // (8 waves: 5.3), 4096 -> 14336 9.6 (16: 11.3), 1280 -> 5120 gated 5.1 (16: 5.9).
   const int64_t cols = wide ? 32 : 16, groups = (f.N + cols - 1) / cols;
