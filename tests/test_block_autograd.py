@@ -157,3 +157,18 @@ def test_a_broadcast_gradient_is_laid_out_once(device, kind, gate):
     size = 4 * x.numel()  # the gradient laid out, dx, the residual's, and that times 1 behind it
     assert torch.cuda.max_memory_allocated(device) - before < 4 * size + size // 2
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["gate_add of a number", "gate_add, a frozen gate", "gate_add's residual", "gate_add_norm's stream"])
+def test_compiled_where_an_input_is_not_kept(device, name):
+    _say("compiled", name)
+    torch._dynamo.reset()
+    norms._ops()
+    call, train = LINEAR[name]
+    compiled = torch.compile(lambda t: call(t) * 2, backend="aot_eager", fullgraph=True)
+    t, dy = _inputs(device), _rand(device, 2, 5, 40, seed=9)
+    leaves = [t[k] for k in train]
+    want = torch.autograd.grad(call(t) * 2, leaves, dy)
+    for a, b in zip(torch.autograd.grad(compiled(t), leaves, dy), want):
+        assert torch.equal(a, b)

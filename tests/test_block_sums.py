@@ -124,3 +124,27 @@ def test_the_norms_sums_are_exact(device, kind, rows, dtype):
         _exact({n: got[n] for n in names[3:]}, {"w2": s1, "b2": s0, "scale": s1, "shift": s0}, dtype, dy, f"gate_add_norm's norm {rows} x {cols}")
         got = _sums(call, t, [dy, torch.zeros_like(dy)], names, dtype)
         _exact(got, {"w": s1, "b": s0, "gate": s1, **{n: zero for n in names[3:]}}, dtype, dy, f"gate_add_norm's branch {rows} x {cols}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [8, 130])
+def test_more_groups_than_workgroups(device, cols):
+    """A gate, scale and shift of each row's own, for more rows than a grid has workgroups (2^20): each row's gradient, and what all rows
+    share, of whole numbers."""
+    rows = 2**20 + 77
+    _say("groups", rows, cols)
+    x, dy = _whole(device, rows, cols, seed=1).float(), _whole(device, rows, cols, seed=2).float()
+    gate = torch.ones_like(x).requires_grad_(True)
+    x.requires_grad_(True)
+    y = norms.gate_add(x, dy, gate=gate)
+    assert torch.equal(y, x + dy)
+    dx, dgate = torch.autograd.grad(y, (x, gate), dy)
+    assert torch.equal(dx, dy) and torch.equal(dgate, dy * x)
+    del y, dx, dgate, gate
+    zero = torch.zeros(rows, cols, device=device)
+    scale, shift, bias = (t.requires_grad_(True) for t in (zero.clone(), zero, torch.zeros(cols, device=device)))
+    ds, db, dscale = torch.autograd.grad(norms.norm(x.detach(), None, bias, kind="rms", scale=scale, shift=shift), (shift, bias, scale), dy)
+    assert torch.equal(ds, dy) and torch.equal(db.double(), dy.double().sum(0))
+    want = dy.double() * (x.detach().double() / (x.detach().double().square().mean(-1, keepdim=True) + 1e-5).sqrt())
+    # squares are exact; 1 / cols, their mean with eps, the root to within 3 units, the norm and the product: 8 roundings at most
+    assert bool(((dscale.double() - want).abs() <= 8 * 2.0**-24 * want.abs()).all())

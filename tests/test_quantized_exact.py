@@ -90,3 +90,21 @@ def test_an_infinity_at_every_number_of_rows(device, rows, dtype):
         assert torch.equal(got[keep], want[keep])
         exact = values[:, 49] * bad
         assert bool(torch.isnan(exact).any()) and torch.equal(got[at].cpu().double().nan_to_num(0.5, 1.0, -1.0), exact.nan_to_num(0.5, 1.0, -1.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows", [5, 80, 150])
+def test_rows_of_larger_matrices_give_the_same_bits(device, rows, dtype):
+    """Strides and odd bases change no sum, in float32 neither."""
+    w, _ = _weight(device, 40, 72, seed=3)
+    g = torch.Generator().manual_seed(6)
+    x, b, r = (torch.randn(*s, generator=g).to(dtype).to(device) for s in ((rows, 72), (40,), (rows, 40)))
+    want = q4.quantized_linear(x, w, b, r)
+    for left, right in ((8, 8), (1, 2), (16, 3)):
+        wide = []
+        for m in (x, r):
+            big = torch.full((rows + 1, left + m.shape[1] + right), math.nan, dtype=dtype, device=device)
+            big[:-1, left:left + m.shape[1]] = m
+            wide.append(big[:-1, left:left + m.shape[1]])
+        assert torch.equal(q4.quantized_linear(wide[0], w, b, wide[1]), want)
